@@ -294,6 +294,55 @@ int or_varlen_fwd(const or_varlen_args* args, void* stream);
  * serialised by the caller; calls on one stream are ordered. */
 int or_varlen_fwd_noalloc(const or_varlen_args* args, void* stream);
 
+/* Arguments of or_varlen_bwd. Segment s has query rows [cu_q[s], cu_q[s+1]) of q, o, d_o and dq, and key rows
+ * [k_start, k_start + k_len) of k, v, dk and dv, with k_start = k_off ? k_off[s] : cu_k[s] and the count
+ * k_len ? k_len[s] : cu_k[s+1] - k_start. The key ranges of segments may overlap. Offsets are read on the device; rows past
+ * n_q and n_k are not touched whatever they say. */
+typedef struct or_varlen_bwd_args {
+  const void* q;            /* bf16 [n_q, H, D], row stride q_row_stride */
+  const void* k;            /* bf16 [n_k, H, D], row stride k_row_stride */
+  const void* v;            /* bf16 [n_k, H, D], row stride k_row_stride */
+  const void* o;            /* bf16 [n_q, H, D], row stride o_row_stride: the forward call's output */
+  const void* d_o;          /* bf16 [n_q, H, D], row stride do_row_stride: the gradient of o */
+  const float* lse;         /* fp32 [H, n_q], head stride lse_stride: the forward call's log-sum-exp */
+  const float* dlse;        /* optional fp32, as lse: the gradient of lse */
+  void* dq;                 /* bf16 [n_q, H, D], contiguous; every row is written (zeros where nothing is attended to) */
+  void* dk;                 /* bf16 [n_k, H, D], contiguous; every row is written (zeros where no segment reads it) */
+  void* dv;                 /* bf16 [n_k, H, D], contiguous, likewise */
+  const int32_t* cu_q;      /* [n_seg + 1] */
+  const int32_t* cu_k;      /* [n_seg + 1] or NULL with k_off and k_len */
+  const int32_t* k_off;     /* optional [n_seg] */
+  const int32_t* k_len;     /* optional [n_seg] */
+  int64_t q_row_stride;     /* elements; multiples of 8 */
+  int64_t k_row_stride;
+  int64_t o_row_stride;
+  int64_t do_row_stride;
+  int64_t lse_stride;       /* elements between the heads of lse and of dlse */
+  int32_t n_seg;            /* 1 to 4096 */
+  int32_t n_q;
+  int32_t n_k;
+  int32_t max_q;            /* most queries and keys of a segment: they choose tiles and splits, not results' validity */
+  int32_t max_k;
+  int32_t H;
+  int32_t D;                /* 64 or 128 */
+  float scale;              /* the forward call's softmax scale */
+  void* workspace;          /* device scratch of or_varlen_bwd_workspace_size() bytes for the same sizes */
+  int64_t workspace_bytes;
+} or_varlen_bwd_args;
+
+/* Bytes of device workspace or_varlen_bwd needs: tile tables, two statistics per query row and head, and fp32 partial
+ * gradients where the call has so few tiles that a streamed axis is split. -1 for sizes it refuses. */
+int64_t or_varlen_bwd_workspace_size(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H,
+                                     int32_t D);
+
+/* The gradient of or_varlen_fwd (and so of attention.varlen, varlen_lse and overlapping_ranges, src/onereel/attention.py:
+ * 39-53,74-84, which the reference leaves to FlashAttention's own): with P = exp(scale q k^T - lse) and
+ * delta = rowsum(d_o * o) - dlse, dS = P * (d_o v^T - delta), dv = P^T d_o, dq = scale dS k, dk = scale dS^T q, each summed
+ * in fp32 over every segment that reads the row and rounded to bf16 once (P and dS are rounded to bf16 as operands). No
+ * atomics: a call's results have the same bits every time. Three launches (tile planner, dq, dk with dv), a fourth that adds
+ * partial gradients where an axis is split. */
+int or_varlen_bwd(const or_varlen_bwd_args* args, void* stream);
+
 /* Replaces the log-sum-exp merge of partial attention results: ring._merge (src/onereel/parallel/ring.py:63-70) and
  * the merge in Processor._far_lse (src/onereel/models/hunyuan15.py:270-275). o: fp32 [n_rows, H, D] (row stride
  * o_row_stride elements), lse: fp32 [H, n_rows], both updated in place with the partial result o_s: bf16

@@ -60,6 +60,14 @@ class VarlenArgs(ctypes.Structure):
                 ('k_tok_rows', i64), ('v_runs', vp)]
 
 
+class VarlenBwdArgs(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ('q', 'k', 'v', 'o', 'd_o', 'lse', 'dlse', 'dq', 'dk', 'dv', 'cu_q', 'cu_k', 'k_off',
+                                  'k_len')] + \
+               [(n, i64) for n in ('q_row_stride', 'k_row_stride', 'o_row_stride', 'do_row_stride', 'lse_stride')] + \
+               [(n, i32) for n in ('n_seg', 'n_q', 'n_k', 'max_q', 'max_k', 'H', 'D')] + \
+               [('scale', ctypes.c_float), ('workspace', vp), ('workspace_bytes', i64)]
+
+
 class PackArgs(ctypes.Structure):
     _fields_ = [('k_video', vp), ('k_text', vp), ('v_video', vp), ('v_text', vp), ('video_row_stride', i64),
                 ('text_row_stride', i64), ('n_video', i64), ('k_src', vp), ('k_rope', vp), ('k_move_from', vp),
@@ -80,6 +88,8 @@ SIGNATURES = {
     'or_varlen_workspace_size': (i64, [i32, i32, i32, i32]),
     'or_varlen_fwd': (i32, [ctypes.POINTER(VarlenArgs), vp]),
     'or_varlen_fwd_noalloc': (i32, [ctypes.POINTER(VarlenArgs), vp]),
+    'or_varlen_bwd_workspace_size': (i64, [i32] * 7),
+    'or_varlen_bwd': (i32, [ctypes.POINTER(VarlenBwdArgs), vp]),
     'or_lse_merge': (i32, [vp, vp, vp, vp, i64, i32, i32, i64, i64, vp]),
     'or_rmsnorm_rope': (i32, [vp, vp, vp, vp, i64, i64, i64, i32, i32, ctypes.c_float, vp, vp, vp, i64, vp, vp, i64,
                               i64, vp]),

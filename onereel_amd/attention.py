@@ -3,10 +3,16 @@
 Same names, shapes and semantics: packed q [Nq, H, D], k / v [Nk, H, D], bf16, non-causal, softmax scale D^-0.5;
 `cu_seqlens` int32 on the device. The reference's FlashAttention backends (`BACKEND` 'fa2' / 'fa3' / 'auto') map to
 the one HIP kernel; `backend()` reports 'hip'. Errors raise `onereel_amd._lib.HipPathError` (a RuntimeError).
+
+`dense`, `varlen`, `varlen_lse`, `packed`, `packed_lse`, `overlapping_ranges` and `overlapping_ranges_lse` are
+differentiable in q, k and v, as FlashAttention's are (once; the gradient itself has no graph): when autograd records and
+one of them requires a gradient, the call keeps its output and log-sum-exp for `or_varlen_bwd`. `varlen_backward` and
+`overlapping_ranges_backward` are the same gradients as plain calls, without autograd.
 """
 from __future__ import annotations
 
 import array
+import ctypes
 import functools
 import operator
 
@@ -39,12 +45,111 @@ def cu_seqlens(lengths, device='cuda') -> torch.Tensor:
     return torch.tensor(_offsets(lengths), dtype=torch.int32, device=device)
 
 
+def wants_grad(*xs) -> bool:
+    """whether autograd records a call on these tensors (None: no tensor)"""
+    return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in xs)
+
+
+def refuse_captured_leaves(what: str, *xs):
+    """A backward pass recorded into a graph adds into its leaves' gradients on the stream of the first pass that used
+    them; when that is another stream (an eager pass whose graph still lives), the capture ends the process. So a call
+    under capture takes no leaves that require gradients; the backward entry points without autograd can be captured."""
+    if any(x is not None and x.requires_grad and x.is_leaf for x in xs) and torch.cuda.is_current_stream_capturing():
+        raise _L.HipValueError(f'{what}: a leaf that requires a gradient cannot be differentiated under graph capture: '
+                               f'capture the call without autograd and its backward entry point')
+
+
+def _rows_for(x, H: int, D: int):
+    """x itself where its rows are as the kernels read them, else a copy (a gradient may come expanded or transposed)"""
+    if x.dim() != 3 or tuple(x.shape[1:]) != (H, D):
+        raise _L.HipValueError(f'expected [rows, {H}, {D}], got {tuple(x.shape)}')
+    fits = x.stride(2) == 1 and x.stride(1) == D and x.stride(0) >= H * D and x.stride(0) % 8 == 0
+    if x.shape[0] and not (fits and x.data_ptr() % 16 == 0):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, max(x.stride(0), H * D) if x.shape[0] else H * D
+
+
+def _backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse=None, k_off=None, k_len=None):
+    """or_varlen_bwd on torch tensors: (dq, dk, dv), bf16 and contiguous"""
+    _scene._check_bf16(do, q, k, v, o)
+    if k.dim() != 3 or q.dim() != 3:
+        raise _L.HipValueError('q, k and v must be [rows, heads, head_dim]')
+    (n_q, H, D), n_k = q.shape, k.shape[0]
+    if v.shape != k.shape or o.shape != q.shape or do.shape != q.shape or tuple(k.shape[1:]) != (H, D):
+        raise _L.HipValueError(f'q, o and do must have one shape and k and v one with the same [{H}, {D}] rows')
+    for x in (lse, dlse):
+        if x is not None and (x.dtype != torch.float32 or tuple(x.shape) != (H, n_q)):
+            raise _L.HipTypeError(f'lse and its gradient must be float32 [{H}, {n_q}]')
+    for x in (cu_q, cu_k, k_off, k_len):
+        if x is not None and (x.dtype != torch.int32 or not x.is_cuda or not x.is_contiguous()):
+            raise _L.HipTypeError('index arrays must be contiguous int32 GPU tensors')
+    dev = q.device
+    if any(x is not None and x.device != dev for x in (do, k, v, o, lse, dlse, cu_q, cu_k, k_off, k_len)):
+        raise _L.HipTypeError('all tensors of a call must be on one GPU')
+    (q, qs), (o, os_), (do, dos) = (_rows_for(x, H, D) for x in (q, o, do))
+    (k, ks), (v, vs) = (_rows_for(x, H, D) for x in (k, v))
+    if ks != vs:
+        (k, ks), v = (k.clone(memory_format=torch.contiguous_format), H * D), v.clone(memory_format=torch.contiguous_format)
+    lse = lse.contiguous()
+    dlse = None if dlse is None else dlse.contiguous()
+    dq = torch.empty(n_q, H, D, dtype=torch.bfloat16, device=dev)
+    dk, dv = (torch.empty(n_k, H, D, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    a = _L.VarlenBwdArgs()
+    a.q, a.k, a.v, a.o, a.d_o, a.lse, a.dlse = (_L.ptr(x) for x in (q, k, v, o, do, lse, dlse))
+    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    a.cu_q, a.cu_k, a.k_off, a.k_len = (_L.ptr(x) for x in (cu_q, cu_k, k_off, k_len))
+    a.q_row_stride, a.k_row_stride, a.o_row_stride, a.do_row_stride, a.lse_stride = qs, ks, os_, dos, n_q
+    a.n_seg, a.n_q, a.n_k, a.max_q, a.max_k, a.H, a.D = cu_q.numel() - 1, n_q, n_k, int(max_q), int(max_k), H, D
+    a.scale = float(D ** -0.5)
+    n = _L.lib().or_varlen_bwd_workspace_size(a.n_seg, n_q, n_k, a.max_q, a.max_k, H, D)
+    _L.check(min(int(n), 0), 'or_varlen_bwd_workspace_size')
+    ws = torch.empty(int(n), dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    with torch.cuda.device(dev):
+        _L.check(_L.lib().or_varlen_bwd(ctypes.byref(a), _L.stream_handle(dev)), 'or_varlen_bwd')
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    """or_varlen_fwd with its log-sum-exp, and or_varlen_bwd"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, k_off, k_len, max_q, max_k):
+        lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
+        o = _scene.varlen(q, k, v, cu_q, cu_k, max_q, max_k, k_off=k_off, k_len=k_len, lse=lse)
+        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k, k_off, k_len)
+        ctx.longest = max_q, max_k
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dlse):
+        q, k, v, o, lse, cu_q, cu_k, k_off, k_len = ctx.saved_tensors
+        grads = (None,) * 3
+        if do is not None or dlse is not None:
+            do = torch.zeros_like(o) if do is None else do
+            grads = _backward(do, q, k, v, o, lse, cu_q, cu_k, *ctx.longest, dlse, k_off, k_len)
+        return *grads, None, None, None, None, None, None
+
+
+def _attend(q, k, v, cu_q, cu_k, max_q, max_k, k_off=None, k_len=None, lse=False):
+    """the varlen call of every entry point: o, or (o, lse)"""
+    if wants_grad(q, k, v):
+        refuse_captured_leaves('attention', q, k, v)
+        o, l = _Attention.apply(q, k, v, cu_q, cu_k, k_off, k_len, max_q, max_k)
+        return (o, l) if lse else o
+    l = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if lse else None
+    o = _scene.varlen(q, k, v, cu_q, cu_k, max_q, max_k, k_off=k_off, k_len=k_len, lse=l)
+    return (o, l) if lse else o
+
+
 def dense(q, k, v):
     """q, k, v [B, S, H, D] -> [B, S, H, D] (attention.py:32-36)"""
     B, S, H, D = q.shape
     Sk = k.shape[1]
     cu_q, cu_k = _L.device_ints([_offsets([S] * B), _offsets([Sk] * B)], q.device)
-    o = _scene.varlen(q.reshape(B * S, H, D), k.reshape(B * Sk, H, D), v.reshape(B * Sk, H, D), cu_q, cu_k, S, Sk)
+    o = _attend(q.reshape(B * S, H, D), k.reshape(B * Sk, H, D), v.reshape(B * Sk, H, D), cu_q, cu_k, S, Sk)
     return o.view(B, S, H, D)
 
 
@@ -71,7 +176,7 @@ def varlen(q, k, v, cu_q, cu_k, max_q, max_k, check: bool = True):
         check_cu_seqlens(cu_k, min(k.shape[0], v.shape[0]), max_k, 'cu_k')
         if cu_q.numel() != cu_k.numel():
             raise _L.HipValueError('cu_q and cu_k must hold one offset per segment boundary each')
-    return _scene.varlen(q, k, v, cu_q, cu_k, max_q, max_k)
+    return _attend(q, k, v, cu_q, cu_k, max_q, max_k)
 
 
 def varlen_lse(q, k, v, cu_q, cu_k, max_q, max_k, check: bool = True):
@@ -81,9 +186,19 @@ def varlen_lse(q, k, v, cu_q, cu_k, max_q, max_k, check: bool = True):
         check_cu_seqlens(cu_k, min(k.shape[0], v.shape[0]), max_k, 'cu_k')
         if cu_q.numel() != cu_k.numel():
             raise _L.HipValueError('cu_q and cu_k must hold one offset per segment boundary each')
-    lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
-    o = _scene.varlen(q, k, v, cu_q, cu_k, max_q, max_k, lse=lse)
-    return o, lse
+    return _attend(q, k, v, cu_q, cu_k, max_q, max_k, lse=True)
+
+
+def varlen_backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse=None, check: bool = True):
+    """The gradient of varlen / varlen_lse: (dq, dk, dv) bf16 from do [Nq, H, D], the call's inputs, its output o and lse
+    [H, Nq] fp32, and dlse [H, Nq] fp32 when the lse was used too. Rows of q behind the last segment and rows of k / v
+    that no segment reads get zeros. Sums are fp32 in a fixed order: the same bits every time. check as in varlen."""
+    if check:
+        check_cu_seqlens(cu_q, q.shape[0], max_q, 'cu_q')
+        check_cu_seqlens(cu_k, min(k.shape[0], v.shape[0]), max_k, 'cu_k')
+    if cu_q.numel() != cu_k.numel():
+        raise _L.HipValueError('cu_q and cu_k must hold one offset per segment boundary each')
+    return _backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse)
 
 
 def _concat_table(xs):
@@ -112,7 +227,8 @@ def _concat(segments):
     if n > 112:
         nq, nk = [x.shape[0] for x in qs], [x.shape[0] for x in ks]
     long = n <= 112 or (sum(nq) + 2 * sum(nk)) * qs[0].shape[1:].numel() >= n << 19
-    table = _concat_table(qs + ks + vs) if long else None
+    # autograd records torch.cat
+    table = _concat_table(qs + ks + vs) if long and not wants_grad(*qs, *ks, *vs) else None
     if table is not None and table[1][n:2 * n] == table[1][2 * n:] and sum(table[1]) < 2 ** 31:
         at, rows, *row = table
         nq, nk = rows[:n], rows[n:2 * n]
@@ -145,10 +261,8 @@ def packed(segments):
     return varlen(*args, check=False).split(nq)    # offsets built here from the segments' lengths
 
 
-def overlapping_ranges(q, k, v, q_ranges, k_ranges):
-    """attention of q rows q_ranges[j] to k / v rows k_ranges[j] without copying k / v: the kernel reads the
-    overlapping contiguous key ranges in place (per-segment key offset and length, as FA3's cu_seqlens_k offsets
-    with seqused_k). q_ranges must tile q in order (attention.py:74-84)."""
+def _range_args(q, k, v, q_ranges, k_ranges):
+    """(cu_q, key starts, key counts, most queries, most keys) of overlapping_ranges, checked"""
     nq = [hi - lo for lo, hi in q_ranges]
     starts = [lo for lo, _ in q_ranges]
     if sum(nq) != q.shape[0] or any(lo != sum(nq[:j]) for j, lo in enumerate(starts)):
@@ -160,7 +274,28 @@ def overlapping_ranges(q, k, v, q_ranges, k_ranges):
         raise _L.HipValueError(f'k_ranges must lie inside the {n_k} rows of k and v')
     nk = [hi - lo for lo, hi in k_ranges]
     cu_q, k_start, k_count = _L.device_ints([_offsets(nq), [lo for lo, _ in k_ranges], nk], q.device)
-    return _scene.varlen(q, k, v, cu_q, None, max(nq), max(nk), k_off=k_start, k_len=k_count)
+    return cu_q, k_start, k_count, max(nq), max(nk)
+
+
+def overlapping_ranges(q, k, v, q_ranges, k_ranges):
+    """attention of q rows q_ranges[j] to k / v rows k_ranges[j] without copying k / v: the kernel reads the
+    overlapping contiguous key ranges in place (per-segment key offset and length, as FA3's cu_seqlens_k offsets
+    with seqused_k). q_ranges must tile q in order (attention.py:74-84)."""
+    cu_q, k_start, k_count, max_q, max_k = _range_args(q, k, v, q_ranges, k_ranges)
+    return _attend(q, k, v, cu_q, None, max_q, max_k, k_start, k_count)
+
+
+def overlapping_ranges_lse(q, k, v, q_ranges, k_ranges):
+    """overlapping_ranges with the softmax log-sum-exp: (out, lse [H, Nq] fp32), what its backward call needs"""
+    cu_q, k_start, k_count, max_q, max_k = _range_args(q, k, v, q_ranges, k_ranges)
+    return _attend(q, k, v, cu_q, None, max_q, max_k, k_start, k_count, lse=True)
+
+
+def overlapping_ranges_backward(do, q, k, v, o, lse, q_ranges, k_ranges, dlse=None):
+    """the gradient of overlapping_ranges / overlapping_ranges_lse, as varlen_backward: a row of k and v sums the
+    gradients of every range that reads it"""
+    cu_q, k_start, k_count, max_q, max_k = _range_args(q, k, v, q_ranges, k_ranges)
+    return _backward(do, q, k, v, o, lse, cu_q, None, max_q, max_k, dlse, k_start, k_count)
 
 
 def merge_lse(o, lse, o_s, lse_s):

@@ -1,0 +1,833 @@
+// Gradient of the packed varlen attention (attention.hip) for gfx950: dq, dk, dv of softmax(q k^T * scale) v per segment,
+// bf16 in and out, fp32 accumulation, nothing kept from the forward pass but its output and its log-sum-exp.
+//
+//   P = exp(scale q k^T - lse)      delta = rowsum(do * o) - dlse      dS = P * (do v^T - delta)
+//   dv = P^T do                     dq = scale dS k                    dk = scale dS^T q
+//
+// Two passes, each recomputing P: one over query tiles for dq (3 products), one over key tiles for dk and dv (4). One pass
+// of 5 products would have to add dq into memory from every key tile, with atomics whose order changes the bits; the
+// two passes sum every gradient in registers in a fixed order, so a call gives the same bits every time.
+//
+// - A wavefront owns 32 T rows (T = 1 or 2 blocks of 32 queries, or keys) of its work-group's tile and keeps their
+//   operands and their fp32 gradient in registers; the rows of the other side stream past in blocks of 32 through a ring of
+//   LDS slots filled by LDS DMA, three blocks ahead.
+// - Both products of scores put the streamed rows on the MFMA rows and the owned rows on its columns, so a lane holds
+//   scores of one owned row, and the bf16 P and dS of a lane are the B operand of the next products as they lie.
+//   Their A operand is the streamed block transposed, read from the same slot by transposing LDS reads. The slot's
+//   swizzle serves both kinds of read without bank conflicts.
+// - P and dS are rounded to bf16 once, as the operands of the bf16 matrix cores (the forward pass rounds its P the same way);
+//   scores, P, dS, delta and all sums are fp32.
+// - Key rows may belong to several segments (overlapping ranges): the key axis is cut at every range boundary, so that all
+//   rows of a key tile have the same segments, and the tile streams the queries of all of them. Rows past an end load as
+//   zeros: a zero query row adds nothing to dk and dv, and the scores of key rows past the end are set to P = 0.
+// - Few tiles (few queries against long keys, or few keys against long queries): the streamed axis is split, the parts
+//   write fp32 partial gradients, and a last launch adds them in order.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.h"
+
+namespace onereel {
+
+namespace {
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+
+constexpr int kThreads = 256;        // 4 wavefronts
+constexpr int kBlk = 32;             // streamed rows per block
+constexpr int kRing = 4;             // LDS slots of the ring
+constexpr int kPlanThreads = 1024;
+constexpr int kMaxSeg = 4096;
+constexpr int kMaxSplit = 32;
+constexpr int kHeader = 8;           // int32 words ahead of the tile tables: query tile count, key tile count
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct BwdArgs {
+  const uint16_t *q, *k, *v, *o, *d_o;
+  const float *lse, *dlse;
+  uint16_t *dq, *dk, *dv;
+  const int32_t *cu_q, *cu_k, *k_off, *k_len;
+  int64_t qs, ks, os, dos;           // row strides (elements) of q, of k and v, of o, of do
+  int64_t lse_stride;                // elements between the heads of lse and dlse
+  int32_t n_seg, n_q, n_k, H;
+  float scale;
+  int32_t split_q, split_k;          // parts of the streamed axis in the dq pass and in the dk / dv pass
+  int32_t max_q_tiles, max_k_tiles;
+  // workspace
+  int32_t* head;
+  i32x4* q_tiles;                    // first query, rows, first key, keys
+  i32x4* k_tiles;                    // first key, rows, first and last segment that may read them
+  float* stat;                       // [2][H][n_q]: -lse / scale, then -delta
+  float* part_q;                     // [split_q][n_q][H][D]
+  float* part_k;                     // [split_k][2][n_k][H][D]: dk, then dv
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
+// a value that is the same in every lane, in a scalar register
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ i32x4 uni(i32x4 x) { return i32x4{uni(x[0]), uni(x[1]), uni(x[2]), uni(x[3])}; }
+
+// a segment's queries and keys, kept inside the tensors whatever the offsets say
+__device__ __forceinline__ void seg_q(const BwdArgs& a, int s, int& lo, int& n) {
+  lo = clampi(a.cu_q[s], 0, a.n_q);
+  n = max(clampi(a.cu_q[s + 1], 0, a.n_q) - lo, 0);
+}
+__device__ __forceinline__ void seg_k(const BwdArgs& a, int s, int& lo, int& n) {
+  const int64_t beg = a.k_off ? a.k_off[s] : a.cu_k[s];
+  const int64_t len = a.k_len ? a.k_len[s] : a.cu_k[s + 1] - beg;
+  lo = (int)min(max(beg, (int64_t)0), (int64_t)a.n_k);
+  n = (int)max(min(beg + len, (int64_t)a.n_k) - lo, (int64_t)0);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// planner: one block. Query tiles: every segment's queries in pieces of tq rows, then the rows behind the last segment
+// (no keys: their gradient is zero). Key tiles: the key axis cut at the segments' key range boundaries, every interval in
+// pieces of tk rows, with the first and last segment that cover it.
+__device__ int block_scan(int v, int* wsum) {   // exclusive sum over the block's threads; wsum[16] is the total
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int x = v;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) wsum[w] = x;
+  __syncthreads();
+  int base = 0, all = 0;
+  for (int i = 0; i < kPlanThreads / 64; ++i) {
+    if (i < w) base += wsum[i];
+    all += wsum[i];
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) wsum[16] = all;
+  __syncthreads();
+  return base + x - v;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void bwd_plan_kernel(BwdArgs a, int tq, int tk) {
+  __shared__ int bnd[2 * kMaxSeg];
+  __shared__ int lo_seg[2 * kMaxSeg + 1];
+  __shared__ int hi_seg[2 * kMaxSeg + 1];
+  __shared__ int wsum[17];
+  const int t = threadIdx.x, n = a.n_seg;
+  // query tiles
+  int at = 0;
+  for (int s0 = 0; s0 <= n; s0 += kPlanThreads) {
+    const int s = s0 + t;
+    int lo = 0, len = 0, k0 = 0, nk = 0;
+    if (s < n) {
+      seg_q(a, s, lo, len);
+      seg_k(a, s, k0, nk);
+    } else if (s == n) {
+      lo = clampi(a.cu_q[n], 0, a.n_q);
+      len = a.n_q - lo;
+    }
+    const int tiles = (len + tq - 1) / tq;
+    const int first = at + block_scan(tiles, wsum);
+    for (int i = 0; i < tiles && first + i < a.max_q_tiles; ++i)
+      a.q_tiles[first + i] = i32x4{lo + i * tq, min(tq, len - i * tq), k0, nk};
+    at += wsum[16];
+    __syncthreads();
+  }
+  if (t == 0) a.head[0] = min(at, a.max_q_tiles);
+  // boundaries of the key ranges, sorted (a power of two of them, the rest past the end)
+  int m = 2;
+  while (m < 2 * n) m <<= 1;
+  for (int i = t; i < m; i += kPlanThreads) {
+    int b = a.n_k;
+    if (i < 2 * n) {
+      int lo, len;
+      seg_k(a, i >> 1, lo, len);
+      b = i & 1 ? lo + len : lo;
+    }
+    bnd[i] = b;
+  }
+  for (int i = t; i <= m; i += kPlanThreads) {
+    lo_seg[i] = 0x7fffffff;
+    hi_seg[i] = -1;
+  }
+  __syncthreads();
+  for (int size = 2; size <= m; size <<= 1)
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      for (int i = t; i < m / 2; i += kPlanThreads) {
+        const int x = 2 * d * (i / d) + i % d, y = x + d;
+        const bool up = (x & size) == 0;
+        const int p = bnd[x], r = bnd[y];
+        if ((p > r) == up) {
+          bnd[x] = r;
+          bnd[y] = p;
+        }
+      }
+      __syncthreads();
+    }
+  // interval i is [bnd[i - 1], bnd[i]): from 0 at i = 0, to n_k at i = m
+  for (int s = t; s < n; s += kPlanThreads) {
+    int lo, len;
+    seg_k(a, s, lo, len);
+    if (len == 0) continue;
+    int x = 0, y = m;   // the first boundary at lo
+    while (x < y) {
+      const int mid = (x + y) >> 1;
+      if (bnd[mid] < lo) x = mid + 1; else y = mid;
+    }
+    for (int i = x + 1; i < m && bnd[i] <= lo + len; ++i) {
+      if (bnd[i] == bnd[i - 1]) continue;
+      atomicMin(&lo_seg[i], s);
+      atomicMax(&hi_seg[i], s);
+    }
+  }
+  __syncthreads();
+  at = 0;
+  for (int i0 = 0; i0 <= m; i0 += kPlanThreads) {
+    const int i = i0 + t;
+    int lo = 0, len = 0;
+    if (i <= m) {
+      lo = i > 0 ? bnd[i - 1] : 0;
+      len = (i < m ? bnd[i] : a.n_k) - lo;
+    }
+    const int tiles = (len + tk - 1) / tk;
+    const int first = at + block_scan(tiles, wsum);
+    for (int j = 0; j < tiles && first + j < a.max_k_tiles; ++j)
+      a.k_tiles[first + j] = i32x4{lo + j * tk, min(tk, len - j * tk), lo_seg[i], hi_seg[i]};
+    at += wsum[16];
+    __syncthreads();
+  }
+  if (t == 0) a.head[1] = min(at, a.max_k_tiles);
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// streamed blocks: 32 rows of D bf16 in an LDS slot, row r's 16-byte chunk c at position c ^ swz(r). A b128 read of one
+// chunk of 16 consecutive rows, and a transposing b64 read (4 rows x 32 columns per half wavefront), both touch every
+// bank once: the low row bits move whole 64-byte pieces, the next ones chunks inside them.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const lds_void*)p; }
+
+template <int D>
+struct Str {
+  static constexpr int CH = D / 8;                 // 16-byte chunks per row
+  static constexpr int KS = D / 16;                // MFMA steps over the head dims
+  static constexpr int DB = D / 32;                // blocks of 32 head dims
+  static constexpr int SLOT = kBlk * D * 2;        // bytes of one block
+  static constexpr int LPB = kBlk * CH / kThreads; // DMA loads per lane and block
+};
+
+// one block of `rows` valid rows at `base` into LDS: the descriptor ends at the last valid row, the rows past it read zeros.
+// Inline asm, so that the compiler adds no waits for these LDS writes to unrelated reads: the loop waits itself. One
+// wait state is needed between the write of M0 and the LDS DMA that reads it (the s_nop).
+template <int D>
+__device__ __forceinline__ void dma_rows(const uint16_t* base, int64_t rs, int rows, const uint32_t* voff, uint32_t m0) {
+  const uint64_t b = (uint64_t)base;
+  const int32_t nrec = rows > 0 ? (int32_t)((rows - 1) * rs * 2 + D * 2) : 0;
+  const i32x4 r = {__builtin_amdgcn_readfirstlane((int32_t)(uint32_t)b),
+                   __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)(b >> 32)), __builtin_amdgcn_readfirstlane(nrec),
+                   0x00020000};
+#pragma unroll
+  for (int i = 0; i < Str<D>::LPB; ++i)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff[i]), "s"(r),
+                 "s"(__builtin_amdgcn_readfirstlane(m0 + i * kThreads * 16))
+                 : "memory");
+}
+
+// 64 statistics (32 rows of two arrays n elements apart) into LDS, zeros past `rows`
+__device__ __forceinline__ void dma_stats(const float* base, int64_t apart, int rows, int lane, uint32_t m0) {
+  const uint64_t b = (uint64_t)base;
+  const i32x4 r = {__builtin_amdgcn_readfirstlane((int32_t)(uint32_t)b),
+                   __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)(b >> 32)), (int32_t)0x7fffffff, 0x00020000};
+  const uint32_t off = (lane & 31) < rows ? (uint32_t)((lane & 31) * 4 + (lane >> 5) * apart * 4) : 0x80000000u;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(off), "s"(r),
+               "s"(__builtin_amdgcn_readfirstlane(m0))
+               : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// read addresses of a lane inside a slot
+template <int D>
+struct Lds {
+  uint32_t row[Str<D>::KS];        // 8 dims 16 ks + 8 (lane / 32) .. of row lane % 32
+  uint32_t tr[Str<D>::DB][2];      // transposing: dims 32 db + .., rows 4 (lane / 32) + 8 t + (0 .. 3)
+  __device__ __forceinline__ void init(int lane) {
+    const int l32 = lane & 31, h = lane >> 5, r = lane & 15, g = (lane >> 4) & 1;
+#pragma unroll
+    for (int ks = 0; ks < Str<D>::KS; ++ks) row[ks] = l32 * D * 2 + ((2 * ks + h) ^ swz<D>(l32)) * 16;
+#pragma unroll
+    for (int db = 0; db < Str<D>::DB; ++db)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int rr = 4 * h + 8 * t + (r >> 2);
+        tr[db][t] = rr * D * 2 + ((4 * db + 2 * g + ((r >> 1) & 1)) ^ swz<D>(rr)) * 16 + (r & 1) * 8;
+      }
+  }
+};
+
+template <int D>
+__device__ __forceinline__ bf16x8 row_frag(uint32_t slot, const Lds<D>& ad, int ks) {
+  return *(const __attribute__((address_space(3))) bf16x8*)(uintptr_t)(slot + ad.row[ks]);
+}
+
+// dims 32 db + lane % 32 of the 8 rows that a lane's scores of step hs belong to: 16 hs + 4 (lane / 32) + {0..3, 8..11}
+template <int D>
+__device__ __forceinline__ bf16x8 tr_frag(uint32_t slot, const Lds<D>& ad, int db, int hs) {
+  u32x2 x[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    x[t] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                                         (lds_bf16x4*)(uintptr_t)(slot + ad.tr[db][t] + 16 * hs * D * 2)));
+  const u32x4 y = {x[0][0], x[0][1], x[1][0], x[1][1]};
+  return __builtin_bit_cast(bf16x8, y);
+}
+
+__device__ __forceinline__ bf16x8 pack8(const f32x16& x, int half) {
+  u32x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = pack2(x[8 * half + 2 * i], x[8 * half + 2 * i + 1]);
+  return __builtin_bit_cast(bf16x8, y);
+}
+
+// operand of 32 owned rows: 8 dims 16 ks + 8 (lane / 32) of row lane % 32, zeros past `rows`
+template <int D>
+__device__ __forceinline__ void load_owned(bf16x8 (&f)[Str<D>::KS], const uint16_t* p, int64_t rs, int rows, int lane) {
+  const int l32 = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int ks = 0; ks < Str<D>::KS; ++ks) {
+    u32x4 x = {0, 0, 0, 0};
+    if (l32 < rows) x = *(const u32x4*)(p + l32 * rs + 16 * ks + 8 * h);
+    f[ks] = __builtin_bit_cast(bf16x8, x);
+  }
+}
+
+// gradient of 32 owned rows (dims on the accumulators' rows, owned row lane % 32 on the column)
+template <int D>
+__device__ __forceinline__ void store_bf16(uint16_t* p, int64_t rs, const f32x16 (&acc)[Str<D>::DB], float f, int rows,
+                                           int lane) {
+  const int l32 = lane & 31, h = lane >> 5;
+  if (l32 >= rows) return;
+#pragma unroll
+  for (int db = 0; db < Str<D>::DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const u32x2 y = {pack2(acc[db][4 * g] * f, acc[db][4 * g + 1] * f),
+                       pack2(acc[db][4 * g + 2] * f, acc[db][4 * g + 3] * f)};
+      *(u32x2*)(p + l32 * rs + 32 * db + 8 * g + 4 * h) = y;
+    }
+}
+template <int D>
+__device__ __forceinline__ void store_f32(float* p, int64_t rs, const f32x16 (&acc)[Str<D>::DB], float f, int rows,
+                                          int lane) {
+  const int l32 = lane & 31, h = lane >> 5;
+  if (l32 >= rows) return;
+#pragma unroll
+  for (int db = 0; db < Str<D>::DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *(f32x4*)(p + l32 * rs + 32 * db + 8 * g + 4 * h) =
+          f32x4{acc[db][4 * g] * f, acc[db][4 * g + 1] * f, acc[db][4 * g + 2] * f, acc[db][4 * g + 3] * f};
+}
+
+// this block's item of n: the blocks of one XCD (block index modulo 8) take consecutive items, which share their head's
+// streamed rows in that XCD's L2
+__device__ __forceinline__ int64_t xcd_item(int64_t n) {
+  const int64_t per = (n + 7) / 8, j = blockIdx.x >> 3, i = (blockIdx.x & 7) * per + j;
+  return j < per && i < n ? i : -1;
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// dq: a block owns 128 T queries of one head and streams the keys and values of their segment
+template <int D, int T>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void bwd_q_kernel(BwdArgs a) {
+  using C = Str<D>;
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT];
+  const int n_tiles = uni(a.head[0]);
+  const int64_t item = xcd_item((int64_t)n_tiles * a.H * a.split_q);
+  if (item < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = (int)(item % a.split_q);
+  const int head = (int)(item / a.split_q / n_tiles);
+  const i32x4 tile = uni(a.q_tiles[item / a.split_q % n_tiles]);
+  const int row0 = tile[0] + w * 32 * T, n_keys = tile[3];
+  const int rows = clampi(tile[1] - w * 32 * T, 0, 32 * T);
+
+  uint32_t voff[C::LPB];
+#pragma unroll
+  for (int i = 0; i < C::LPB; ++i) {
+    const int x = i * kThreads + tid, r = x / C::CH, c = x % C::CH;
+    voff[i] = (uint32_t)(r * a.ks * 2 + (c ^ swz<D>(r)) * 16);
+  }
+  const uint32_t lds = lds_addr(ring), m0 = lds + w * 1024;
+  const int blocks = (n_keys + kBlk - 1) / kBlk;
+  const int b0 = (int)((int64_t)blocks * part / a.split_q), b1 = (int)((int64_t)blocks * (part + 1) / a.split_q);
+  const uint16_t* kp = a.k + (int64_t)tile[2] * a.ks + (int64_t)head * D;
+  const uint16_t* vp = a.v + (int64_t)tile[2] * a.ks + (int64_t)head * D;
+  auto fetch = [&](int b) {
+    const int n = b < b1 ? min(n_keys - b * kBlk, kBlk) : 0;
+    const int64_t off = (int64_t)(b < b1 ? b : b0) * kBlk * a.ks;
+    const uint32_t at = m0 + (b & (kRing - 1)) * C::SLOT;
+    dma_rows<D>(kp + off, a.ks, n, voff, at);
+    dma_rows<D>(vp + off, a.ks, n, voff, at + kRing * C::SLOT);
+  };
+
+  // the owned queries, their output gradients and their statistics
+  bf16x8 qf[T][C::KS], df[T][C::KS];
+  float neg_lse[T], neg_delta[T];
+  f32x16 acc[T][C::DB];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int n = clampi(rows - 32 * t, 0, 32);
+    const int64_t r = row0 + 32 * t;
+    bf16x8 of[C::KS];
+    load_owned<D>(qf[t], a.q + r * a.qs + (int64_t)head * D, a.qs, n, lane);
+    load_owned<D>(df[t], a.d_o + r * a.dos + (int64_t)head * D, a.dos, n, lane);
+    load_owned<D>(of, a.o + r * a.os + (int64_t)head * D, a.os, n, lane);
+    float d = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) {
+      const u32x4 x = __builtin_bit_cast(u32x4, of[ks]), y = __builtin_bit_cast(u32x4, df[t][ks]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        d = fmaf(bf2f((uint16_t)(x[i] & 0xffffu)), bf2f((uint16_t)(y[i] & 0xffffu)), d);
+        d = fmaf(bf2f((uint16_t)(x[i] >> 16)), bf2f((uint16_t)(y[i] >> 16)), d);
+      }
+    }
+    d += __shfl_xor(d, 32);
+    const bool mine = (lane & 31) < n;
+    const int64_t at = r + (lane & 31);
+    const float l = mine ? a.lse[head * a.lse_stride + at] : 0.0f;
+    if (mine && a.dlse) d -= a.dlse[head * a.lse_stride + at];
+    neg_lse[t] = -l * kLog2e;
+    neg_delta[t] = -d;
+    if (mine && lane < 32 && part == 0) {
+      a.stat[(int64_t)head * a.n_q + at] = -l / a.scale;
+      a.stat[(int64_t)(a.H + head) * a.n_q + at] = -d;
+    }
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[t][db][e] = 0.0f;
+  }
+
+  Lds<D> ad;
+  ad.init(lane);
+  const float c = a.scale * kLog2e;
+  const f32x16 zero = {};
+#pragma unroll 1
+  for (int b = b0; b < b0 + kRing - 1; ++b) fetch(b);
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) {
+    wait_loads_barrier<(kRing - 2) * 2 * C::LPB>();
+    fetch(b + kRing - 1);
+    const uint32_t ks_ = lds + (b & (kRing - 1)) * C::SLOT, vs_ = ks_ + kRing * C::SLOT;
+    f32x16 s[T], dp[T];
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) {
+      const bf16x8 kf = row_frag<D>(ks_, ad, ks);
+#pragma unroll
+      for (int t = 0; t < T; ++t) s[t] = mfma(kf, qf[t][ks], ks ? s[t] : zero);
+    }
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) {
+      const bf16x8 vf = row_frag<D>(vs_, ad, ks);
+#pragma unroll
+      for (int t = 0; t < T; ++t) dp[t] = mfma(vf, df[t][ks], ks ? dp[t] : zero);
+    }
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, neg_lse[t]));
+    if (n_keys - b * kBlk < kBlk) {   // the key rows past the end
+      const int n = n_keys - b * kBlk - 4 * (lane >> 5);
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] = 8 * (e >> 2) + (e & 3) < n ? s[t][e] : 0.0f;
+    }
+    bf16x8 ds[T][2];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[t][e] = s[t][e] * (dp[t][e] + neg_delta[t]);
+#pragma unroll
+      for (int hs = 0; hs < 2; ++hs) ds[t][hs] = pack8(dp[t], hs);
+    }
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+      for (int hs = 0; hs < 2; ++hs) {
+        const bf16x8 kt = tr_frag<D>(ks_, ad, db, hs);
+#pragma unroll
+        for (int t = 0; t < T; ++t) acc[t][db] = mfma(kt, ds[t][hs], acc[t][db]);
+      }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no DMA into LDS of a block that has ended
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int n = clampi(rows - 32 * t, 0, 32);
+    const int64_t at = ((int64_t)(row0 + 32 * t) * a.H + head) * D, rs = (int64_t)a.H * D;
+    if (a.split_q == 1) store_bf16<D>(a.dq + at, rs, acc[t], a.scale, n, lane);
+    else store_f32<D>(a.part_q + (int64_t)part * a.n_q * rs + at, rs, acc[t], a.scale, n, lane);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// dk, dv: a block owns 128 T keys of one head and streams the queries of every segment that reads them
+
+// walks the blocks of 32 queries of the segments that cover a key tile
+struct Walk {
+  int seg, last, row, left;          // the segment, the last one to look at, the next query row and the rows after it
+  __device__ __forceinline__ bool next_segment(const BwdArgs& a, int k0) {
+    for (; seg <= last; ++seg) {
+      int lo, n;
+      seg_k(a, seg, lo, n);
+      if (uni(lo) > k0 || uni(lo + n) <= k0) continue;
+      seg_q(a, seg, row, left);
+      row = uni(row);
+      left = uni(left);
+      if (left > 0) {
+        ++seg;
+        return true;
+      }
+    }
+    left = 0;
+    return false;
+  }
+};
+
+template <int D, int T>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void bwd_kv_kernel(BwdArgs a) {
+  using C = Str<D>;
+  constexpr int kStat = 256;         // bytes of one wavefront's statistics of a block
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT + kRing * 4 * kStat];
+  const int n_tiles = uni(a.head[1]);
+  const int64_t item = xcd_item((int64_t)n_tiles * a.H * a.split_k);
+  if (item < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = (int)(item % a.split_k);
+  const int head = (int)(item / a.split_k / n_tiles);
+  const i32x4 tile = uni(a.k_tiles[item / a.split_k % n_tiles]);
+  const int row0 = tile[0] + w * 32 * T;
+  const int rows = clampi(tile[1] - w * 32 * T, 0, 32 * T);
+
+  uint32_t voq[C::LPB], vod[C::LPB];
+#pragma unroll
+  for (int i = 0; i < C::LPB; ++i) {
+    const int x = i * kThreads + tid, r = x / C::CH, c = x % C::CH;
+    voq[i] = (uint32_t)(r * a.qs * 2 + (c ^ swz<D>(r)) * 16);
+    vod[i] = (uint32_t)(r * a.dos * 2 + (c ^ swz<D>(r)) * 16);
+  }
+  const uint32_t lds = lds_addr(ring), m0 = lds + w * 1024, st0 = lds + 2 * kRing * C::SLOT + w * kStat;
+
+  // this part's blocks of the segments' blocks in order
+  Walk wk{tile[2], tile[3], 0, 0};
+  int total = 0;
+  while (wk.next_segment(a, tile[0])) total += (wk.left + kBlk - 1) / kBlk;
+  const int b0 = (int)((int64_t)total * part / a.split_k), b1 = (int)((int64_t)total * (part + 1) / a.split_k);
+  wk = Walk{tile[2], tile[3], 0, 0};
+  for (int skip = b0; wk.next_segment(a, tile[0]);) {
+    const int n = (wk.left + kBlk - 1) / kBlk;
+    if (skip < n) {
+      wk.row += skip * kBlk;
+      wk.left -= skip * kBlk;
+      break;
+    }
+    skip -= n;
+  }
+  auto fetch = [&](int b) {
+    if (b < b1 && wk.left <= 0) wk.next_segment(a, tile[0]);
+    const int n = b < b1 ? min(wk.left, kBlk) : 0, slot = b & (kRing - 1);
+    const int64_t r = b < b1 ? wk.row : 0;
+    const uint32_t at = m0 + slot * C::SLOT;
+    dma_rows<D>(a.q + r * a.qs + (int64_t)head * D, a.qs, n, voq, at);
+    dma_rows<D>(a.d_o + r * a.dos + (int64_t)head * D, a.dos, n, vod, at + kRing * C::SLOT);
+    dma_stats(a.stat + (int64_t)head * a.n_q + r, (int64_t)a.H * a.n_q, n, lane, st0 + slot * 4 * kStat);
+    wk.row += kBlk;
+    wk.left -= kBlk;
+  };
+
+  bf16x8 kf[T][C::KS], vf[T][C::KS];
+  f32x16 dk[T][C::DB], dv[T][C::DB];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int n = clampi(rows - 32 * t, 0, 32);
+    const int64_t at = (int64_t)(row0 + 32 * t) * a.ks + (int64_t)head * D;
+    load_owned<D>(kf[t], a.k + at, a.ks, n, lane);
+    load_owned<D>(vf[t], a.v + at, a.ks, n, lane);
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dk[t][db][e] = dv[t][db][e] = 0.0f;
+  }
+
+  Lds<D> ad;
+  ad.init(lane);
+  const float c = a.scale * kLog2e;
+#pragma unroll 1
+  for (int b = b0; b < b0 + kRing - 1; ++b) fetch(b);
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) {
+    wait_loads_barrier<(kRing - 2) * (2 * C::LPB + 1)>();
+    fetch(b + kRing - 1);
+    const int slot = b & (kRing - 1);
+    const uint32_t qs_ = lds + slot * C::SLOT, ds_ = qs_ + kRing * C::SLOT, st = st0 + slot * 4 * kStat;
+    // -lse / scale and -delta start the sums of the scores and of do v^T: rows 8 g + 4 (lane / 32) ..
+    f32x16 s0, d0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 x = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)(st + 32 * g + 16 * (lane >> 5));
+      const f32x4 y = *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)(st + 128 + 32 * g + 16 * (lane >> 5));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s0[4 * g + i] = x[i];
+        d0[4 * g + i] = y[i];
+      }
+    }
+    f32x16 s[T], dp[T];
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) {
+      const bf16x8 qf = row_frag<D>(qs_, ad, ks);
+#pragma unroll
+      for (int t = 0; t < T; ++t) s[t] = mfma(qf, kf[t][ks], ks ? s[t] : s0);
+    }
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) {
+      const bf16x8 df = row_frag<D>(ds_, ad, ks);
+#pragma unroll
+      for (int t = 0; t < T; ++t) dp[t] = mfma(df, vf[t][ks], ks ? dp[t] : d0);
+    }
+    bf16x8 p[T][2], ds[T][2];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t][e] = __builtin_amdgcn_exp2f(s[t][e] * c);
+#pragma unroll
+      for (int hs = 0; hs < 2; ++hs) p[t][hs] = pack8(s[t], hs);
+    }
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+      for (int hs = 0; hs < 2; ++hs) {
+        const bf16x8 dt = tr_frag<D>(ds_, ad, db, hs);
+#pragma unroll
+        for (int t = 0; t < T; ++t) dv[t][db] = mfma(dt, p[t][hs], dv[t][db]);
+      }
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[t][e] *= s[t][e];
+#pragma unroll
+      for (int hs = 0; hs < 2; ++hs) ds[t][hs] = pack8(dp[t], hs);
+    }
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+      for (int hs = 0; hs < 2; ++hs) {
+        const bf16x8 qt = tr_frag<D>(qs_, ad, db, hs);
+#pragma unroll
+        for (int t = 0; t < T; ++t) dk[t][db] = mfma(qt, ds[t][hs], dk[t][db]);
+      }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no DMA into LDS of a block that has ended
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int n = clampi(rows - 32 * t, 0, 32);
+    const int64_t at = ((int64_t)(row0 + 32 * t) * a.H + head) * D, rs = (int64_t)a.H * D, all = a.n_k * rs;
+    if (a.split_k == 1) {
+      store_bf16<D>(a.dk + at, rs, dk[t], a.scale, n, lane);
+      store_bf16<D>(a.dv + at, rs, dv[t], 1.0f, n, lane);
+    } else {
+      store_f32<D>(a.part_k + 2 * part * all + at, rs, dk[t], a.scale, n, lane);
+      store_f32<D>(a.part_k + (2 * part + 1) * all + at, rs, dv[t], 1.0f, n, lane);
+    }
+  }
+}
+
+// the partial gradients of split passes, added in the order of the parts: 8 elements a thread of dq, then dk, then dv
+__global__ __launch_bounds__(kThreads) void bwd_add_kernel(BwdArgs a, int64_t q8, int64_t k8) {
+  const int64_t step = (int64_t)gridDim.x * kThreads, n = q8 + 2 * k8;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) {
+    const bool is_q = i < q8;
+    const int64_t which = is_q ? 0 : (i - q8) / k8, e = is_q ? i : (i - q8) % k8;
+    const float* p = is_q ? a.part_q : a.part_k + which * k8 * 8;
+    const int64_t apart = is_q ? q8 * 8 : 2 * k8 * 8;
+    const int parts = is_q ? a.split_q : a.split_k;
+    f32x4 x = {}, y = {};
+    for (int j = 0; j < parts; ++j) {
+      x += *(const f32x4*)(p + j * apart + e * 8);
+      y += *(const f32x4*)(p + j * apart + e * 8 + 4);
+    }
+    const u32x4 r = {pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3])};
+    *(u32x4*)((is_q ? a.dq : which ? a.dv : a.dk) + e * 8) = r;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// tiles and splits of a call, from its sizes alone (the offsets are on the device)
+struct Shape {
+  int tq, tk;                        // rows of a query tile and of a key tile
+  int64_t max_q_tiles, max_k_tiles;
+  int split_q, split_k;
+};
+
+// parts of a streamed axis: enough for two rounds of blocks on 256 CUs, none shorter than four blocks of rows
+int split_of(int64_t items, int64_t streamed) {
+  const int64_t want = (512 + items - 1) / std::max<int64_t>(items, 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, streamed / (4 * kBlk), kMaxSplit}));
+}
+
+Shape shape_of(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H) {
+  Shape s;
+  s.tq = max_q <= 128 ? 128 : 256;
+  s.tk = max_k <= 128 ? 128 : 256;
+  s.max_q_tiles = n_q / s.tq + n_seg + 1;
+  s.max_k_tiles = n_k / s.tk + 2 * (int64_t)n_seg + 1;
+  s.split_q = split_of((int64_t)H * ((n_q + s.tq - 1) / s.tq), max_k);
+  s.split_k = split_of((int64_t)H * ((n_k + s.tk - 1) / s.tk), max_q);
+  return s;
+}
+
+struct Layout {
+  int64_t q_tiles, k_tiles, stat, part_q, part_k, bytes;
+};
+Layout layout_of(const Shape& s, int32_t n_q, int32_t n_k, int32_t H, int32_t D) {
+  Layout l;
+  int64_t at = kHeader * 4;
+  auto take = [&](int64_t n) {
+    const int64_t was = (at + 255) & ~(int64_t)255;
+    at = was + n;
+    return was;
+  };
+  l.q_tiles = take(s.max_q_tiles * 16);
+  l.k_tiles = take(s.max_k_tiles * 16);
+  l.stat = take((int64_t)2 * H * n_q * 4);
+  l.part_q = take(s.split_q > 1 ? (int64_t)s.split_q * n_q * H * D * 4 : 0);
+  l.part_k = take(s.split_k > 1 ? (int64_t)s.split_k * 2 * n_k * H * D * 4 : 0);
+  l.bytes = (at + 255) & ~(int64_t)255;
+  return l;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+template <int D>
+void launch(const BwdArgs& a, const Shape& s, hipStream_t st) {
+  auto grid = [](int64_t items) { return dim3((unsigned)((items + 7) / 8 * 8)); };
+  const dim3 gq = grid(s.max_q_tiles * a.H * s.split_q), gk = grid(s.max_k_tiles * a.H * s.split_k);
+  if (a.n_q > 0) {
+    if (s.tq == 128) hipLaunchKernelGGL((bwd_q_kernel<D, 1>), gq, dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((bwd_q_kernel<D, 2>), gq, dim3(kThreads), 0, st, a);
+  }
+  if (a.n_k > 0) {
+    if (s.tk == 128) hipLaunchKernelGGL((bwd_kv_kernel<D, 1>), gk, dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((bwd_kv_kernel<D, 2>), gk, dim3(kThreads), 0, st, a);
+  }
+}
+
+}  // namespace
+}  // namespace onereel
+
+using namespace onereel;
+
+extern "C" int64_t or_varlen_bwd_workspace_size(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k,
+                                                int32_t H, int32_t D) {
+  if (n_seg < 1 || n_seg > kMaxSeg || n_q < 0 || n_k < 0 || max_q < 0 || max_k < 0 || H < 1 || H > 256 ||
+      (D != 64 && D != 128))
+    return fail_arg("or_varlen_bwd_workspace_size: 1 to %d segments, 1 to 256 heads of 64 or 128 and sizes of at least 0 are "
+                    "needed", kMaxSeg);
+  return layout_of(shape_of(n_seg, n_q, n_k, max_q, max_k, H), n_q, n_k, H, D).bytes;
+}
+
+extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
+  if (!p) return fail_arg("or_varlen_bwd: args is NULL");
+  const or_varlen_bwd_args& x = *p;
+  if (x.D != 64 && x.D != 128) return fail_arg("or_varlen_bwd: head_dim must be 64 or 128 (got %d)", x.D);
+  if (x.H < 1 || x.H > 256) return fail_arg("or_varlen_bwd: 1 to 256 heads (got %d)", x.H);
+  if (x.n_seg < 1 || x.n_seg > kMaxSeg) return fail_arg("or_varlen_bwd: 1 to %d segments (got %d)", kMaxSeg, x.n_seg);
+  if (x.n_q < 0 || x.n_k < 0 || x.max_q < 0 || x.max_k < 0) return fail_arg("or_varlen_bwd: negative sizes");
+  if (!(x.scale > 0.0f) || !isfinite(x.scale)) return fail_arg("or_varlen_bwd: scale must be positive and finite");
+  if (x.n_q == 0 && x.n_k == 0) return 0;
+  if (x.n_q > 0 && (!x.q || !x.o || !x.d_o || !x.lse || !x.dq))
+    return fail_arg("or_varlen_bwd: q, o, do, lse and dq are required");
+  if (x.n_k > 0 && (!x.k || !x.v || !x.dk || !x.dv)) return fail_arg("or_varlen_bwd: k, v, dk and dv are required");
+  if (!x.cu_q || (!x.cu_k && !(x.k_off && x.k_len)))
+    return fail_arg("or_varlen_bwd: cu_q and cu_k (or k_off and k_len) are required");
+  const int64_t row = (int64_t)x.H * x.D, far = (int64_t)1 << 24;
+  for (int64_t s : {x.q_row_stride, x.k_row_stride, x.o_row_stride, x.do_row_stride})
+    if (s < row || s % 8 || s > far)
+      return fail_arg("or_varlen_bwd: row strides must be multiples of 8 elements from H * D = %lld to 2^24",
+                      (long long)row);
+  if (!aligned16(x.q) || !aligned16(x.k) || !aligned16(x.v) || !aligned16(x.o) || !aligned16(x.d_o) || !aligned16(x.dq) ||
+      !aligned16(x.dk) || !aligned16(x.dv))
+    return fail_arg("or_varlen_bwd: pointers must be 16-byte aligned");
+  if (x.lse_stride < x.n_q) return fail_arg("or_varlen_bwd: lse_stride must cover the query rows");
+  const Shape s = shape_of(x.n_seg, x.n_q, x.n_k, x.max_q, x.max_k, x.H);
+  const Layout l = layout_of(s, x.n_q, x.n_k, x.H, x.D);
+  if (!x.workspace || x.workspace_bytes < l.bytes || !aligned16(x.workspace))
+    return fail_arg("or_varlen_bwd: a 16-byte aligned workspace of %lld bytes is needed", (long long)l.bytes);
+  // the second array of statistics lies 4 H n_q bytes after the first, within the 32 bits of a buffer offset
+  if ((int64_t)x.H * x.n_q * 4 + 256 >= (int64_t)0x7fffffff)
+    return fail_arg("or_varlen_bwd: H * n_q must stay under 2^29");
+  if (std::max(s.max_q_tiles * s.split_q, s.max_k_tiles * s.split_k) * x.H >= (int64_t)0x7ffffff0)
+    return fail_arg("or_varlen_bwd: too many tiles");
+  char* ws = (char*)x.workspace;
+  BwdArgs a;
+  a.q = (const uint16_t*)x.q;
+  a.k = (const uint16_t*)x.k;
+  a.v = (const uint16_t*)x.v;
+  a.o = (const uint16_t*)x.o;
+  a.d_o = (const uint16_t*)x.d_o;
+  a.lse = x.lse;
+  a.dlse = x.dlse;
+  a.dq = (uint16_t*)x.dq;
+  a.dk = (uint16_t*)x.dk;
+  a.dv = (uint16_t*)x.dv;
+  a.cu_q = x.cu_q;
+  a.cu_k = x.cu_k;
+  a.k_off = x.k_off;
+  a.k_len = x.k_len;
+  a.qs = x.q_row_stride;
+  a.ks = x.k_row_stride;
+  a.os = x.o_row_stride;
+  a.dos = x.do_row_stride;
+  a.lse_stride = x.lse_stride;
+  a.n_seg = x.n_seg;
+  a.n_q = x.n_q;
+  a.n_k = x.n_k;
+  a.H = x.H;
+  a.scale = x.scale;
+  a.split_q = s.split_q;
+  a.split_k = s.split_k;
+  a.max_q_tiles = (int32_t)s.max_q_tiles;
+  a.max_k_tiles = (int32_t)s.max_k_tiles;
+  a.head = (int32_t*)ws;
+  a.q_tiles = (i32x4*)(ws + l.q_tiles);
+  a.k_tiles = (i32x4*)(ws + l.k_tiles);
+  a.stat = (float*)(ws + l.stat);
+  a.part_q = (float*)(ws + l.part_q);
+  a.part_k = (float*)(ws + l.part_k);
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(bwd_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a, s.tq, s.tk);
+  if (x.D == 128) launch<128>(a, s, st);
+  else launch<64>(a, s, st);
+  const int64_t q8 = s.split_q > 1 ? (int64_t)x.n_q * row / 8 : 0, k8 = s.split_k > 1 ? (int64_t)x.n_k * row / 8 : 0;
+  if (q8 + k8 > 0) {
+    const int64_t blocks = std::min<int64_t>((q8 + 2 * k8 + kThreads - 1) / kThreads, 4096);
+    hipLaunchKernelGGL(bwd_add_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, a, q8, k8);
+  }
+  return check_hip(hipGetLastError(), "attention backward launch");
+}
