@@ -364,6 +364,22 @@ int or_rmsnorm_rope(const void* q, const void* k, const void* wq, const void* wk
                     const float* sin_table, const int32_t* rope_row, int64_t n_rope_rows, void* q_out, void* k_out,
                     int64_t qo_row_stride, int64_t ko_row_stride, void* stream);
 
+/* Bytes of device workspace or_rmsnorm_rope_bwd needs (-1 for sizes it refuses). */
+int64_t or_rmsnorm_rope_bwd_workspace_size(int64_t n_rows, int32_t C);
+
+/* The gradient of or_rmsnorm_rope (src/onereel/models/wan.py:64-74, which the reference leaves to torch.compile): with
+ * n = x / sqrt(mean(x^2) + eps) and g the output's gradient rotated back, dx = (g w - n mean(g w n)) / sqrt(mean(x^2) + eps)
+ * and dw = the sum over rows of g n; fp32 throughout, dx rounded to bf16 once. dq, dk: gradients of the outputs, q, k: the
+ * forward call's inputs, all bf16 rows of C elements with the given strides; q_grad, k_grad: bf16 [n_rows, C],
+ * contiguous; wq_grad, wk_grad: fp32 [C]. wk NULL: q alone. The other arguments as forward. The sums over rows are taken in
+ * a fixed order. Two launches. */
+int or_rmsnorm_rope_bwd(const void* dq, const void* dk, const void* q, const void* k, const void* wq, const void* wk,
+                        int64_t dq_row_stride, int64_t dk_row_stride, int64_t q_row_stride, int64_t k_row_stride,
+                        int64_t n_rows, int32_t C, int32_t D, float eps, const float* cos_table,
+                        const float* sin_table, const int32_t* rope_row, int64_t n_rope_rows, void* q_grad,
+                        void* k_grad, float* wq_grad, float* wk_grad, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
 /* Replaces the pooling of FrameMemory.collect (src/onereel/frame_memory.py:76-85, index_add_ of one layer's video rows
  * into per-frame sums and counts): for the frame-major rows r of hs (bf16, row stride row_stride elements, C wide),
  * frame (row0 + r) / T, sums[frame] += the row (fp32 [n_frames, C]) and counts[frame] += 1 (fp32 [n_frames]). Rows

@@ -55,6 +55,15 @@ def _qk(q, k, wq, wk, eps: float, cos, sin, heads: int):
         raise L.HipValueError(f'q / k of width {C} do not split into {heads} heads (k {tuple(k.shape)})')
     if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16:
         raise L.HipTypeError('q and k must be bfloat16')
+    if A.wants_grad(q, k, wq, wk):
+        A.refuse_captured_leaves('_qk', q, k, wq, wk)
+        return _QK.apply(q, k, wq, wk, eps, cos, sin, heads)
+    return _qk_forward(q, k, wq, wk, eps, cos, sin, heads)
+
+
+def _qk_forward(q, k, wq, wk, eps, cos, sin, heads):
+    C = q.shape[-1]
+    D = C // heads
     lead = q.shape[:-1]
     q2, k2 = q.reshape(-1, C), k.reshape(-1, C)
     if q2.stride(1) != 1 or k2.stride(1) != 1:
@@ -81,6 +90,9 @@ def rms_norm(x, weight, eps: float):
     C = x.shape[-1]
     if x.dtype != torch.bfloat16:
         raise L.HipTypeError('x must be bfloat16')
+    if A.wants_grad(x, weight):
+        A.refuse_captured_leaves('rms_norm', x, weight)
+        return _RMSNorm.apply(x, weight, eps)
     x2 = x.reshape(-1, C)
     if x2.stride(1) != 1:
         raise L.HipValueError('x rows must be contiguous')
@@ -90,6 +102,101 @@ def rms_norm(x, weight, eps: float):
                                     float(eps), None, None, None, 0, out.data_ptr(), None, C, 0,
                                     L.stream_handle(x.device)), 'or_rmsnorm_rope')
     return out.view(x.shape)
+
+
+def _grad_rows(x, C: int):
+    """x as [rows, C] bf16 rows that the gradient kernel reads: contiguous elements, whole 16-byte pieces (a copy where x
+    is not such rows, e.g. an expanded gradient)"""
+    if x.dtype != torch.bfloat16 or not x.is_cuda:
+        raise L.HipTypeError(f'expected a bf16 GPU tensor, got {x.dtype} on {x.device}')
+    x2 = x.reshape(-1, C)
+    if x2.shape[0] and not (x2.stride(1) == 1 and x2.stride(0) >= C and x2.stride(0) % 8 == 0 and x2.data_ptr() % 16 == 0):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2, max(x2.stride(0), C) if x2.shape[0] else C
+
+
+def _norm_backward(dys, xs, ws, eps, C: int, D: int, cos=None, sin=None):
+    """or_rmsnorm_rope_bwd of one or two tensors: ([dx, ..] [rows, C] bf16, [dw, ..] [C] fp32)"""
+    dev = xs[0].device
+    if any(t.device != dev for t in (*dys, *xs, *ws)) or (cos is not None and (cos.device != dev or sin.device != dev)):
+        raise L.HipTypeError('all tensors of a call must be on one GPU')
+    (dys, dss), (xs, xss) = (zip(*(_grad_rows(t, C) for t in ts)) for ts in (dys, xs))
+    S = xs[0].shape[0]
+    if any(t.shape[0] != S for t in (*dys, *xs)):
+        raise L.HipValueError('gradients and inputs must have the same rows')
+    if any(w.numel() != C for w in ws):
+        raise L.HipValueError(f'weights must hold {C} elements')
+    ws = [w.reshape(C).to(torch.bfloat16).contiguous() for w in ws]
+    ws = [w if w.data_ptr() % 16 == 0 else w.clone() for w in ws]
+    dx = [torch.empty(S, C, dtype=torch.bfloat16, device=dev) for _ in xs]
+    dw = [torch.empty(C, dtype=torch.float32, device=dev) for _ in xs]
+    n = L.lib().or_rmsnorm_rope_bwd_workspace_size(S, C)
+    L.check(min(int(n), 0), 'or_rmsnorm_rope_bwd_workspace_size')
+    space = torch.empty(int(n), dtype=torch.uint8, device=dev)
+    two = lambda ts, none=None: [t.data_ptr() for t in ts] + [none] * (2 - len(ts))
+    dss, xss = ([*t, *(0,) * (2 - len(t))] for t in (dss, xss))
+    with torch.cuda.device(dev):
+        L.check(L.lib().or_rmsnorm_rope_bwd(*two(dys), *two(xs), *two(ws), *dss, *xss, S, C, D, float(eps), L.ptr(cos),
+                                            L.ptr(sin), None, S if cos is not None else 0, *two(dx), *two(dw),
+                                            space.data_ptr(), space.numel(), L.stream_handle(dev)),
+                'or_rmsnorm_rope_bwd')
+    return dx, dw
+
+
+def qk_backward(dq, dk, q, k, wq, wk, eps: float, cos, sin, heads: int):
+    """The gradient of _qk: (q_grad, k_grad) bf16 in the shapes of q and k, (wq_grad, wk_grad) fp32 [C]. dq, dk
+    [..., S, heads, D] bf16: the gradients of its outputs; the other arguments are the call's own. fp32 inside, one
+    rounding; the weights' sums over rows are taken in a fixed order."""
+    C = q.shape[-1]
+    D = C // heads
+    if heads * D != C or k.shape != q.shape or dq.numel() != q.numel() or dk.numel() != q.numel():
+        raise L.HipValueError(f'q, k and their gradients must have one size of {heads} heads (q {tuple(q.shape)}, '
+                              f'k {tuple(k.shape)}, dq {tuple(dq.shape)}, dk {tuple(dk.shape)})')
+    S = q.numel() // C if C else 0
+    c, s = (t.reshape(-1, D).to(torch.float32).contiguous() for t in (cos, sin))
+    if c.shape[0] != S or s.shape[0] != S:
+        raise L.HipValueError(f'rotary tables hold {c.shape[0]} rows for {S} tokens')
+    (gq, gk), (gwq, gwk) = _norm_backward([dq, dk], [q, k], [wq, wk], eps, C, D, c, s)
+    return gq.view(q.shape), gk.view(k.shape), gwq, gwk
+
+
+def rms_norm_backward(dy, x, weight, eps: float):
+    """The gradient of rms_norm: (dx bf16 in the shape of x, dw fp32 [C])"""
+    C = x.shape[-1]
+    if dy.shape != x.shape:
+        raise L.HipValueError(f'x {tuple(x.shape)} and its output\'s gradient {tuple(dy.shape)} must have one shape')
+    (dx,), (dw,) = _norm_backward([dy], [x], [weight], eps, C, 128)
+    return dx.view(x.shape), dw
+
+
+class _QK(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, eps, cos, sin, heads):
+        ctx.save_for_backward(q, k, wq, wk, cos, sin)
+        ctx.eps, ctx.heads = eps, heads
+        return _qk_forward(q, k, wq, wk, eps, cos, sin, heads)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, wq, wk, cos, sin = ctx.saved_tensors
+        gq, gk, gwq, gwk = qk_backward(dq, dk, q, k, wq, wk, ctx.eps, cos, sin, ctx.heads)
+        return gq, gk, gwq.view(wq.shape).to(wq.dtype), gwk.view(wk.shape).to(wk.dtype), None, None, None, None
+
+
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps):
+        ctx.save_for_backward(x, weight)
+        ctx.eps = eps
+        return rms_norm(x, weight, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight = ctx.saved_tensors
+        dx, dw = rms_norm_backward(dy, x, weight, ctx.eps)
+        return dx, dw.view(weight.shape).to(weight.dtype), None
 
 
 def _token_ranges(lay, T: int) -> list:

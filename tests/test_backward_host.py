@@ -83,9 +83,10 @@ def test_python_refusals():
 def test_gradient_rows_are_copied_only_where_they_must_be():
     x = torch.zeros(6, 2, 64, dtype=torch.bfloat16)
     assert A._rows_for(x, 2, 64) == (x, 128) and A._rows_for(x[::2], 2, 64)[1] == 256
-    for odd in (x[:1].expand(6, 2, 64), x.transpose(1, 2).reshape(6, 64, 2).transpose(1, 2)):
+    for odd in (x[:1].expand(6, 2, 64), x.transpose(1, 2).reshape(6, 64, 2).transpose(1, 2),
+                torch.zeros(6, 64, 2, dtype=torch.bfloat16).transpose(1, 2)):
         y, stride = A._rows_for(odd, 2, 64)
-        assert stride == 128 and y.is_contiguous() and y.data_ptr() != odd.data_ptr()
+        assert stride == 128 and y.is_contiguous() and (y.data_ptr() == odd.data_ptr()) == odd.is_contiguous()
     assert A._rows_for(x[:0], 2, 64)[1] == 128
     with pytest.raises(L.HipValueError):
         A._rows_for(x, 2, 32)
