@@ -77,6 +77,23 @@ class PackArgs(ctypes.Structure):
                 ('cos_table', vp), ('sin_table', vp), ('n_rope_rows', i64), ('H', i32), ('D', i32)]
 
 
+# activations of or_linear (OR_ACT_*)
+ACTIVATIONS = {None: 0, 'gelu_tanh': 1, 'silu': 2}
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ('x', 'weight', 'bias', 'gate', 'residual', 'y', 'preactivation')] + \
+               [(n, i64) for n in ('n_rows', 'x_row_stride', 'weight_row_stride', 'residual_row_stride',
+                                   'y_row_stride')] + \
+               [(n, i32) for n in ('n_in', 'n_out', 'activation')] + [('workspace', vp), ('workspace_bytes', i64)]
+
+
+class LinearBwdArgs(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ('dy', 'x', 'weight', 'preactivation', 'gate', 'dx', 'dweight', 'dbias', 'dgate')] + \
+               [(n, i64) for n in ('n_rows', 'dy_row_stride', 'x_row_stride', 'weight_row_stride')] + \
+               [(n, i32) for n in ('n_in', 'n_out', 'activation')] + [('workspace', vp), ('workspace_bytes', i64)]
+
+
 # every exported symbol with its ctypes signature: include/onereel_hip.h
 SIGNATURES = {
     'or_layout_plan': (i32, [ctypes.POINTER(LayoutDesc), ctypes.POINTER(LayoutSizes)]),
@@ -115,6 +132,10 @@ DIT_SIGNATURES = {
     'or_gated_residual': (i32, [vp, vp, vp, i64, i32, i64, i64, vp]),
     'or_residual_layernorm_modulate': (i32, [vp, vp, vp, vp, i64, i32, i64, i64, i64, ctypes.c_float, vp, vp, vp, vp,
                                              vp]),
+    'or_linear_workspace_size': (i64, [i64, i32, i32]),
+    'or_linear': (i32, [ctypes.POINTER(LinearArgs), vp]),
+    'or_linear_bwd_workspace_size': (i64, [i64, i32, i32, i32]),
+    'or_linear_bwd': (i32, [ctypes.POINTER(LinearBwdArgs), vp]),
 }
 
 # libonereel_bench.so: include/onereel_bench.h

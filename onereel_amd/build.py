@@ -20,12 +20,12 @@ DIT_LIB = PKG / 'libonereel_dit.so'
 BENCH_LIB = PKG / 'libonereel_bench.so'
 OBJ = PKG / 'csrc' / '_obj'
 SOURCES = ['layout.hip', 'gather.hip', 'attention.hip', 'attention_bwd.hip', 'merge.hip', 'norm_rope.hip', 'frame_memory.hip', 'memory.hip']
-DIT_SOURCES = ['dit_fused.hip']
+DIT_SOURCES = ['dit_fused.hip', 'linear.hip']
 BENCH_SOURCES = ['mfma_ceiling.hip']
 # attention: no NaN operands reach the softmax max, so fmax needs no quieting of its inputs (v_max3_f32 directly)
 SOURCE_FLAGS = {'attention.hip': ['-fno-honor-nans']}
-# attention_bwd: its fp32 gradients (up to 256 registers) are only added to by MFMAs: they stay in AGPRs
-SOURCE_DROPS = {'attention_bwd.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form=1']}
+# attention_bwd, linear: their accumulators (up to 256 registers) are only added to by MFMAs: they stay in AGPRs
+SOURCE_DROPS = {s: ['-mllvm', '-amdgpu-mfma-vgpr-form=1'] for s in ('attention_bwd.hip', 'linear.hip')}
 ARCH = os.environ.get('ONEREEL_ARCH', 'gfx950')
 
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')

@@ -253,7 +253,7 @@ __device__ __forceinline__ void dma_stats(const float* base, int64_t apart, int 
 
 template <int N>
 __device__ __forceinline__ void wait_loads_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {

@@ -1,0 +1,674 @@
+// Linear layers of the DiT block for gfx950: y = residual + gate * act(x W^T + b) with everything after the product in its
+// epilogue, and the gradient of it. bf16 operands, fp32 accumulation, one rounding.
+//
+//   z = x W^T + b      y = residual + gate * act(z)
+//   dz = dy * gate * act'(z)    dx = dz W    dW = dz^T x    db = sum dz    dgate = sum dy * act(z)   (sums over rows)
+//
+// One product kernel for the three layouts: C[i][j] = sum_k A(i, k) B(j, k), where an operand's rows are contiguous either
+// along k (x and W forward, dz in dx) or along their own index (W in dx, dz and x in dW).
+// - A work-group of 4 wavefronts owns a TI x TJ tile, each wavefront a quarter of it in fp32 accumulators; 64 steps of k of
+//   both operands go into one of two LDS buffers by LDS DMA while the other is multiplied. An operand contiguous along k
+//   is read as it lies (16 bytes a lane); the others are read by transposing LDS reads. XOR swizzles of the 16-byte
+//   chunks keep both free of bank conflicts.
+// - C's columns j are the rows of the MFMA tiles, so that a lane holds runs of 4 columns of one row; the epilogue brings
+//   32 rows at a time through LDS into rows of 16-byte pieces, with the residual read and the results written in whole
+//   lines.
+// - Rows and columns past an operand's end load as zeros through the buffer descriptor (and an offset out of its range
+//   for the pieces past the end of a row that is not the last), so ragged sizes take the same path.
+// - Tiles of 256 x 256 are bound by the matrix cores; smaller tiles and a k axis split over several work-groups (fp32
+//   partial products, added in order by the epilogue's own launch) fill the GPU when there are few tiles. Up to 32 rows
+//   of x take a kernel of their own that streams W once, bound by HBM.
+#include <math.h>
+
+#include <algorithm>
+
+#include "../../include/onereel_dit.h"
+#include "common.h"
+
+namespace onereel {
+
+namespace {
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+
+constexpr int kThreads = 256;
+constexpr int kStep = 64;            // k per LDS buffer
+constexpr int64_t kMaxStride = 1 << 21;
+
+// ------------------------------------------------------------------------------------------------------------------
+// epilogue
+struct Epilogue {
+  uint16_t* y;
+  int64_t y_stride;
+  uint16_t* z;                       // optional: the pre-activation, [rows, cols] contiguous
+  const float* bias;                 // optional [cols]
+  const float* gate;                 // optional [cols]
+  const uint16_t* residual;          // optional
+  int64_t residual_stride;
+  int act;
+};
+
+__device__ __forceinline__ float act_of(float z, int act) {
+  if (act == OR_ACT_SILU) return z / (1.0f + __expf(-z));
+  if (act == OR_ACT_GELU_TANH) {
+    // 0.5 z (1 + tanh u) = z / (1 + exp(-2 u))
+    const float u = 0.7978845608028654f * (z + 0.044715f * z * z * z);
+    return z / (1.0f + __expf(-2.0f * u));
+  }
+  return z;
+}
+
+// act(z) and act'(z). The derivative is taken at z clamped to +-20, where it has reached 0 or 1 in fp32: no 0 * inf.
+__device__ __forceinline__ void act_grad(float z, int act, float& f, float& d) {
+  f = z;
+  d = 1.0f;
+  if (act == OR_ACT_NONE) return;
+  const float c = fminf(fmaxf(z, -20.0f), 20.0f);
+  if (act == OR_ACT_SILU) {
+    const float p = 1.0f / (1.0f + __expf(-c));
+    d = p + c * p * (1.0f - p);
+  } else {
+    const float u = 0.7978845608028654f * (c + 0.044715f * c * c * c);
+    const float p = 1.0f / (1.0f + __expf(-2.0f * u)), q = 1.0f / (1.0f + __expf(2.0f * u));
+    d = p + 2.0f * c * p * q * (0.7978845608028654f * (1.0f + 3.0f * 0.044715f * c * c));
+  }
+  if (z != z) d = z;
+  f = act_of(z, act);
+}
+
+// 8 columns col .. of one row from the fp32 products v
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int col, int cols, float (&v)[8]) {
+  if (e.bias) {
+    const f32x4 b0 = *(const f32x4*)(e.bias + col), b1 = *(const f32x4*)(e.bias + col + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += i < 4 ? b0[i] : b1[i - 4];
+  }
+  if (e.z) *(u32x4*)(e.z + row * cols + col) = u32x4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
+  if (e.act != OR_ACT_NONE)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = act_of(v[i], e.act);
+  if (e.gate) {
+    const f32x4 b0 = *(const f32x4*)(e.gate + col), b1 = *(const f32x4*)(e.gate + col + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= i < 4 ? b0[i] : b1[i - 4];
+  }
+  if (e.residual) {
+    const u32x4 r = *(const u32x4*)(e.residual + row * e.residual_stride + col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] += bf2f((uint16_t)(r[i] & 0xffffu));
+      v[2 * i + 1] += bf2f((uint16_t)(r[i] >> 16));
+    }
+  }
+  *(u32x4*)(e.y + row * e.y_stride + col) = u32x4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// products
+struct Operand {
+  const uint16_t* p;
+  int64_t stride;                    // elements between its rows (rows of i or j, or rows of k when transposed)
+};
+
+struct GemmArgs {
+  Operand a, b;
+  int64_t I;                         // rows of C
+  int J;                             // columns of C, a multiple of 8
+  int64_t K;
+  int split;                         // parts of the k axis
+  int tiles_i, tiles_j;
+  float* part;                       // [split][I][J] when split > 1
+  Epilogue e;
+};
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const lds_void*)p; }
+
+__device__ __forceinline__ void dma16(const i32x4& r, uint32_t off, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r),
+               "s"(__builtin_amdgcn_readfirstlane(m0))
+               : "memory");
+}
+
+__device__ __forceinline__ i32x4 descriptor(const uint16_t* p, int64_t bytes) {
+  const uint64_t b = (uint64_t)p;
+  return i32x4{__builtin_amdgcn_readfirstlane((int32_t)(uint32_t)b),
+               __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)(b >> 32)),
+               __builtin_amdgcn_readfirstlane((int32_t)(bytes > 0 ? bytes : 0)), 0x00020000};
+}
+
+// One operand's tile of N rows x kStep in LDS. TR false: N rows of 64 k (128 bytes each); TR true: 64 rows of k of N
+// elements. Chunk c (16 bytes) of row r lies at position c ^ swz(r).
+template <int N, bool TR>
+struct Tile {
+  static constexpr int CH = TR ? N / 8 : kStep / 8;      // chunks per row
+  static constexpr int BYTES = N * kStep * 2;
+  static constexpr int LOADS = BYTES / 16 / kThreads;    // DMA loads per lane
+  static constexpr int W = N / 2, F = W / 32;            // a wavefront's share and its blocks of 32
+  static_assert(LOADS >= 1, "tile");
+
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (!TR) return (r >> 1) & 7;
+    else if constexpr (CH == 8) return ((r >> 1) & 1) << 2;
+    else return (r & 3) << 2;
+  }
+  uint32_t off[LOADS];               // byte offset of each load from the tile's first element
+  int chunk[LOADS];                  // its column of the row, in chunks
+  __device__ __forceinline__ void init(int tid, int64_t stride) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int x = i * kThreads + tid, r = x / CH, c = (x % CH) ^ swz(r);
+      off[i] = (uint32_t)(r * stride * 2 + c * 16);
+      chunk[i] = c;
+    }
+  }
+  // the tile at rows n0 .. (of n) and k0 .. (of k)
+  __device__ __forceinline__ void load(const Operand& o, int64_t n0, int64_t n, int64_t k0, int64_t k, uint32_t m0) const {
+    const int64_t rows = TR ? min(k - k0, (int64_t)kStep) : min(n - n0, (int64_t)N);
+    const int64_t wide = TR ? min(n - n0, (int64_t)N) : min(k - k0, (int64_t)kStep);
+    const uint16_t* p = o.p + (TR ? k0 * o.stride + n0 : n0 * o.stride + k0);
+    const i32x4 r = descriptor(p, rows > 0 && wide > 0 ? ((rows - 1) * o.stride + wide) * 2 : 0);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      dma16(r, chunk[i] * 8 < wide ? off[i] : 0x80000000u, m0 + i * kThreads * 16);
+  }
+};
+
+// operand fragments of a wavefront: block f of 32 rows, step ks of 16 k (8 (lane / 32) + 0 .. 7 of them in this lane)
+template <int N, bool TR>
+struct Frag {
+  static constexpr int FS = TR ? (N / 2 / 32) : kStep / 16;
+  uint32_t at[FS];                   // TR: one per block of 32, else one per step
+  __device__ __forceinline__ void init(int lane, int half) {
+    using T = Tile<N, TR>;
+    const int l32 = lane & 31, h = lane >> 5, r = lane & 15, g = (lane >> 4) & 1;
+#pragma unroll
+    for (int x = 0; x < FS; ++x) {
+      if constexpr (TR) {
+        const int row = 8 * h + (r >> 2), c = (half * T::W + 32 * x) / 8 + 2 * g + ((r >> 1) & 1);
+        at[x] = row * N * 2 + (c ^ T::swz(row)) * 16 + (r & 1) * 8;
+      } else {
+        const int row = half * T::W + l32;
+        at[x] = row * kStep * 2 + ((2 * x + h) ^ T::swz(row)) * 16;
+      }
+    }
+  }
+  __device__ __forceinline__ bf16x8 get(uint32_t buf, int f, int ks) const {
+    if constexpr (TR) {
+      u32x2 x[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        x[t] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                                             (lds_bf16x4*)(uintptr_t)(buf + at[f] + (16 * ks + 4 * t) * N * 2)));
+      return __builtin_bit_cast(bf16x8, u32x4{x[0][0], x[0][1], x[1][0], x[1][1]});
+    } else {
+      return *(const __attribute__((address_space(3))) bf16x8*)(uintptr_t)(buf + at[ks] + f * 32 * kStep * 2);
+    }
+  }
+};
+
+// Tiles in groups of 8 rows of tiles: the work-groups of one XCD (index modulo 8) take consecutive tiles, which share
+// their operands' rows in that XCD's L2.
+__device__ __forceinline__ bool tile_of(const GemmArgs& g, int& ti, int& tj, int& part) {
+  const int64_t n = (int64_t)g.tiles_i * g.tiles_j * g.split, per = (n + 7) / 8, j = blockIdx.x >> 3;
+  int64_t x = (blockIdx.x & 7) * per + j;
+  if (j >= per || x >= n) return false;
+  part = (int)(x % g.split);
+  x /= g.split;
+  constexpr int kGroup = 8;
+  const int64_t group = x / ((int64_t)kGroup * g.tiles_j), in = x % ((int64_t)kGroup * g.tiles_j);
+  const int high = min(kGroup, g.tiles_i - (int)group * kGroup);
+  ti = (int)(group * kGroup + in % high);
+  tj = (int)(in / high);
+  return true;
+}
+
+template <int TI, int TJ, bool TRA, bool TRB>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void gemm_kernel(GemmArgs g) {
+  using TA = Tile<TI, TRA>;
+  using TB = Tile<TJ, TRB>;
+  constexpr int FI = TA::F, FJ = TB::F, BUF = TA::BYTES + TB::BYTES;
+  constexpr int kPad = TJ / 2 + 4;                         // floats per staged row of the epilogue
+  constexpr int kStage = 4 * 32 * kPad * 4;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * BUF > kStage ? 2 * BUF : kStage];
+  int ti, tj, part;
+  if (!tile_of(g, ti, tj, part)) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = w >> 1, wj = w & 1;
+  const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * TJ;
+  const int64_t steps = (g.K + kStep - 1) / kStep;
+  const int64_t s0 = steps * part / g.split, s1 = steps * (part + 1) / g.split;
+
+  TA la;
+  TB lb;
+  la.init(tid, g.a.stride);
+  lb.init(tid, g.b.stride);
+  Frag<TI, TRA> fa;
+  Frag<TJ, TRB> fb;
+  fa.init(lane, wi);
+  fb.init(lane, wj);
+  const uint32_t base = lds_addr(lds), m0 = base + w * 1024;
+  auto fetch = [&](int64_t s, uint32_t buf) {
+    la.load(g.a, i0, g.I, s * kStep, g.K, m0 + buf);
+    lb.load(g.b, j0, g.J, s * kStep, g.K, m0 + buf + TA::BYTES);
+  };
+
+  f32x16 acc[FI][FJ];
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < FJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+  uint32_t cur = 0;
+  if (s0 < s1) fetch(s0, 0);
+#pragma unroll 1
+  for (int64_t s = s0; s < s1; ++s) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + 1 < s1) fetch(s + 1, BUF - cur);
+    const uint32_t ba = base + cur, bb = ba + TA::BYTES;
+#pragma unroll
+    for (int ks = 0; ks < kStep / 16; ++ks) {
+      bf16x8 a[FI], b[FJ];
+#pragma unroll
+      for (int i = 0; i < FI; ++i) a[i] = fa.get(ba, i, ks);
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) b[j] = fb.get(bb, j, ks);
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+    }
+    cur = BUF - cur;
+  }
+  __syncthreads();
+
+  // epilogue: 32 rows at a time through this wavefront's part of LDS
+  const int l32 = lane & 31, h = lane >> 5;
+  float* st = (float*)lds + w * 32 * kPad;
+  constexpr int LPR = TJ / 2 / 8;                          // lanes per row of 16-byte pieces
+  const int64_t ib = i0 + wi * (TI / 2);
+  const int64_t jc = j0 + wj * (TJ / 2) + (lane % LPR) * 8;
+#pragma unroll
+  for (int i = 0; i < FI; ++i) {
+#pragma unroll
+    for (int j = 0; j < FJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(f32x4*)(st + l32 * kPad + 32 * j + 8 * q + 4 * h) =
+            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+    for (int r = lane / LPR; r < 32; r += 64 / LPR) {
+      const int64_t row = ib + 32 * i + r;
+      const f32x4 x = *(const f32x4*)(st + r * kPad + (lane % LPR) * 8), y = *(const f32x4*)(st + r * kPad + (lane % LPR) * 8 + 4);
+      if (row < g.I && jc < g.J) {
+        if (g.split > 1) {
+          float* p = g.part + ((int64_t)part * g.I + row) * g.J + jc;
+          *(f32x4*)p = x;
+          *(f32x4*)(p + 4) = y;
+        } else {
+          float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+          finish8(g.e, row, (int)jc, g.J, v);
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// the parts of a split product, added in order, and the epilogue
+__global__ __launch_bounds__(kThreads) void join_kernel(GemmArgs g) {
+  const int64_t n8 = g.I * g.J / 8, step = (int64_t)gridDim.x * kThreads;
+  for (int64_t x = (int64_t)blockIdx.x * kThreads + threadIdx.x; x < n8; x += step) {
+    f32x4 lo = {}, hi = {};
+    for (int p = 0; p < g.split; ++p) {
+      const float* at = g.part + (int64_t)p * g.I * g.J + x * 8;
+      lo += *(const f32x4*)at;
+      hi += *(const f32x4*)(at + 4);
+    }
+    float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    finish8(g.e, x * 8 / g.J, (int)(x * 8 % g.J), g.J, v);
+  }
+}
+
+// Up to 16 MB rows of x: a work-group takes 16 columns and reads their rows of W once, its wavefronts dealing out k in
+// pieces of 128; no LDS but for the sum of the wavefronts. W's lanes hold 64 contiguous bytes of a row (k within a piece is
+// dealt to the MFMA steps in that order, on both operands).
+constexpr int kSkinnyWaves = 8;
+template <int MB>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(GemmArgs g) {
+  __shared__ float sum[kSkinnyWaves][16 * MB][17];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, q = lane >> 4;
+  const int j0 = blockIdx.x * 16;
+  const int K = (int)g.K;
+  f32x4 acc[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) acc[m] = f32x4{0, 0, 0, 0};
+  const uint16_t* wp = g.b.p + (int64_t)min(j0 + l16, g.J - 1) * g.b.stride;
+  for (int k0 = w * 128; k0 < K; k0 += kSkinnyWaves * 128) {
+    u32x4 wf[4], xf[MB][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int k = k0 + 32 * q + 8 * s;
+      const bool in = k < K;
+      wf[s] = in ? *(const u32x4*)(wp + k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const int r = 16 * m + l16;
+        xf[m][s] = in && r < g.I ? *(const u32x4*)(g.a.p + r * g.a.stride + k) : u32x4{0, 0, 0, 0};
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wf[s]),
+                                                         __builtin_bit_cast(bf16x8, xf[m][s]), acc[m], 0, 0, 0);
+  }
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[w][16 * m + l16][4 * q + i] = acc[m][i];
+  __syncthreads();
+  for (int x = threadIdx.x; x < 32 * MB; x += 64 * kSkinnyWaves) {
+    const int r = x >> 1, c = 8 * (x & 1);
+    if (r >= g.I || j0 + c >= g.J) continue;
+    float v[8] = {};
+    for (int i = 0; i < kSkinnyWaves; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += sum[i][r][c + e];
+    finish8(g.e, r, j0 + c, g.J, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// dz = dy * gate * act'(z) and the sums over rows db = sum dz, dgate = sum dy * act(z): 256 columns x kSumRows rows a
+// work-group, 8 columns a lane; the work-groups' partial sums are added up in order by a second launch
+constexpr int kSumRows = 128;
+struct DzArgs {
+  const uint16_t *dy, *z;
+  int64_t dy_stride;
+  const float* gate;
+  uint16_t* dz;                      // optional
+  float* part;                       // [2][chunks][N]: db, dgate
+  float *db, *dgate;                 // optional
+  int64_t M;
+  int N, act, chunks;
+};
+
+__global__ __launch_bounds__(kThreads) void dz_kernel(DzArgs g) {
+  __shared__ float sum[2][8][256];
+  const int c = threadIdx.x & 31, rr = threadIdx.x >> 5, col = blockIdx.x * 256 + c * 8;
+  const int64_t r0 = (int64_t)blockIdx.y * kSumRows, r1 = min(r0 + kSumRows, g.M);
+  float db[8] = {}, dg[8] = {}, gate[8];
+  const bool in = col < g.N;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) gate[i] = in && g.gate ? g.gate[col + i] : 1.0f;
+  if (in)
+    for (int64_t r = r0 + rr; r < r1; r += 8) {
+      const u32x4 y = *(const u32x4*)(g.dy + r * g.dy_stride + col);
+      const u32x4 z = g.z ? *(const u32x4*)(g.z + r * g.N + col) : u32x4{0, 0, 0, 0};
+      float dz[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = bf2f((uint16_t)(i & 1 ? y[i / 2] >> 16 : y[i / 2] & 0xffffu));
+        const float zz = bf2f((uint16_t)(i & 1 ? z[i / 2] >> 16 : z[i / 2] & 0xffffu));
+        float f, d;
+        act_grad(zz, g.act, f, d);
+        dg[i] += e * f;
+        dz[i] = g.act == OR_ACT_NONE ? e * gate[i] : e * gate[i] * d;
+        db[i] += dz[i];
+      }
+      if (g.dz)
+        *(u32x4*)(g.dz + r * g.N + col) = u32x4{pack2(dz[0], dz[1]), pack2(dz[2], dz[3]), pack2(dz[4], dz[5]), pack2(dz[6], dz[7])};
+    }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    sum[0][rr][c * 8 + i] = db[i];
+    sum[1][rr][c * 8 + i] = dg[i];
+  }
+  __syncthreads();
+  const int x = blockIdx.x * 256 + threadIdx.x;
+  if (x >= g.N) return;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    if (!(which ? g.dgate : g.db)) continue;
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += sum[which][i][threadIdx.x];
+    g.part[((int64_t)which * g.chunks + blockIdx.y) * g.N + x] = v;
+  }
+}
+
+constexpr int kSumWaves = 16;
+__global__ __launch_bounds__(64 * kSumWaves) void column_sum_kernel(DzArgs g) {
+  __shared__ float sum[kSumWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, which = blockIdx.y, col = blockIdx.x * 64 + lane;
+  float* out = which ? g.dgate : g.db;
+  if (!out) return;
+  float v = 0.0f;
+  if (col < g.N) {
+    const float* p = g.part + (int64_t)which * g.chunks * g.N + col;
+#pragma unroll 8
+    for (int b = wave; b < g.chunks; b += kSumWaves) v += p[(int64_t)b * g.N];
+  }
+  sum[wave][lane] = v;
+  __syncthreads();
+  if (wave == 0 && col < g.N) {
+    v = 0.0f;
+    for (int i = 0; i < kSumWaves; ++i) v += sum[i][lane];
+    out[col] = v;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// which kernel a product takes, and its workspace
+struct Plan {
+  int tile;                          // 256, 128 or 64; 0: the skinny kernel
+  int tiles_i, tiles_j, split;
+  int64_t part_bytes;
+};
+
+Plan plan_of(int64_t I, int64_t J, int64_t K, bool rows_of_k) {
+  Plan p = {};
+  p.split = 1;
+  if (rows_of_k && I <= 32) return p;
+  const int64_t steps = (K + kStep - 1) / kStep;
+  auto tiles = [&](int t) { return ((I + t - 1) / t) * ((J + t - 1) / t); };
+  p.tile = tiles(256) >= 192 ? 256 : tiles(128) >= 128 ? 128 : 64;
+  p.tiles_i = (int)((I + p.tile - 1) / p.tile);
+  p.tiles_j = (int)((J + p.tile - 1) / p.tile);
+  const int64_t n = (int64_t)p.tiles_i * p.tiles_j;
+  // few tiles and a long k: parts of at least 8 steps, up to 512 work-groups
+  p.split = (int)std::max<int64_t>(1, std::min<int64_t>({(384 + n - 1) / std::max<int64_t>(n, 1), steps / 8, 32}));
+  if (n >= 256) p.split = 1;
+  p.part_bytes = p.split > 1 ? (int64_t)p.split * I * J * 4 : 0;
+  return p;
+}
+
+template <bool TRA, bool TRB>
+void launch_tiles(const GemmArgs& g, int tile, hipStream_t st) {
+  const int64_t n = (int64_t)g.tiles_i * g.tiles_j * g.split;
+  const dim3 grid((unsigned)((n + 7) / 8 * 8));
+  if (tile == 256) hipLaunchKernelGGL((gemm_kernel<256, 256, TRA, TRB>), grid, dim3(kThreads), 0, st, g);
+  else if (tile == 128) hipLaunchKernelGGL((gemm_kernel<128, 128, TRA, TRB>), grid, dim3(kThreads), 0, st, g);
+  else hipLaunchKernelGGL((gemm_kernel<64, 64, TRA, TRB>), grid, dim3(kThreads), 0, st, g);
+}
+
+void launch_product(GemmArgs g, bool tra, bool trb, float* part, hipStream_t st) {
+  const Plan p = plan_of(g.I, g.J, g.K, !tra && !trb);
+  if (p.tile == 0) {
+    const dim3 grid((unsigned)((g.J + 15) / 16));
+    if (g.I <= 16) hipLaunchKernelGGL(skinny_kernel<1>, grid, dim3(64 * kSkinnyWaves), 0, st, g);
+    else hipLaunchKernelGGL(skinny_kernel<2>, grid, dim3(64 * kSkinnyWaves), 0, st, g);
+    return;
+  }
+  g.tiles_i = p.tiles_i;
+  g.tiles_j = p.tiles_j;
+  g.split = p.split;
+  g.part = part;
+  if (!tra && !trb) launch_tiles<false, false>(g, p.tile, st);
+  else if (!tra) launch_tiles<false, true>(g, p.tile, st);
+  else launch_tiles<true, true>(g, p.tile, st);
+  if (p.split > 1) {
+    const int64_t blocks = std::min<int64_t>((g.I * g.J / 8 + kThreads - 1) / kThreads, 8192);
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, g);
+  }
+}
+
+bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
+
+int check_sizes(const char* what, int64_t M, int32_t N, int32_t K, int32_t act) {
+  if (M < 0 || M >= (int64_t)1 << 31) return fail_arg("%s: 0 to 2^31 - 1 rows (got %lld)", what, (long long)M);
+  if (N < 8 || N % 8 || K < 8 || K % 8 || N > kMaxStride || K > kMaxStride)
+    return fail_arg("%s: n_in and n_out must be multiples of 8 up to 2^21 (got %d and %d)", what, K, N);
+  if (act != OR_ACT_NONE && act != OR_ACT_GELU_TANH && act != OR_ACT_SILU) return fail_arg("%s: unknown activation %d", what, act);
+  // tiles of 64 in a grid of 32 bits
+  if ((M + 63) / 64 * ((N + 63) / 64) >= (int64_t)1 << 30 || (M + 63) / 64 * ((K + 63) / 64) >= (int64_t)1 << 30)
+    return fail_arg("%s: too many tiles", what);
+  return 0;
+}
+
+int bad_stride(const char* what, int64_t stride, int64_t width) {
+  if (stride < width || stride % 8 || stride > kMaxStride)
+    return fail_arg("%s: row strides must be multiples of 8 elements that cover a row, up to 2^21", what);
+  return 0;
+}
+
+struct BwdLayout {
+  int64_t dz, sums, part, bytes;
+};
+BwdLayout bwd_layout(int64_t M, int32_t N, int32_t K, bool makes_dz) {
+  BwdLayout l;
+  l.dz = 0;
+  l.sums = makes_dz ? round256(M * N * 2) : 0;
+  const int64_t chunks = (M + kSumRows - 1) / kSumRows;
+  l.part = l.sums + round256(2 * chunks * N * 4);
+  l.bytes = l.part + round256(std::max(plan_of(M, K, N, false).part_bytes, plan_of(N, K, M, false).part_bytes)) + 256;
+  return l;
+}
+
+}  // namespace
+}  // namespace onereel
+
+using namespace onereel;
+
+extern "C" int64_t or_linear_workspace_size(int64_t n_rows, int32_t n_in, int32_t n_out) {
+  if (int rc = check_sizes("or_linear_workspace_size", n_rows, n_out, n_in, OR_ACT_NONE)) return rc;
+  return plan_of(n_rows, n_out, n_in, true).part_bytes + 256;
+}
+
+extern "C" int or_linear(const or_linear_args* p, void* stream) {
+  if (!p) return fail_arg("or_linear: args is NULL");
+  const or_linear_args& x = *p;
+  if (int rc = check_sizes("or_linear", x.n_rows, x.n_out, x.n_in, x.activation)) return rc;
+  if (x.n_rows == 0) return 0;
+  if (!x.x || !x.weight || !x.y) return fail_arg("or_linear: x, weight and y are required");
+  if (int rc = bad_stride("or_linear: x", x.x_row_stride, x.n_in)) return rc;
+  if (int rc = bad_stride("or_linear: weight", x.weight_row_stride, x.n_in)) return rc;
+  if (int rc = bad_stride("or_linear: y", x.y_row_stride, x.n_out)) return rc;
+  if (x.residual)
+    if (int rc = bad_stride("or_linear: residual", x.residual_row_stride, x.n_out)) return rc;
+  if (!al16(x.x) || !al16(x.weight) || !al16(x.bias) || !al16(x.gate) || !al16(x.residual) || !al16(x.y) ||
+      !al16(x.preactivation))
+    return fail_arg("or_linear: pointers must be 16-byte aligned");
+  const int64_t need = or_linear_workspace_size(x.n_rows, x.n_in, x.n_out);
+  if (!x.workspace || !al16(x.workspace) || x.workspace_bytes < need)
+    return fail_arg("or_linear: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
+  GemmArgs g = {};
+  g.a = Operand{(const uint16_t*)x.x, x.x_row_stride};
+  g.b = Operand{(const uint16_t*)x.weight, x.weight_row_stride};
+  g.I = x.n_rows;
+  g.J = x.n_out;
+  g.K = x.n_in;
+  g.e = Epilogue{(uint16_t*)x.y, x.y_row_stride, (uint16_t*)x.preactivation, x.bias, x.gate, (const uint16_t*)x.residual,
+                 x.residual_row_stride, x.activation};
+  launch_product(g, false, false, (float*)x.workspace, (hipStream_t)stream);
+  return check_hip(hipGetLastError(), "or_linear launch");
+}
+
+extern "C" int64_t or_linear_bwd_workspace_size(int64_t n_rows, int32_t n_in, int32_t n_out, int32_t scaled) {
+  if (int rc = check_sizes("or_linear_bwd_workspace_size", n_rows, n_out, n_in, OR_ACT_NONE)) return rc;
+  return bwd_layout(n_rows, n_out, n_in, scaled != 0).bytes;
+}
+
+extern "C" int or_linear_bwd(const or_linear_bwd_args* p, void* stream) {
+  if (!p) return fail_arg("or_linear_bwd: args is NULL");
+  const or_linear_bwd_args& x = *p;
+  if (int rc = check_sizes("or_linear_bwd", x.n_rows, x.n_out, x.n_in, x.activation)) return rc;
+  const bool scaled = x.activation != OR_ACT_NONE || x.gate;
+  if (x.n_rows > 0 && !x.dy) return fail_arg("or_linear_bwd: dy is required");
+  if (x.dx && !x.weight) return fail_arg("or_linear_bwd: dx needs the weight");
+  if (x.dweight && x.n_rows > 0 && !x.x) return fail_arg("or_linear_bwd: dweight needs x");
+  if (x.dgate && !x.gate) return fail_arg("or_linear_bwd: dgate needs the gate");
+  if ((x.activation != OR_ACT_NONE || x.dgate) && x.n_rows > 0 && !x.preactivation)
+    return fail_arg("or_linear_bwd: an activation's gradient and dgate need the pre-activation");
+  if (int rc = bad_stride("or_linear_bwd: dy", x.dy_row_stride, x.n_out)) return rc;
+  if (x.x)
+    if (int rc = bad_stride("or_linear_bwd: x", x.x_row_stride, x.n_in)) return rc;
+  if (x.weight)
+    if (int rc = bad_stride("or_linear_bwd: weight", x.weight_row_stride, x.n_in)) return rc;
+  if (!al16(x.dy) || !al16(x.x) || !al16(x.weight) || !al16(x.preactivation) || !al16(x.gate) || !al16(x.dx) ||
+      !al16(x.dweight) || !al16(x.dbias) || !al16(x.dgate))
+    return fail_arg("or_linear_bwd: pointers must be 16-byte aligned");
+  const BwdLayout l = bwd_layout(x.n_rows, x.n_out, x.n_in, scaled);
+  if (!x.workspace || !al16(x.workspace) || x.workspace_bytes < l.bytes)
+    return fail_arg("or_linear_bwd: a 16-byte aligned workspace of %lld bytes is needed", (long long)l.bytes);
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)x.workspace;
+  const bool sums = x.dbias || x.dgate, products = x.dx || x.dweight;
+  Operand dz{(const uint16_t*)x.dy, x.dy_row_stride};
+  if (sums || (scaled && products)) {
+    DzArgs d = {};
+    d.dy = (const uint16_t*)x.dy;
+    d.dy_stride = x.dy_row_stride;
+    d.z = x.activation != OR_ACT_NONE || x.dgate ? (const uint16_t*)x.preactivation : nullptr;
+    d.gate = x.gate;
+    d.dz = scaled && products ? (uint16_t*)(ws + l.dz) : nullptr;
+    d.part = (float*)(ws + l.sums);
+    d.db = x.dbias;
+    d.dgate = x.dgate;
+    d.M = x.n_rows;
+    d.N = x.n_out;
+    d.act = x.activation;
+    d.chunks = (int)((x.n_rows + kSumRows - 1) / kSumRows);
+    if (d.chunks > 65535) return fail_arg("or_linear_bwd: at most %d rows", 65535 * kSumRows);
+    if (d.chunks > 0)
+      hipLaunchKernelGGL(dz_kernel, dim3((unsigned)((x.n_out + 255) / 256), (unsigned)d.chunks), dim3(kThreads), 0, st, d);
+    if (sums)
+      hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((x.n_out + 63) / 64), 2), dim3(64 * kSumWaves), 0, st, d);
+    if (d.dz) dz = Operand{d.dz, x.n_out};
+  }
+  if (x.dx && x.n_rows > 0) {
+    GemmArgs g = {};
+    g.a = dz;
+    g.b = Operand{(const uint16_t*)x.weight, x.weight_row_stride};
+    g.I = x.n_rows;
+    g.J = x.n_in;
+    g.K = x.n_out;
+    g.e.y = (uint16_t*)x.dx;
+    g.e.y_stride = x.n_in;
+    launch_product(g, false, true, (float*)(ws + l.part), st);
+  }
+  if (x.dweight) {
+    GemmArgs g = {};
+    g.a = dz;
+    g.b = Operand{(const uint16_t*)x.x, x.x_row_stride};
+    g.I = x.n_out;
+    g.J = x.n_in;
+    g.K = x.n_rows;
+    g.e.y = (uint16_t*)x.dweight;
+    g.e.y_stride = x.n_in;
+    launch_product(g, true, true, (float*)(ws + l.part), st);
+  }
+  return check_hip(hipGetLastError(), "or_linear_bwd launch");
+}
