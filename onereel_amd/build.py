@@ -24,8 +24,8 @@ DIT_SOURCES = ['dit_fused.hip', 'linear.hip']
 BENCH_SOURCES = ['mfma_ceiling.hip']
 # attention: no NaN operands reach the softmax max, so fmax needs no quieting of its inputs (v_max3_f32 directly)
 SOURCE_FLAGS = {'attention.hip': ['-fno-honor-nans']}
-# attention_bwd, linear: their accumulators (up to 256 registers) are only added to by MFMAs: they stay in AGPRs
-SOURCE_DROPS = {s: ['-mllvm', '-amdgpu-mfma-vgpr-form=1'] for s in ('attention_bwd.hip', 'linear.hip')}
+# linear: its accumulators (up to 256 registers) are only added to by MFMAs: they stay in AGPRs
+SOURCE_DROPS = {'linear.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form=1']}
 ARCH = os.environ.get('ONEREEL_ARCH', 'gfx950')
 
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
