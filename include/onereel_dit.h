@@ -48,8 +48,8 @@ int or_residual_layernorm_modulate(void* x, const void* a, const float* gate, vo
 typedef struct or_linear_args {
   const void* x;            /* bf16 [n_rows, n_in], row stride x_row_stride */
   const void* weight;       /* bf16 [n_out, n_in], row stride weight_row_stride */
-  const float* bias;        /* optional fp32 [n_out] */
-  const float* gate;        /* optional fp32 [n_out], the same for every row */
+  const void* bias;         /* optional fp32 [n_out] (bf16 with bias_bf16) */
+  const void* gate;         /* optional fp32 [n_out] (bf16 with gate_bf16), the same for every row */
   const void* residual;     /* optional bf16 [n_rows, n_out], row stride residual_row_stride; may be y itself */
   void* y;                  /* bf16 [n_rows, n_out], row stride y_row_stride */
   void* preactivation;      /* optional bf16 [n_rows, n_out], contiguous: z, for or_linear_bwd */
@@ -61,6 +61,8 @@ typedef struct or_linear_args {
   int32_t n_in;             /* multiples of 8 up to 2^21 */
   int32_t n_out;
   int32_t activation;       /* OR_ACT_* */
+  int32_t bias_bf16;
+  int32_t gate_bf16;
   void* workspace;          /* device scratch of or_linear_workspace_size() bytes */
   int64_t workspace_bytes;
 } or_linear_args;
@@ -81,7 +83,7 @@ typedef struct or_linear_bwd_args {
   const void* x;             /* the call's x (for dweight) */
   const void* weight;        /* its weight (for dx) */
   const void* preactivation; /* its preactivation, contiguous (for an activation, and for dgate) */
-  const float* gate;         /* its gate or NULL */
+  const void* gate;          /* its gate or NULL */
   void* dx;                  /* bf16 [n_rows, n_in], contiguous */
   void* dweight;             /* bf16 [n_out, n_in], contiguous */
   float* dbias;              /* fp32 [n_out] */
@@ -93,6 +95,7 @@ typedef struct or_linear_bwd_args {
   int32_t n_in;
   int32_t n_out;
   int32_t activation;
+  int32_t gate_bf16;
   void* workspace;           /* device scratch of or_linear_bwd_workspace_size() bytes */
   int64_t workspace_bytes;
 } or_linear_bwd_args;

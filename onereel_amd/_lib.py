@@ -79,19 +79,23 @@ class PackArgs(ctypes.Structure):
 
 # activations of or_linear (OR_ACT_*)
 ACTIVATIONS = {None: 0, 'gelu_tanh': 1, 'silu': 2}
+# the largest row stride of its operands, in elements
+MAX_LINEAR_STRIDE = 1 << 21
 
 
 class LinearArgs(ctypes.Structure):
     _fields_ = [(n, vp) for n in ('x', 'weight', 'bias', 'gate', 'residual', 'y', 'preactivation')] + \
                [(n, i64) for n in ('n_rows', 'x_row_stride', 'weight_row_stride', 'residual_row_stride',
                                    'y_row_stride')] + \
-               [(n, i32) for n in ('n_in', 'n_out', 'activation')] + [('workspace', vp), ('workspace_bytes', i64)]
+               [(n, i32) for n in ('n_in', 'n_out', 'activation', 'bias_bf16', 'gate_bf16')] + \
+               [('workspace', vp), ('workspace_bytes', i64)]
 
 
 class LinearBwdArgs(ctypes.Structure):
     _fields_ = [(n, vp) for n in ('dy', 'x', 'weight', 'preactivation', 'gate', 'dx', 'dweight', 'dbias', 'dgate')] + \
                [(n, i64) for n in ('n_rows', 'dy_row_stride', 'x_row_stride', 'weight_row_stride')] + \
-               [(n, i32) for n in ('n_in', 'n_out', 'activation')] + [('workspace', vp), ('workspace_bytes', i64)]
+               [(n, i32) for n in ('n_in', 'n_out', 'activation', 'gate_bf16')] + \
+               [('workspace', vp), ('workspace_bytes', i64)]
 
 
 # every exported symbol with its ctypes signature: include/onereel_hip.h
@@ -251,6 +255,16 @@ def device_ints(lists, device):
         check(lib().or_index_fill(flat.buffer_info()[0], len(flat), out.data_ptr(), stream_handle(out.device)),
               'or_index_fill')
     return list(out.split([len(values) for values in lists]))
+
+
+def call(device, f, *args):
+    """f(*args, the device's current stream) with the device as the current one. The context manager that sets the device
+    costs more than a launch, so it is entered only for another device than the current one."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        return f(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(device):
+        return f(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def stream_handle(device=None):

@@ -60,13 +60,18 @@ def refuse_captured_leaves(what: str, *xs):
 
 
 def _rows_for(x, H: int, D: int):
-    """x itself where its rows are as the kernels read them, else a copy (a gradient may come expanded or transposed)"""
-    if x.dim() != 3 or tuple(x.shape[1:]) != (H, D):
-        raise _L.HipValueError(f'expected [rows, {H}, {D}], got {tuple(x.shape)}')
-    fits = x.stride(2) == 1 and x.stride(1) == D and x.stride(0) >= H * D and x.stride(0) % 8 == 0
-    if x.shape[0] and not (fits and x.data_ptr() % 16 == 0):
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x, max(x.stride(0), H * D) if x.shape[0] else H * D
+    """(x, row stride), x itself where its rows are as the kernels read them, else a copy (a gradient may come expanded or
+    transposed)"""
+    shape, stride = x.shape, x.stride()    # asked for once, as in scene._rows2d: a small call's time is the host's
+    if len(shape) != 3 or shape[1] != H or shape[2] != D:
+        raise _L.HipValueError(f'expected [rows, {H}, {D}], got {tuple(shape)}')
+    row = stride[0]
+    if stride[2] == 1 and stride[1] == D and row >= H * D and row % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x, row
+    return (x, H * D) if not shape[0] else (x.clone(memory_format=torch.contiguous_format), H * D)
+
+
+_GRAD_SIZES = functools.lru_cache(256)(lambda *sizes: int(_L.lib().or_varlen_bwd_workspace_size(*sizes)))
 
 
 def _backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse=None, k_off=None, k_len=None):
@@ -74,39 +79,35 @@ def _backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse=None, k_off=No
     _scene._check_bf16(do, q, k, v, o)
     if k.dim() != 3 or q.dim() != 3:
         raise _L.HipValueError('q, k and v must be [rows, heads, head_dim]')
-    (n_q, H, D), n_k = q.shape, k.shape[0]
-    if v.shape != k.shape or o.shape != q.shape or do.shape != q.shape or tuple(k.shape[1:]) != (H, D):
-        raise _L.HipValueError(f'q, o and do must have one shape and k and v one with the same [{H}, {D}] rows')
+    (n_q, H, D), n_k, dev, at = q.shape, k.shape[0], q.device, q.get_device()
+    if v.shape[0] != n_k or o.shape[0] != n_q or do.shape[0] != n_q:
+        raise _L.HipValueError('q, o and do must have the same rows, and k and v')
     for x in (lse, dlse):
-        if x is not None and (x.dtype != torch.float32 or tuple(x.shape) != (H, n_q)):
-            raise _L.HipTypeError(f'lse and its gradient must be float32 [{H}, {n_q}]')
+        if x is not None and (x.dtype != torch.float32 or x.shape != (H, n_q) or x.get_device() != at):
+            raise _L.HipTypeError(f'lse and its gradient must be float32 [{H}, {n_q}] on the GPU of q')
     for x in (cu_q, cu_k, k_off, k_len):
-        if x is not None and (x.dtype != torch.int32 or not x.is_cuda or not x.is_contiguous()):
-            raise _L.HipTypeError('index arrays must be contiguous int32 GPU tensors')
-    dev = q.device
-    if any(x is not None and x.device != dev for x in (do, k, v, o, lse, dlse, cu_q, cu_k, k_off, k_len)):
+        if x is not None and (x.dtype != torch.int32 or x.get_device() != at or not x.is_contiguous()):
+            raise _L.HipTypeError('index arrays must be contiguous int32 tensors on the GPU of q')
+    if do.get_device() != at or k.get_device() != at or v.get_device() != at or o.get_device() != at:
         raise _L.HipTypeError('all tensors of a call must be on one GPU')
-    (q, qs), (o, os_), (do, dos) = (_rows_for(x, H, D) for x in (q, o, do))
-    (k, ks), (v, vs) = (_rows_for(x, H, D) for x in (k, v))
+    (q, qs), (o, os_), (do, dos) = _rows_for(q, H, D), _rows_for(o, H, D), _rows_for(do, H, D)
+    (k, ks), (v, vs) = _rows_for(k, H, D), _rows_for(v, H, D)
     if ks != vs:
         (k, ks), v = (k.clone(memory_format=torch.contiguous_format), H * D), v.clone(memory_format=torch.contiguous_format)
     lse = lse.contiguous()
     dlse = None if dlse is None else dlse.contiguous()
-    dq = torch.empty(n_q, H, D, dtype=torch.bfloat16, device=dev)
-    dk, dv = (torch.empty(n_k, H, D, dtype=torch.bfloat16, device=dev) for _ in range(2))
-    a = _L.VarlenBwdArgs()
-    a.q, a.k, a.v, a.o, a.d_o, a.lse, a.dlse = (_L.ptr(x) for x in (q, k, v, o, do, lse, dlse))
-    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    a.cu_q, a.cu_k, a.k_off, a.k_len = (_L.ptr(x) for x in (cu_q, cu_k, k_off, k_len))
-    a.q_row_stride, a.k_row_stride, a.o_row_stride, a.do_row_stride, a.lse_stride = qs, ks, os_, dos, n_q
-    a.n_seg, a.n_q, a.n_k, a.max_q, a.max_k, a.H, a.D = cu_q.numel() - 1, n_q, n_k, int(max_q), int(max_k), H, D
-    a.scale = float(D ** -0.5)
-    n = _L.lib().or_varlen_bwd_workspace_size(a.n_seg, n_q, n_k, a.max_q, a.max_k, H, D)
-    _L.check(min(int(n), 0), 'or_varlen_bwd_workspace_size')
-    ws = torch.empty(int(n), dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    with torch.cuda.device(dev):
-        _L.check(_L.lib().or_varlen_bwd(ctypes.byref(a), _L.stream_handle(dev)), 'or_varlen_bwd')
+    new = lambda n: torch.empty(n, H, D, dtype=torch.bfloat16, device=dev)
+    dq, dk, dv = new(n_q), new(n_k), new(n_k)
+    n_seg, max_q, max_k = cu_q.numel() - 1, int(max_q), int(max_k)
+    n = _GRAD_SIZES(n_seg, n_q, n_k, max_q, max_k, H, D)
+    if n < 0:
+        _L.check(_L.lib().or_varlen_bwd_workspace_size(n_seg, n_q, n_k, max_q, max_k, H, D), 'or_varlen_bwd_workspace_size')
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    p = _L.ptr
+    a = _L.VarlenBwdArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), p(dlse),
+                         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_q.data_ptr(), p(cu_k), p(k_off), p(k_len),
+                         qs, ks, os_, dos, n_q, n_seg, n_q, n_k, max_q, max_k, H, D, D ** -0.5, ws.data_ptr(), n)
+    _L.check(_L.call(dev, _L.lib().or_varlen_bwd, ctypes.byref(a)), 'or_varlen_bwd')
     return dq, dk, dv
 
 

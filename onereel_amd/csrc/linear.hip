@@ -47,12 +47,29 @@ struct Epilogue {
   uint16_t* y;
   int64_t y_stride;
   uint16_t* z;                       // optional: the pre-activation, [rows, cols] contiguous
-  const float* bias;                 // optional [cols]
-  const float* gate;                 // optional [cols]
+  const void* bias;                  // optional [cols], fp32 or bf16
+  const void* gate;                  // optional [cols], fp32 or bf16
+  int bias_bf16, gate_bf16;
   const uint16_t* residual;          // optional
   int64_t residual_stride;
   int act;
 };
+
+// 8 columns of a parameter
+__device__ __forceinline__ void load8(const void* p, int bf16, int col, float (&v)[8]) {
+  if (bf16) {
+    const u32x4 r = *(const u32x4*)((const uint16_t*)p + col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = bf2f((uint16_t)(r[i] & 0xffffu));
+      v[2 * i + 1] = bf2f((uint16_t)(r[i] >> 16));
+    }
+  } else {
+    const f32x4 a = *(const f32x4*)((const float*)p + col), b = *(const f32x4*)((const float*)p + col + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < 4 ? a[i] : b[i - 4];
+  }
+}
 
 __device__ __forceinline__ float act_of(float z, int act) {
   if (act == OR_ACT_SILU) return z / (1.0f + __expf(-z));
@@ -84,19 +101,20 @@ __device__ __forceinline__ void act_grad(float z, int act, float& f, float& d) {
 
 // 8 columns col .. of one row from the fp32 products v
 __device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int col, int cols, float (&v)[8]) {
+  float t[8];
   if (e.bias) {
-    const f32x4 b0 = *(const f32x4*)(e.bias + col), b1 = *(const f32x4*)(e.bias + col + 4);
+    load8(e.bias, e.bias_bf16, col, t);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += i < 4 ? b0[i] : b1[i - 4];
+    for (int i = 0; i < 8; ++i) v[i] += t[i];
   }
   if (e.z) *(u32x4*)(e.z + row * cols + col) = u32x4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
   if (e.act != OR_ACT_NONE)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = act_of(v[i], e.act);
   if (e.gate) {
-    const f32x4 b0 = *(const f32x4*)(e.gate + col), b1 = *(const f32x4*)(e.gate + col + 4);
+    load8(e.gate, e.gate_bf16, col, t);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= i < 4 ? b0[i] : b1[i - 4];
+    for (int i = 0; i < 8; ++i) v[i] *= t[i];
   }
   if (e.residual) {
     const u32x4 r = *(const u32x4*)(e.residual + row * e.residual_stride + col);
@@ -396,7 +414,8 @@ constexpr int kSumRows = 128;
 struct DzArgs {
   const uint16_t *dy, *z;
   int64_t dy_stride;
-  const float* gate;
+  const void* gate;
+  int gate_bf16;
   uint16_t* dz;                      // optional
   float* part;                       // [2][chunks][N]: db, dgate
   float *db, *dgate;                 // optional
@@ -411,7 +430,8 @@ __global__ __launch_bounds__(kThreads) void dz_kernel(DzArgs g) {
   float db[8] = {}, dg[8] = {}, gate[8];
   const bool in = col < g.N;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) gate[i] = in && g.gate ? g.gate[col + i] : 1.0f;
+  for (int i = 0; i < 8; ++i) gate[i] = 1.0f;
+  if (in && g.gate) load8(g.gate, g.gate_bf16, col, gate);
   if (in)
     for (int64_t r = r0 + rr; r < r1; r += 8) {
       const u32x4 y = *(const u32x4*)(g.dy + r * g.dy_stride + col);
@@ -590,8 +610,8 @@ extern "C" int or_linear(const or_linear_args* p, void* stream) {
   g.I = x.n_rows;
   g.J = x.n_out;
   g.K = x.n_in;
-  g.e = Epilogue{(uint16_t*)x.y, x.y_row_stride, (uint16_t*)x.preactivation, x.bias, x.gate, (const uint16_t*)x.residual,
-                 x.residual_row_stride, x.activation};
+  g.e = Epilogue{(uint16_t*)x.y, x.y_row_stride, (uint16_t*)x.preactivation, x.bias, x.gate, x.bias_bf16, x.gate_bf16,
+                 (const uint16_t*)x.residual, x.residual_row_stride, x.activation};
   launch_product(g, false, false, (float*)x.workspace, (hipStream_t)stream);
   return check_hip(hipGetLastError(), "or_linear launch");
 }
@@ -633,6 +653,7 @@ extern "C" int or_linear_bwd(const or_linear_bwd_args* p, void* stream) {
     d.dy_stride = x.dy_row_stride;
     d.z = x.activation != OR_ACT_NONE || x.dgate ? (const uint16_t*)x.preactivation : nullptr;
     d.gate = x.gate;
+    d.gate_bf16 = x.gate_bf16;
     d.dz = scaled && products ? (uint16_t*)(ws + l.dz) : nullptr;
     d.part = (float*)(ws + l.sums);
     d.db = x.dbias;

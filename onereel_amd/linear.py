@@ -8,6 +8,7 @@ plain call. bf16 in and out, fp32 inside. Errors raise `onereel_amd._lib.HipPath
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -26,30 +27,44 @@ def _rows(t, width: int, what: str):
     rows are not such, e.g. an expanded gradient)"""
     if t.dtype != torch.bfloat16 or not t.is_cuda:
         raise L.HipTypeError(f'{what} must be a bf16 GPU tensor, got {t.dtype} on {t.device}')
-    if t.dim() < 1 or t.shape[-1] != width:
-        raise L.HipValueError(f'{what} must have rows of {width} elements, got {tuple(t.shape)}')
-    t = t.reshape(-1, width)
-    if t.shape[0] and not (t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= width and t.stride(0) % 8 == 0) and
-                           t.data_ptr() % 16 == 0):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride(0) if t.shape[0] > 1 else width
+    shape = t.shape
+    if not shape or shape[-1] != width:
+        raise L.HipValueError(f'{what} must have rows of {width} elements, got {tuple(shape)}')
+    if len(shape) != 2:
+        t = t.reshape(-1, width)
+    row, one = t.stride()
+    if one == 1 and row >= width and row % 8 == 0 and row <= L.MAX_LINEAR_STRIDE and t.data_ptr() % 16 == 0:
+        return t, row
+    return (t, width) if not t.shape[0] else (t.clone(memory_format=torch.contiguous_format), width)
 
 
 def _vector(t, n: int, what: str):
-    """a parameter of n columns as contiguous fp32 at a 16-byte aligned address"""
+    """(a parameter of n columns, contiguous at a 16-byte aligned address, whether it is bf16)"""
     if t is None:
-        return None
+        return None, 0
     if t.dtype not in (torch.bfloat16, torch.float32) or not t.is_cuda:
         raise L.HipTypeError(f'{what} must be a bf16 or fp32 GPU tensor, got {t.dtype} on {t.device}')
     if t.numel() != n:
         raise L.HipValueError(f'{what} must hold {n} elements, got {tuple(t.shape)}')
-    v = t.reshape(n).to(torch.float32).contiguous()
-    return v if v.data_ptr() % 16 == 0 else v.clone()
+    v = t if t.is_contiguous() else t.reshape(n).contiguous()
+    return v if v.data_ptr() % 16 == 0 else v.clone(), int(t.dtype == torch.bfloat16)
 
 
 def _on_one_gpu(x, *others):
-    if any(t is not None and t.device != x.device for t in others):
-        raise L.HipTypeError('all tensors of a call must be on one GPU')
+    at = x.get_device()
+    for t in others:
+        if t is not None and t.get_device() != at:
+            raise L.HipTypeError('all tensors of a call must be on one GPU')
+
+
+_SIZES = functools.lru_cache(256)(lambda name, *sizes: int(getattr(L.dit_lib(), name)(*sizes)))
+
+
+def _workspace(device, name, *sizes):
+    n = _SIZES(name, *sizes)
+    if n < 0:
+        L.dit_check(getattr(L.dit_lib(), name)(*sizes), name)
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _sizes(x, weight):
@@ -70,20 +85,14 @@ def _forward(x, weight, bias, act: int, gate, residual, keep: bool):
     x2, xs = _rows(x, n_in, 'x')
     w, ws = _rows(weight, n_in, 'weight')
     r, rs = (None, 0) if residual is None else _rows(residual, n_out, 'residual')
-    b, g = _vector(bias, n_out, 'bias'), _vector(gate, n_out, 'gate')
-    M, d = x2.shape[0], L.dit_lib()
-    y = torch.empty(M, n_out, dtype=torch.bfloat16, device=x.device)
+    (b, b16), (g, g16) = _vector(bias, n_out, 'bias'), _vector(gate, n_out, 'gate')
+    M, dev, p = x2.shape[0], x.device, L.ptr
+    y = torch.empty(M, n_out, dtype=torch.bfloat16, device=dev)
     z = torch.empty_like(y) if keep else None
-    n = d.or_linear_workspace_size(M, n_in, n_out)
-    L.dit_check(min(int(n), 0), 'or_linear_workspace_size')
-    space = torch.empty(int(n), dtype=torch.uint8, device=x.device)
-    a = L.LinearArgs()
-    a.x, a.weight, a.bias, a.gate, a.residual, a.y, a.preactivation = (L.ptr(t) for t in (x2, w, b, g, r, y, z))
-    a.n_rows, a.x_row_stride, a.weight_row_stride, a.residual_row_stride, a.y_row_stride = M, xs, ws, rs, n_out
-    a.n_in, a.n_out, a.activation = n_in, n_out, act
-    a.workspace, a.workspace_bytes = space.data_ptr(), space.numel()
-    with torch.cuda.device(x.device):
-        L.dit_check(d.or_linear(ctypes.byref(a), L.stream_handle(x.device)), 'or_linear')
+    space = _workspace(dev, 'or_linear_workspace_size', M, n_in, n_out)
+    a = L.LinearArgs(x2.data_ptr(), w.data_ptr(), p(b), p(g), p(r), y.data_ptr(), p(z), M, xs, ws, rs, n_out, n_in, n_out,
+                     act, b16, g16, space.data_ptr(), space.numel())
+    L.dit_check(L.call(dev, L.dit_lib().or_linear, ctypes.byref(a)), 'or_linear')
     return y.view(shape), None if z is None else z.view(shape)
 
 
@@ -124,23 +133,15 @@ def linear_backward(dy, x, weight, bias: bool = False, activation=None, gate=Non
             raise L.HipValueError(f'the pre-activation must be {tuple(dy.shape)}, got {tuple(preactivation.shape)}')
         z, zs = _rows(preactivation, n_out, 'preactivation')
         z = z if zs == n_out else z.contiguous()
-    g = _vector(gate, n_out, 'gate')
-    M, d, dev = x2.shape[0], L.dit_lib(), x.device
-    dx = torch.empty(M, n_in, dtype=torch.bfloat16, device=dev) if needs[0] else None
-    dw = torch.empty(n_out, n_in, dtype=torch.bfloat16, device=dev) if needs[1] else None
-    db = torch.empty(n_out, dtype=torch.float32, device=dev) if bias else None
-    dg = torch.empty(n_out, dtype=torch.float32, device=dev) if gate is not None else None
-    n = d.or_linear_bwd_workspace_size(M, n_in, n_out, int(bool(act) or g is not None))
-    L.dit_check(min(int(n), 0), 'or_linear_bwd_workspace_size')
-    space = torch.empty(int(n), dtype=torch.uint8, device=dev)
-    a = L.LinearBwdArgs()
-    a.dy, a.x, a.weight, a.preactivation, a.gate = (L.ptr(t) for t in (dy2, x2, w, z, g))
-    a.dx, a.dweight, a.dbias, a.dgate = (L.ptr(t) for t in (dx, dw, db, dg))
-    a.n_rows, a.dy_row_stride, a.x_row_stride, a.weight_row_stride = M, ds, xs, ws
-    a.n_in, a.n_out, a.activation = n_in, n_out, act
-    a.workspace, a.workspace_bytes = space.data_ptr(), space.numel()
-    with torch.cuda.device(dev):
-        L.dit_check(d.or_linear_bwd(ctypes.byref(a), L.stream_handle(dev)), 'or_linear_bwd')
+    g, g16 = _vector(gate, n_out, 'gate')
+    M, dev, p = x2.shape[0], x.device, L.ptr
+    new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=dev)
+    dx, dw = new(torch.bfloat16, M, n_in) if needs[0] else None, new(torch.bfloat16, n_out, n_in) if needs[1] else None
+    db, dg = new(torch.float32, n_out) if bias else None, new(torch.float32, n_out) if gate is not None else None
+    space = _workspace(dev, 'or_linear_bwd_workspace_size', M, n_in, n_out, int(act != 0 or g is not None))
+    a = L.LinearBwdArgs(dy2.data_ptr(), x2.data_ptr(), w.data_ptr(), p(z), p(g), p(dx), p(dw), p(db), p(dg), M, ds, xs, ws,
+                        n_in, n_out, act, g16, space.data_ptr(), space.numel())
+    L.dit_check(L.call(dev, L.dit_lib().or_linear_bwd, ctypes.byref(a)), 'or_linear_bwd')
     return None if dx is None else dx.view(x.shape), dw, db, dg
 
 

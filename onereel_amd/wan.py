@@ -105,42 +105,47 @@ def rms_norm(x, weight, eps: float):
 
 
 def _grad_rows(x, C: int):
-    """x as [rows, C] bf16 rows that the gradient kernel reads: contiguous elements, whole 16-byte pieces (a copy where x
-    is not such rows, e.g. an expanded gradient)"""
+    """x as ([rows, C] bf16 rows that the gradient kernel reads, their stride): contiguous elements, whole 16-byte pieces (a
+    copy where x is not such rows, e.g. an expanded gradient)"""
     if x.dtype != torch.bfloat16 or not x.is_cuda:
         raise L.HipTypeError(f'expected a bf16 GPU tensor, got {x.dtype} on {x.device}')
-    x2 = x.reshape(-1, C)
-    if x2.shape[0] and not (x2.stride(1) == 1 and x2.stride(0) >= C and x2.stride(0) % 8 == 0 and x2.data_ptr() % 16 == 0):
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    return x2, max(x2.stride(0), C) if x2.shape[0] else C
+    x = x.reshape(-1, C)
+    row, one = x.stride()
+    if one == 1 and row >= C and row % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x, row
+    return (x, C) if not x.shape[0] else (x.clone(memory_format=torch.contiguous_format), C)
+
+
+def _weight(w, C: int):
+    if w.numel() != C:
+        raise L.HipValueError(f'weights must hold {C} elements, got {tuple(w.shape)}')
+    w = w.reshape(C).to(torch.bfloat16).contiguous()
+    return w if w.data_ptr() % 16 == 0 else w.clone()
 
 
 def _norm_backward(dys, xs, ws, eps, C: int, D: int, cos=None, sin=None):
     """or_rmsnorm_rope_bwd of one or two tensors: ([dx, ..] [rows, C] bf16, [dw, ..] [C] fp32)"""
-    dev = xs[0].device
-    if any(t.device != dev for t in (*dys, *xs, *ws)) or (cos is not None and (cos.device != dev or sin.device != dev)):
-        raise L.HipTypeError('all tensors of a call must be on one GPU')
-    (dys, dss), (xs, xss) = (zip(*(_grad_rows(t, C) for t in ts)) for ts in (dys, xs))
-    S = xs[0].shape[0]
-    if any(t.shape[0] != S for t in (*dys, *xs)):
+    at, dev = xs[0].get_device(), xs[0].device
+    for t in (*dys, *xs, *ws, *(() if cos is None else (cos, sin))):
+        if t.get_device() != at:
+            raise L.HipTypeError('all tensors of a call must be on one GPU')
+    both = len(xs) == 2
+    (x0, xs0), (d0, ds0), w0 = _grad_rows(xs[0], C), _grad_rows(dys[0], C), _weight(ws[0], C)
+    (x1, xs1), (d1, ds1), w1 = (_grad_rows(xs[1], C), _grad_rows(dys[1], C), _weight(ws[1], C)) if both else \
+        ((None, 0), (None, 0), None)
+    S = x0.shape[0]
+    if d0.shape[0] != S or both and (x1.shape[0] != S or d1.shape[0] != S):
         raise L.HipValueError('gradients and inputs must have the same rows')
-    if any(w.numel() != C for w in ws):
-        raise L.HipValueError(f'weights must hold {C} elements')
-    ws = [w.reshape(C).to(torch.bfloat16).contiguous() for w in ws]
-    ws = [w if w.data_ptr() % 16 == 0 else w.clone() for w in ws]
-    dx = [torch.empty(S, C, dtype=torch.bfloat16, device=dev) for _ in xs]
-    dw = [torch.empty(C, dtype=torch.float32, device=dev) for _ in xs]
-    n = L.lib().or_rmsnorm_rope_bwd_workspace_size(S, C)
-    L.check(min(int(n), 0), 'or_rmsnorm_rope_bwd_workspace_size')
-    space = torch.empty(int(n), dtype=torch.uint8, device=dev)
-    two = lambda ts, none=None: [t.data_ptr() for t in ts] + [none] * (2 - len(ts))
-    dss, xss = ([*t, *(0,) * (2 - len(t))] for t in (dss, xss))
-    with torch.cuda.device(dev):
-        L.check(L.lib().or_rmsnorm_rope_bwd(*two(dys), *two(xs), *two(ws), *dss, *xss, S, C, D, float(eps), L.ptr(cos),
-                                            L.ptr(sin), None, S if cos is not None else 0, *two(dx), *two(dw),
-                                            space.data_ptr(), space.numel(), L.stream_handle(dev)),
-                'or_rmsnorm_rope_bwd')
-    return dx, dw
+    new = lambda: (torch.empty(S, C, dtype=torch.bfloat16, device=dev), torch.empty(C, dtype=torch.float32, device=dev))
+    (dx0, dw0), (dx1, dw1) = new(), new() if both else (None, None)
+    n = int(L.lib().or_rmsnorm_rope_bwd_workspace_size(S, C))
+    L.check(min(n, 0), 'or_rmsnorm_rope_bwd_workspace_size')
+    space = torch.empty(n, dtype=torch.uint8, device=dev)
+    p = L.ptr
+    L.check(L.call(dev, L.lib().or_rmsnorm_rope_bwd, d0.data_ptr(), p(d1), x0.data_ptr(), p(x1), w0.data_ptr(), p(w1), ds0,
+                   ds1, xs0, xs1, S, C, D, float(eps), p(cos), p(sin), None, S if cos is not None else 0,
+                   dx0.data_ptr(), p(dx1), dw0.data_ptr(), p(dw1), space.data_ptr(), n), 'or_rmsnorm_rope_bwd')
+    return ([dx0, dx1], [dw0, dw1]) if both else ([dx0], [dw0])
 
 
 def qk_backward(dq, dk, q, k, wq, wk, eps: float, cos, sin, heads: int):
