@@ -8,7 +8,7 @@
 // of 5 products would have to add dq into memory from every key tile, with atomics whose order changes the bits; the
 // two passes sum every gradient in registers in a fixed order, so a call gives the same bits every time.
 //
-// - A wavefront owns 32 T rows (T = 1 or 2 blocks of 32 queries, or keys) of its work-group's tile and keeps their
+// - A wavefront owns 32 rows (keys, or queries; 64 queries with heads of 64) of its work-group's tile and keeps their
 //   operands and their fp32 gradient in registers; the rows of the other side stream past in blocks of 32 through a ring of
 //   LDS slots filled by LDS DMA, three blocks ahead.
 // - Both products of scores put the streamed rows on the MFMA rows and the owned rows on its columns, so a lane holds
@@ -68,6 +68,12 @@ struct BwdArgs {
   float* part_q;                     // [split_q][n_q][H][D]
   float* part_k;                     // [split_k][2][n_k][H][D]: dk, then dv
 };
+
+// rows of a query tile. 32 queries a wavefront leave room for two wavefronts on a SIMD, one's exponentials under the
+// other's matrix work: 3 x 9680 queries x 11440 keys, 16 heads of 128, dq 3.41 ms against 3.88 with 64 (one wavefront); dk
+// and dv 4.80 against 5.36 ms with 32 and 64 keys. With heads of 64, 64 queries fit twice too and halve the LDS reads per
+// query: 2 x 3001 x 3001 131 us against 138 (dk and dv with 64 keys do not fit twice: 239 against 198 us).
+constexpr int query_tile(int D) { return D == 128 ? 128 : 256; }
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 // a value that is the same in every lane, in a scalar register
@@ -260,38 +266,33 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// read addresses of a lane inside a slot
+// Read addresses of a lane inside a slot: one register each, all others an XOR (and an immediate) away, since the dims of
+// a step and the 4 rows of a transposing read are chunk bits that the swizzle only XORs.
 template <int D>
 struct Lds {
-  uint32_t row[Str<D>::KS];        // 8 dims 16 ks + 8 (lane / 32) .. of row lane % 32
-  uint32_t tr[Str<D>::DB][2];      // transposing: dims 32 db + .., rows 4 (lane / 32) + 8 t + (0 .. 3)
+  uint32_t row;                    // dims 8 (lane / 32) .. of row lane % 32; step ks: ^ 32 ks
+  uint32_t tr;                     // transposing: dims 0 .., rows 4 (lane / 32) + (0 .. 3); block db: ^ 64 db, rows + 8: + 8 rows, ^ 32
   __device__ __forceinline__ void init(int lane) {
-    const int l32 = lane & 31, h = lane >> 5, r = lane & 15, g = (lane >> 4) & 1;
-#pragma unroll
-    for (int ks = 0; ks < Str<D>::KS; ++ks) row[ks] = l32 * D * 2 + ((2 * ks + h) ^ swz<D>(l32)) * 16;
-#pragma unroll
-    for (int db = 0; db < Str<D>::DB; ++db)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int rr = 4 * h + 8 * t + (r >> 2);
-        tr[db][t] = rr * D * 2 + ((4 * db + 2 * g + ((r >> 1) & 1)) ^ swz<D>(rr)) * 16 + (r & 1) * 8;
-      }
+    const int l32 = lane & 31, h = lane >> 5, r = lane & 15, g = (lane >> 4) & 1, rr = 4 * h + (r >> 2);
+    row = l32 * D * 2 + (h ^ swz<D>(l32)) * 16;
+    tr = rr * D * 2 + ((2 * g + ((r >> 1) & 1)) ^ swz<D>(rr)) * 16 + (r & 1) * 8;
   }
 };
 
+// `row` and `tr` here are the slot's address plus Lds::row and Lds::tr; `off` an offset of another slot at the same place
 template <int D>
-__device__ __forceinline__ bf16x8 row_frag(uint32_t slot, const Lds<D>& ad, int ks) {
-  return *(const __attribute__((address_space(3))) bf16x8*)(uintptr_t)(slot + ad.row[ks]);
+__device__ __forceinline__ bf16x8 row_frag(uint32_t row, int ks, uint32_t off) {
+  return *(const __attribute__((address_space(3))) bf16x8*)(uintptr_t)((row ^ (32 * ks)) + off);
 }
 
 // dims 32 db + lane % 32 of the 8 rows that a lane's scores of step hs belong to: 16 hs + 4 (lane / 32) + {0..3, 8..11}
 template <int D>
-__device__ __forceinline__ bf16x8 tr_frag(uint32_t slot, const Lds<D>& ad, int db, int hs) {
+__device__ __forceinline__ bf16x8 tr_frag(uint32_t tr, int db, int hs, uint32_t off) {
   u32x2 x[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t)
     x[t] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-                                         (lds_bf16x4*)(uintptr_t)(slot + ad.tr[db][t] + 16 * hs * D * 2)));
+                                         (lds_bf16x4*)(uintptr_t)((tr ^ (64 * db + 32 * t)) + (16 * hs + 8 * t) * D * 2 + off)));
   const u32x4 y = {x[0][0], x[0][1], x[1][0], x[1][1]};
   return __builtin_bit_cast(bf16x8, y);
 }
@@ -353,7 +354,7 @@ __device__ __forceinline__ int64_t xcd_item(int64_t n) {
 // ------------------------------------------------------------------------------------------------------------------
 // dq: a block owns 128 T queries of one head and streams the keys and values of their segment
 template <int D, int T>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void bwd_q_kernel(BwdArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void bwd_q_kernel(BwdArgs a) {
   using C = Str<D>;
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT];
   const int n_tiles = uni(a.head[0]);
@@ -434,17 +435,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))
   for (int b = b0; b < b1; ++b) {
     wait_loads_barrier<(kRing - 2) * 2 * C::LPB>();
     fetch(b + kRing - 1);
-    const uint32_t ks_ = lds + (b & (kRing - 1)) * C::SLOT, vs_ = ks_ + kRing * C::SLOT;
+    const uint32_t slot = lds + (b & (kRing - 1)) * C::SLOT, row = slot + ad.row, tr = slot + ad.tr;
     f32x16 s[T], dp[T];
 #pragma unroll
     for (int ks = 0; ks < C::KS; ++ks) {
-      const bf16x8 kf = row_frag<D>(ks_, ad, ks);
+      const bf16x8 kf = row_frag<D>(row, ks, 0), vf = row_frag<D>(row, ks, kRing * C::SLOT);
 #pragma unroll
       for (int t = 0; t < T; ++t) s[t] = mfma(kf, qf[t][ks], ks ? s[t] : zero);
-    }
-#pragma unroll
-    for (int ks = 0; ks < C::KS; ++ks) {
-      const bf16x8 vf = row_frag<D>(vs_, ad, ks);
 #pragma unroll
       for (int t = 0; t < T; ++t) dp[t] = mfma(vf, df[t][ks], ks ? dp[t] : zero);
     }
@@ -471,7 +468,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))
     for (int db = 0; db < C::DB; ++db)
 #pragma unroll
       for (int hs = 0; hs < 2; ++hs) {
-        const bf16x8 kt = tr_frag<D>(ks_, ad, db, hs);
+        const bf16x8 kt = tr_frag<D>(tr, db, hs, 0);
 #pragma unroll
         for (int t = 0; t < T; ++t) acc[t][db] = mfma(kt, ds[t][hs], acc[t][db]);
       }
@@ -487,7 +484,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// dk, dv: a block owns 128 T keys of one head and streams the queries of every segment that reads them
+// dk, dv: a block owns 128 keys of one head and streams the queries of every segment that reads them
 
 // walks the blocks of 32 queries of the segments that cover a key tile
 struct Walk {
@@ -510,8 +507,8 @@ struct Walk {
   }
 };
 
-template <int D, int T>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void bwd_kv_kernel(BwdArgs a) {
+template <int D>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))) void bwd_kv_kernel(BwdArgs a) {
   using C = Str<D>;
   constexpr int kStat = 256;         // bytes of one wavefront's statistics of a block
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT + kRing * 4 * kStat];
@@ -522,8 +519,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))
   const int part = (int)(item % a.split_k);
   const int head = (int)(item / a.split_k / n_tiles);
   const i32x4 tile = uni(a.k_tiles[item / a.split_k % n_tiles]);
-  const int row0 = tile[0] + w * 32 * T;
-  const int rows = clampi(tile[1] - w * 32 * T, 0, 32 * T);
+  const int row0 = tile[0] + w * 32;
+  const int rows = clampi(tile[1] - w * 32, 0, 32);
 
   uint32_t voq[C::LPB], vod[C::LPB];
 #pragma unroll
@@ -561,19 +558,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))
     wk.left -= kBlk;
   };
 
-  bf16x8 kf[T][C::KS], vf[T][C::KS];
-  f32x16 dk[T][C::DB], dv[T][C::DB];
+  bf16x8 kf[C::KS], vf[C::KS];
+  f32x16 dk[C::DB], dv[C::DB];
+  const int64_t own = (int64_t)row0 * a.ks + (int64_t)head * D;
+  load_owned<D>(kf, a.k + own, a.ks, rows, lane);
+  load_owned<D>(vf, a.v + own, a.ks, rows, lane);
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int n = clampi(rows - 32 * t, 0, 32);
-    const int64_t at = (int64_t)(row0 + 32 * t) * a.ks + (int64_t)head * D;
-    load_owned<D>(kf[t], a.k + at, a.ks, n, lane);
-    load_owned<D>(vf[t], a.v + at, a.ks, n, lane);
+  for (int db = 0; db < C::DB; ++db)
 #pragma unroll
-    for (int db = 0; db < C::DB; ++db)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) dk[t][db][e] = dv[t][db][e] = 0.0f;
-  }
+    for (int e = 0; e < 16; ++e) dk[db][e] = dv[db][e] = 0.0f;
 
   Lds<D> ad;
   ad.init(lane);
@@ -585,7 +578,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))
     wait_loads_barrier<(kRing - 2) * (2 * C::LPB + 1)>();
     fetch(b + kRing - 1);
     const int slot = b & (kRing - 1);
-    const uint32_t qs_ = lds + slot * C::SLOT, ds_ = qs_ + kRing * C::SLOT, st = st0 + slot * 4 * kStat;
+    const uint32_t row = lds + slot * C::SLOT + ad.row, tr = lds + slot * C::SLOT + ad.tr, st = st0 + slot * 4 * kStat;
     // -lse / scale and -delta start the sums of the scores and of do v^T: rows 8 g + 4 (lane / 32) ..
     f32x16 s0, d0;
 #pragma unroll
@@ -598,63 +591,34 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 2))
         d0[4 * g + i] = y[i];
       }
     }
-    f32x16 s[T], dp[T];
+    f32x16 s, dp;
 #pragma unroll
     for (int ks = 0; ks < C::KS; ++ks) {
-      const bf16x8 qf = row_frag<D>(qs_, ad, ks);
-#pragma unroll
-      for (int t = 0; t < T; ++t) s[t] = mfma(qf, kf[t][ks], ks ? s[t] : s0);
+      s = mfma(row_frag<D>(row, ks, 0), kf[ks], ks ? s : s0);
+      dp = mfma(row_frag<D>(row, ks, kRing * C::SLOT), vf[ks], ks ? dp : d0);
     }
 #pragma unroll
-    for (int ks = 0; ks < C::KS; ++ks) {
-      const bf16x8 df = row_frag<D>(ds_, ad, ks);
-#pragma unroll
-      for (int t = 0; t < T; ++t) dp[t] = mfma(df, vf[t][ks], ks ? dp[t] : d0);
+    for (int e = 0; e < 16; ++e) {
+      s[e] = __builtin_amdgcn_exp2f(s[e] * c);
+      dp[e] *= s[e];
     }
-    bf16x8 p[T][2], ds[T][2];
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[t][e] = __builtin_amdgcn_exp2f(s[t][e] * c);
-#pragma unroll
-      for (int hs = 0; hs < 2; ++hs) p[t][hs] = pack8(s[t], hs);
-    }
+    const bf16x8 p[2] = {pack8(s, 0), pack8(s, 1)}, ds[2] = {pack8(dp, 0), pack8(dp, 1)};
 #pragma unroll
     for (int db = 0; db < C::DB; ++db)
 #pragma unroll
       for (int hs = 0; hs < 2; ++hs) {
-        const bf16x8 dt = tr_frag<D>(ds_, ad, db, hs);
-#pragma unroll
-        for (int t = 0; t < T; ++t) dv[t][db] = mfma(dt, p[t][hs], dv[t][db]);
-      }
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) dp[t][e] *= s[t][e];
-#pragma unroll
-      for (int hs = 0; hs < 2; ++hs) ds[t][hs] = pack8(dp[t], hs);
-    }
-#pragma unroll
-    for (int db = 0; db < C::DB; ++db)
-#pragma unroll
-      for (int hs = 0; hs < 2; ++hs) {
-        const bf16x8 qt = tr_frag<D>(qs_, ad, db, hs);
-#pragma unroll
-        for (int t = 0; t < T; ++t) dk[t][db] = mfma(qt, ds[t][hs], dk[t][db]);
+        dv[db] = mfma(tr_frag<D>(tr, db, hs, kRing * C::SLOT), p[hs], dv[db]);
+        dk[db] = mfma(tr_frag<D>(tr, db, hs, 0), ds[hs], dk[db]);
       }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no DMA into LDS of a block that has ended
-#pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int n = clampi(rows - 32 * t, 0, 32);
-    const int64_t at = ((int64_t)(row0 + 32 * t) * a.H + head) * D, rs = (int64_t)a.H * D, all = a.n_k * rs;
-    if (a.split_k == 1) {
-      store_bf16<D>(a.dk + at, rs, dk[t], a.scale, n, lane);
-      store_bf16<D>(a.dv + at, rs, dv[t], 1.0f, n, lane);
-    } else {
-      store_f32<D>(a.part_k + 2 * part * all + at, rs, dk[t], a.scale, n, lane);
-      store_f32<D>(a.part_k + (2 * part + 1) * all + at, rs, dv[t], 1.0f, n, lane);
-    }
+  const int64_t at = ((int64_t)row0 * a.H + head) * D, rs = (int64_t)a.H * D, all = a.n_k * rs;
+  if (a.split_k == 1) {
+    store_bf16<D>(a.dk + at, rs, dk, a.scale, rows, lane);
+    store_bf16<D>(a.dv + at, rs, dv, 1.0f, rows, lane);
+  } else {
+    store_f32<D>(a.part_k + 2 * part * all + at, rs, dk, a.scale, rows, lane);
+    store_f32<D>(a.part_k + (2 * part + 1) * all + at, rs, dv, 1.0f, rows, lane);
   }
 }
 
@@ -685,20 +649,23 @@ struct Shape {
   int split_q, split_k;
 };
 
-// parts of a streamed axis: enough for two rounds of blocks on 256 CUs, none shorter than four blocks of rows
+// Parts of a streamed axis: as many as keep every block of the call resident at once (256 CUs, two blocks each), none
+// shorter than 8 blocks of rows. The partial gradients cost more than uneven rounds do, so calls with half that many
+// items or more are not split: 12 sequences of up to 699 x 899 rows, 16 heads (336 items), dk and dv in 2 parts take 59 us
+// and 27 us to add, in one 53 us; 128 keys against 3 x 9680 queries (48 items) in one part 488 us, in 8 104 us and 8 to add.
 int split_of(int64_t items, int64_t streamed) {
-  const int64_t want = (512 + items - 1) / std::max<int64_t>(items, 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, streamed / (4 * kBlk), kMaxSplit}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(items, 1), streamed / (8 * kBlk), kMaxSplit}));
 }
 
-Shape shape_of(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H) {
+Shape shape_of(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H, int32_t D) {
   Shape s;
-  s.tq = max_q <= 128 ? 128 : 256;
-  s.tk = max_k <= 128 ? 128 : 256;
+  s.tq = query_tile(D);
+  s.tk = 128;
   s.max_q_tiles = n_q / s.tq + n_seg + 1;
   s.max_k_tiles = n_k / s.tk + 2 * (int64_t)n_seg + 1;
-  s.split_q = split_of((int64_t)H * ((n_q + s.tq - 1) / s.tq), max_k);
-  s.split_k = split_of((int64_t)H * ((n_k + s.tk - 1) / s.tk), max_q);
+  // a segment ends in a half-filled tile on average
+  s.split_q = split_of(H * ((n_q + s.tq - 1) / s.tq + n_seg / 2), max_k);
+  s.split_k = split_of(H * ((n_k + s.tk - 1) / s.tk + n_seg / 2), max_q);
   return s;
 }
 
@@ -728,14 +695,8 @@ template <int D>
 void launch(const BwdArgs& a, const Shape& s, hipStream_t st) {
   auto grid = [](int64_t items) { return dim3((unsigned)((items + 7) / 8 * 8)); };
   const dim3 gq = grid(s.max_q_tiles * a.H * s.split_q), gk = grid(s.max_k_tiles * a.H * s.split_k);
-  if (a.n_q > 0) {
-    if (s.tq == 128) hipLaunchKernelGGL((bwd_q_kernel<D, 1>), gq, dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL((bwd_q_kernel<D, 2>), gq, dim3(kThreads), 0, st, a);
-  }
-  if (a.n_k > 0) {
-    if (s.tk == 128) hipLaunchKernelGGL((bwd_kv_kernel<D, 1>), gk, dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL((bwd_kv_kernel<D, 2>), gk, dim3(kThreads), 0, st, a);
-  }
+  if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, query_tile(D) / 128>), gq, dim3(kThreads), 0, st, a);
+  if (a.n_k > 0) hipLaunchKernelGGL((bwd_kv_kernel<D>), gk, dim3(kThreads), 0, st, a);
 }
 
 }  // namespace
@@ -749,7 +710,7 @@ extern "C" int64_t or_varlen_bwd_workspace_size(int32_t n_seg, int32_t n_q, int3
       (D != 64 && D != 128))
     return fail_arg("or_varlen_bwd_workspace_size: 1 to %d segments, 1 to 256 heads of 64 or 128 and sizes of at least 0 are "
                     "needed", kMaxSeg);
-  return layout_of(shape_of(n_seg, n_q, n_k, max_q, max_k, H), n_q, n_k, H, D).bytes;
+  return layout_of(shape_of(n_seg, n_q, n_k, max_q, max_k, H, D), n_q, n_k, H, D).bytes;
 }
 
 extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
@@ -775,7 +736,7 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
       !aligned16(x.dk) || !aligned16(x.dv))
     return fail_arg("or_varlen_bwd: pointers must be 16-byte aligned");
   if (x.lse_stride < x.n_q) return fail_arg("or_varlen_bwd: lse_stride must cover the query rows");
-  const Shape s = shape_of(x.n_seg, x.n_q, x.n_k, x.max_q, x.max_k, x.H);
+  const Shape s = shape_of(x.n_seg, x.n_q, x.n_k, x.max_q, x.max_k, x.H, x.D);
   const Layout l = layout_of(s, x.n_q, x.n_k, x.H, x.D);
   if (!x.workspace || x.workspace_bytes < l.bytes || !aligned16(x.workspace))
     return fail_arg("or_varlen_bwd: a 16-byte aligned workspace of %lld bytes is needed", (long long)l.bytes);

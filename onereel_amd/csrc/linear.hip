@@ -408,9 +408,9 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(GemmArgs g) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// dz = dy * gate * act'(z) and the sums over rows db = sum dz, dgate = sum dy * act(z): 256 columns x kSumRows rows a
-// work-group, 8 columns a lane; the work-groups' partial sums are added up in order by a second launch
-constexpr int kSumRows = 128;
+// dz = dy * gate * act'(z) and the sums over rows db = sum dz, dgate = sum dy * act(z): 256 columns x 8 to 128 rows a
+// work-group, 8 columns a lane; the work-groups' partial sums are added up in order by a second launch. HBM-bound with
+// many rows; with few of them by the latency of a work-group's rows, so they are dealt to 1024 work-groups or more
 struct DzArgs {
   const uint16_t *dy, *z;
   int64_t dy_stride;
@@ -420,13 +420,13 @@ struct DzArgs {
   float* part;                       // [2][chunks][N]: db, dgate
   float *db, *dgate;                 // optional
   int64_t M;
-  int N, act, chunks;
+  int N, act, chunks, chunk_rows;
 };
 
 __global__ __launch_bounds__(kThreads) void dz_kernel(DzArgs g) {
   __shared__ float sum[2][8][256];
   const int c = threadIdx.x & 31, rr = threadIdx.x >> 5, col = blockIdx.x * 256 + c * 8;
-  const int64_t r0 = (int64_t)blockIdx.y * kSumRows, r1 = min(r0 + kSumRows, g.M);
+  const int64_t r0 = (int64_t)blockIdx.y * g.chunk_rows, r1 = min(r0 + g.chunk_rows, g.M);
   float db[8] = {}, dg[8] = {}, gate[8];
   const bool in = col < g.N;
 #pragma unroll
@@ -564,6 +564,13 @@ int bad_stride(const char* what, int64_t stride, int64_t width) {
   return 0;
 }
 
+// rows of a work-group of dz_kernel: a multiple of the 8 it takes at once
+int chunk_rows_of(int64_t M, int32_t N) {
+  const int64_t chunks = (1024 + (N + 255) / 256 - 1) / ((N + 255) / 256);
+  const int64_t rows = ((M + chunks - 1) / chunks + 7) / 8 * 8;
+  return (int)std::max<int64_t>(8, std::min<int64_t>(rows, 128));
+}
+
 struct BwdLayout {
   int64_t dz, sums, part, bytes;
 };
@@ -571,7 +578,8 @@ BwdLayout bwd_layout(int64_t M, int32_t N, int32_t K, bool makes_dz) {
   BwdLayout l;
   l.dz = 0;
   l.sums = makes_dz ? round256(M * N * 2) : 0;
-  const int64_t chunks = (M + kSumRows - 1) / kSumRows;
+  const int rows = chunk_rows_of(M, N);
+  const int64_t chunks = (M + rows - 1) / rows;
   l.part = l.sums + round256(2 * chunks * N * 4);
   l.bytes = l.part + round256(std::max(plan_of(M, K, N, false).part_bytes, plan_of(N, K, M, false).part_bytes)) + 256;
   return l;
@@ -661,8 +669,9 @@ extern "C" int or_linear_bwd(const or_linear_bwd_args* p, void* stream) {
     d.M = x.n_rows;
     d.N = x.n_out;
     d.act = x.activation;
-    d.chunks = (int)((x.n_rows + kSumRows - 1) / kSumRows);
-    if (d.chunks > 65535) return fail_arg("or_linear_bwd: at most %d rows", 65535 * kSumRows);
+    d.chunk_rows = chunk_rows_of(x.n_rows, x.n_out);
+    if (x.n_rows > (int64_t)65535 * 128) return fail_arg("or_linear_bwd: at most %d rows", 65535 * 128);
+    d.chunks = (int)((x.n_rows + d.chunk_rows - 1) / d.chunk_rows);
     if (d.chunks > 0)
       hipLaunchKernelGGL(dz_kernel, dim3((unsigned)((x.n_out + 255) / 256), (unsigned)d.chunks), dim3(kThreads), 0, st, d);
     if (sums)
