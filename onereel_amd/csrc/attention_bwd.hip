@@ -591,18 +591,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
         d0[4 * g + i] = y[i];
       }
     }
+    // the matrix work of a wavefront first: the other one on its SIMD fills the gaps with its exponentials (5.05 -> 4.60 ms,
+    // 3 x 9680 queries x 11440 keys, 16 heads; dq gains nothing from it)
     f32x16 s, dp;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int ks = 0; ks < C::KS; ++ks) {
       s = mfma(row_frag<D>(row, ks, 0), kf[ks], ks ? s : s0);
       dp = mfma(row_frag<D>(row, ks, kRing * C::SLOT), vf[ks], ks ? dp : d0);
     }
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       s[e] = __builtin_amdgcn_exp2f(s[e] * c);
       dp[e] *= s[e];
     }
     const bf16x8 p[2] = {pack8(s, 0), pack8(s, 1)}, ds[2] = {pack8(dp, 0), pack8(dp, 1)};
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int db = 0; db < C::DB; ++db)
 #pragma unroll
@@ -610,6 +615,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
         dv[db] = mfma(tr_frag<D>(tr, db, hs, kRing * C::SLOT), p[hs], dv[db]);
         dk[db] = mfma(tr_frag<D>(tr, db, hs, 0), ds[hs], dk[db]);
       }
+    __builtin_amdgcn_s_setprio(0);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no DMA into LDS of a block that has ended
   const int64_t at = ((int64_t)row0 * a.H + head) * D, rs = (int64_t)a.H * D, all = a.n_k * rs;
