@@ -25,6 +25,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -431,8 +432,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   const f32x16 zero = {};
 #pragma unroll 1
   for (int b = b0; b < b0 + kRing - 1; ++b) fetch(b);
-#pragma unroll 1
-  for (int b = b0; b < b1; ++b) {
+  auto step = [&](int b, auto tail) {
     wait_loads_barrier<(kRing - 2) * 2 * C::LPB>();
     fetch(b + kRing - 1);
     const uint32_t slot = lds + (b & (kRing - 1)) * C::SLOT, row = slot + ad.row, tr = slot + ad.tr;
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, neg_lse[t]));
-    if (n_keys - b * kBlk < kBlk) {   // the key rows past the end
+    if constexpr (decltype(tail)::value) {   // the key rows past the end
       const int n = n_keys - b * kBlk - 4 * (lane >> 5);
 #pragma unroll
       for (int t = 0; t < T; ++t)
@@ -472,7 +472,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int t = 0; t < T; ++t) acc[t][db] = mfma(kt, ds[t][hs], acc[t][db]);
       }
-  }
+  };
+  const int whole = min(b1, n_keys / kBlk);
+#pragma unroll 1
+  for (int b = b0; b < whole; ++b) step(b, std::false_type{});
+  if (max(whole, b0) < b1) step(max(whole, b0), std::true_type{});
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no DMA into LDS of a block that has ended
 #pragma unroll
   for (int t = 0; t < T; ++t) {
