@@ -74,6 +74,7 @@ struct BwdArgs {
 // other's matrix work: 3 x 9680 queries x 11440 keys, 16 heads of 128, dq 3.41 ms against 3.88 with 64 (one wavefront); dk
 // and dv 4.80 against 5.36 ms with 32 and 64 keys. With heads of 64, 64 queries fit twice too and halve the LDS reads per
 // query: 2 x 3001 x 3001 131 us against 138 (dk and dv with 64 keys do not fit twice: 239 against 198 us).
+constexpr int kKeyTile = 128;
 constexpr int query_tile(int D) { return D == 128 ? 128 : 256; }
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -94,120 +95,225 @@ __device__ __forceinline__ void seg_k(const BwdArgs& a, int s, int& lo, int& n) 
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// planner: one block. Query tiles: every segment's queries in pieces of tq rows, then the rows behind the last segment
-// (no keys: their gradient is zero). Key tiles: the key axis cut at the segments' key range boundaries, every interval in
-// pieces of tk rows, with the first and last segment that cover it.
-__device__ int block_scan(int v, int* wsum) {   // exclusive sum over the block's threads; wsum[16] is the total
+// planner. Query tiles: every segment's queries in pieces of tq rows, then the rows behind the last segment (no keys: their
+// gradient is zero). Key tiles: the key axis cut at the segments' key range boundaries, every interval in pieces of tk rows,
+// with the first and last segment that cover it.
+//
+// Calls of up to kFewSeg segments need no launch for it: a block of the dq pass finds its query tile in a wavefront's scan of
+// cu_q, and the first block of that pass writes the key tiles that the dk / dv pass reads (a planner launch of one block
+// took 7 to 17 us, the dk / dv pass of 12 ragged sequences 49). With more segments one block plans both ahead.
+constexpr int kFewSeg = 256;
+
+// exclusive sum over the block's threads; all: the total
+template <int THREADS>
+__device__ int block_scan(int v, int* wsum, int& all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int x = v;
+#pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const int y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
-  __syncthreads();
   if (lane == 63) wsum[w] = x;
   __syncthreads();
-  int base = 0, all = 0;
-  for (int i = 0; i < kPlanThreads / 64; ++i) {
-    if (i < w) base += wsum[i];
-    all += wsum[i];
+  int base = 0;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) {
+    const int y = wsum[i];
+    if (i < w) base += y;
+    all += y;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) wsum[16] = all;
   __syncthreads();
   return base + x - v;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void bwd_plan_kernel(BwdArgs a, int tq, int tk) {
-  __shared__ int bnd[2 * kMaxSeg];
-  __shared__ int lo_seg[2 * kMaxSeg + 1];
-  __shared__ int hi_seg[2 * kMaxSeg + 1];
-  __shared__ int wsum[17];
-  const int t = threadIdx.x, n = a.n_seg;
-  // query tiles
+// the tiles of n pieces (piece i: `count(i)` tiles), dealt out to the threads: emit(piece, tile of the piece, tile). first: n + 1
+// ints of LDS
+template <int THREADS, class Count, class Emit>
+__device__ int deal_tiles(int n, int most, int* first, int* wsum, Count&& count, Emit&& emit) {
+  const int t = threadIdx.x;
   int at = 0;
-  for (int s0 = 0; s0 <= n; s0 += kPlanThreads) {
-    const int s = s0 + t;
-    int lo = 0, len = 0, k0 = 0, nk = 0;
-    if (s < n) {
-      seg_q(a, s, lo, len);
-      seg_k(a, s, k0, nk);
-    } else if (s == n) {
-      lo = clampi(a.cu_q[n], 0, a.n_q);
-      len = a.n_q - lo;
-    }
-    const int tiles = (len + tq - 1) / tq;
-    const int first = at + block_scan(tiles, wsum);
-    for (int i = 0; i < tiles && first + i < a.max_q_tiles; ++i)
-      a.q_tiles[first + i] = i32x4{lo + i * tq, min(tq, len - i * tq), k0, nk};
-    at += wsum[16];
-    __syncthreads();
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
+    int all;
+    const int x = block_scan<THREADS>(i0 + t < n ? count(i0 + t) : 0, wsum, all);
+    if (i0 + t < n) first[i0 + t] = at + x;
+    at += all;
   }
-  if (t == 0) a.head[0] = min(at, a.max_q_tiles);
+  if (t == 0) first[n] = at;
+  __syncthreads();
+  at = min(at, most);
+  for (int x = t; x < at; x += THREADS) {
+    int lo = 0, hi = n - 1;   // the last piece that starts at or before x
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    emit(lo, x - first[lo], x);
+  }
+  return at;
+}
+
+template <int SEG>
+struct PlanLds {
+  int bnd[2 * SEG], lo_seg[2 * SEG + 1], hi_seg[2 * SEG + 1], first[2 * SEG + 2], wsum[16];
+};
+
+template <int THREADS, int SEG>
+__device__ void plan_keys(const BwdArgs& a, int tk, PlanLds<SEG>& l) {
+  const int t = threadIdx.x, n = a.n_seg;
   // boundaries of the key ranges, sorted (a power of two of them, the rest past the end)
   int m = 2;
   while (m < 2 * n) m <<= 1;
-  for (int i = t; i < m; i += kPlanThreads) {
+  int* raw = l.first;   // unsorted, until the tiles are dealt out
+  for (int i = t; i < m; i += THREADS) {
     int b = a.n_k;
     if (i < 2 * n) {
       int lo, len;
       seg_k(a, i >> 1, lo, len);
       b = i & 1 ? lo + len : lo;
     }
-    bnd[i] = b;
+    raw[i] = b;
+    l.bnd[i] = b;
   }
-  for (int i = t; i <= m; i += kPlanThreads) {
-    lo_seg[i] = 0x7fffffff;
-    hi_seg[i] = -1;
+  for (int i = t; i <= m; i += THREADS) {
+    l.lo_seg[i] = 0x7fffffff;
+    l.hi_seg[i] = -1;
   }
   __syncthreads();
-  for (int size = 2; size <= m; size <<= 1)
-    for (int d = size >> 1; d > 0; d >>= 1) {
-      for (int i = t; i < m / 2; i += kPlanThreads) {
-        const int x = 2 * d * (i / d) + i % d, y = x + d;
-        const bool up = (x & size) == 0;
-        const int p = bnd[x], r = bnd[y];
-        if ((p > r) == up) {
-          bnd[x] = r;
-          bnd[y] = p;
-        }
-      }
-      __syncthreads();
+  if (m <= 512) {   // by rank: no barriers
+    for (int i = t; i < m; i += THREADS) {
+      const int b = raw[i];
+      int rank = 0;
+      for (int j = 0; j < m; ++j) rank += raw[j] < b || (raw[j] == b && j < i);
+      l.bnd[rank] = b;
     }
+    __syncthreads();
+  } else {
+    for (int size = 2; size <= m; size <<= 1)
+      for (int d = size >> 1; d > 0; d >>= 1) {
+        for (int i = t; i < m / 2; i += THREADS) {
+          const int x = 2 * d * (i / d) + i % d, y = x + d;
+          const bool up = (x & size) == 0;
+          const int p = l.bnd[x], r = l.bnd[y];
+          if ((p > r) == up) {
+            l.bnd[x] = r;
+            l.bnd[y] = p;
+          }
+        }
+        __syncthreads();
+      }
+  }
   // interval i is [bnd[i - 1], bnd[i]): from 0 at i = 0, to n_k at i = m
-  for (int s = t; s < n; s += kPlanThreads) {
+  for (int s = t; s < n; s += THREADS) {
     int lo, len;
     seg_k(a, s, lo, len);
     if (len == 0) continue;
     int x = 0, y = m;   // the first boundary at lo
     while (x < y) {
       const int mid = (x + y) >> 1;
-      if (bnd[mid] < lo) x = mid + 1; else y = mid;
+      if (l.bnd[mid] < lo) x = mid + 1; else y = mid;
     }
-    for (int i = x + 1; i < m && bnd[i] <= lo + len; ++i) {
-      if (bnd[i] == bnd[i - 1]) continue;
-      atomicMin(&lo_seg[i], s);
-      atomicMax(&hi_seg[i], s);
+    for (int i = x + 1; i < m && l.bnd[i] <= lo + len; ++i) {
+      if (l.bnd[i] == l.bnd[i - 1]) continue;
+      atomicMin(&l.lo_seg[i], s);
+      atomicMax(&l.hi_seg[i], s);
     }
   }
   __syncthreads();
-  at = 0;
-  for (int i0 = 0; i0 <= m; i0 += kPlanThreads) {
-    const int i = i0 + t;
-    int lo = 0, len = 0;
-    if (i <= m) {
-      lo = i > 0 ? bnd[i - 1] : 0;
-      len = (i < m ? bnd[i] : a.n_k) - lo;
-    }
-    const int tiles = (len + tk - 1) / tk;
-    const int first = at + block_scan(tiles, wsum);
-    for (int j = 0; j < tiles && first + j < a.max_k_tiles; ++j)
-      a.k_tiles[first + j] = i32x4{lo + j * tk, min(tk, len - j * tk), lo_seg[i], hi_seg[i]};
-    at += wsum[16];
-    __syncthreads();
-  }
-  if (t == 0) a.head[1] = min(at, a.max_k_tiles);
+  auto start = [&](int i) { return i > 0 ? l.bnd[i - 1] : 0; };
+  auto length = [&](int i) { return (i < m ? l.bnd[i] : a.n_k) - start(i); };
+  const int tiles = deal_tiles<THREADS>(
+      m + 1, a.max_k_tiles, l.first, l.wsum, [&](int i) { return (length(i) + tk - 1) / tk; },
+      [&](int i, int j, int x) {
+        a.k_tiles[x] = i32x4{start(i) + j * tk, min(tk, length(i) - j * tk), l.lo_seg[i], l.hi_seg[i]};
+      });
+  if (t == 0) a.head[1] = tiles;
 }
+
+__global__ __launch_bounds__(kPlanThreads) void bwd_plan_kernel(BwdArgs a, int tq, int tk) {
+  __shared__ PlanLds<kMaxSeg> l;
+  const int n = a.n_seg;
+  auto piece = [&](int s, int& lo, int& len) {
+    if (s < n) {
+      seg_q(a, s, lo, len);
+    } else {
+      lo = clampi(a.cu_q[n], 0, a.n_q);
+      len = a.n_q - lo;
+    }
+  };
+  const int tiles = deal_tiles<kPlanThreads>(
+      n + 1, a.max_q_tiles, l.first, l.wsum,
+      [&](int s) {
+        int lo, len;
+        piece(s, lo, len);
+        return (len + tq - 1) / tq;
+      },
+      [&](int s, int j, int x) {
+        int lo, len, k0 = 0, nk = 0;
+        piece(s, lo, len);
+        if (s < n) seg_k(a, s, k0, nk);
+        a.q_tiles[x] = i32x4{lo + j * tq, min(tq, len - j * tq), k0, nk};
+      });
+  if (threadIdx.x == 0) a.head[0] = tiles;
+  __syncthreads();
+  plan_keys<kPlanThreads, kMaxSeg>(a, tk, l);
+}
+
+// The query tiles of a call of at most kFewSeg segments: how many there are, and the one with index x, from every
+// wavefront's own scan.
+struct QueryTiles {
+  int incl[kFewSeg / 64], tiles[kFewSeg / 64], n_seg_tiles, tail, tail_lo;
+  __device__ __forceinline__ int count(const BwdArgs& a, int tq, int lane) {
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < kFewSeg / 64; ++i) {
+      incl[i] = at;
+      tiles[i] = 0;
+      if (64 * i < a.n_seg) {
+        int lo, len = 0;
+        if (64 * i + lane < a.n_seg) seg_q(a, 64 * i + lane, lo, len);
+        tiles[i] = (len + tq - 1) / tq;
+        int x = tiles[i];
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+          const int y = __shfl_up(x, d);
+          if (lane >= d) x += y;
+        }
+        incl[i] = at + x;
+        at += __shfl(x, 63);
+      }
+    }
+    n_seg_tiles = uni(at);
+    tail_lo = uni(clampi(a.cu_q[a.n_seg], 0, a.n_q));
+    tail = a.n_q - tail_lo;
+    return min(n_seg_tiles + (tail + tq - 1) / tq, a.max_q_tiles);
+  }
+  __device__ __forceinline__ i32x4 at(const BwdArgs& a, int tq, int x) const {
+    if (x >= n_seg_tiles) {
+      const int j = (x - n_seg_tiles) * tq;
+      return i32x4{tail_lo + j, min(tq, tail - j), 0, 0};
+    }
+    int s = 0, j = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < kFewSeg / 64; ++i) {
+      const uint64_t hit = __ballot(incl[i] > x && tiles[i] > 0);
+      if (!found && hit) {
+        const int l = __builtin_ctzll(hit);
+        s = 64 * i + l;
+        j = x - (__shfl(incl[i], l) - __shfl(tiles[i], l));
+        found = true;
+      }
+    }
+    s = uni(s);
+    j = uni(j) * tq;
+    int lo, len, k0, nk;
+    seg_q(a, s, lo, len);
+    seg_k(a, s, k0, nk);
+    return uni(i32x4{lo + j, min(tq, len - j), k0, nk});
+  }
+};
 
 // ------------------------------------------------------------------------------------------------------------------
 // streamed blocks: 32 rows of D bf16 in an LDS slot, row r's 16-byte chunk c at position c ^ swz(r). A b128 read of one
@@ -347,24 +453,38 @@ __device__ __forceinline__ void store_f32(float* p, int64_t rs, const f32x16 (&a
 
 // this block's item of n: the blocks of one XCD (block index modulo 8) take consecutive items, which share their head's
 // streamed rows in that XCD's L2
-__device__ __forceinline__ int64_t xcd_item(int64_t n) {
-  const int64_t per = (n + 7) / 8, j = blockIdx.x >> 3, i = (blockIdx.x & 7) * per + j;
+__device__ __forceinline__ int64_t xcd_item(int64_t n, unsigned block) {
+  const int64_t per = (n + 7) / 8, j = block >> 3, i = (block & 7) * per + j;
   return j < per && i < n ? i : -1;
 }
 
 // ------------------------------------------------------------------------------------------------------------------
 // dq: a block owns 128 T queries of one head and streams the keys and values of their segment
-template <int D, int T>
+template <int D, int T, bool FEW>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void bwd_q_kernel(BwdArgs a) {
   using C = Str<D>;
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT];
-  const int n_tiles = uni(a.head[0]);
-  const int64_t item = xcd_item((int64_t)n_tiles * a.H * a.split_q);
+  const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
+  QueryTiles qt;
+  int n_tiles;
+  if constexpr (FEW) {
+    static_assert(sizeof(PlanLds<kFewSeg>) <= sizeof(ring), "plan");
+    if (blockIdx.x < 8) {   // ahead of the blocks with an item, eight of them so that those keep their XCDs
+      if (blockIdx.x == 0) plan_keys<kThreads, kFewSeg>(a, kKeyTile, *(PlanLds<kFewSeg>*)ring);
+      return;
+    }
+    n_tiles = qt.count(a, 128 * T, lane);
+  } else {
+    n_tiles = uni(a.head[0]);
+  }
+  const int64_t item = xcd_item((int64_t)n_tiles * a.H * a.split_q, blockIdx.x - (FEW ? 8 : 0));
   if (item < 0) return;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = (int)(item % a.split_q);
   const int head = (int)(item / a.split_q / n_tiles);
-  const i32x4 tile = uni(a.q_tiles[item / a.split_q % n_tiles]);
+  const int which = (int)(item / a.split_q % n_tiles);
+  i32x4 tile;
+  if constexpr (FEW) tile = qt.at(a, 128 * T, which);
+  else tile = uni(a.q_tiles[which]);
   const int row0 = tile[0] + w * 32 * T, n_keys = tile[3];
   const int rows = clampi(tile[1] - w * 32 * T, 0, 32 * T);
 
@@ -517,7 +637,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
   constexpr int kStat = 256;         // bytes of one wavefront's statistics of a block
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT + kRing * 4 * kStat];
   const int n_tiles = uni(a.head[1]);
-  const int64_t item = xcd_item((int64_t)n_tiles * a.H * a.split_k);
+  const int64_t item = xcd_item((int64_t)n_tiles * a.H * a.split_k, blockIdx.x);
   if (item < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = (int)(item % a.split_k);
@@ -670,7 +790,7 @@ int split_of(int64_t items, int64_t streamed) {
 Shape shape_of(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H, int32_t D) {
   Shape s;
   s.tq = query_tile(D);
-  s.tk = 128;
+  s.tk = kKeyTile;
   s.max_q_tiles = n_q / s.tq + n_seg + 1;
   s.max_k_tiles = n_k / s.tk + 2 * (int64_t)n_seg + 1;
   // a segment ends in a half-filled tile on average
@@ -705,7 +825,13 @@ template <int D>
 void launch(const BwdArgs& a, const Shape& s, hipStream_t st) {
   auto grid = [](int64_t items) { return dim3((unsigned)((items + 7) / 8 * 8)); };
   const dim3 gq = grid(s.max_q_tiles * a.H * s.split_q), gk = grid(s.max_k_tiles * a.H * s.split_k);
-  if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, query_tile(D) / 128>), gq, dim3(kThreads), 0, st, a);
+  constexpr int T = query_tile(D) / 128;
+  if (a.n_seg <= kFewSeg) {
+    hipLaunchKernelGGL((bwd_q_kernel<D, T, true>), dim3(gq.x + 8), dim3(kThreads), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(bwd_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a, s.tq, s.tk);
+    if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, T, false>), gq, dim3(kThreads), 0, st, a);
+  }
   if (a.n_k > 0) hipLaunchKernelGGL((bwd_kv_kernel<D>), gk, dim3(kThreads), 0, st, a);
 }
 
@@ -753,7 +879,7 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
   // the second array of statistics lies 4 H n_q bytes after the first, within the 32 bits of a buffer offset
   if ((int64_t)x.H * x.n_q * 4 + 256 >= (int64_t)0x7fffffff)
     return fail_arg("or_varlen_bwd: H * n_q must stay under 2^29");
-  if (std::max(s.max_q_tiles * s.split_q, s.max_k_tiles * s.split_k) * x.H >= (int64_t)0x7ffffff0)
+  if (std::max(s.max_q_tiles * s.split_q, s.max_k_tiles * s.split_k) * x.H >= (int64_t)0x7fffffe0)
     return fail_arg("or_varlen_bwd: too many tiles");
   char* ws = (char*)x.workspace;
   BwdArgs a;
@@ -792,7 +918,6 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
   a.part_q = (float*)(ws + l.part_q);
   a.part_k = (float*)(ws + l.part_k);
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(bwd_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a, s.tq, s.tk);
   if (x.D == 128) launch<128>(a, s, st);
   else launch<64>(a, s, st);
   const int64_t q8 = s.split_q > 1 ? (int64_t)x.n_q * row / 8 : 0, k8 = s.split_k > 1 ? (int64_t)x.n_k * row / 8 : 0;

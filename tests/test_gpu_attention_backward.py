@@ -77,7 +77,9 @@ CASES = [
     ([8], [5000], 2, 128),                                  # few queries: keys split
     ([4000], [16], 1, 64),                                  # few keys: queries split
     ([3] * 90, [7] * 90, 1, 128),
-    ([1] * 300 + [2] * 213, [3] * 513, 1, 64),
+    ([1] * 300 + [2] * 213, [3] * 513, 1, 64),               # planned by a launch of its own
+    ([2] * 255 + [130], [3] * 255 + [140], 2, 128),          # the most segments that are not
+    ([2] * 256 + [130], [3] * 256 + [140], 2, 128),
 ]
 
 
