@@ -24,8 +24,6 @@ DIT_SOURCES = ['dit_fused.hip', 'linear.hip']
 BENCH_SOURCES = ['mfma_ceiling.hip']
 # attention: no NaN operands reach the softmax max, so fmax needs no quieting of its inputs (v_max3_f32 directly)
 SOURCE_FLAGS = {'attention.hip': ['-fno-honor-nans']}
-# linear: its accumulators (up to 256 registers) are only added to by MFMAs: they stay in AGPRs
-SOURCE_DROPS = {'linear.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form=1']}
 ARCH = os.environ.get('ONEREEL_ARCH', 'gfx950')
 
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
@@ -35,14 +33,6 @@ FLAGS = [f'--offload-arch={ARCH}', '-O3', '-std=c++17', '-fPIC', '-I', str(INCLU
          # MFMA accumulators in VGPRs: the softmax rescales them with VALU ops, which cannot address AGPRs
          '-mllvm', '-amdgpu-mfma-vgpr-form=1',
          '-Wno-unused-result']
-
-
-def source_flags(src: str) -> list:
-    """the hipcc flags of one source file"""
-    drop = SOURCE_DROPS.get(src, [])
-    at = next((i for i in range(len(FLAGS)) if drop and FLAGS[i:i + len(drop)] == drop), None)
-    flags = FLAGS if at is None else FLAGS[:at] + FLAGS[at + len(drop):]
-    return flags + SOURCE_FLAGS.get(src, [])
 
 
 def _run(cmd):
@@ -64,7 +54,7 @@ def build(verbose: bool = False) -> Path:
 
     def one(src_obj):
         src, obj = src_obj
-        return _run([HIPCC, *source_flags(src), '-c', str(CSRC / src), '-o', str(obj)])
+        return _run([HIPCC, *FLAGS, *SOURCE_FLAGS.get(src, []), '-c', str(CSRC / src), '-o', str(obj)])
 
     srcs = SOURCES + DIT_SOURCES + BENCH_SOURCES
     with ThreadPoolExecutor(max_workers=len(srcs)) as ex:
