@@ -19,8 +19,8 @@
 // - Tiles of 256 x 256 are bound by the matrix cores; smaller tiles and a k axis split over several work-groups (fp32
 //   partial products, added in order by the epilogue's own launch) fill the GPU when there are few tiles. Up to 32 rows
 //   of x take a kernel of their own that streams W once, bound by HBM.
-// Measured (bf16, fp32 sums): 12720 x 2048 -> 8192 with bias, GELU and the pre-activation written 472 us, the product alone
-// 440 (a library product of that size, without epilogue, 375 to 400); dx 392 us (library 422), dW 363 us (library 469).
+// Measured (bf16, fp32 sums): 12720 x 2048 -> 8192 with bias, GELU and the pre-activation written 455 us, the product alone
+// 400 to 450 (a library product of that size, without epilogue, 375 to 400); dx 400 us (library 425), dW 360 us (library 460).
 #include <math.h>
 
 #include <algorithm>
@@ -75,13 +75,18 @@ __device__ __forceinline__ void load8(const void* p, int bf16, int col, float (&
   }
 }
 
+// 1 / (1 + exp(-x)) with v_exp_f32 and v_rcp_f32, good to 2^-22 (a full division costs the epilogue of a 256 x 256 tile as
+// much again as the rest of a GELU: the layer of 12720 x 2048 -> 8192 478 us with it, 455 so)
+__device__ __forceinline__ float logistic(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));
+}
+
+// 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3)
+constexpr float kGelu1 = 2 * 0.7978845608028654f, kGelu3 = kGelu1 * 0.044715f;
+
 __device__ __forceinline__ float act_of(float z, int act) {
-  if (act == OR_ACT_SILU) return z / (1.0f + __expf(-z));
-  if (act == OR_ACT_GELU_TANH) {
-    // 0.5 z (1 + tanh u) = z / (1 + exp(-2 u))
-    const float u = 0.7978845608028654f * (z + 0.044715f * z * z * z);
-    return z / (1.0f + __expf(-2.0f * u));
-  }
+  if (act == OR_ACT_SILU) return z * logistic(z);
+  if (act == OR_ACT_GELU_TANH) return z * logistic(z * (kGelu1 + kGelu3 * z * z));
   return z;
 }
 
@@ -92,12 +97,11 @@ __device__ __forceinline__ void act_grad(float z, int act, float& f, float& d) {
   if (act == OR_ACT_NONE) return;
   const float c = fminf(fmaxf(z, -20.0f), 20.0f);
   if (act == OR_ACT_SILU) {
-    const float p = 1.0f / (1.0f + __expf(-c));
+    const float p = logistic(c);
     d = p + c * p * (1.0f - p);
   } else {
-    const float u = 0.7978845608028654f * (c + 0.044715f * c * c * c);
-    const float p = 1.0f / (1.0f + __expf(-2.0f * u)), q = 1.0f / (1.0f + __expf(2.0f * u));
-    d = p + 2.0f * c * p * q * (0.7978845608028654f * (1.0f + 3.0f * 0.044715f * c * c));
+    const float u = c * (kGelu1 + kGelu3 * c * c), p = logistic(u), q = logistic(-u);
+    d = p + c * p * q * (kGelu1 + 3.0f * kGelu3 * c * c);
   }
   if (z != z) d = z;
   f = act_of(z, act);
@@ -737,6 +741,7 @@ extern "C" int or_linear_bwd(const or_linear_bwd_args* p, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)x.workspace;
   const bool sums = x.dbias || x.dgate, products = x.dx || x.dweight;
+  if (!sums && !products) return 0;
   Operand dz{(const uint16_t*)x.dy, x.dy_row_stride};
   if (sums || (scaled && products)) {
     DzArgs d = {};

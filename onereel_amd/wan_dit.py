@@ -20,9 +20,15 @@ chains of torch kernels over fp32 temporaries: every residual add runs in one pa
 and only the first norm runs alone (`or_layernorm_modulate`). Shapes of
 Wan2.2-TI2V-5B: hidden 3072 = 24 heads x 128, FFN 14336, 30 blocks, eps 1e-6, patch (1, 2, 2) over 48 latent
 channels, text width 4096 projected to 3072.
+
+`WanDiT.differentiable_forward` is the same pass for fine-tuning, with gradients of every weight: the projections and the
+feed forward are `linear` calls (bias, GELU, gate and residual in their epilogues), the attention and its norms the
+differentiable calls of the processors (halo scopes; the packed frame-memory scopes and the bounded memory have no
+gradient), the LayerNorm + modulation torch operations in fp32. Nothing is updated in place.
 """
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
@@ -31,6 +37,7 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from . import wan
+from .linear import linear
 from .layout import SceneLayout
 
 
@@ -125,6 +132,17 @@ class Linear:
         return y.view(*x.shape[:-1], y.shape[-1])
 
 
+def _norm(x, eps, weight=None, bias=None, scale=None, shift=None):
+    """layernorm_modulate in torch operations, for autograd"""
+    y = F.layer_norm(x.float(), x.shape[-1:], weight, bias, eps)
+    return (y if scale is None else y * (1 + scale) + shift).to(torch.bfloat16)
+
+
+def _apply(layer, x, **epilogue):
+    """a Linear layer through or_linear, differentiable"""
+    return linear(x, layer.weight, layer.bias, **epilogue)
+
+
 class RMSNorm:
     def __init__(self, n, eps, gen, device):
         self.weight = (1 + 0.1 * torch.randn(n, generator=gen, device=device)).to(torch.bfloat16)
@@ -144,6 +162,16 @@ class Attention:
         self.to_q, self.to_k, self.to_v = (Linear(d, d, cfg.std, gen, device) for _ in range(3))
         self.to_out = [Linear(d, d, cfg.std, gen, device), lambda x: x]
         self.norm_q, self.norm_k = RMSNorm(d, cfg.eps, gen, device), RMSNorm(d, cfg.eps, gen, device)
+
+
+class _Projections:
+    """an Attention as a processor sees it in the differentiable pass: projections by or_linear, the output's left to the
+    caller, who has its gate and residual"""
+
+    def __init__(self, attn: Attention):
+        self.heads, self.norm_q, self.norm_k = attn.heads, attn.norm_q, attn.norm_k
+        self.to_q, self.to_k, self.to_v = (functools.partial(_apply, l) for l in (attn.to_q, attn.to_k, attn.to_v))
+        self.to_out = [lambda x: x, lambda x: x]
 
 
 class Block:
@@ -174,6 +202,24 @@ class Block:
         n = residual_layernorm_modulate_(x, p_cross(self.attn2, n, encoder_hidden_states=text), eps, scale=c_scale,
                                          shift=c_shift)
         return self.ffn_out(self.ffn_in.gelu_tanh(n)), c_gate
+
+    def differentiable(self, x, mod, text, rotary, p_self, p_cross):
+        """x [1, S, dim] bf16 -> the block's output, a new tensor, with gradients of x and of every weight"""
+        eps = self.cfg.eps
+        shift, scale, gate, c_shift, c_scale, c_gate = mod
+        o = p_self(_Projections(self.attn1), _norm(x, eps, scale=scale, shift=shift), rotary_emb=rotary)
+        x = _apply(self.attn1.to_out[0], o, gate=gate, residual=x)
+        o = p_cross(_Projections(self.attn2), _norm(x, eps, self.norm2_w, self.norm2_b), encoder_hidden_states=text)
+        x = _apply(self.attn2.to_out[0], o, residual=x)
+        h = _apply(self.ffn_in, _norm(x, eps, scale=c_scale, shift=c_shift), activation='gelu_tanh')
+        return _apply(self.ffn_out, h, gate=c_gate, residual=x)
+
+    def parameters(self):
+        layers = [l for a in (self.attn1, self.attn2) for l in (a.to_q, a.to_k, a.to_v, a.to_out[0])]
+        layers += [self.ffn_in, self.ffn_out]
+        return [p for l in layers for p in (l.weight, l.bias)] + \
+            [n.weight for a in (self.attn1, self.attn2) for n in (a.norm_q, a.norm_k)] + \
+            [self.norm2_w, self.norm2_b, self.scale_shift_table]
 
 
 def timestep_features(t: float, n: int, device) -> torch.Tensor:
@@ -219,6 +265,27 @@ class WanDiT:
             shift, scale = (mods[i + 1][0], mods[i + 1][1]) if i + 1 < len(self.blocks) else (out_shift, out_scale)
             n = residual_layernorm_modulate_(x, f, eps, gate=gate, scale=scale, shift=shift)
         return self.proj_out(n)[0]
+
+    def differentiable_forward(self, tokens, t: float, text, rotary):
+        """forward with gradients of tokens, text and `parameters()` (those of them that require one)"""
+        if self.ctx.memory or any(self.ctx.layout.extra.get(j) for j in range(self.ctx.layout.n_scenes)):
+            raise L.HipValueError('the frame-memory scopes and the bounded memory have no gradient: train with halo scopes')
+        d, eps = self.cfg.dim, self.cfg.eps
+        x = _apply(self.patch_embed, tokens)[None]
+        features = timestep_features(t, self.cfg.freq_dim, tokens.device).to(torch.bfloat16)[None]
+        temb = _apply(self.time_out, _apply(self.time_in, features, activation='silu'))
+        temb6 = _apply(self.time_proj, F.silu(temb)).float().view(6, d)
+        ctx_text = _apply(self.text_out, _apply(self.text_in, text, activation='gelu_tanh'))[None]
+        for blk in self.blocks:
+            x = blk.differentiable(x, blk.modulation(temb6), ctx_text, rotary, self.p_self, self.p_cross)
+        out_shift, out_scale = (self.scale_shift_table + temb.float()).chunk(2, 0)
+        return _apply(self.proj_out, _norm(x, eps, scale=out_scale, shift=out_shift))[0]
+
+    def parameters(self):
+        """every weight, for an optimizer; none requires a gradient until the caller says so (requires_grad_())"""
+        layers = [self.patch_embed, self.text_in, self.text_out, self.time_in, self.time_out, self.time_proj, self.proj_out]
+        return [p for l in layers for p in (l.weight, l.bias)] + [p for b in self.blocks for p in b.parameters()] + \
+            [self.scale_shift_table]
 
     def flops(self, text_rows: int) -> dict:
         """useful FLOP of one forward: GEMMs (2 m n k each) and attention (4 Lq Lk H D per scope, self and cross)"""
