@@ -46,7 +46,7 @@ constexpr int kBlk = 32;             // streamed rows per block
 constexpr int kRing = 4;             // LDS slots of the ring
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxSeg = 4096;
-constexpr int kMaxSplit = 32;
+constexpr int kMaxSplit = 64;
 constexpr int kHeader = 8;           // int32 words ahead of the tile tables: query tile count, key tile count
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -61,21 +61,23 @@ struct BwdArgs {
   float scale;
   int32_t split_q, split_k;          // parts of the streamed axis in the dq pass and in the dk / dv pass
   int32_t max_q_tiles, max_k_tiles;
+  int32_t tq, tk;                    // rows of a query tile and of a key tile
   // workspace
   int32_t* head;
   i32x4* q_tiles;                    // first query, rows, first key, keys
-  i32x4* k_tiles;                    // first key, rows, first and last segment that may read them
+  i32x4* k_tiles;                    // two a tile: first key, rows, first and last segment that may read them; first query and
+                                     // queries of the segment where only one may
   float* stat;                       // [2][H][n_q]: -lse / scale, then -delta
   float* part_q;                     // [split_q][n_q][H][D]
   float* part_k;                     // [split_k][2][n_k][H][D]: dk, then dv
 };
 
-// rows of a query tile. 32 queries a wavefront leave room for two wavefronts on a SIMD, one's exponentials under the
-// other's matrix work: 3 x 9680 queries x 11440 keys, 16 heads of 128, dq 3.41 ms against 3.88 with 64 (one wavefront); dk
-// and dv 4.80 against 5.36 ms with 32 and 64 keys. With heads of 64, 64 queries fit twice too and halve the LDS reads per
-// query: 2 x 3001 x 3001 131 us against 138 (dk and dv with 64 keys do not fit twice: 239 against 198 us).
+// Blocks of 32 queries that a wavefront owns. One leaves room for two wavefronts on a SIMD, one's exponentials under the
+// other's matrix work: 3 x 9680 queries x 11440 keys, 16 heads of 128, dq 3.41 ms against 3.88 with two blocks (one
+// wavefront); dk and dv 4.80 against 5.36 ms with 32 and 64 keys. With heads of 64, two blocks fit twice too and halve the
+// LDS reads per query: 2 x 3001 x 3001 131 us against 138 (dk and dv with 64 keys do not fit twice: 239 against 198 us).
+constexpr int query_blocks(int D) { return D == 64 ? 2 : 1; }
 constexpr int kKeyTile = 128;
-constexpr int query_tile(int D) { return D == 128 ? 128 : 256; }
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 // a value that is the same in every lane, in a scalar register
@@ -160,8 +162,8 @@ struct PlanLds {
 };
 
 template <int THREADS, int SEG>
-__device__ void plan_keys(const BwdArgs& a, int tk, PlanLds<SEG>& l) {
-  const int t = threadIdx.x, n = a.n_seg;
+__device__ void plan_keys(const BwdArgs& a, PlanLds<SEG>& l) {
+  const int t = threadIdx.x, n = a.n_seg, tk = a.tk;
   // boundaries of the key ranges, sorted (a power of two of them, the rest past the end)
   int m = 2;
   while (m < 2 * n) m <<= 1;
@@ -226,14 +228,17 @@ __device__ void plan_keys(const BwdArgs& a, int tk, PlanLds<SEG>& l) {
   const int tiles = deal_tiles<THREADS>(
       m + 1, a.max_k_tiles, l.first, l.wsum, [&](int i) { return (length(i) + tk - 1) / tk; },
       [&](int i, int j, int x) {
-        a.k_tiles[x] = i32x4{start(i) + j * tk, min(tk, length(i) - j * tk), l.lo_seg[i], l.hi_seg[i]};
+        int lo = 0, len = 0;
+        if (l.lo_seg[i] == l.hi_seg[i]) seg_q(a, l.lo_seg[i], lo, len);
+        a.k_tiles[2 * x] = i32x4{start(i) + j * tk, min(tk, length(i) - j * tk), l.lo_seg[i], l.hi_seg[i]};
+        a.k_tiles[2 * x + 1] = i32x4{lo, len, 0, 0};
       });
   if (t == 0) a.head[1] = tiles;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void bwd_plan_kernel(BwdArgs a, int tq, int tk) {
+__global__ __launch_bounds__(kPlanThreads) void bwd_plan_kernel(BwdArgs a) {
   __shared__ PlanLds<kMaxSeg> l;
-  const int n = a.n_seg;
+  const int n = a.n_seg, tq = a.tq;
   auto piece = [&](int s, int& lo, int& len) {
     if (s < n) {
       seg_q(a, s, lo, len);
@@ -257,24 +262,32 @@ __global__ __launch_bounds__(kPlanThreads) void bwd_plan_kernel(BwdArgs a, int t
       });
   if (threadIdx.x == 0) a.head[0] = tiles;
   __syncthreads();
-  plan_keys<kPlanThreads, kMaxSeg>(a, tk, l);
+  plan_keys<kPlanThreads, kMaxSeg>(a, l);
 }
 
 // The query tiles of a call of at most kFewSeg segments: how many there are, and the one with index x, from every
 // wavefront's own scan.
 struct QueryTiles {
-  int incl[kFewSeg / 64], tiles[kFewSeg / 64], n_seg_tiles, tail, tail_lo;
+  static constexpr int N = kFewSeg / 64;
+  int lo[N], len[N], k0[N], nk[N], incl[N], n_seg_tiles, tail, tail_lo;
   __device__ __forceinline__ int count(const BwdArgs& a, int tq, int lane) {
+    // every load at once: what follows waits for one round of them
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      lo[i] = len[i] = k0[i] = nk[i] = 0;
+      if (64 * i < a.n_seg && 64 * i + lane < a.n_seg) {
+        seg_q(a, 64 * i + lane, lo[i], len[i]);
+        seg_k(a, 64 * i + lane, k0[i], nk[i]);
+      }
+    }
+    tail_lo = uni(clampi(a.cu_q[a.n_seg], 0, a.n_q));
+    tail = a.n_q - tail_lo;
     int at = 0;
 #pragma unroll
-    for (int i = 0; i < kFewSeg / 64; ++i) {
+    for (int i = 0; i < N; ++i) {
       incl[i] = at;
-      tiles[i] = 0;
       if (64 * i < a.n_seg) {
-        int lo, len = 0;
-        if (64 * i + lane < a.n_seg) seg_q(a, 64 * i + lane, lo, len);
-        tiles[i] = (len + tq - 1) / tq;
-        int x = tiles[i];
+        int x = (len[i] + tq - 1) / tq;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
           const int y = __shfl_up(x, d);
@@ -285,33 +298,23 @@ struct QueryTiles {
       }
     }
     n_seg_tiles = uni(at);
-    tail_lo = uni(clampi(a.cu_q[a.n_seg], 0, a.n_q));
-    tail = a.n_q - tail_lo;
     return min(n_seg_tiles + (tail + tq - 1) / tq, a.max_q_tiles);
   }
-  __device__ __forceinline__ i32x4 at(const BwdArgs& a, int tq, int x) const {
-    if (x >= n_seg_tiles) {
-      const int j = (x - n_seg_tiles) * tq;
-      return i32x4{tail_lo + j, min(tq, tail - j), 0, 0};
-    }
-    int s = 0, j = 0;
-    bool found = false;
+  __device__ __forceinline__ i32x4 at(int tq, int x) const {
+    i32x4 tile = {tail_lo + (x - n_seg_tiles) * tq, 0, 0, 0};
+    tile[1] = min(tq, tail - (tile[0] - tail_lo));
+    bool found = x >= n_seg_tiles;
 #pragma unroll
-    for (int i = 0; i < kFewSeg / 64; ++i) {
-      const uint64_t hit = __ballot(incl[i] > x && tiles[i] > 0);
+    for (int i = 0; i < N; ++i) {
+      // the first lane whose sum passes x: its segment has tiles
+      const uint64_t hit = __ballot(incl[i] > x && len[i] > 0);
       if (!found && hit) {
-        const int l = __builtin_ctzll(hit);
-        s = 64 * i + l;
-        j = x - (__shfl(incl[i], l) - __shfl(tiles[i], l));
+        const int l = __builtin_ctzll(hit), n = __shfl(len[i], l), j = (x - (__shfl(incl[i], l) - (n + tq - 1) / tq)) * tq;
+        tile = i32x4{__shfl(lo[i], l) + j, min(tq, n - j), __shfl(k0[i], l), __shfl(nk[i], l)};
         found = true;
       }
     }
-    s = uni(s);
-    j = uni(j) * tq;
-    int lo, len, k0, nk;
-    seg_q(a, s, lo, len);
-    seg_k(a, s, k0, nk);
-    return uni(i32x4{lo + j, min(tq, len - j), k0, nk});
+    return uni(tile);
   }
 };
 
@@ -460,9 +463,10 @@ __device__ __forceinline__ int64_t xcd_item(int64_t n, unsigned block) {
 
 // ------------------------------------------------------------------------------------------------------------------
 // dq: a block owns 128 T queries of one head and streams the keys and values of their segment
-template <int D, int T, bool FEW>
+template <int D, bool FEW>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void bwd_q_kernel(BwdArgs a) {
   using C = Str<D>;
+  constexpr int T = query_blocks(D);
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT];
   const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
   QueryTiles qt;
@@ -470,7 +474,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   if constexpr (FEW) {
     static_assert(sizeof(PlanLds<kFewSeg>) <= sizeof(ring), "plan");
     if (blockIdx.x < 8) {   // ahead of the blocks with an item, eight of them so that those keep their XCDs
-      if (blockIdx.x == 0) plan_keys<kThreads, kFewSeg>(a, kKeyTile, *(PlanLds<kFewSeg>*)ring);
+      if (blockIdx.x == 0) plan_keys<kThreads, kFewSeg>(a, *(PlanLds<kFewSeg>*)ring);
       return;
     }
     n_tiles = qt.count(a, 128 * T, lane);
@@ -483,7 +487,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int head = (int)(item / a.split_q / n_tiles);
   const int which = (int)(item / a.split_q % n_tiles);
   i32x4 tile;
-  if constexpr (FEW) tile = qt.at(a, 128 * T, which);
+  if constexpr (FEW) tile = qt.at(128 * T, which);
   else tile = uni(a.q_tiles[which]);
   const int row0 = tile[0] + w * 32 * T, n_keys = tile[3];
   const int rows = clampi(tile[1] - w * 32 * T, 0, 32 * T);
@@ -506,6 +510,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     dma_rows<D>(kp + off, a.ks, n, voff, at);
     dma_rows<D>(vp + off, a.ks, n, voff, at + kRing * C::SLOT);
   };
+  // the first blocks are under way while the owned rows load
+#pragma unroll
+  for (int b = 0; b < kRing - 1; ++b) fetch(b0 + b);
 
   // the owned queries, their output gradients and their statistics
   bf16x8 qf[T][C::KS], df[T][C::KS];
@@ -550,8 +557,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   ad.init(lane);
   const float c = a.scale * kLog2e;
   const f32x16 zero = {};
-#pragma unroll 1
-  for (int b = b0; b < b0 + kRing - 1; ++b) fetch(b);
+  const int end = min(n_keys, b1 * kBlk);
   auto step = [&](int b, auto tail) {
     wait_loads_barrier<(kRing - 2) * 2 * C::LPB>();
     fetch(b + kRing - 1);
@@ -570,7 +576,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, neg_lse[t]));
     if constexpr (decltype(tail)::value) {   // the key rows past the end
-      const int n = n_keys - b * kBlk - 4 * (lane >> 5);
+      const int n = end - b * kBlk - 4 * (lane >> 5);
 #pragma unroll
       for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -593,10 +599,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         for (int t = 0; t < T; ++t) acc[t][db] = mfma(kt, ds[t][hs], acc[t][db]);
       }
   };
-  const int whole = min(b1, n_keys / kBlk);
+  int b = b0;
 #pragma unroll 1
-  for (int b = b0; b < whole; ++b) step(b, std::false_type{});
-  if (max(whole, b0) < b1) step(max(whole, b0), std::true_type{});
+  for (; (b + 1) * kBlk <= end; ++b) step(b, std::false_type{});
+  if (b * kBlk < end) step(b, std::true_type{});
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no DMA into LDS of a block that has ended
 #pragma unroll
   for (int t = 0; t < T; ++t) {
@@ -642,7 +648,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = (int)(item % a.split_k);
   const int head = (int)(item / a.split_k / n_tiles);
-  const i32x4 tile = uni(a.k_tiles[item / a.split_k % n_tiles]);
+  const int64_t which = item / a.split_k % n_tiles;
+  const i32x4 tile = uni(a.k_tiles[2 * which]), only = uni(a.k_tiles[2 * which + 1]);
   const int row0 = tile[0] + w * 32;
   const int rows = clampi(tile[1] - w * 32, 0, 32);
 
@@ -656,31 +663,39 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
   const uint32_t lds = lds_addr(ring), m0 = lds + w * 1024, st0 = lds + 2 * kRing * C::SLOT + w * kStat;
 
   // this part's blocks of the segments' blocks in order
-  Walk wk{tile[2], tile[3], 0, 0};
-  int total = 0;
-  while (wk.next_segment(a, tile[0])) total += (wk.left + kBlk - 1) / kBlk;
+  Walk walk{tile[3] + 1, tile[3], only[0], only[1]};
+  int total = (only[1] + kBlk - 1) / kBlk;
+  if (tile[2] < tile[3]) {
+    Walk all{tile[2], tile[3], 0, 0};
+    for (total = 0; all.next_segment(a, tile[0]);) total += (all.left + kBlk - 1) / kBlk;
+    walk = Walk{tile[2], tile[3], 0, 0};
+    walk.next_segment(a, tile[0]);
+  }
   const int b0 = (int)((int64_t)total * part / a.split_k), b1 = (int)((int64_t)total * (part + 1) / a.split_k);
-  wk = Walk{tile[2], tile[3], 0, 0};
-  for (int skip = b0; wk.next_segment(a, tile[0]);) {
-    const int n = (wk.left + kBlk - 1) / kBlk;
+  for (int skip = b0; walk.left > 0;) {
+    const int n = (walk.left + kBlk - 1) / kBlk;
     if (skip < n) {
-      wk.row += skip * kBlk;
-      wk.left -= skip * kBlk;
+      walk.row += skip * kBlk;
+      walk.left -= skip * kBlk;
       break;
     }
     skip -= n;
+    walk.next_segment(a, tile[0]);
   }
   auto fetch = [&](int b) {
-    if (b < b1 && wk.left <= 0) wk.next_segment(a, tile[0]);
-    const int n = b < b1 ? min(wk.left, kBlk) : 0, slot = b & (kRing - 1);
-    const int64_t r = b < b1 ? wk.row : 0;
+    if (b < b1 && walk.left <= 0) walk.next_segment(a, tile[0]);
+    const int n = b < b1 ? min(walk.left, kBlk) : 0, slot = b & (kRing - 1);
+    const int64_t r = b < b1 ? walk.row : 0;
     const uint32_t at = m0 + slot * C::SLOT;
     dma_rows<D>(a.q + r * a.qs + (int64_t)head * D, a.qs, n, voq, at);
     dma_rows<D>(a.d_o + r * a.dos + (int64_t)head * D, a.dos, n, vod, at + kRing * C::SLOT);
     dma_stats(a.stat + (int64_t)head * a.n_q + r, (int64_t)a.H * a.n_q, n, lane, st0 + slot * 4 * kStat);
-    wk.row += kBlk;
-    wk.left -= kBlk;
+    walk.row += kBlk;
+    walk.left -= kBlk;
   };
+  // the first blocks are under way while the owned rows load
+#pragma unroll
+  for (int b = 0; b < kRing - 1; ++b) fetch(b0 + b);
 
   bf16x8 kf[C::KS], vf[C::KS];
   f32x16 dk[C::DB], dv[C::DB];
@@ -695,8 +710,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
   Lds<D> ad;
   ad.init(lane);
   const float c = a.scale * kLog2e;
-#pragma unroll 1
-  for (int b = b0; b < b0 + kRing - 1; ++b) fetch(b);
 #pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     wait_loads_barrier<(kRing - 2) * (2 * C::LPB + 1)>();
@@ -715,30 +728,52 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
         d0[4 * g + i] = y[i];
       }
     }
-    // the matrix work of a wavefront first: the other one on its SIMD fills the gaps with its exponentials (5.05 -> 4.60 ms,
-    // 3 x 9680 queries x 11440 keys, 16 heads; dq gains nothing from it)
+    // The matrix work of a wavefront first: the other one on its SIMD fills the gaps with its exponentials (5.05 -> 4.60 ms,
+    // 3 x 9680 queries x 11440 keys, 16 heads; dq gains nothing from it). Operands are read two steps early, which is what
+    // the registers have room for, in an order set here: the compiler reads each pair just before its use (4.74 -> 4.35 ms).
     f32x16 s, dp;
     __builtin_amdgcn_s_setprio(1);
+    bf16x8 fq[2] = {row_frag<D>(row, 0, 0), row_frag<D>(row, 1, 0)};
+    bf16x8 fd[2] = {row_frag<D>(row, 0, kRing * C::SLOT), row_frag<D>(row, 1, kRing * C::SLOT)};
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int ks = 0; ks < C::KS; ++ks) {
-      s = mfma(row_frag<D>(row, ks, 0), kf[ks], ks ? s : s0);
-      dp = mfma(row_frag<D>(row, ks, kRing * C::SLOT), vf[ks], ks ? dp : d0);
+      s = mfma(fq[ks & 1], kf[ks], ks ? s : s0);
+      dp = mfma(fd[ks & 1], vf[ks], ks ? dp : d0);
+      if (ks + 2 < C::KS) {
+        fq[ks & 1] = row_frag<D>(row, ks + 2, 0);
+        fd[ks & 1] = row_frag<D>(row, ks + 2, kRing * C::SLOT);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
+    // by halves: the first half's registers hold the first transposed operands while the second half is worked on
+    bf16x8 p[2], ds[2], ft[2][2];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      s[e] = __builtin_amdgcn_exp2f(s[e] * c);
-      dp[e] *= s[e];
+    for (int hs = 0; hs < 2; ++hs) {
+#pragma unroll
+      for (int e = 8 * hs; e < 8 * hs + 8; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(s[e] * c);
+        dp[e] *= s[e];
+      }
+      p[hs] = pack8(s, hs);
+      ds[hs] = pack8(dp, hs);
+      ft[hs][0] = tr_frag<D>(tr, hs % C::DB, hs / C::DB, kRing * C::SLOT);
+      ft[hs][1] = tr_frag<D>(tr, hs % C::DB, hs / C::DB, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const bf16x8 p[2] = {pack8(s, 0), pack8(s, 1)}, ds[2] = {pack8(dp, 0), pack8(dp, 1)};
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int db = 0; db < C::DB; ++db)
-#pragma unroll
-      for (int hs = 0; hs < 2; ++hs) {
-        dv[db] = mfma(tr_frag<D>(tr, db, hs, kRing * C::SLOT), p[hs], dv[db]);
-        dk[db] = mfma(tr_frag<D>(tr, db, hs, 0), ds[hs], dk[db]);
+    for (int i = 0; i < 2 * C::DB; ++i) {
+      const int db = i % C::DB, hs = i / C::DB, n = i + 2;
+      dv[db] = mfma(ft[i & 1][0], p[hs], dv[db]);
+      dk[db] = mfma(ft[i & 1][1], ds[hs], dk[db]);
+      if (n < 2 * C::DB) {
+        ft[i & 1][0] = tr_frag<D>(tr, n % C::DB, n / C::DB, kRing * C::SLOT);
+        ft[i & 1][1] = tr_frag<D>(tr, n % C::DB, n / C::DB, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     __builtin_amdgcn_s_setprio(0);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no DMA into LDS of a block that has ended
@@ -762,6 +797,7 @@ __global__ __launch_bounds__(kThreads) void bwd_add_kernel(BwdArgs a, int64_t q8
     const int64_t apart = is_q ? q8 * 8 : 2 * k8 * 8;
     const int parts = is_q ? a.split_q : a.split_k;
     f32x4 x = {}, y = {};
+#pragma unroll 8
     for (int j = 0; j < parts; ++j) {
       x += *(const f32x4*)(p + j * apart + e * 8);
       y += *(const f32x4*)(p + j * apart + e * 8 + 4);
@@ -779,23 +815,29 @@ struct Shape {
   int split_q, split_k;
 };
 
-// Parts of a streamed axis: as many as keep every block of the call resident at once (256 CUs, two blocks each), none
-// shorter than 8 blocks of rows. The partial gradients cost more than uneven rounds do, so calls with half that many
-// items or more are not split: 12 sequences of up to 699 x 899 rows, 16 heads (336 items), dk and dv in 2 parts take 59 us
-// and 27 us to add, in one 53 us; 128 keys against 3 x 9680 queries (48 items) in one part 488 us, in 8 104 us and 8 to add.
+// Parts of a streamed axis: as many as give every one of 256 CUs a work-group, none shorter than 8 blocks of rows; twice as
+// many where the parts would still be 64 blocks or longer, since two work-groups on a CU fill each other's gaps. Splitting
+// further, or calls that have 256 items, gains less than the partial gradients cost (16 heads of 128; dq, then dk and dv):
+// 2048 x 2048 64 + 90 us, in 2 parts 59 + 71 and 18 to add; 256 keys against 4096 queries 149 us for dk and dv in 1 part, 35 in
+// 8, 37 in 16; 128 against 3 x 9680 488 us in 1, 104 in 8, 95 in 10.
+constexpr int kCUs = 256;
 int split_of(int64_t items, int64_t streamed) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(items, 1), streamed / (8 * kBlk), kMaxSplit}));
+  const int64_t blocks = streamed / kBlk;
+  int64_t parts = std::max<int64_t>(1, std::min<int64_t>({kCUs / std::max<int64_t>(items, 1), blocks / 8, kMaxSplit / 2}));
+  if (items * parts <= kCUs && blocks / parts >= 64) parts *= 2;
+  return (int)parts;
 }
 
 Shape shape_of(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H, int32_t D) {
   Shape s;
-  s.tq = query_tile(D);
+  // a segment ends in a half-filled tile on average
+  auto items = [&](int64_t n, int tile) { return H * ((n + tile - 1) / tile + n_seg / 2); };
+  s.tq = 128 * query_blocks(D);
   s.tk = kKeyTile;
   s.max_q_tiles = n_q / s.tq + n_seg + 1;
   s.max_k_tiles = n_k / s.tk + 2 * (int64_t)n_seg + 1;
-  // a segment ends in a half-filled tile on average
-  s.split_q = split_of(H * ((n_q + s.tq - 1) / s.tq + n_seg / 2), max_k);
-  s.split_k = split_of(H * ((n_k + s.tk - 1) / s.tk + n_seg / 2), max_q);
+  s.split_q = split_of(items(n_q, s.tq), max_k);
+  s.split_k = split_of(items(n_k, s.tk), max_q);
   return s;
 }
 
@@ -811,7 +853,7 @@ Layout layout_of(const Shape& s, int32_t n_q, int32_t n_k, int32_t H, int32_t D)
     return was;
   };
   l.q_tiles = take(s.max_q_tiles * 16);
-  l.k_tiles = take(s.max_k_tiles * 16);
+  l.k_tiles = take(s.max_k_tiles * 32);
   l.stat = take((int64_t)2 * H * n_q * 4);
   l.part_q = take(s.split_q > 1 ? (int64_t)s.split_q * n_q * H * D * 4 : 0);
   l.part_k = take(s.split_k > 1 ? (int64_t)s.split_k * 2 * n_k * H * D * 4 : 0);
@@ -824,15 +866,14 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 template <int D>
 void launch(const BwdArgs& a, const Shape& s, hipStream_t st) {
   auto grid = [](int64_t items) { return dim3((unsigned)((items + 7) / 8 * 8)); };
-  const dim3 gq = grid(s.max_q_tiles * a.H * s.split_q), gk = grid(s.max_k_tiles * a.H * s.split_k);
-  constexpr int T = query_tile(D) / 128;
+  const dim3 gq = grid(s.max_q_tiles * a.H * s.split_q), gk = grid(s.max_k_tiles * a.H * s.split_k), t(kThreads);
   if (a.n_seg <= kFewSeg) {
-    hipLaunchKernelGGL((bwd_q_kernel<D, T, true>), dim3(gq.x + 8), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((bwd_q_kernel<D, true>), dim3(gq.x + 8), t, 0, st, a);
   } else {
-    hipLaunchKernelGGL(bwd_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a, s.tq, s.tk);
-    if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, T, false>), gq, dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(bwd_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+    if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, false>), gq, t, 0, st, a);
   }
-  if (a.n_k > 0) hipLaunchKernelGGL((bwd_kv_kernel<D>), gk, dim3(kThreads), 0, st, a);
+  if (a.n_k > 0) hipLaunchKernelGGL((bwd_kv_kernel<D>), gk, t, 0, st, a);
 }
 
 }  // namespace
@@ -909,6 +950,8 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
   a.scale = x.scale;
   a.split_q = s.split_q;
   a.split_k = s.split_k;
+  a.tq = s.tq;
+  a.tk = s.tk;
   a.max_q_tiles = (int32_t)s.max_q_tiles;
   a.max_k_tiles = (int32_t)s.max_k_tiles;
   a.head = (int32_t*)ws;

@@ -80,6 +80,11 @@ CASES = [
     ([1] * 300 + [2] * 213, [3] * 513, 1, 64),               # planned by a launch of its own
     ([2] * 255 + [130], [3] * 255 + [140], 2, 128),          # the most segments that are not
     ([2] * 256 + [130], [3] * 256 + [140], 2, 128),
+    # many heads and segments: more than one round of work-groups
+    ([130] * 33 + [300, 1], [70] * 33 + [513, 200], 16, 64),
+    ([130] * 33 + [300, 1], [70] * 33 + [513, 200], 16, 128),
+    ([33] * 30, [1, 2, 31, 32, 33, 64, 65, 95, 96, 97] * 3, 64, 128),
+    ([1, 2, 31, 32, 33, 64, 65, 95, 96, 97] * 3, [33] * 30, 64, 64),
 ]
 
 
@@ -97,14 +102,15 @@ def test_varlen_backward(lq, lk, H, D):
     assert all(torch.equal(x, y) for x, y in zip(got, again))
 
 
+@pytest.mark.parametrize('H', [2, 96])
 @pytest.mark.parametrize('D', [64, 128])
-def test_ranges_backward_shares_key_rows(D):
+def test_ranges_backward_shares_key_rows(D, H):
     """rows read by none, one, two and three ranges; a range inside another, equal ones, an empty one"""
     lq, kr = [70, 140, 1, 300, 33], [(10, 200), (150, 600), (150, 600), (20, 20), (180, 181)]
-    print(f'ranges D={D}', flush=True)
+    print(f'ranges D={D} H={H}', flush=True)
     qr, _ = cut(lq)
-    q, k, v, do = inputs(sum(lq), 700, 2, D, 5)
-    dlse = torch.randn(2, sum(lq), generator=torch.Generator().manual_seed(9))
+    q, k, v, do = inputs(sum(lq), 700, H, D, 5)
+    dlse = torch.randn(H, sum(lq), generator=torch.Generator().manual_seed(9))
     g = [x.to(DEV) for x in (q, k, v, do)]
     o, lse = A.overlapping_ranges_lse(*g[:3], qr, kr)
     got = A.overlapping_ranges_backward(g[3], *g[:3], o, lse, qr, kr, dlse=dlse.to(DEV))
