@@ -74,8 +74,17 @@ def _rows_for(x, H: int, D: int):
 _GRAD_SIZES = functools.lru_cache(256)(lambda *sizes: int(_L.lib().or_varlen_bwd_workspace_size(*sizes)))
 
 
-def _backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse=None, k_off=None, k_len=None):
-    """or_varlen_bwd on torch tensors: (dq, dk, dv), bf16 and contiguous"""
+def _index_pointers(q, *index):
+    """the addresses of a call's index arrays (None: no array)"""
+    at = q.get_device()
+    for x in index:
+        if x is not None and (x.dtype != torch.int32 or x.get_device() != at or not x.is_contiguous()):
+            raise _L.HipTypeError('index arrays must be contiguous int32 tensors on the GPU of q')
+    return [_L.ptr(x) for x in index]
+
+
+def _backward(do, q, k, v, o, lse, index, n_seg, max_q, max_k, dlse=None):
+    """or_varlen_bwd on torch tensors: (dq, dk, dv), bf16 and contiguous. index: the addresses of cu_q, cu_k, k_off, k_len"""
     _scene._check_bf16(do, q, k, v, o)
     if k.dim() != 3 or q.dim() != 3:
         raise _L.HipValueError('q, k and v must be [rows, heads, head_dim]')
@@ -85,9 +94,6 @@ def _backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse=None, k_off=No
     for x in (lse, dlse):
         if x is not None and (x.dtype != torch.float32 or x.shape != (H, n_q) or x.get_device() != at):
             raise _L.HipTypeError(f'lse and its gradient must be float32 [{H}, {n_q}] on the GPU of q')
-    for x in (cu_q, cu_k, k_off, k_len):
-        if x is not None and (x.dtype != torch.int32 or x.get_device() != at or not x.is_contiguous()):
-            raise _L.HipTypeError('index arrays must be contiguous int32 tensors on the GPU of q')
     if do.get_device() != at or k.get_device() != at or v.get_device() != at or o.get_device() != at:
         raise _L.HipTypeError('all tensors of a call must be on one GPU')
     (q, qs), (o, os_), (do, dos) = _rows_for(q, H, D), _rows_for(o, H, D), _rows_for(do, H, D)
@@ -98,15 +104,14 @@ def _backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse=None, k_off=No
     dlse = None if dlse is None else dlse.contiguous()
     new = lambda n: torch.empty(n, H, D, dtype=torch.bfloat16, device=dev)
     dq, dk, dv = new(n_q), new(n_k), new(n_k)
-    n_seg, max_q, max_k = cu_q.numel() - 1, int(max_q), int(max_k)
+    max_q, max_k = int(max_q), int(max_k)
     n = _GRAD_SIZES(n_seg, n_q, n_k, max_q, max_k, H, D)
     if n < 0:
         _L.check(_L.lib().or_varlen_bwd_workspace_size(n_seg, n_q, n_k, max_q, max_k, H, D), 'or_varlen_bwd_workspace_size')
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     p = _L.ptr
     a = _L.VarlenBwdArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), p(dlse),
-                         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_q.data_ptr(), p(cu_k), p(k_off), p(k_len),
-                         qs, ks, os_, dos, n_q, n_seg, n_q, n_k, max_q, max_k, H, D, D ** -0.5, ws.data_ptr(), n)
+                         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *index, qs, ks, os_, dos, n_q, n_seg, n_q, n_k, max_q, max_k, H, D, D ** -0.5, ws.data_ptr(), n)
     _L.check(_L.call(dev, _L.lib().or_varlen_bwd, ctypes.byref(a)), 'or_varlen_bwd')
     return dq, dk, dv
 
@@ -130,7 +135,8 @@ class _Attention(torch.autograd.Function):
         grads = (None,) * 3
         if do is not None or dlse is not None:
             do = torch.zeros_like(o) if do is None else do
-            grads = _backward(do, q, k, v, o, lse, cu_q, cu_k, *ctx.longest, dlse, k_off, k_len)
+            grads = _backward(do, q, k, v, o, lse, _index_pointers(q, cu_q, cu_k, k_off, k_len), cu_q.numel() - 1,
+                              *ctx.longest, dlse)
         return *grads, None, None, None, None, None, None
 
 
@@ -199,7 +205,8 @@ def varlen_backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse=None, ch
         check_cu_seqlens(cu_k, min(k.shape[0], v.shape[0]), max_k, 'cu_k')
     if cu_q.numel() != cu_k.numel():
         raise _L.HipValueError('cu_q and cu_k must hold one offset per segment boundary each')
-    return _backward(do, q, k, v, o, lse, cu_q, cu_k, max_q, max_k, dlse)
+    return _backward(do, q, k, v, o, lse, _index_pointers(q, cu_q, cu_k, None, None), cu_q.numel() - 1, max_q, max_k,
+                     dlse)
 
 
 def _concat_table(xs):
@@ -263,40 +270,50 @@ def packed(segments):
 
 
 def _range_args(q, k, v, q_ranges, k_ranges):
-    """(cu_q, key starts, key counts, most queries, most keys) of overlapping_ranges, checked"""
+    """(cu_q, key starts, key counts) of overlapping_ranges as lists, checked"""
     nq = [hi - lo for lo, hi in q_ranges]
-    starts = [lo for lo, _ in q_ranges]
-    if sum(nq) != q.shape[0] or any(lo != sum(nq[:j]) for j, lo in enumerate(starts)):
+    cu_q = _offsets(nq)
+    if cu_q[-1] != q.shape[0] or [lo for lo, _ in q_ranges] != cu_q[:-1]:
         raise _L.HipValueError('q_ranges must tile q in order')
     if len(k_ranges) != len(q_ranges):
         raise _L.HipValueError('q_ranges and k_ranges must pair up')
     n_k = min(k.shape[0], v.shape[0])
     if any(not 0 <= lo <= hi <= n_k for lo, hi in k_ranges):
         raise _L.HipValueError(f'k_ranges must lie inside the {n_k} rows of k and v')
-    nk = [hi - lo for lo, hi in k_ranges]
-    cu_q, k_start, k_count = _L.device_ints([_offsets(nq), [lo for lo, _ in k_ranges], nk], q.device)
-    return cu_q, k_start, k_count, max(nq), max(nk)
+    return cu_q, [lo for lo, _ in k_ranges], [hi - lo for lo, hi in k_ranges]
+
+
+def _ranges(q, k, v, q_ranges, k_ranges, lse):
+    cu_q, starts, counts = _range_args(q, k, v, q_ranges, k_ranges)
+    index = _L.device_ints([cu_q, starts, counts], q.device)
+    longest = max(hi - lo for lo, hi in q_ranges)
+    return _attend(q, k, v, index[0], None, longest, max(counts), *index[1:], lse=lse)
 
 
 def overlapping_ranges(q, k, v, q_ranges, k_ranges):
     """attention of q rows q_ranges[j] to k / v rows k_ranges[j] without copying k / v: the kernel reads the
     overlapping contiguous key ranges in place (per-segment key offset and length, as FA3's cu_seqlens_k offsets
     with seqused_k). q_ranges must tile q in order (attention.py:74-84)."""
-    cu_q, k_start, k_count, max_q, max_k = _range_args(q, k, v, q_ranges, k_ranges)
-    return _attend(q, k, v, cu_q, None, max_q, max_k, k_start, k_count)
+    return _ranges(q, k, v, q_ranges, k_ranges, False)
 
 
 def overlapping_ranges_lse(q, k, v, q_ranges, k_ranges):
     """overlapping_ranges with the softmax log-sum-exp: (out, lse [H, Nq] fp32), what its backward call needs"""
-    cu_q, k_start, k_count, max_q, max_k = _range_args(q, k, v, q_ranges, k_ranges)
-    return _attend(q, k, v, cu_q, None, max_q, max_k, k_start, k_count, lse=True)
+    return _ranges(q, k, v, q_ranges, k_ranges, True)
 
 
 def overlapping_ranges_backward(do, q, k, v, o, lse, q_ranges, k_ranges, dlse=None):
     """the gradient of overlapping_ranges / overlapping_ranges_lse, as varlen_backward: a row of k and v sums the
     gradients of every range that reads it"""
-    cu_q, k_start, k_count, max_q, max_k = _range_args(q, k, v, q_ranges, k_ranges)
-    return _backward(do, q, k, v, o, lse, cu_q, None, max_q, max_k, dlse, k_start, k_count)
+    cu_q, starts, counts = _range_args(q, k, v, q_ranges, k_ranges)
+    if not q.is_cuda:
+        raise _L.HipTypeError(f'expected a bf16 GPU tensor, got {q.dtype} on {q.device}')
+    values = array.array('i', cu_q + starts + counts)
+    index, n = torch.empty(len(values), dtype=torch.int32, device=q.device), len(starts)
+    at = index.data_ptr()
+    _L.check(_L.call(q.device, _L.lib().or_index_fill, values.buffer_info()[0], len(values), at), 'or_index_fill')
+    return _backward(do, q, k, v, o, lse, (at, None, at + 4 * n + 4, at + 8 * n + 4), n,
+                     max(hi - lo for lo, hi in q_ranges), max(counts), dlse)
 
 
 def merge_lse(o, lse, o_s, lse_s):
