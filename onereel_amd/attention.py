@@ -15,6 +15,7 @@ import array
 import ctypes
 import functools
 import operator
+import warnings
 
 import torch
 
@@ -50,13 +51,24 @@ def wants_grad(*xs) -> bool:
     return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in xs)
 
 
-def refuse_captured_leaves(what: str, *xs):
-    """A backward pass recorded into a graph adds into its leaves' gradients on the stream of the first pass that used
-    them; when that is another stream (an eager pass whose graph still lives), the capture ends the process. So a call
-    under capture takes no leaves that require gradients; the backward entry points without autograd can be captured."""
-    if any(x is not None and x.requires_grad and x.is_leaf for x in xs) and torch.cuda.is_current_stream_capturing():
-        raise _L.HipValueError(f'{what}: a leaf that requires a gradient cannot be differentiated under graph capture: '
-                               f'capture the call without autograd and its backward entry point')
+def captured_leaves(*xs) -> bool:
+    """Whether this call is being captured and one of xs is a leaf that requires a gradient. A backward pass recorded into a
+    graph adds into its leaves' gradients on the stream of the first pass that used them; when that is another stream (an
+    eager pass whose graph still lives), the capture ends the process. So autograd records no such call; the backward entry
+    points without autograd can be captured."""
+    return any(x is not None and x.requires_grad and x.is_leaf for x in xs) and torch.cuda.is_current_stream_capturing()
+
+
+def records(what: str, *xs) -> bool:
+    """whether a call on these tensors is recorded by autograd: when wants_grad says so, but for captured_leaves, whose call
+    runs as it does without autograd (with a warning)"""
+    if not wants_grad(*xs):
+        return False
+    if captured_leaves(*xs):
+        warnings.warn(f'{what}: under graph capture a call on leaves that require gradients is not recorded: capture the '
+                      f'backward entry point instead', stacklevel=3)
+        return False
+    return True
 
 
 def _rows_for(x, H: int, D: int):
@@ -142,8 +154,7 @@ class _Attention(torch.autograd.Function):
 
 def _attend(q, k, v, cu_q, cu_k, max_q, max_k, k_off=None, k_len=None, lse=False):
     """the varlen call of every entry point: o, or (o, lse)"""
-    if wants_grad(q, k, v):
-        refuse_captured_leaves('attention', q, k, v)
+    if records('attention', q, k, v):
         o, l = _Attention.apply(q, k, v, cu_q, cu_k, k_off, k_len, max_q, max_k)
         return (o, l) if lse else o
     l = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if lse else None

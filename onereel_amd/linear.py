@@ -13,7 +13,7 @@ import functools
 import torch
 
 from . import _lib as L
-from .attention import refuse_captured_leaves, wants_grad
+from .attention import captured_leaves, wants_grad
 
 
 def _activation(name) -> int:
@@ -104,7 +104,9 @@ def linear(x, weight, bias=None, activation=None, gate=None, residual=None, keep
     for the gate's gradient."""
     act = _activation(activation)
     if wants_grad(x, weight, bias, gate, residual):
-        refuse_captured_leaves('linear', x, weight, bias, gate, residual)
+        if captured_leaves(x, weight, bias, gate, residual):
+            raise L.HipValueError('linear: a leaf that requires a gradient cannot be differentiated under graph capture: '
+                                  'capture the call without autograd, and linear_backward')
         y, z = _Linear.apply(x, weight, bias, activation, gate, residual, bool(keep_preactivation))
         return (y, z) if keep_preactivation else y
     y, z = _forward(x, weight, bias, act, gate, residual, bool(keep_preactivation))

@@ -55,8 +55,7 @@ def _qk(q, k, wq, wk, eps: float, cos, sin, heads: int):
         raise L.HipValueError(f'q / k of width {C} do not split into {heads} heads (k {tuple(k.shape)})')
     if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16:
         raise L.HipTypeError('q and k must be bfloat16')
-    if A.wants_grad(q, k, wq, wk):
-        A.refuse_captured_leaves('_qk', q, k, wq, wk)
+    if A.records('_qk', q, k, wq, wk):
         return _QK.apply(q, k, wq, wk, eps, cos, sin, heads)
     return _qk_forward(q, k, wq, wk, eps, cos, sin, heads)
 
@@ -90,8 +89,7 @@ def rms_norm(x, weight, eps: float):
     C = x.shape[-1]
     if x.dtype != torch.bfloat16:
         raise L.HipTypeError('x must be bfloat16')
-    if A.wants_grad(x, weight):
-        A.refuse_captured_leaves('rms_norm', x, weight)
+    if A.records('rms_norm', x, weight):
         return _RMSNorm.apply(x, weight, eps)
     x2 = x.reshape(-1, C)
     if x2.stride(1) != 1:

@@ -243,18 +243,30 @@ def test_graph_replays_and_two_graphs():
             assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
 
 
-def test_capture_refuses_leaves():
+def test_capture_does_not_record_leaves():
+    """a captured call on leaves that require gradients runs as without autograd, and says so"""
     print('capture of leaves', flush=True)
     x = [t.to(DEV).requires_grad_() for t in inputs(40, 40, 1, 64)[:3]]
     cu = torch.tensor([0, 40], dtype=torch.int32, device=DEV)
-    keep = torch.ones(4, device=DEV)
+    with torch.no_grad():
+        want = A.varlen(*x, cu, cu, 40, 40)
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
-        keep.add_(1)
-        with pytest.raises(A._L.HipValueError, match='leaf'):
-            A.varlen(*x, cu, cu, 40, 40, check=False)
-    g.replay()
-    torch.cuda.synchronize()
+        with pytest.warns(UserWarning, match='leaves'):
+            out = A.varlen(*x, cu, cu, 40, 40, check=False)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert not out.requires_grad and torch.equal(out, want)
+
+
+@pytest.mark.parametrize('nq,nk', [(0, 70), (70, 0), (0, 0)])
+def test_no_rows_at_all(nq, nk):
+    print(f'no rows {nq} {nk}', flush=True)
+    q, k, v, do = (x.to(DEV) for x in inputs(nq, nk, 2, 128))
+    cq, ck = (torch.tensor([0, n, n], dtype=torch.int32, device=DEV) for n in (nq, nk))
+    got = A.varlen_backward(do, q, k, v, q.clone(), torch.zeros(2, nq, device=DEV), cq, ck, nq, nk)
+    assert [x.shape for x in got] == [q.shape, k.shape, v.shape] and not any(x.any() for x in got)
 
 
 def test_another_stream():

@@ -197,6 +197,32 @@ def test_autograd():
     assert (num - (grads[0].double().view(90, 64) * d).sum()).abs() <= room
 
 
+def test_capture_refuses_leaves():
+    print('capture of leaves', flush=True)
+    x, w, *_ = inputs(40, 64, 48)
+    w.requires_grad_()
+    keep = torch.ones(4, device=DEV)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        keep.add_(1)
+        with pytest.raises(F.L.HipValueError, match='leaf'):
+            F.linear(x, w)
+    g.replay()
+    torch.cuda.synchronize()
+
+
+def test_transposed_weight_and_one_row_of_a_wider_tensor():
+    print('odd layouts', flush=True)
+    x, w, *_ = inputs(70, 64, 48, 2)
+    wt = w.t().contiguous().t()
+    assert torch.equal(F.linear(x, wt), F.linear(x, w))
+    one = x[:1, :].expand(5, 64)[2:3]
+    assert torch.equal(F.linear(one, w), F.linear(x[:1], w))
+    dy = rand_bf16((70, 48), 1).to(DEV)
+    got = F.linear_backward(dy.t().contiguous().t(), x, wt, bias=True)
+    assert all(torch.equal(a, b) for a, b in zip(got[:3], F.linear_backward(dy, x, w, bias=True)))
+
+
 def test_graph_replays():
     print('graph', flush=True)
     M, K, N = 700, 1024, 136                   # few tiles: both passes split their k axis
