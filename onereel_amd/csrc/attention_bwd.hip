@@ -16,7 +16,7 @@
 //   Their A operand is the streamed block transposed, read from the same slot by transposing LDS reads. The slot's
 //   swizzle serves both kinds of read without bank conflicts.
 // - P and dS are rounded to bf16 once, as the operands of the bf16 matrix cores (the forward pass rounds its P the same way);
-//   scores, P, dS, delta and all sums are fp32.
+//   scores, P, dS, delta and all sums are fp32. Calls of few scores carry what that rounding leaves out in a second product.
 // - Key rows may belong to several segments (overlapping ranges): the key axis is cut at every range boundary, so that all
 //   rows of a key tile have the same segments, and the tile streams the queries of all of them. Rows past an end load as
 //   zeros: a zero query row adds nothing to dk and dv, and the scores of key rows past the end are set to P = 0.
@@ -414,6 +414,16 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& x, int half) {
   return __builtin_bit_cast(bf16x8, y);
 }
 
+// what the rounding of pack8(x, half) left out, rounded itself
+__device__ __forceinline__ bf16x8 pack8_rest(const f32x16& x, int half, bf16x8 rounded) {
+  const u32x4 r = __builtin_bit_cast(u32x4, rounded);
+  u32x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    y[i] = pack2(x[8 * half + 2 * i] - bf2f((uint16_t)(r[i] & 0xffffu)), x[8 * half + 2 * i + 1] - bf2f((uint16_t)(r[i] >> 16)));
+  return __builtin_bit_cast(bf16x8, y);
+}
+
 // operand of 32 owned rows: 8 dims 16 ks + 8 (lane / 32) of row lane % 32, zeros past `rows`
 template <int D>
 __device__ __forceinline__ void load_owned(bf16x8 (&f)[Str<D>::KS], const uint16_t* p, int64_t rs, int rows, int lane) {
@@ -463,8 +473,8 @@ __device__ __forceinline__ int64_t xcd_item(int64_t n, unsigned block) {
 
 // ------------------------------------------------------------------------------------------------------------------
 // dq: a block owns 128 T queries of one head and streams the keys and values of their segment
-template <int D, bool FEW>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void bwd_q_kernel(BwdArgs a) {
+template <int D, bool FEW, bool FINE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ? 1 : 2, 2))) void bwd_q_kernel(BwdArgs a) {
   using C = Str<D>;
   constexpr int T = query_blocks(D);
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT];
@@ -582,13 +592,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[t][e] = 8 * (e >> 2) + (e & 3) < n ? s[t][e] : 0.0f;
     }
-    bf16x8 ds[T][2];
+    bf16x8 ds[T][2], rest[T][2];
 #pragma unroll
     for (int t = 0; t < T; ++t) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[t][e] = s[t][e] * (dp[t][e] + neg_delta[t]);
 #pragma unroll
-      for (int hs = 0; hs < 2; ++hs) ds[t][hs] = pack8(dp[t], hs);
+      for (int hs = 0; hs < 2; ++hs) {
+        ds[t][hs] = pack8(dp[t], hs);
+        if constexpr (FINE) rest[t][hs] = pack8_rest(dp[t], hs, ds[t][hs]);
+      }
     }
 #pragma unroll
     for (int db = 0; db < C::DB; ++db)
@@ -596,7 +609,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       for (int hs = 0; hs < 2; ++hs) {
         const bf16x8 kt = tr_frag<D>(tr, db, hs, 0);
 #pragma unroll
-        for (int t = 0; t < T; ++t) acc[t][db] = mfma(kt, ds[t][hs], acc[t][db]);
+        for (int t = 0; t < T; ++t) {
+          acc[t][db] = mfma(kt, ds[t][hs], acc[t][db]);
+          if constexpr (FINE) acc[t][db] = mfma(kt, rest[t][hs], acc[t][db]);
+        }
       }
   };
   int b = b0;
@@ -637,8 +653,8 @@ struct Walk {
   }
 };
 
-template <int D>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))) void bwd_kv_kernel(BwdArgs a) {
+template <int D, bool FINE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ? 1 : 2, 4))) void bwd_kv_kernel(BwdArgs a) {
   using C = Str<D>;
   constexpr int kStat = 256;         // bytes of one wavefront's statistics of a block
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT + kRing * 4 * kStat];
@@ -748,7 +764,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
     }
     __builtin_amdgcn_s_setprio(0);
     // by halves: the first half's registers hold the first transposed operands while the second half is worked on
-    bf16x8 p[2], ds[2], ft[2][2];
+    bf16x8 p[2], ds[2], p_rest[2], ds_rest[2], ft[2][2];
 #pragma unroll
     for (int hs = 0; hs < 2; ++hs) {
 #pragma unroll
@@ -758,6 +774,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
       }
       p[hs] = pack8(s, hs);
       ds[hs] = pack8(dp, hs);
+      if constexpr (FINE) {
+        p_rest[hs] = pack8_rest(s, hs, p[hs]);
+        ds_rest[hs] = pack8_rest(dp, hs, ds[hs]);
+      }
       ft[hs][0] = tr_frag<D>(tr, hs % C::DB, hs / C::DB, kRing * C::SLOT);
       ft[hs][1] = tr_frag<D>(tr, hs % C::DB, hs / C::DB, 0);
       __builtin_amdgcn_sched_barrier(0);
@@ -768,6 +788,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 4))
       const int db = i % C::DB, hs = i / C::DB, n = i + 2;
       dv[db] = mfma(ft[i & 1][0], p[hs], dv[db]);
       dk[db] = mfma(ft[i & 1][1], ds[hs], dk[db]);
+      if constexpr (FINE) {
+        dv[db] = mfma(ft[i & 1][0], p_rest[hs], dv[db]);
+        dk[db] = mfma(ft[i & 1][1], ds_rest[hs], dk[db]);
+      }
       if (n < 2 * C::DB) {
         ft[i & 1][0] = tr_frag<D>(tr, n % C::DB, n / C::DB, kRing * C::SLOT);
         ft[i & 1][1] = tr_frag<D>(tr, n % C::DB, n / C::DB, 0);
@@ -863,17 +887,27 @@ Layout layout_of(const Shape& s, int32_t n_q, int32_t n_k, int32_t H, int32_t D)
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-template <int D>
+template <int D, bool FINE>
 void launch(const BwdArgs& a, const Shape& s, hipStream_t st) {
   auto grid = [](int64_t items) { return dim3((unsigned)((items + 7) / 8 * 8)); };
   const dim3 gq = grid(s.max_q_tiles * a.H * s.split_q), gk = grid(s.max_k_tiles * a.H * s.split_k), t(kThreads);
   if (a.n_seg <= kFewSeg) {
-    hipLaunchKernelGGL((bwd_q_kernel<D, true>), dim3(gq.x + 8), t, 0, st, a);
+    hipLaunchKernelGGL((bwd_q_kernel<D, true, FINE>), dim3(gq.x + 8), t, 0, st, a);
   } else {
     hipLaunchKernelGGL(bwd_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
-    if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, false>), gq, t, 0, st, a);
+    if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, false, FINE>), gq, t, 0, st, a);
   }
-  if (a.n_k > 0) hipLaunchKernelGGL((bwd_kv_kernel<D>), gk, t, 0, st, a);
+  if (a.n_k > 0) hipLaunchKernelGGL((bwd_kv_kernel<D, FINE>), gk, t, 0, st, a);
+}
+
+// Whether P and dS go into their products as two bf16 numbers, the rounded value and what that rounding left out: in calls
+// of few scores, which latency bounds. A result rounded once has its own rounding and that of its operand, 1.41 times the
+// error of its own rounding alone with many scores and up to 1.55 times with few, where the roundings do not average out;
+// with the second product it is 1.00 times. Kernel times with one product / two: 13.5 / 14.2 us at 2 heads x 64 x 64
+// scores (D 64), 18.8 / 20.3 at 4 x 128 x 128; above the limit 31.5 / 35.6 at 8 x 256 x 256 (D 128), 75.8 / 87.0 at
+// 8 x 1400 x 1400.
+bool is_fine(const or_varlen_bwd_args& x) {
+  return (int64_t)x.H * x.n_q * x.max_k <= (int64_t)1 << 18;
 }
 
 }  // namespace
@@ -961,8 +995,9 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
   a.part_q = (float*)(ws + l.part_q);
   a.part_k = (float*)(ws + l.part_k);
   hipStream_t st = (hipStream_t)stream;
-  if (x.D == 128) launch<128>(a, s, st);
-  else launch<64>(a, s, st);
+  const bool fine = is_fine(x);
+  if (x.D == 128) fine ? launch<128, true>(a, s, st) : launch<128, false>(a, s, st);
+  else fine ? launch<64, true>(a, s, st) : launch<64, false>(a, s, st);
   const int64_t q8 = s.split_q > 1 ? (int64_t)x.n_q * row / 8 : 0, k8 = s.split_k > 1 ? (int64_t)x.n_k * row / 8 : 0;
   if (q8 + k8 > 0) {
     const int64_t blocks = std::min<int64_t>((q8 + 2 * k8 + kThreads - 1) / kThreads, 4096);

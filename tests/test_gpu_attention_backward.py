@@ -102,6 +102,35 @@ def test_varlen_backward(lq, lk, H, D):
     assert all(torch.equal(x, y) for x, y in zip(got, again))
 
 
+@pytest.mark.parametrize('n,m,H,D', [(1, 3, 2, 64), (64, 64, 2, 64), (111, 77, 3, 128), (300, 5, 4, 64), (5, 700, 8, 128)])
+def test_few_scores_round_only_the_result(n, m, H, D):
+    """P and dS as two bf16 numbers each: what is left out of an operand is 2^-16 of it, half a step of half a step. fp32 around
+    them: scores, dP and delta of D products and a sum, at most (D + 2) 2^-24 of their terms' sum (for a score: its absolute
+    error, hence the relative error of P), 2^-20 for the exponent's own arithmetic (lse and scores below 16, exp2, the
+    factor log2 e) and (n + 2) 2^-24 for the sums over rows. So beside the result's own half step:
+    |error| <= e_p sum P |do| for dv, e_p sum |dS| |k| + (D + 2) 2^-24 sum P (|do| |v| + |do o|) |k| for dq, and so for dk."""
+    print(f'few scores {n} x {m} H={H} D={D}', flush=True)
+    q, k, v, do = inputs(n, m, H, D)
+    g = [x.to(DEV) for x in (q, k, v, do)]
+    (_, cq), (_, ck) = cut([n]), cut([m])
+    args = (cq.to(DEV), ck.to(DEV), n, m)
+    o, lse = A.varlen_lse(*g[:3], *args)
+    got = A.varlen_backward(g[3], *g[:3], o, lse, *args)
+    qh, kh, vh, doh, oh = (x.cpu().double().transpose(0, 1) for x in (q, k, v, do, o))
+    scale = D ** -0.5
+    p = torch.exp(qh @ kh.transpose(1, 2) * scale - lse.cpu().double()[:, :, None])
+    ds = p * (doh @ vh.transpose(1, 2) - (doh * oh).sum(2)[:, :, None])
+    fp32 = (D + 2) * 2 ** -24
+    e_p = 2 ** -16 + fp32 * scale * (qh.abs() @ kh.abs().transpose(1, 2)).max().item() + 2 ** -20 + (max(n, m) + 2) * 2 ** -24
+    ds_err = e_p * ds.abs() + fp32 * p * (doh.abs() @ vh.abs().transpose(1, 2) + (doh * oh).abs().sum(2)[:, :, None])
+    for name, x, want, err in (('dq', got[0], ds @ kh * scale, ds_err @ kh.abs() * scale),
+                               ('dk', got[1], ds.transpose(1, 2) @ qh * scale, ds_err.transpose(1, 2) @ qh.abs() * scale),
+                               ('dv', got[2], p.transpose(1, 2) @ doh, e_p * p.transpose(1, 2) @ doh.abs())):
+        off = (x.cpu().double().transpose(0, 1) - want).abs()
+        worst = (off - HALF * want.abs() - (1 + HALF) * err).max().item()
+        assert worst <= 1e-30, f'{name}: {worst:.3e} past the bound (max error {off.max():.3e})'
+
+
 @pytest.mark.parametrize('H', [2, 96])
 @pytest.mark.parametrize('D', [64, 128])
 def test_ranges_backward_shares_key_rows(D, H):
