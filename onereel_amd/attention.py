@@ -71,6 +71,15 @@ def records(what: str, *xs) -> bool:
     return True
 
 
+def unrecorded_capture(what: str, *xs):
+    """xs, detached where records would not have autograd record a call on them, for entry points that reshape or
+    concatenate them first: what that makes of a leaf is none"""
+    return [x.detach() for x in xs] if wants_grad(*xs) and not records(what, *xs) else xs
+
+
+_MAX_STRIDE = 1 << 24      # of or_varlen_bwd's rows
+
+
 def _rows_for(x, H: int, D: int):
     """(x, row stride), x itself where its rows are as the kernels read them, else a copy (a gradient may come expanded or
     transposed)"""
@@ -78,7 +87,7 @@ def _rows_for(x, H: int, D: int):
     if len(shape) != 3 or shape[1] != H or shape[2] != D:
         raise _L.HipValueError(f'expected [rows, {H}, {D}], got {tuple(shape)}')
     row = stride[0]
-    if stride[2] == 1 and stride[1] == D and row >= H * D and row % 8 == 0 and x.data_ptr() % 16 == 0:
+    if stride[2] == 1 and stride[1] == D and H * D <= row <= _MAX_STRIDE and row % 8 == 0 and x.data_ptr() % 16 == 0:
         return x, row
     return (x, H * D) if not shape[0] else (x.clone(memory_format=torch.contiguous_format), H * D)
 
@@ -100,9 +109,12 @@ def _backward(do, q, k, v, o, lse, index, n_seg, max_q, max_k, dlse=None):
     _scene._check_bf16(do, q, k, v, o)
     if k.dim() != 3 or q.dim() != 3:
         raise _L.HipValueError('q, k and v must be [rows, heads, head_dim]')
-    (n_q, H, D), n_k, dev, at = q.shape, k.shape[0], q.device, q.get_device()
-    if v.shape[0] != n_k or o.shape[0] != n_q or do.shape[0] != n_q:
-        raise _L.HipValueError('q, o and do must have the same rows, and k and v')
+    (n_q, H, D), more_k, more_v, dev, at = q.shape, k.shape[0], v.shape[0], q.device, q.get_device()
+    if o.shape[0] != n_q or do.shape[0] != n_q:
+        raise _L.HipValueError('q, o and do must have the same rows')
+    n_k = min(more_k, more_v)
+    if more_k != more_v:     # rows that only one of them has are read by no segment
+        k, v = k[:n_k], v[:n_k]
     for x in (lse, dlse):
         if x is not None and (x.dtype != torch.float32 or x.shape != (H, n_q) or x.get_device() != at):
             raise _L.HipTypeError(f'lse and its gradient must be float32 [{H}, {n_q}] on the GPU of q')
@@ -115,7 +127,9 @@ def _backward(do, q, k, v, o, lse, index, n_seg, max_q, max_k, dlse=None):
     lse = lse.contiguous()
     dlse = None if dlse is None else dlse.contiguous()
     new = lambda n: torch.empty(n, H, D, dtype=torch.bfloat16, device=dev)
-    dq, dk, dv = new(n_q), new(n_k), new(n_k)
+    dq, dk, dv = new(n_q), new(more_k), new(more_v)
+    if more_k != more_v:
+        (dk if more_k > n_k else dv)[n_k:].zero_()
     max_q, max_k = int(max_q), int(max_k)
     n = _GRAD_SIZES(n_seg, n_q, n_k, max_q, max_k, H, D)
     if n < 0:
@@ -123,7 +137,8 @@ def _backward(do, q, k, v, o, lse, index, n_seg, max_q, max_k, dlse=None):
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     p = _L.ptr
     a = _L.VarlenBwdArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), p(dlse),
-                         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *index, qs, ks, os_, dos, n_q, n_seg, n_q, n_k, max_q, max_k, H, D, D ** -0.5, ws.data_ptr(), n)
+                         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *index, qs, ks, os_, dos, n_q, n_seg, n_q, n_k, max_q,
+                         max_k, H, D, D ** -0.5, ws.data_ptr(), n)
     _L.check(_L.call(dev, _L.lib().or_varlen_bwd, ctypes.byref(a)), 'or_varlen_bwd')
     return dq, dk, dv
 
@@ -166,6 +181,7 @@ def dense(q, k, v):
     """q, k, v [B, S, H, D] -> [B, S, H, D] (attention.py:32-36)"""
     B, S, H, D = q.shape
     Sk = k.shape[1]
+    q, k, v = unrecorded_capture('dense', q, k, v)
     cu_q, cu_k = _L.device_ints([_offsets([S] * B), _offsets([Sk] * B)], q.device)
     o = _attend(q.reshape(B * S, H, D), k.reshape(B * Sk, H, D), v.reshape(B * Sk, H, D), cu_q, cu_k, S, Sk)
     return o.view(B, S, H, D)
@@ -239,6 +255,10 @@ def _concat(segments):
     """the segments' q, k and v end to end, as the varlen call takes them, and the query count of each segment"""
     qs, ks, vs = zip(*segments)
     n, dev = len(qs), qs[0].device
+    grad = wants_grad(*qs, *ks, *vs)
+    if grad:
+        xs = unrecorded_capture('packed', *qs, *ks, *vs)
+        qs, ks, vs, grad = xs[:n], xs[n:2 * n], xs[2 * n:], wants_grad(*xs)
     # past one launch of or_concat (112 sequences) the host is what counts, and torch.cat needs less of it per tensor (225
     # sequences of 20 rows x 16 x 128: 297 us a call with or_concat, 258 so), unless the sequences are long enough for the
     # GPU to be the slower side (300 of 100 rows: 428 and 594, of 300: 984 and 1453)
@@ -247,7 +267,7 @@ def _concat(segments):
         nq, nk = [x.shape[0] for x in qs], [x.shape[0] for x in ks]
     long = n <= 112 or (sum(nq) + 2 * sum(nk)) * qs[0].shape[1:].numel() >= n << 19
     # autograd records torch.cat
-    table = _concat_table(qs + ks + vs) if long and not wants_grad(*qs, *ks, *vs) else None
+    table = _concat_table(qs + ks + vs) if long and not grad else None
     if table is not None and table[1][n:2 * n] == table[1][2 * n:] and sum(table[1]) < 2 ** 31:
         at, rows, *row = table
         nq, nk = rows[:n], rows[n:2 * n]

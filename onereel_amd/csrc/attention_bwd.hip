@@ -67,7 +67,7 @@ struct BwdArgs {
   i32x4* q_tiles;                    // first query, rows, first key, keys
   i32x4* k_tiles;                    // two a tile: first key, rows, first and last segment that may read them; first query and
                                      // queries of the segment where only one may
-  float* stat;                       // [2][H][n_q]: -lse / scale, then -delta
+  float* stat;                       // [H][2][n_q]: -lse / scale, then -delta
   float* part_q;                     // [split_q][n_q][H][D]
   float* part_k;                     // [split_k][2][n_k][H][D]: dk, then dv
 };
@@ -356,7 +356,7 @@ __device__ __forceinline__ void dma_rows(const uint16_t* base, int64_t rs, int r
                  : "memory");
 }
 
-// 64 statistics (32 rows of two arrays n elements apart) into LDS, zeros past `rows`
+// 64 statistics (32 rows of two arrays `apart` elements apart) into LDS, zeros past `rows`
 __device__ __forceinline__ void dma_stats(const float* base, int64_t apart, int rows, int lane, uint32_t m0) {
   const uint64_t b = (uint64_t)base;
   const i32x4 r = {__builtin_amdgcn_readfirstlane((int32_t)(uint32_t)b),
@@ -554,8 +554,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
     neg_lse[t] = -l * kLog2e;
     neg_delta[t] = -d;
     if (mine && lane < 32 && part == 0) {
-      a.stat[(int64_t)head * a.n_q + at] = -l / a.scale;
-      a.stat[(int64_t)(a.H + head) * a.n_q + at] = -d;
+      a.stat[(int64_t)2 * head * a.n_q + at] = -l / a.scale;
+      a.stat[(int64_t)(2 * head + 1) * a.n_q + at] = -d;
     }
 #pragma unroll
     for (int db = 0; db < C::DB; ++db)
@@ -705,7 +705,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
     const uint32_t at = m0 + slot * C::SLOT;
     dma_rows<D>(a.q + r * a.qs + (int64_t)head * D, a.qs, n, voq, at);
     dma_rows<D>(a.d_o + r * a.dos + (int64_t)head * D, a.dos, n, vod, at + kRing * C::SLOT);
-    dma_stats(a.stat + (int64_t)head * a.n_q + r, (int64_t)a.H * a.n_q, n, lane, st0 + slot * 4 * kStat);
+    dma_stats(a.stat + (int64_t)2 * head * a.n_q + r, a.n_q, n, lane, st0 + slot * 4 * kStat);
     walk.row += kBlk;
     walk.left -= kBlk;
   };
@@ -951,10 +951,9 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
   const Layout l = layout_of(s, x.n_q, x.n_k, x.H, x.D);
   if (!x.workspace || x.workspace_bytes < l.bytes || !aligned16(x.workspace))
     return fail_arg("or_varlen_bwd: a 16-byte aligned workspace of %lld bytes is needed", (long long)l.bytes);
-  // the second array of statistics lies 4 H n_q bytes after the first, within the 32 bits of a buffer offset
-  if ((int64_t)x.H * x.n_q * 4 + 256 >= (int64_t)0x7fffffff)
-    return fail_arg("or_varlen_bwd: H * n_q must stay under 2^29");
-  if (std::max(s.max_q_tiles * s.split_q, s.max_k_tiles * s.split_k) * x.H >= (int64_t)0x7fffffe0)
+  // a head's second row of statistics lies 4 n_q bytes after the first, within the 32 bits of a buffer offset
+  if ((int64_t)x.n_q * 4 + 256 >= (int64_t)0x7fffffff) return fail_arg("or_varlen_bwd: n_q must stay under 2^29");
+  if (std::max(s.max_q_tiles * s.split_q, s.max_k_tiles * s.split_k) * x.H >= (int64_t)1 << 24)   // 2^32 threads
     return fail_arg("or_varlen_bwd: too many tiles");
   char* ws = (char*)x.workspace;
   BwdArgs a;

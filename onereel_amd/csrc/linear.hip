@@ -575,6 +575,7 @@ struct Plan {
 // with two of 64 x 64 and one (128 x 8192 x 2048: 11 us). A work-group's start and epilogue count as 3 steps. Parts of k add
 // the launch that joins them and its traffic (1536 x 8192 in 2 parts: 19 us).
 constexpr int kCUs = 256;
+constexpr int64_t kMaxBlocks = ((int64_t)1 << 23) - 8;   // of 512 threads: a grid has under 2^32
 Plan plan_of(int64_t I, int64_t J, int64_t K, bool rows_of_k) {
   Plan p = {};
   p.split = 1;
@@ -585,6 +586,7 @@ Plan plan_of(int64_t I, int64_t J, int64_t K, bool rows_of_k) {
     const int64_t ti = (I + tile - 1) / tile, tj = (J + tile - 1) / tile;
     for (int split : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
       if (split > 1 && steps / split < 4) break;
+      if (ti * tj * split > kMaxBlocks) break;
       const int64_t n = ti * tj * split, two = (n + 2 * kCUs - 1) / (2 * kCUs);
       const double step = tile == 256 ? 1.6 * ((n + kCUs - 1) / kCUs)
                           : tile == 128 ? (n <= kCUs ? 0.6 : 1.05 * two) : (n <= kCUs ? 0.32 : 0.43 * two);
@@ -637,13 +639,12 @@ bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 int check_sizes(const char* what, int64_t M, int32_t N, int32_t K, int32_t act) {
-  if (M < 0 || M >= (int64_t)1 << 31) return fail_arg("%s: 0 to 2^31 - 1 rows (got %lld)", what, (long long)M);
+  if (M < 0 || M > (int64_t)1 << 30) return fail_arg("%s: 0 to 2^30 rows (got %lld)", what, (long long)M);
   if (N < 8 || N % 8 || K < 8 || K % 8 || N > kMaxStride || K > kMaxStride)
     return fail_arg("%s: n_in and n_out must be multiples of 8 up to 2^21 (got %d and %d)", what, K, N);
   if (act != OR_ACT_NONE && act != OR_ACT_GELU_TANH && act != OR_ACT_SILU) return fail_arg("%s: unknown activation %d", what, act);
-  // tiles of 64 in a grid of 32 bits
-  if ((M + 63) / 64 * ((N + 63) / 64) >= (int64_t)1 << 30 || (M + 63) / 64 * ((K + 63) / 64) >= (int64_t)1 << 30)
-    return fail_arg("%s: too many tiles", what);
+  for (int64_t width : {N, K})
+    if ((M + 255) / 256 * ((width + 255) / 256) > kMaxBlocks) return fail_arg("%s: too many tiles", what);
   return 0;
 }
 
@@ -653,11 +654,11 @@ int bad_stride(const char* what, int64_t stride, int64_t width) {
   return 0;
 }
 
-// rows of a work-group of dz_kernel: a multiple of the 8 it takes at once
+// rows of a work-group of dz_kernel: a multiple of the 8 it takes at once, and at most 65535 groups of them
 int chunk_rows_of(int64_t M, int32_t N) {
   const int64_t chunks = (1024 + (N + 255) / 256 - 1) / ((N + 255) / 256);
   const int64_t rows = ((M + chunks - 1) / chunks + 7) / 8 * 8;
-  return (int)std::max<int64_t>(8, std::min<int64_t>(rows, 128));
+  return (int)std::max<int64_t>({8, std::min<int64_t>(rows, 128), (M + 65534) / 65535 + 7 & ~(int64_t)7});
 }
 
 struct BwdLayout {
@@ -760,7 +761,6 @@ extern "C" int or_linear_bwd(const or_linear_bwd_args* p, void* stream) {
     d.N = x.n_out;
     d.act = x.activation;
     d.chunk_rows = chunk_rows_of(x.n_rows, x.n_out);
-    if (x.n_rows > (int64_t)65535 * 128) return fail_arg("or_linear_bwd: at most %d rows", 65535 * 128);
     d.chunks = (int)((x.n_rows + d.chunk_rows - 1) / d.chunk_rows);
     if (d.chunks > 0)
       hipLaunchKernelGGL(dz_kernel, dim3((unsigned)((x.n_out + 255) / 256), (unsigned)d.chunks), dim3(kThreads), 0, st, d);

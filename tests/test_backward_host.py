@@ -92,6 +92,9 @@ def test_gradient_rows_are_copied_only_where_they_must_be():
         y, stride = A._rows_for(odd, 2, 64)
         assert stride == 128 and y.is_contiguous() and (y.data_ptr() == odd.data_ptr()) == odd.is_contiguous()
     assert A._rows_for(x[:0], 2, 64)[1] == 128
+    far = torch.zeros((1 << 24) + 136, dtype=torch.bfloat16).as_strided((2, 2, 64), ((1 << 24) + 8, 64, 1))
+    y, stride = A._rows_for(far, 2, 64)     # rows further apart than or_varlen_bwd takes
+    assert stride == 128 and y.is_contiguous() and torch.equal(y, far)
     with pytest.raises(L.HipValueError):
         A._rows_for(x, 2, 32)
 
@@ -156,6 +159,7 @@ def linear_args(**kw):
     (dict(x_row_stride=56), 'strides'), (dict(weight_row_stride=68), 'strides'), (dict(y_row_stride=1 << 22), 'strides'),
     (dict(residual_row_stride=64), 'strides'), (dict(bias=4100), 'aligned'), (dict(preactivation=4104), 'aligned'),
     (dict(workspace=None), 'workspace'), (dict(workspace_bytes=10), 'workspace'),
+    (dict(n_rows=1 << 31), 'rows'), (dict(n_rows=1 << 30, n_in=1 << 12, x_row_stride=1 << 12, weight_row_stride=1 << 12), 'tiles'),
 ])
 def test_linear_refuses(kw, message):
     with pytest.raises(L.HipPathError, match=message):
@@ -179,7 +183,8 @@ def linear_bwd_args(**kw):
     (dict(weight=None), 'dx needs'), (dict(x=None), 'dweight needs'), (dict(gate=None), 'dgate needs'),
     (dict(preactivation=None), 'pre-activation'), (dict(preactivation=None, activation=0), 'pre-activation'),
     (dict(dy_row_stride=120), 'strides'), (dict(x_row_stride=8), 'strides'), (dict(dx=4098), 'aligned'),
-    (dict(workspace_bytes=10), 'workspace'), (dict(n_rows=65535 * 128 + 1), 'at most'),
+    (dict(workspace_bytes=10), 'workspace'), (dict(n_rows=(1 << 30) + 1), '2\\^30 rows'),
+    (dict(n_rows=1 << 30, n_out=1 << 12, dy_row_stride=1 << 12), 'tiles'),
 ])
 def test_linear_bwd_refuses(kw, message):
     with pytest.raises(L.HipPathError, match=message):

@@ -289,6 +289,42 @@ def test_capture_does_not_record_leaves():
         assert not out.requires_grad and torch.equal(out, want)
 
 
+@pytest.mark.parametrize('call', ['dense', 'packed', 'packed_lse'])
+def test_capture_does_not_record_what_is_made_of_leaves(call):
+    """as above, where the call reshapes or concatenates the leaves first"""
+    print(f'capture of leaves through {call}', flush=True)
+    x = [t.to(DEV).requires_grad_() for t in inputs(40, 40, 1, 64)[:3]]
+    y = [t.to(DEV).requires_grad_() for t in inputs(9, 33, 1, 64, 5)[:3]]
+    z = [t.detach()[None].requires_grad_() for t in x]
+    run = {'dense': lambda: [A.dense(*z)], 'packed': lambda: list(A.packed([x, y])),
+           'packed_lse': lambda: [t for pair in A.packed_lse([x, y]) for t in pair]}[call]
+    with torch.no_grad():
+        want = run()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.warns(UserWarning, match='leaves'):
+            out = run()
+    assert not any(t.requires_grad for t in out)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize('more_k,more_v', [(7, 0), (0, 200)])
+def test_rows_that_only_k_or_v_has(more_k, more_v):
+    """the forward call takes such k and v, so does its gradient: zeros there"""
+    print(f'k + {more_k}, v + {more_v} rows', flush=True)
+    q, k, v, do = (x.to(DEV) for x in inputs(70, 300, 2, 64))
+    cu_q, cu_k = (torch.tensor([0, n], dtype=torch.int32, device=DEV) for n in (70, 100))
+    xs = [x.detach().requires_grad_() for x in (q, k[:100 + more_k], v[:100 + more_v])]
+    A.varlen(*xs, cu_q, cu_k, 70, 100).backward(do)
+    o, lse = A.varlen_lse(q, k[:100], v[:100], cu_q, cu_k, 70, 100)
+    want = A.varlen_backward(do, q, k[:100], v[:100], o, lse, cu_q, cu_k, 70, 100)
+    assert all(x.grad.shape == x.shape for x in xs)
+    assert all(torch.equal(x.grad[:len(w)], w) and not x.grad[len(w):].any() for x, w in zip(xs, want))
+
+
 @pytest.mark.parametrize('nq,nk', [(0, 70), (70, 0), (0, 0)])
 def test_no_rows_at_all(nq, nk):
     print(f'no rows {nq} {nk}', flush=True)
