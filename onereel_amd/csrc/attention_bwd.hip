@@ -90,8 +90,8 @@ __device__ __forceinline__ void seg_q(const BwdArgs& a, int s, int& lo, int& n) 
   n = max(clampi(a.cu_q[s + 1], 0, a.n_q) - lo, 0);
 }
 __device__ __forceinline__ void seg_k(const BwdArgs& a, int s, int& lo, int& n) {
-  const int64_t beg = a.k_off ? a.k_off[s] : a.cu_k[s];
-  const int64_t len = a.k_len ? a.k_len[s] : a.cu_k[s + 1] - beg;
+  const int64_t beg = (a.k_off ? a.k_off : a.cu_k)[s], end = (a.k_len ? a.k_len : a.cu_k + 1)[s];   // no branches: loads
+  const int64_t len = a.k_len ? end : end - beg;                                                   // are under way at once
   lo = (int)min(max(beg, (int64_t)0), (int64_t)a.n_k);
   n = (int)max(min(beg + len, (int64_t)a.n_k) - lo, (int64_t)0);
 }
@@ -275,9 +275,11 @@ struct QueryTiles {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       lo[i] = len[i] = k0[i] = nk[i] = 0;
-      if (64 * i < a.n_seg && 64 * i + lane < a.n_seg) {
-        seg_q(a, 64 * i + lane, lo[i], len[i]);
-        seg_k(a, 64 * i + lane, k0[i], nk[i]);
+      if (64 * i < a.n_seg) {
+        const int s = min(64 * i + lane, a.n_seg - 1);
+        seg_q(a, s, lo[i], len[i]);
+        seg_k(a, s, k0[i], nk[i]);
+        if (64 * i + lane >= a.n_seg) len[i] = 0;
       }
     }
     tail_lo = uni(clampi(a.cu_q[a.n_seg], 0, a.n_q));
@@ -424,44 +426,50 @@ __device__ __forceinline__ bf16x8 pack8_rest(const f32x16& x, int half, bf16x8 r
   return __builtin_bit_cast(bf16x8, y);
 }
 
-// operand of 32 owned rows: 8 dims 16 ks + 8 (lane / 32) of row lane % 32, zeros past `rows`
+// operand of 32 owned rows: 8 dims 16 ks + 8 (lane / 32) of row lane % 32, zeros past `rows` by way of a buffer descriptor that
+// ends there (with a branch around the loads they wait for one another)
 template <int D>
 __device__ __forceinline__ void load_owned(bf16x8 (&f)[Str<D>::KS], const uint16_t* p, int64_t rs, int rows, int lane) {
   const int l32 = lane & 31, h = lane >> 5;
+  const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, rows > 0 ? (int)((rows - 1) * rs * 2 + D * 2) : 0, 0x00020000);
+  const int at = (int)(l32 * rs * 2) + 16 * h;
 #pragma unroll
-  for (int ks = 0; ks < Str<D>::KS; ++ks) {
-    u32x4 x = {0, 0, 0, 0};
-    if (l32 < rows) x = *(const u32x4*)(p + l32 * rs + 16 * ks + 8 * h);
-    f[ks] = __builtin_bit_cast(bf16x8, x);
-  }
+  for (int ks = 0; ks < Str<D>::KS; ++ks)
+    f[ks] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, at + 32 * ks, 0, 0));
 }
 
-// gradient of 32 owned rows (dims on the accumulators' rows, owned row lane % 32 on the column)
-template <int D>
-__device__ __forceinline__ void store_bf16(uint16_t* p, int64_t rs, const f32x16 (&acc)[Str<D>::DB], float f, int rows,
-                                           int lane) {
+// Gradient of 32 owned rows (dims on the accumulators' rows, owned row lane % 32 on the column) times f, bf16 or fp32, in whole
+// lines by way of 16 (bf16) or 32 rows' bytes of this wavefront's LDS at `lds`: stored as they lie, a lane's 4 dims at a time,
+// dk and dv of 12720 keys against 64 queries take STORE_FIGURES.
+template <int D, class T>
+__device__ __forceinline__ void store_rows(T* p, int64_t rs, const f32x16 (&acc)[Str<D>::DB], float f, int rows, int lane,
+                                           uint32_t lds) {
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int BYTES = D * sizeof(T), CH = BYTES / 16, PER = 16 / sizeof(T);
+  typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+  typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+  // chunk c (16 bytes) of row r lies at c ^ (r or r / 2), and in rows of bf16 the halves of a chunk are swapped from row 16
+  auto at = [&](int r, int c) { return lds + r * BYTES + ((c ^ (CH == 8 ? r >> 1 : r)) & (CH - 1)) * 16; };
   const int l32 = lane & 31, h = lane >> 5;
-  if (l32 >= rows) return;
 #pragma unroll
   for (int db = 0; db < Str<D>::DB; ++db)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const u32x2 y = {pack2(acc[db][4 * g] * f, acc[db][4 * g + 1] * f),
-                       pack2(acc[db][4 * g + 2] * f, acc[db][4 * g + 3] * f)};
-      *(u32x2*)(p + l32 * rs + 32 * db + 8 * g + 4 * h) = y;
+      const float x[4] = {acc[db][4 * g] * f, acc[db][4 * g + 1] * f, acc[db][4 * g + 2] * f, acc[db][4 * g + 3] * f};
+      if constexpr (F32)
+        *(lds_u32x4*)(uintptr_t)at(l32, 8 * db + 2 * g + h) = __builtin_bit_cast(u32x4, f32x4{x[0], x[1], x[2], x[3]});
+      else
+        *(lds_u32x2*)(uintptr_t)(at(l32, 4 * db + g) + 8 * (h ^ (l32 >> 4))) = u32x2{pack2(x[0], x[1]), pack2(x[2], x[3])};
     }
-}
-template <int D>
-__device__ __forceinline__ void store_f32(float* p, int64_t rs, const f32x16 (&acc)[Str<D>::DB], float f, int rows,
-                                          int lane) {
-  const int l32 = lane & 31, h = lane >> 5;
-  if (l32 >= rows) return;
+  __builtin_amdgcn_wave_barrier();
 #pragma unroll
-  for (int db = 0; db < Str<D>::DB; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *(f32x4*)(p + l32 * rs + 32 * db + 8 * g + 4 * h) =
-          f32x4{acc[db][4 * g] * f, acc[db][4 * g + 1] * f, acc[db][4 * g + 2] * f, acc[db][4 * g + 3] * f};
+  for (int i = 0; i < CH / 2; ++i) {
+    const int r = i * (64 / CH) + lane / CH, c = lane % CH;
+    u32x4 y = *(const lds_u32x4*)(uintptr_t)at(r, c);
+    if (!F32 && i >= CH / 4) y = u32x4{y[2], y[3], y[0], y[1]};
+    if (r < rows) *(u32x4*)(p + r * rs + c * PER) = y;
+  }
+  __builtin_amdgcn_wave_barrier();
 }
 
 // this block's item of n: the blocks of one XCD (block index modulo 8) take consecutive items, which share their head's
@@ -526,8 +534,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
 
   // the owned queries, their output gradients and their statistics
   bf16x8 qf[T][C::KS], df[T][C::KS];
-  float neg_lse[T], neg_delta[T];
+  float lse[T], dlse[T], neg_lse[T], neg_delta[T];
   f32x16 acc[T][C::DB];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int64_t at = head * a.lse_stride + min(row0 + 32 * t + (lane & 31), a.n_q - 1);
+    lse[t] = a.lse[at];
+    dlse[t] = (a.dlse ? a.dlse : a.lse)[at];
+  }
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     const int n = clampi(rows - 32 * t, 0, 32);
@@ -549,8 +563,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
     d += __shfl_xor(d, 32);
     const bool mine = (lane & 31) < n;
     const int64_t at = r + (lane & 31);
-    const float l = mine ? a.lse[head * a.lse_stride + at] : 0.0f;
-    if (mine && a.dlse) d -= a.dlse[head * a.lse_stride + at];
+    const float l = mine ? lse[t] : 0.0f;
+    if (a.dlse) d -= mine ? dlse[t] : 0.0f;
     neg_lse[t] = -l * kLog2e;
     neg_delta[t] = -d;
     if (mine && lane < 32 && part == 0) {
@@ -619,13 +633,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
 #pragma unroll 1
   for (; (b + 1) * kBlk <= end; ++b) step(b, std::false_type{});
   if (b * kBlk < end) step(b, std::true_type{});
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no DMA into LDS of a block that has ended
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the blocks asked for past the end, before the ring is used again
+  __syncthreads();
+  const uint32_t own = lds + w * (2 * kRing * C::SLOT / 4);
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     const int n = clampi(rows - 32 * t, 0, 32);
     const int64_t at = ((int64_t)(row0 + 32 * t) * a.H + head) * D, rs = (int64_t)a.H * D;
-    if (a.split_q == 1) store_bf16<D>(a.dq + at, rs, acc[t], a.scale, n, lane);
-    else store_f32<D>(a.part_q + (int64_t)part * a.n_q * rs + at, rs, acc[t], a.scale, n, lane);
+    if (a.split_q == 1) store_rows<D>(a.dq + at, rs, acc[t], a.scale, n, lane, own);
+    else store_rows<D>(a.part_q + (int64_t)part * a.n_q * rs + at, rs, acc[t], a.scale, n, lane, own);
   }
 }
 
@@ -800,14 +816,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
     }
     __builtin_amdgcn_s_setprio(0);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no DMA into LDS of a block that has ended
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the blocks asked for past the end, before the ring is used again
+  __syncthreads();
+  const uint32_t mine = lds + w * (2 * kRing * C::SLOT / 4);
   const int64_t at = ((int64_t)row0 * a.H + head) * D, rs = (int64_t)a.H * D, all = a.n_k * rs;
   if (a.split_k == 1) {
-    store_bf16<D>(a.dk + at, rs, dk, a.scale, rows, lane);
-    store_bf16<D>(a.dv + at, rs, dv, 1.0f, rows, lane);
+    store_rows<D>(a.dk + at, rs, dk, a.scale, rows, lane, mine);
+    store_rows<D>(a.dv + at, rs, dv, 1.0f, rows, lane, mine);
   } else {
-    store_f32<D>(a.part_k + 2 * part * all + at, rs, dk, a.scale, rows, lane);
-    store_f32<D>(a.part_k + (2 * part + 1) * all + at, rs, dv, 1.0f, rows, lane);
+    store_rows<D>(a.part_k + 2 * part * all + at, rs, dk, a.scale, rows, lane, mine);
+    store_rows<D>(a.part_k + (2 * part + 1) * all + at, rs, dv, 1.0f, rows, lane, mine);
   }
 }
 
