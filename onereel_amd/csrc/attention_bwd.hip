@@ -20,8 +20,10 @@
 // - Key rows may belong to several segments (overlapping ranges): the key axis is cut at every range boundary, so that all
 //   rows of a key tile have the same segments, and the tile streams the queries of all of them. Rows past an end load as
 //   zeros: a zero query row adds nothing to dk and dv, and the scores of key rows past the end are set to P = 0.
-// - Few tiles (few queries against long keys, or few keys against long queries): the streamed axis is split, the parts
-//   write fp32 partial gradients, and a last launch adds them in order.
+// - Tiles with long streamed axes (few queries against long keys, few keys against long queries, one long segment among short
+//   ones) are split; the parts write fp32 partial gradients, and a last launch adds them in order.
+// Measured: 3 x 9680 queries against overlapping 11440 keys, 16 heads of 128: dq 3.27 ms, dk and dv 4.14 ms, 1180 to 1220
+// TFLOP/s of the 7 products executed (a large bf16 product of the vendor library reaches 1390 to 1490 on the same card).
 #include <math.h>
 
 #include <algorithm>
@@ -42,12 +44,12 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 constexpr int kThreads = 256;        // 4 wavefronts
+constexpr int kCUs = 256;
 constexpr int kBlk = 32;             // streamed rows per block
 constexpr int kRing = 4;             // LDS slots of the ring
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxSeg = 4096;
-constexpr int kMaxSplit = 64;
-constexpr int kHeader = 8;           // int32 words ahead of the tile tables: query tile count, key tile count
+constexpr int kHeader = 8;           // int32 words ahead of the tables
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct BwdArgs {
@@ -59,17 +61,18 @@ struct BwdArgs {
   int64_t lse_stride;                // elements between the heads of lse and dlse
   int32_t n_seg, n_q, n_k, H;
   float scale;
-  int32_t split_q, split_k;          // parts of the streamed axis in the dq pass and in the dk / dv pass
-  int32_t max_q_tiles, max_k_tiles;
+  int32_t max_q_items, max_k_items;  // of one head
+  int32_t slots_q, slots_k;          // partial gradients of tiles that a head may have; 0: no tile is split
   int32_t tq, tk;                    // rows of a query tile and of a key tile
   // workspace
-  int32_t* head;
-  i32x4* q_tiles;                    // first query, rows, first key, keys
-  i32x4* k_tiles;                    // two a tile: first key, rows, first and last segment that may read them; first query and
-                                     // queries of the segment where only one may
+  int32_t* head;                     // query items (calls that are planned ahead), key items, split query tiles, split key tiles
+  i32x4* q_items;                    // first query, rows, first key, keys
+  i32x4* k_items;                    // two an item: first key, rows, first and last segment that may read them; first query and
+                                     // queries of the segment where only one may, part and parts, the part's slot
+  i32x4 *q_split, *k_split;          // split tiles: first row, rows, first slot, parts
   float* stat;                       // [H][2][n_q]: -lse / scale, then -delta
-  float* part_q;                     // [split_q][n_q][H][D]
-  float* part_k;                     // [split_k][2][n_k][H][D]: dk, then dv
+  float* part_q;                     // [slots_q][H][tq][D]
+  float* part_k;                     // [2][slots_k][H][tk][D]: dk, dv
 };
 
 // Blocks of 32 queries that a wavefront owns. One leaves room for two wavefronts on a SIMD, one's exponentials under the
@@ -105,6 +108,27 @@ __device__ __forceinline__ void seg_k(const BwdArgs& a, int s, int& lo, int& n) 
 // cu_q, and the first block of that pass writes the key tiles that the dk / dv pass reads (a planner launch of one block
 // took 7 to 17 us, the dk / dv pass of 12 ragged sequences 49). With more segments one block plans both ahead.
 constexpr int kFewSeg = 256;
+// Of up to kSorted segments the tiles with the longest streamed axes come first, and long ones are split (parts_of): 12 ragged
+// sequences of 1 to 899 rows, 16 heads of 128, dq in 36 us, 42 in the order of the segments, dk and dv in 36 and 40;
+// 3 x 9680 queries against overlapping ranges, dk and dv, 4.14 ms and 4.33. Calls of more segments have short ones, or items
+// enough to even out.
+constexpr int kSorted = 64;
+
+// Parts of a tile that streams `blocks` blocks, in a call whose heads' tiles stream `total` blocks each: the nearest number that
+// gives every one of 256 CUs a share of the call's blocks as long as a part, no part shorter than 8 blocks or so; and where
+// such parts are 48 blocks long, nearly twice as many, since two work-groups on a CU fill each other's gaps. A tile of 2 parts
+// or more has at most blocks / share + 1/2 <= 4/3 blocks / share of them, so a head's split tiles have at most
+// 4/3 total / share, kMaxParts over all heads, and never more than the workspace's slots. 24 calls of 1 to 24 segments of 1
+// to 12720 rows, 1 to 8 heads: 2.4 to 6 times as fast where one segment outweighs the others, 1.5 times on (geometric)
+// average, as with one number of parts for all tiles; 128 keys against 3 x 9680 queries, 16 heads: 488 us for dk and dv in 1
+// part, 103 in 5, 80 in 10.
+constexpr int kMaxParts = 700;
+__device__ __forceinline__ int share_of(int64_t total, int H, int slots) {
+  int64_t share = max((total * H + kCUs - 1) / kCUs, (int64_t)8);
+  if (share >= 48) share = share * 9 / 16;
+  return (int)min(max(share, (4 * total + 3 * slots - 1) / (3 * slots)), (int64_t)1 << 30);
+}
+__device__ __forceinline__ int parts_of(int blocks, int share) { return max((int)(((int64_t)blocks + share / 2) / share), 1); }
 
 // exclusive sum over the block's threads; all: the total
 template <int THREADS>
@@ -159,6 +183,8 @@ __device__ int deal_tiles(int n, int most, int* first, int* wsum, Count&& count,
 template <int SEG>
 struct PlanLds {
   int bnd[2 * SEG], lo_seg[2 * SEG + 1], hi_seg[2 * SEG + 1], first[2 * SEG + 2], wsum[16];
+  unsigned long long total;
+  int order[2 * kSorted + 1], blocks[2 * kSorted + 1], n_q[kSorted], k_lo[kSorted], k_end[kSorted];
 };
 
 template <int THREADS, int SEG>
@@ -225,15 +251,59 @@ __device__ void plan_keys(const BwdArgs& a, PlanLds<SEG>& l) {
   __syncthreads();
   auto start = [&](int i) { return i > 0 ? l.bnd[i - 1] : 0; };
   auto length = [&](int i) { return (i < m ? l.bnd[i] : a.n_k) - start(i); };
-  const int tiles = deal_tiles<THREADS>(
-      m + 1, a.max_k_tiles, l.first, l.wsum, [&](int i) { return (length(i) + tk - 1) / tk; },
-      [&](int i, int j, int x) {
+  const bool sorted = SEG == kFewSeg && n <= kSorted;
+  int share = 1 << 30;
+  if (sorted) {
+    // blocks of queries that read an interval; its rank among them
+    if (t < n) {
+      int lo, len;
+      seg_q(a, t, lo, l.n_q[t]);
+      seg_k(a, t, lo, len);
+      l.k_lo[t] = lo;
+      l.k_end[t] = lo + len;
+    }
+    if (t == 0) l.total = 0;
+    __syncthreads();
+    int mine = 0;
+    if (t <= m) {
+      if (length(t) > 0)
+        for (int s = l.lo_seg[t]; s <= l.hi_seg[t]; ++s)
+          if (l.k_lo[s] <= start(t) && start(t) < l.k_end[s]) mine += (l.n_q[s] + kBlk - 1) / kBlk;
+      l.blocks[t] = mine;
+      if (mine) atomicAdd(&l.total, (unsigned long long)mine * ((length(t) + tk - 1) / tk));
+    }
+    __syncthreads();
+    if (a.slots_k) share = share_of((int64_t)l.total, a.H, a.slots_k);
+    int rank = 0;
+    if (t <= m) {
+      for (int i = 0; i <= m; ++i) rank += l.blocks[i] > mine || (l.blocks[i] == mine && i < t);
+      l.order[rank] = t;
+    }
+    __syncthreads();
+  }
+  auto nth = [&](int i) { return sorted ? l.order[i] : i; };
+  auto parts = [&](int i) { return sorted ? parts_of(l.blocks[i], share) : 1; };
+  auto tiles = [&](int i) { return (length(i) + tk - 1) / tk; };
+  const int items = deal_tiles<THREADS>(
+      m + 1, a.max_k_items, l.first, l.wsum, [&](int r) { return tiles(nth(r)) * parts(nth(r)); },
+      [&](int r, int j, int x) {
+        const int i = nth(r), n_parts = parts(i), at = j / n_parts * tk;
         int lo = 0, len = 0;
         if (l.lo_seg[i] == l.hi_seg[i]) seg_q(a, l.lo_seg[i], lo, len);
-        a.k_tiles[2 * x] = i32x4{start(i) + j * tk, min(tk, length(i) - j * tk), l.lo_seg[i], l.hi_seg[i]};
-        a.k_tiles[2 * x + 1] = i32x4{lo, len, 0, 0};
+        a.k_items[2 * x] = i32x4{start(i) + at, min(tk, length(i) - at), l.lo_seg[i], l.hi_seg[i]};
+        a.k_items[2 * x + 1] = i32x4{lo, len, j % n_parts | n_parts << 16, x};   // split tiles come first: the item is the slot
       });
-  if (t == 0) a.head[1] = tiles;
+  int n_split = 0;
+  if (a.slots_k && sorted) {   // interval t's tiles, when split
+    const int i = t <= m ? nth(t) : 0, n_parts = t <= m ? parts(i) : 1, n_tiles = n_parts > 1 ? tiles(i) : 0;
+    const int base = block_scan<THREADS>(n_tiles, l.wsum, n_split);
+    for (int j = 0; j < n_tiles; ++j)
+      a.k_split[base + j] = i32x4{start(i) + j * tk, min(tk, length(i) - j * tk), l.first[t] + j * n_parts, n_parts};
+  }
+  if (t == 0) {
+    a.head[1] = items;
+    a.head[3] = n_split;
+  }
 }
 
 __global__ __launch_bounds__(kPlanThreads) void bwd_plan_kernel(BwdArgs a) {
@@ -248,7 +318,7 @@ __global__ __launch_bounds__(kPlanThreads) void bwd_plan_kernel(BwdArgs a) {
     }
   };
   const int tiles = deal_tiles<kPlanThreads>(
-      n + 1, a.max_q_tiles, l.first, l.wsum,
+      n + 1, a.max_q_items, l.first, l.wsum,
       [&](int s) {
         int lo, len;
         piece(s, lo, len);
@@ -258,18 +328,26 @@ __global__ __launch_bounds__(kPlanThreads) void bwd_plan_kernel(BwdArgs a) {
         int lo, len, k0 = 0, nk = 0;
         piece(s, lo, len);
         if (s < n) seg_k(a, s, k0, nk);
-        a.q_tiles[x] = i32x4{lo + j * tq, min(tq, len - j * tq), k0, nk};
+        a.q_items[x] = i32x4{lo + j * tq, min(tq, len - j * tq), k0, nk};
       });
   if (threadIdx.x == 0) a.head[0] = tiles;
   __syncthreads();
   plan_keys<kPlanThreads, kMaxSeg>(a, l);
 }
 
-// The query tiles of a call of at most kFewSeg segments: how many there are, and the one with index x, from every
+// The query items of a call of at most kFewSeg segments: how many there are, and the one with index x, from every
 // wavefront's own scan.
-struct QueryTiles {
+struct QueryItems {
   static constexpr int N = kFewSeg / 64;
-  int lo[N], len[N], k0[N], nk[N], incl[N], n_seg_tiles, tail, tail_lo;
+  int lo[N], len[N], k0[N], nk[N], incl[N], parts, n_seg_items, tail, tail_lo;
+  static __device__ __forceinline__ int scan(int x, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(x, d);
+      if (lane >= d) x += y;
+    }
+    return x;
+  }
   __device__ __forceinline__ int count(const BwdArgs& a, int tq, int lane) {
     // every load at once: what follows waits for one round of them
 #pragma unroll
@@ -284,39 +362,67 @@ struct QueryTiles {
     }
     tail_lo = uni(clampi(a.cu_q[a.n_seg], 0, a.n_q));
     tail = a.n_q - tail_lo;
+    parts = 1;
+    if (a.n_seg <= kSorted) {   // longest first, equal ones in order
+      int rank = 0;
+      for (int s = 0; s < a.n_seg; ++s) {
+        const int x = __builtin_amdgcn_readlane(nk[0], s);
+        rank += x > nk[0] || (x == nk[0] && s < lane);
+      }
+      rank = lane < a.n_seg ? 4 * rank : 4 * lane;
+      lo[0] = __builtin_amdgcn_ds_permute(rank, lo[0]);
+      len[0] = __builtin_amdgcn_ds_permute(rank, len[0]);
+      k0[0] = __builtin_amdgcn_ds_permute(rank, k0[0]);
+      nk[0] = __builtin_amdgcn_ds_permute(rank, nk[0]);
+      if (a.slots_q) {
+        const int blocks = (nk[0] + kBlk - 1) / kBlk;
+        int64_t total = (int64_t)((len[0] + tq - 1) / tq) * blocks;
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor((long long)total, d);
+        parts = parts_of(blocks, share_of(total, a.H, a.slots_q));
+      }
+    }
     int at = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       incl[i] = at;
       if (64 * i < a.n_seg) {
-        int x = (len[i] + tq - 1) / tq;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const int y = __shfl_up(x, d);
-          if (lane >= d) x += y;
-        }
-        incl[i] = at + x;
-        at += __shfl(x, 63);
+        incl[i] = at + scan(items(i, tq), lane);
+        at = __shfl(incl[i], 63);
       }
     }
-    n_seg_tiles = uni(at);
-    return min(n_seg_tiles + (tail + tq - 1) / tq, a.max_q_tiles);
+    n_seg_items = uni(at);
+    return min(n_seg_items + (tail + tq - 1) / tq, a.max_q_items);
   }
-  __device__ __forceinline__ i32x4 at(int tq, int x) const {
-    i32x4 tile = {tail_lo + (x - n_seg_tiles) * tq, 0, 0, 0};
+  __device__ __forceinline__ int items(int i, int tq) const { return (len[i] + tq - 1) / tq * (i ? 1 : parts); }
+  // first query, rows, first key, keys; the part and the parts
+  __device__ __forceinline__ i32x4 at(int tq, int x, int& part, int& n_parts) const {
+    i32x4 tile = {tail_lo + (x - n_seg_items) * tq, 0, 0, 0};
     tile[1] = min(tq, tail - (tile[0] - tail_lo));
-    bool found = x >= n_seg_tiles;
+    part = 0;
+    n_parts = 1;
+    bool found = x >= n_seg_items;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       // the first lane whose sum passes x: its segment has tiles
       const uint64_t hit = __ballot(incl[i] > x && len[i] > 0);
       if (!found && hit) {
-        const int l = __builtin_ctzll(hit), n = __shfl(len[i], l), j = (x - (__shfl(incl[i], l) - (n + tq - 1) / tq)) * tq;
-        tile = i32x4{__shfl(lo[i], l) + j, min(tq, n - j), __shfl(k0[i], l), __shfl(nk[i], l)};
+        const int l = __builtin_ctzll(hit), n = __shfl(len[i], l), j = x - __shfl(incl[i] - items(i, tq), l);
+        if (i == 0) n_parts = uni(__shfl(parts, l));
+        part = uni(j % n_parts);
+        const int row = j / n_parts * tq;
+        tile = i32x4{__shfl(lo[i], l) + row, min(tq, n - row), __shfl(k0[i], l), __shfl(nk[i], l)};
         found = true;
       }
     }
     return uni(tile);
+  }
+  // the split tiles, by one wavefront
+  __device__ __forceinline__ void write_split(const BwdArgs& a, int tq, int lane) const {
+    const int n = parts > 1 ? (len[0] + tq - 1) / tq : 0, end = scan(n, lane);
+    for (int j = 0; j < n; ++j)
+      a.q_split[end - n + j] = i32x4{lo[0] + j * tq, min(tq, len[0] - j * tq), incl[0] + (j - n) * parts, parts};
+    if (lane == 63) a.head[2] = end;
   }
 };
 
@@ -439,8 +545,8 @@ __device__ __forceinline__ void load_owned(bf16x8 (&f)[Str<D>::KS], const uint16
 }
 
 // Gradient of 32 owned rows (dims on the accumulators' rows, owned row lane % 32 on the column) times f, bf16 or fp32, in whole
-// lines by way of 16 (bf16) or 32 rows' bytes of this wavefront's LDS at `lds`: stored as they lie, a lane's 4 dims at a time,
-// dk and dv of 12720 keys against 64 queries take STORE_FIGURES.
+// lines by way of this wavefront's quarter of the ring at `lds`: stored as they lie, a lane's 4 dims at a time,
+// dk and dv of 12720 keys against 64 queries take 62 us (16 bytes a write request), 47 so.
 template <int D, class T>
 __device__ __forceinline__ void store_rows(T* p, int64_t rs, const f32x16 (&acc)[Str<D>::DB], float f, int rows, int lane,
                                            uint32_t lds) {
@@ -472,11 +578,25 @@ __device__ __forceinline__ void store_rows(T* p, int64_t rs, const f32x16 (&acc)
   __builtin_amdgcn_wave_barrier();
 }
 
-// this block's item of n: the blocks of one XCD (block index modulo 8) take consecutive items, which share their head's
-// streamed rows in that XCD's L2
-__device__ __forceinline__ int64_t xcd_item(int64_t n, unsigned block) {
+// This block's head and item of n_items x H; false: none. The blocks of one XCD (block index modulo 8) take consecutive items
+// of few heads, which share their streamed rows in that XCD's L2. Few items are dealt out by their length instead (they
+// come longest first), all heads' longest ahead of their shorter ones; where they all run at once, two work-groups on a
+// CU, a CU's second one, a kCUs of blocks later, is the shorter the longer its first one is.
+__device__ __forceinline__ bool item_of(int n_items, int H, int block, int& head, int& item) {
+  const int64_t n = (int64_t)n_items * H;
+  if (n <= 4 * kCUs) {
+    if (block >= n) return false;
+    const int first = (kCUs + H - 1) / H;
+    item = block / H;
+    head = block % H;
+    if (n <= 2 * kCUs && item >= first) item = n_items - 1 - (item - first);
+    return true;
+  }
   const int64_t per = (n + 7) / 8, j = block >> 3, i = (block & 7) * per + j;
-  return j < per && i < n ? i : -1;
+  if (j >= per || i >= n) return false;
+  head = (int)(i / n_items);
+  item = (int)(i % n_items);
+  return true;
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -487,26 +607,27 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
   constexpr int T = query_blocks(D);
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT];
   const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
-  QueryTiles qt;
-  int n_tiles;
+  QueryItems qi;
+  int n_items;
   if constexpr (FEW) {
     static_assert(sizeof(PlanLds<kFewSeg>) <= sizeof(ring), "plan");
     if (blockIdx.x < 8) {   // ahead of the blocks with an item, eight of them so that those keep their XCDs
       if (blockIdx.x == 0) plan_keys<kThreads, kFewSeg>(a, *(PlanLds<kFewSeg>*)ring);
+      if (blockIdx.x == 1 && w == 0 && a.slots_q) {
+        qi.count(a, 128 * T, lane);
+        qi.write_split(a, 128 * T, lane);
+      }
       return;
     }
-    n_tiles = qt.count(a, 128 * T, lane);
+    n_items = qi.count(a, 128 * T, lane);
   } else {
-    n_tiles = uni(a.head[0]);
+    n_items = uni(a.head[0]);
   }
-  const int64_t item = xcd_item((int64_t)n_tiles * a.H * a.split_q, blockIdx.x - (FEW ? 8 : 0));
-  if (item < 0) return;
-  const int part = (int)(item % a.split_q);
-  const int head = (int)(item / a.split_q / n_tiles);
-  const int which = (int)(item / a.split_q % n_tiles);
+  int head, item, part = 0, parts = 1;
+  if (!item_of(n_items, a.H, blockIdx.x - (FEW ? 8 : 0), head, item)) return;
   i32x4 tile;
-  if constexpr (FEW) tile = qt.at(128 * T, which);
-  else tile = uni(a.q_tiles[which]);
+  if constexpr (FEW) tile = qi.at(128 * T, item, part, parts);
+  else tile = uni(a.q_items[item]);
   const int row0 = tile[0] + w * 32 * T, n_keys = tile[3];
   const int rows = clampi(tile[1] - w * 32 * T, 0, 32 * T);
 
@@ -518,7 +639,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
   }
   const uint32_t lds = lds_addr(ring), m0 = lds + w * 1024;
   const int blocks = (n_keys + kBlk - 1) / kBlk;
-  const int b0 = (int)((int64_t)blocks * part / a.split_q), b1 = (int)((int64_t)blocks * (part + 1) / a.split_q);
+  const int b0 = (int)((int64_t)blocks * part / parts), b1 = (int)((int64_t)blocks * (part + 1) / parts);
   const uint16_t* kp = a.k + (int64_t)tile[2] * a.ks + (int64_t)head * D;
   const uint16_t* vp = a.v + (int64_t)tile[2] * a.ks + (int64_t)head * D;
   auto fetch = [&](int b) {
@@ -639,9 +760,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     const int n = clampi(rows - 32 * t, 0, 32);
-    const int64_t at = ((int64_t)(row0 + 32 * t) * a.H + head) * D, rs = (int64_t)a.H * D;
-    if (a.split_q == 1) store_rows<D>(a.dq + at, rs, acc[t], a.scale, n, lane, own);
-    else store_rows<D>(a.part_q + (int64_t)part * a.n_q * rs + at, rs, acc[t], a.scale, n, lane, own);
+    if (parts == 1) {
+      store_rows<D>(a.dq + ((int64_t)(row0 + 32 * t) * a.H + head) * D, (int64_t)a.H * D, acc[t], a.scale, n, lane, own);
+    } else {   // split tiles come first: the item is the slot
+      const int64_t row = ((int64_t)item * a.H + head) * 128 * T + w * 32 * T + 32 * t;
+      store_rows<D>(a.part_q + row * D, D, acc[t], a.scale, n, lane, own);
+    }
   }
 }
 
@@ -674,14 +798,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
   using C = Str<D>;
   constexpr int kStat = 256;         // bytes of one wavefront's statistics of a block
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT + kRing * 4 * kStat];
-  const int n_tiles = uni(a.head[1]);
-  const int64_t item = xcd_item((int64_t)n_tiles * a.H * a.split_k, blockIdx.x);
-  if (item < 0) return;
+  int head, item;
+  if (!item_of(uni(a.head[1]), a.H, blockIdx.x, head, item)) return;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int part = (int)(item % a.split_k);
-  const int head = (int)(item / a.split_k / n_tiles);
-  const int64_t which = item / a.split_k % n_tiles;
-  const i32x4 tile = uni(a.k_tiles[2 * which]), only = uni(a.k_tiles[2 * which + 1]);
+  const i32x4 tile = uni(a.k_items[2 * (int64_t)item]), only = uni(a.k_items[2 * (int64_t)item + 1]);
+  const int part = only[2] & 0xffff, parts = only[2] >> 16;
   const int row0 = tile[0] + w * 32;
   const int rows = clampi(tile[1] - w * 32, 0, 32);
 
@@ -703,7 +824,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
     walk = Walk{tile[2], tile[3], 0, 0};
     walk.next_segment(a, tile[0]);
   }
-  const int b0 = (int)((int64_t)total * part / a.split_k), b1 = (int)((int64_t)total * (part + 1) / a.split_k);
+  const int b0 = (int)((int64_t)total * part / parts), b1 = (int)((int64_t)total * (part + 1) / parts);
   for (int skip = b0; walk.left > 0;) {
     const int n = (walk.left + kBlk - 1) / kBlk;
     if (skip < n) {
@@ -819,74 +940,75 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ?
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the blocks asked for past the end, before the ring is used again
   __syncthreads();
   const uint32_t mine = lds + w * (2 * kRing * C::SLOT / 4);
-  const int64_t at = ((int64_t)row0 * a.H + head) * D, rs = (int64_t)a.H * D, all = a.n_k * rs;
-  if (a.split_k == 1) {
+  if (parts == 1) {
+    const int64_t at = ((int64_t)row0 * a.H + head) * D, rs = (int64_t)a.H * D;
     store_rows<D>(a.dk + at, rs, dk, a.scale, rows, lane, mine);
     store_rows<D>(a.dv + at, rs, dv, 1.0f, rows, lane, mine);
   } else {
-    store_rows<D>(a.part_k + 2 * part * all + at, rs, dk, a.scale, rows, lane, mine);
-    store_rows<D>(a.part_k + (2 * part + 1) * all + at, rs, dv, 1.0f, rows, lane, mine);
+    float* at = a.part_k + (((int64_t)only[3] * a.H + head) * kKeyTile + w * 32) * D;
+    store_rows<D>(at, D, dk, a.scale, rows, lane, mine);
+    store_rows<D>(at + (int64_t)a.slots_k * a.H * kKeyTile * D, D, dv, 1.0f, rows, lane, mine);
   }
 }
 
-// the partial gradients of split passes, added in the order of the parts: 8 elements a thread of dq, then dk, then dv
-__global__ __launch_bounds__(kThreads) void bwd_add_kernel(BwdArgs a, int64_t q8, int64_t k8) {
-  const int64_t step = (int64_t)gridDim.x * kThreads, n = q8 + 2 * k8;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) {
-    const bool is_q = i < q8;
-    const int64_t which = is_q ? 0 : (i - q8) / k8, e = is_q ? i : (i - q8) % k8;
-    const float* p = is_q ? a.part_q : a.part_k + which * k8 * 8;
-    const int64_t apart = is_q ? q8 * 8 : 2 * k8 * 8;
-    const int parts = is_q ? a.split_q : a.split_k;
-    f32x4 x = {}, y = {};
+// the partial gradients of split tiles, added in the order of the parts: 8 elements a thread of dq, then of dk and dv
+template <int D>
+__global__ __launch_bounds__(kThreads) void bwd_add_kernel(BwdArgs a) {
+  constexpr int ROWS = kThreads * 8 / D;
+  const int qc = a.tq / ROWS, kc = a.tk / ROWS;
+  const int64_t nq = a.slots_q ? (int64_t)a.head[2] * a.H * qc : 0, nk = a.slots_k ? (int64_t)a.head[3] * a.H * kc : 0;
+  for (int64_t i = blockIdx.x; i < nq + 2 * nk; i += gridDim.x) {
+    const bool is_q = i < nq;
+    const int which = is_q ? 0 : (int)((i - nq) / nk), tile_rows = is_q ? a.tq : a.tk, chunks = is_q ? qc : kc;
+    const int64_t x = is_q ? i : (i - nq) % nk;
+    const int head = (int)(x / chunks % a.H), row = (int)(x % chunks) * ROWS + threadIdx.x / (D / 8), col = threadIdx.x % (D / 8) * 8;
+    const i32x4 tile = (is_q ? a.q_split : a.k_split)[x / chunks / a.H];
+    if (row >= tile[1]) continue;
+    const int64_t apart = (int64_t)a.H * tile_rows * D;
+    const float* p = (is_q ? a.part_q : a.part_k + which * a.slots_k * apart) + tile[2] * apart + ((int64_t)head * tile_rows + row) * D + col;
+    f32x4 lo = {}, hi = {};
 #pragma unroll 8
-    for (int j = 0; j < parts; ++j) {
-      x += *(const f32x4*)(p + j * apart + e * 8);
-      y += *(const f32x4*)(p + j * apart + e * 8 + 4);
+    for (int j = 0; j < tile[3]; ++j) {
+      lo += *(const f32x4*)(p + j * apart);
+      hi += *(const f32x4*)(p + j * apart + 4);
     }
-    const u32x4 r = {pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3])};
-    *(u32x4*)((is_q ? a.dq : which ? a.dv : a.dk) + e * 8) = r;
+    *(u32x4*)((is_q ? a.dq : which ? a.dv : a.dk) + ((int64_t)(tile[0] + row) * a.H + head) * D + col) =
+        u32x4{pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(hi[0], hi[1]), pack2(hi[2], hi[3])};
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// tiles and splits of a call, from its sizes alone (the offsets are on the device)
+// tiles and parts of a call, from its sizes alone (the offsets are on the device)
 struct Shape {
   int tq, tk;                        // rows of a query tile and of a key tile
-  int64_t max_q_tiles, max_k_tiles;
-  int split_q, split_k;
+  int64_t max_q_items, max_k_items;
+  int slots_q, slots_k;
 };
 
-// Parts of a streamed axis: as many as give every one of 256 CUs a work-group, none shorter than 8 blocks of rows; twice as
-// many where the parts would still be 64 blocks or longer, since two work-groups on a CU fill each other's gaps. Splitting
-// further, or calls that have 256 items, gains less than the partial gradients cost (16 heads of 128; dq, then dk and dv):
-// 2048 x 2048 64 + 90 us, in 2 parts 59 + 71 and 18 to add; 256 keys against 4096 queries 149 us for dk and dv in 1 part, 35 in
-// 8, 37 in 16; 128 against 3 x 9680 488 us in 1, 104 in 8, 95 in 10.
-constexpr int kCUs = 256;
-int split_of(int64_t items, int64_t streamed) {
-  const int64_t blocks = streamed / kBlk;
-  int64_t parts = std::max<int64_t>(1, std::min<int64_t>({kCUs / std::max<int64_t>(items, 1), blocks / 8, kMaxSplit / 2}));
-  if (items * parts <= kCUs && blocks / parts >= 64) parts *= 2;
-  return (int)parts;
+// Partial gradients of tiles that a head may have: parts_of's limits, of at most `tiles` tiles of at most `blocks` blocks. None in
+// calls of more than 16 rounds of work-groups, whose longest tiles come first.
+int slots_of(int32_t n_seg, int64_t tiles, int64_t blocks, int H) {
+  if (n_seg > kSorted || (tiles - n_seg / 2) * H > 32 * kCUs || blocks < 12) return 0;
+  return (int)std::min<int64_t>(kMaxParts / H + 1, tiles * blocks / 6 + 1);
 }
 
 Shape shape_of(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H, int32_t D) {
   Shape s;
-  // a segment ends in a half-filled tile on average
-  auto items = [&](int64_t n, int tile) { return H * ((n + tile - 1) / tile + n_seg / 2); };
   s.tq = 128 * query_blocks(D);
   s.tk = kKeyTile;
-  s.max_q_tiles = n_q / s.tq + n_seg + 1;
-  s.max_k_tiles = n_k / s.tk + 2 * (int64_t)n_seg + 1;
-  s.split_q = split_of(items(n_q, s.tq), max_k);
-  s.split_k = split_of(items(n_k, s.tk), max_q);
+  const int64_t q_tiles = n_q / s.tq + n_seg + 1, k_tiles = n_k / s.tk + 2 * (int64_t)n_seg + 1;
+  s.slots_q = slots_of(n_seg, q_tiles, ((int64_t)max_k + kBlk - 1) / kBlk, H);
+  // overlapping ranges: a key tile may stream every segment's queries
+  s.slots_k = slots_of(n_seg, n_k / s.tk + n_seg + 1, std::min((int64_t)n_q / kBlk, (int64_t)max_q / kBlk * n_seg) + n_seg, H);
+  s.max_q_items = q_tiles + s.slots_q;
+  s.max_k_items = k_tiles + s.slots_k;
   return s;
 }
 
 struct Layout {
-  int64_t q_tiles, k_tiles, stat, part_q, part_k, bytes;
+  int64_t q_items, k_items, q_split, k_split, stat, part_q, part_k, bytes;
 };
-Layout layout_of(const Shape& s, int32_t n_q, int32_t n_k, int32_t H, int32_t D) {
+Layout layout_of(const Shape& s, int32_t n_q, int32_t H, int32_t D) {
   Layout l;
   int64_t at = kHeader * 4;
   auto take = [&](int64_t n) {
@@ -894,11 +1016,13 @@ Layout layout_of(const Shape& s, int32_t n_q, int32_t n_k, int32_t H, int32_t D)
     at = was + n;
     return was;
   };
-  l.q_tiles = take(s.max_q_tiles * 16);
-  l.k_tiles = take(s.max_k_tiles * 32);
+  l.q_items = take(s.max_q_items * 16);
+  l.k_items = take(s.max_k_items * 32);
+  l.q_split = take((int64_t)s.slots_q * 16);
+  l.k_split = take((int64_t)s.slots_k * 16);
   l.stat = take((int64_t)2 * H * n_q * 4);
-  l.part_q = take(s.split_q > 1 ? (int64_t)s.split_q * n_q * H * D * 4 : 0);
-  l.part_k = take(s.split_k > 1 ? (int64_t)s.split_k * 2 * n_k * H * D * 4 : 0);
+  l.part_q = take((int64_t)s.slots_q * H * s.tq * D * 4);
+  l.part_k = take((int64_t)s.slots_k * 2 * H * s.tk * D * 4);
   l.bytes = (at + 255) & ~(int64_t)255;
   return l;
 }
@@ -908,7 +1032,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 template <int D, bool FINE>
 void launch(const BwdArgs& a, const Shape& s, hipStream_t st) {
   auto grid = [](int64_t items) { return dim3((unsigned)((items + 7) / 8 * 8)); };
-  const dim3 gq = grid(s.max_q_tiles * a.H * s.split_q), gk = grid(s.max_k_tiles * a.H * s.split_k), t(kThreads);
+  const dim3 gq = grid(s.max_q_items * a.H), gk = grid(s.max_k_items * a.H), t(kThreads);
   if (a.n_seg <= kFewSeg) {
     hipLaunchKernelGGL((bwd_q_kernel<D, true, FINE>), dim3(gq.x + 8), t, 0, st, a);
   } else {
@@ -916,6 +1040,7 @@ void launch(const BwdArgs& a, const Shape& s, hipStream_t st) {
     if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, false, FINE>), gq, t, 0, st, a);
   }
   if (a.n_k > 0) hipLaunchKernelGGL((bwd_kv_kernel<D, FINE>), gk, t, 0, st, a);
+  if (s.slots_q || s.slots_k) hipLaunchKernelGGL(bwd_add_kernel<D>, dim3(8 * kCUs), t, 0, st, a);
 }
 
 // Whether P and dS go into their products as two bf16 numbers, the rounded value and what that rounding left out: in calls
@@ -939,7 +1064,7 @@ extern "C" int64_t or_varlen_bwd_workspace_size(int32_t n_seg, int32_t n_q, int3
       (D != 64 && D != 128))
     return fail_arg("or_varlen_bwd_workspace_size: 1 to %d segments, 1 to 256 heads of 64 or 128 and sizes of at least 0 are "
                     "needed", kMaxSeg);
-  return layout_of(shape_of(n_seg, n_q, n_k, max_q, max_k, H, D), n_q, n_k, H, D).bytes;
+  return layout_of(shape_of(n_seg, n_q, n_k, max_q, max_k, H, D), n_q, H, D).bytes;
 }
 
 extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
@@ -966,12 +1091,12 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
     return fail_arg("or_varlen_bwd: pointers must be 16-byte aligned");
   if (x.lse_stride < x.n_q) return fail_arg("or_varlen_bwd: lse_stride must cover the query rows");
   const Shape s = shape_of(x.n_seg, x.n_q, x.n_k, x.max_q, x.max_k, x.H, x.D);
-  const Layout l = layout_of(s, x.n_q, x.n_k, x.H, x.D);
+  const Layout l = layout_of(s, x.n_q, x.H, x.D);
   if (!x.workspace || x.workspace_bytes < l.bytes || !aligned16(x.workspace))
     return fail_arg("or_varlen_bwd: a 16-byte aligned workspace of %lld bytes is needed", (long long)l.bytes);
   // a head's second row of statistics lies 4 n_q bytes after the first, within the 32 bits of a buffer offset
   if ((int64_t)x.n_q * 4 + 256 >= (int64_t)0x7fffffff) return fail_arg("or_varlen_bwd: n_q must stay under 2^29");
-  if (std::max(s.max_q_tiles * s.split_q, s.max_k_tiles * s.split_k) * x.H >= (int64_t)1 << 24)   // 2^32 threads
+  if (std::max(s.max_q_items, s.max_k_items) * x.H >= (int64_t)1 << 24)   // 2^32 threads
     return fail_arg("or_varlen_bwd: too many tiles");
   char* ws = (char*)x.workspace;
   BwdArgs a;
@@ -999,15 +1124,17 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
   a.n_k = x.n_k;
   a.H = x.H;
   a.scale = x.scale;
-  a.split_q = s.split_q;
-  a.split_k = s.split_k;
+  a.slots_q = s.slots_q;
+  a.slots_k = s.slots_k;
   a.tq = s.tq;
   a.tk = s.tk;
-  a.max_q_tiles = (int32_t)s.max_q_tiles;
-  a.max_k_tiles = (int32_t)s.max_k_tiles;
+  a.max_q_items = (int32_t)s.max_q_items;
+  a.max_k_items = (int32_t)s.max_k_items;
   a.head = (int32_t*)ws;
-  a.q_tiles = (i32x4*)(ws + l.q_tiles);
-  a.k_tiles = (i32x4*)(ws + l.k_tiles);
+  a.q_items = (i32x4*)(ws + l.q_items);
+  a.k_items = (i32x4*)(ws + l.k_items);
+  a.q_split = (i32x4*)(ws + l.q_split);
+  a.k_split = (i32x4*)(ws + l.k_split);
   a.stat = (float*)(ws + l.stat);
   a.part_q = (float*)(ws + l.part_q);
   a.part_k = (float*)(ws + l.part_k);
@@ -1015,10 +1142,5 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
   const bool fine = is_fine(x);
   if (x.D == 128) fine ? launch<128, true>(a, s, st) : launch<128, false>(a, s, st);
   else fine ? launch<64, true>(a, s, st) : launch<64, false>(a, s, st);
-  const int64_t q8 = s.split_q > 1 ? (int64_t)x.n_q * row / 8 : 0, k8 = s.split_k > 1 ? (int64_t)x.n_k * row / 8 : 0;
-  if (q8 + k8 > 0) {
-    const int64_t blocks = std::min<int64_t>((q8 + 2 * k8 + kThreads - 1) / kThreads, 4096);
-    hipLaunchKernelGGL(bwd_add_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, a, q8, k8);
-  }
   return check_hip(hipGetLastError(), "attention backward launch");
 }

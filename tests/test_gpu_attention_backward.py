@@ -80,6 +80,11 @@ CASES = [
     ([1] * 300 + [2] * 213, [3] * 513, 1, 64),               # planned by a launch of its own
     ([2] * 255 + [130], [3] * 255 + [140], 2, 128),          # the most segments that are not
     ([2] * 256 + [130], [3] * 256 + [140], 2, 128),
+    # one long segment among short ones: some tiles split, their neighbours not
+    ([8, 1, 1000, 130, 40], [3000, 7000, 40, 900, 0], 2, 128),
+    ([3000, 7000, 40, 900, 0], [8, 1, 1000, 130, 40], 2, 64),
+    ([4] * 30 + [700] + [5] * 33, [3] * 30 + [5000] + [6] * 33, 1, 64),    # the most segments that are sorted and split
+    ([4] * 30 + [700] + [5] * 34, [3] * 30 + [5000] + [6] * 34, 1, 128),
     # many heads and segments: more than one round of work-groups
     ([130] * 33 + [300, 1], [70] * 33 + [513, 200], 16, 64),
     ([130] * 33 + [300, 1], [70] * 33 + [513, 200], 16, 128),
@@ -145,6 +150,20 @@ def test_ranges_backward_shares_key_rows(D, H):
     got = A.overlapping_ranges_backward(g[3], *g[:3], o, lse, qr, kr, dlse=dlse.to(DEV))
     check(got, *reference(q, k, v, do, qr, kr, dlse, o.cpu(), lse.cpu()))
     assert not got[1][:10].any() and not got[2][600:].any() and not got[0][211:511].any()
+
+
+@pytest.mark.parametrize('D', [64, 128])
+def test_ranges_backward_splits_shared_key_rows(D):
+    """key rows read by several segments of long queries: parts that begin and end inside any of them"""
+    lq, kr = [700, 1, 1500, 0, 333], [(0, 90), (30, 250), (60, 200), (0, 250), (80, 81)]
+    print(f'shared and split D={D}', flush=True)
+    qr, _ = cut(lq)
+    q, k, v, do = inputs(sum(lq), 260, 2, D)
+    g = [x.to(DEV) for x in (q, k, v, do)]
+    o, lse = A.overlapping_ranges_lse(*g[:3], qr, kr)
+    got = A.overlapping_ranges_backward(g[3], *g[:3], o, lse, qr, kr)
+    check(got, *reference(q, k, v, do, qr, kr, o=o.cpu(), lse=lse.cpu()))
+    assert not got[1][250:].any() and not got[2][250:].any()
 
 
 def test_rows_behind_the_last_segment_and_neighbours_that_are_not_finite():
