@@ -105,7 +105,8 @@ def _index_pointers(q, *index):
 
 
 def _backward(do, q, k, v, o, lse, index, n_seg, max_q, max_k, dlse=None):
-    """or_varlen_bwd on torch tensors: (dq, dk, dv), bf16 and contiguous. index: the addresses of cu_q, cu_k, k_off, k_len"""
+    """or_varlen_bwd on torch tensors: (dq, dk, dv), bf16 and contiguous. index: the addresses of cu_q, cu_k, k_off, k_len,
+    or an array of the ints of cu_q, k_off and k_len, which then lie behind the workspace"""
     _scene._check_bf16(do, q, k, v, o)
     if k.dim() != 3 or q.dim() != 3:
         raise _L.HipValueError('q, k and v must be [rows, heads, head_dim]')
@@ -134,8 +135,14 @@ def _backward(do, q, k, v, o, lse, index, n_seg, max_q, max_k, dlse=None):
     n = _GRAD_SIZES(n_seg, n_q, n_k, max_q, max_k, H, D)
     if n < 0:
         _L.check(_L.lib().or_varlen_bwd_workspace_size(n_seg, n_q, n_k, max_q, max_k, H, D), 'or_varlen_bwd_workspace_size')
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
     p = _L.ptr
+    if isinstance(index, array.array):
+        ws = torch.empty(n + 4 * len(index), dtype=torch.uint8, device=dev)
+        to = ws.data_ptr() + n
+        _L.check(_L.call(dev, _L.lib().or_index_fill, index.buffer_info()[0], len(index), to), 'or_index_fill')
+        index = to, None, to + 4 * n_seg + 4, to + 8 * n_seg + 4
+    else:
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
     a = _L.VarlenBwdArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), p(dlse),
                          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *index, qs, ks, os_, dos, n_q, n_seg, n_q, n_k, max_q,
                          max_k, H, D, D ** -0.5, ws.data_ptr(), n)
@@ -339,11 +346,7 @@ def overlapping_ranges_backward(do, q, k, v, o, lse, q_ranges, k_ranges, dlse=No
     cu_q, starts, counts = _range_args(q, k, v, q_ranges, k_ranges)
     if not q.is_cuda:
         raise _L.HipTypeError(f'expected a bf16 GPU tensor, got {q.dtype} on {q.device}')
-    values = array.array('i', cu_q + starts + counts)
-    index, n = torch.empty(len(values), dtype=torch.int32, device=q.device), len(starts)
-    at = index.data_ptr()
-    _L.check(_L.call(q.device, _L.lib().or_index_fill, values.buffer_info()[0], len(values), at), 'or_index_fill')
-    return _backward(do, q, k, v, o, lse, (at, None, at + 4 * n + 4, at + 8 * n + 4), n,
+    return _backward(do, q, k, v, o, lse, array.array('i', cu_q + starts + counts), len(starts),
                      max(hi - lo for lo, hi in q_ranges), max(counts), dlse)
 
 

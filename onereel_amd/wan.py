@@ -10,6 +10,7 @@ j's queries read only sentence j, all scenes in one varlen launch. The RMSNorm +
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -107,7 +108,8 @@ def _grad_rows(x, C: int):
     copy where x is not such rows, e.g. an expanded gradient)"""
     if x.dtype != torch.bfloat16 or not x.is_cuda:
         raise L.HipTypeError(f'expected a bf16 GPU tensor, got {x.dtype} on {x.device}')
-    x = x.reshape(-1, C)
+    if x.dim() != 2 or x.shape[1] != C:
+        x = x.reshape(-1, C)
     row, one = x.stride()
     if one == 1 and row >= C and row % 8 == 0 and x.data_ptr() % 16 == 0:
         return x, row
@@ -117,8 +119,12 @@ def _grad_rows(x, C: int):
 def _weight(w, C: int):
     if w.numel() != C:
         raise L.HipValueError(f'weights must hold {C} elements, got {tuple(w.shape)}')
-    w = w.reshape(C).to(torch.bfloat16).contiguous()
+    if w.dtype != torch.bfloat16 or not w.is_contiguous():
+        w = w.reshape(C).to(torch.bfloat16).contiguous()
     return w if w.data_ptr() % 16 == 0 else w.clone()
+
+
+_SIZES = functools.lru_cache(256)(lambda S, C: int(L.lib().or_rmsnorm_rope_bwd_workspace_size(S, C)))
 
 
 def _norm_backward(dys, xs, ws, eps, C: int, D: int, cos=None, sin=None):
@@ -136,8 +142,9 @@ def _norm_backward(dys, xs, ws, eps, C: int, D: int, cos=None, sin=None):
         raise L.HipValueError('gradients and inputs must have the same rows')
     new = lambda: (torch.empty(S, C, dtype=torch.bfloat16, device=dev), torch.empty(C, dtype=torch.float32, device=dev))
     (dx0, dw0), (dx1, dw1) = new(), new() if both else (None, None)
-    n = int(L.lib().or_rmsnorm_rope_bwd_workspace_size(S, C))
-    L.check(min(n, 0), 'or_rmsnorm_rope_bwd_workspace_size')
+    n = _SIZES(S, C)
+    if n < 0:
+        L.check(L.lib().or_rmsnorm_rope_bwd_workspace_size(S, C), 'or_rmsnorm_rope_bwd_workspace_size')
     space = torch.empty(n, dtype=torch.uint8, device=dev)
     p = L.ptr
     L.check(L.call(dev, L.lib().or_rmsnorm_rope_bwd, d0.data_ptr(), p(d1), x0.data_ptr(), p(x1), w0.data_ptr(), p(w1), ds0,
@@ -169,7 +176,7 @@ def rms_norm_backward(dy, x, weight, eps: float):
     if dy.shape != x.shape:
         raise L.HipValueError(f'x {tuple(x.shape)} and its output\'s gradient {tuple(dy.shape)} must have one shape')
     (dx,), (dw,) = _norm_backward([dy], [x], [weight], eps, C, 128)
-    return dx.view(x.shape), dw
+    return dx if x.dim() == 2 else dx.view(x.shape), dw
 
 
 class _QK(torch.autograd.Function):
