@@ -12,14 +12,15 @@
  *   or_scatter        packed output rows written back to token order, text padding rows zeroed
  *   or_lse_merge      log-sum-exp merge of two partial attention results (attention split over key sets)
  *   or_rmsnorm_rope   fused RMSNorm + interleaved RoPE of the Wan self-attention's queries and keys
+ *   or_varlen_bwd, or_rmsnorm_rope_bwd         the gradients of or_varlen_fwd and or_rmsnorm_rope
  *   or_frame_pool     frame memory: per-frame sums of hidden states (deterministic)
  *   or_frame_select   frame memory: k-means (cosine) representatives and their medoids, one workgroup
  *   or_memory_select, or_memory_foreign,
  *   or_memory_index                            bounded memory: per-head k-means representatives, each piece's foreign
  *                                              representatives (multi-head form) or key lists (single-head form)
  *
- * The fused elementwise kernels of the Wan-shaped DiT block harness (a measurement harness around the scene path,
- * not part of it) are a separate library, libonereel_dit.so (include/onereel_dit.h).
+ * The linear layers and fused elementwise kernels of the Wan-shaped DiT block around the scene path are a separate library,
+ * libonereel_dit.so (include/onereel_dit.h).
  *
  * Conventions: every tensor is caller-owned device memory passed as a raw pointer; rows are [row][head][dim] with a
  * row stride in elements; bf16 is IEEE bfloat16 stored as uint16_t; index arrays are int32. Every launch goes on the
@@ -331,7 +332,7 @@ typedef struct or_varlen_bwd_args {
 } or_varlen_bwd_args;
 
 /* Bytes of device workspace or_varlen_bwd needs: tile tables, two statistics per query row and head, and fp32 partial
- * gradients where the call has so few tiles that a streamed axis is split. -1 for sizes it refuses. */
+ * gradients of the tiles that a call of up to 64 segments may split (up to 140 MB). -1 for sizes it refuses. */
 int64_t or_varlen_bwd_workspace_size(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H,
                                      int32_t D);
 
@@ -339,9 +340,9 @@ int64_t or_varlen_bwd_workspace_size(int32_t n_seg, int32_t n_q, int32_t n_k, in
  * 39-53,74-84, which the reference leaves to FlashAttention's own): with P = exp(scale q k^T - lse) and
  * delta = rowsum(d_o * o) - dlse, dS = P * (d_o v^T - delta), dv = P^T d_o, dq = scale dS k, dk = scale dS^T q, each summed
  * in fp32 over every segment that reads the row and rounded to bf16 once (P and dS are rounded to bf16 as operands). No
- * atomics: a call's results have the same bits every time. Two launches (dq, dk with dv), a tile planner ahead of
- * them with more than 256 segments, and one that adds
- * partial gradients where an axis is split. */
+ * atomics: a call's results have the same bits every time. Calls of up to 2^18 scores carry what the rounding of P and dS leaves
+ * out in a second product. Two launches (dq, dk with dv), a tile planner ahead of them with more than 256 segments, and one
+ * that adds partial gradients in calls that may split tiles. */
 int or_varlen_bwd(const or_varlen_bwd_args* args, void* stream);
 
 /* Replaces the log-sum-exp merge of partial attention results: ring._merge (src/onereel/parallel/ring.py:63-70) and

@@ -7,6 +7,8 @@ Drop-in modules (same names and semantics as the reference's):
     onereel_amd.attention                   src/onereel/attention.py on the HIP varlen kernel
     onereel_amd.hunyuan15                   Context / Processor / RoPE positions of src/onereel/models/hunyuan15.py
     onereel_amd.wan                         Context / Processor of src/onereel/models/wan.py
+onereel_amd.attention and the norms of onereel_amd.wan are differentiable; onereel_amd.linear has the linear layers of a block
+(bias, activation, gate and residual in the product's epilogue) and their gradient.
 Engine: onereel_amd.scene (ScopePlan, pack_rows, varlen, scatter, scene_attention) over libonereel_hip.so.
 """
 from .layout import SceneLayout

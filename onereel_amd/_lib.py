@@ -15,7 +15,7 @@ from pathlib import Path
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 
 LIB_PATH = Path(os.environ.get('ONEREEL_HIP_LIB', Path(__file__).resolve().parent / 'libonereel_hip.so'))
-# the DiT harness's elementwise kernels (include/onereel_dit.h), not on the scene-attention path
+# the linear layers and elementwise kernels of the Wan-shaped DiT (include/onereel_dit.h), not on the scene-attention path
 DIT_LIB_PATH = Path(__file__).resolve().parent / 'libonereel_dit.so'
 # bench.py's measurement kernels (include/onereel_bench.h), not on the scene-attention path
 BENCH_LIB_PATH = Path(__file__).resolve().parent / 'libonereel_bench.so'
@@ -181,7 +181,7 @@ def lib():
 
 
 def dit_lib():
-    """the DiT harness's library (it loads libonereel_hip.so beside it and reports errors through its or_last_error,
+    """the library of the Wan-shaped DiT (it loads libonereel_hip.so beside it and reports errors through its or_last_error,
     which dit_check reads through this handle)"""
     global _dit_lib
     if _dit_lib is None:

@@ -1,5 +1,5 @@
 """Build libonereel_hip.so (gfx950) in-tree with hipcc: one object per HIP source, then one shared library; and,
-linked against it, libonereel_dit.so (the DiT harness's elementwise kernels) and libonereel_bench.so (bench.py's
+linked against it, libonereel_dit.so (the linear layers and elementwise kernels of the Wan-shaped DiT) and libonereel_bench.so (bench.py's
 measurement kernels).
 
     python -m onereel_amd.build            # or __graft_entry__.build()
@@ -62,7 +62,7 @@ def build(verbose: bool = False) -> Path:
     tmp = LIB.with_suffix('.so.tmp')
     logs.append(_run([HIPCC, f'--offload-arch={ARCH}', '-shared', '-fPIC', *map(str, objs), '-o', str(tmp)]))
     os.replace(tmp, LIB)
-    # the harness and measurement libraries resolve the error helpers from libonereel_hip.so, found beside them at
+    # the DiT's and measurement libraries resolve the error helpers from libonereel_hip.so, found beside them at
     # run time
     for out, lib_objs in ((DIT_LIB, dit_objs), (BENCH_LIB, bench_objs)):
         tmp = out.with_suffix('.so.tmp')
