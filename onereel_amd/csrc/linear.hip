@@ -427,11 +427,85 @@ __global__ __launch_bounds__(kThreads) void join_kernel(GemmArgs g) {
   }
 }
 
-// Up to 16 MB rows of x: a work-group takes 16 columns and reads their rows of W once, its wavefronts dealing out k in
-// pieces of 128; no LDS but for the sum of the wavefronts. Bound by HBM: a load takes 64 contiguous bytes of each of W's 16
-// rows, the next one the other half of their lines (with 64 bytes a lane instead, 16 from each of 64 places a load, one row to
-// 12288 columns from 2048 takes 17.9 us and 32 rows 33, so 15.2 and 23: 3.3 TB/s; a second piece of k in flight and loads
-// past the caches gain nothing).
+// Loads of 16 bytes at a lane's byte offset, zeros where it has none: by way of a buffer descriptor, since with a branch around
+// each load they wait for one another.
+struct Rows {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ Rows(const uint16_t* p, int64_t rows, int64_t stride, int width)
+      : r(__builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)((rows - 1) * stride * 2) + width * 2, 0x00020000)) {}
+  __device__ __forceinline__ u32x4 at(uint32_t off, bool in) const {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, in ? off : 0x80000000u, 0, 0));
+  }
+};
+
+// N sums of a lane's own over all lanes, a half of them kept at each distance D, 32 to 1: at[0] of what a lane then holds
+template <int N, int D, int ALL>
+__device__ __forceinline__ void fold(float (&acc)[ALL], int lane, int& at) {
+  if constexpr (N > 1) {
+    const bool high = lane & D;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float mine = high ? acc[N / 2 + i] : acc[i], other = high ? acc[i] : acc[N / 2 + i];
+      acc[i] = mine + __shfl_xor(other, D);
+    }
+    at += high ? N / 2 : 0;
+  } else {
+    acc[0] += __shfl_xor(acc[0], D);
+  }
+  if constexpr (D > 1) fold<(N > 1 ? N / 2 : 1), D / 2>(acc, lane, at);
+}
+
+// M rows of x, 1 to 4: a work-group takes 8 columns, its wavefronts deal out k in pieces of 512 and read each column's row of W
+// in whole kilobytes; products on the vector units, sums over lanes by halves. Bound by HBM: one
+// row to 12288 columns from 2048 11.6 us (4.3 TB/s), on the matrix cores (below) 14.7; 2 rows of 7680 to 856 columns 6.2 and 11.3,
+// 4 rows of 8192 to 2048 11.5 and 13.4; 8 rows of 2048 to 12288 16.8 and 16.4, so up to 4.
+constexpr int kRowWaves = 4, kFewRows = 4;
+template <int M>
+__global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(GemmArgs g) {
+  constexpr int P = M == 3 ? 4 : M;   // the sums over lanes are dealt out by halves
+  __shared__ float sum[kRowWaves][P * 8];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, j0 = blockIdx.x * 8, K = (int)g.K;
+  const Rows wr(g.b.p + (int64_t)j0 * g.b.stride, 8, g.b.stride, K), xr(g.a.p, g.I, g.a.stride, K);
+  const uint32_t ws = (uint32_t)g.b.stride * 2, xs = (uint32_t)g.a.stride * 2;
+  float acc[P * 8] = {};
+  for (int k0 = w * 512; k0 < K; k0 += kRowWaves * 512) {
+    const uint32_t k = k0 + lane * 8;
+    const bool in = k < (uint32_t)K;
+    u32x4 wf[8], xf[M];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) wf[j] = wr.at(j * ws + k * 2, in);
+#pragma unroll
+    for (int m = 0; m < M; ++m) xf[m] = xr.at(m * xs + k * 2, in);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w0 = bf2f((uint16_t)(wf[j][i] & 0xffffu)), w1 = bf2f((uint16_t)(wf[j][i] >> 16));
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          acc[m * 8 + j] = fmaf(bf2f((uint16_t)(xf[m][i] & 0xffffu)), w0, acc[m * 8 + j]);
+          acc[m * 8 + j] = fmaf(bf2f((uint16_t)(xf[m][i] >> 16)), w1, acc[m * 8 + j]);
+        }
+      }
+  }
+  int at = 0;
+  fold<P * 8, 32>(acc, lane, at);
+  sum[w][at] = acc[0];
+  __syncthreads();
+  if (threadIdx.x < g.I) {
+    float v[8] = {};
+    for (int i = 0; i < kRowWaves; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += sum[i][threadIdx.x * 8 + e];
+    finish8(g.e, threadIdx.x, j0, g.J, v);
+  }
+}
+
+// 5 to 16 MB rows of x: a work-group takes 16 columns and reads their rows of W once, its wavefronts dealing out k in
+// pieces of 128; no LDS but for the sum of the wavefronts. A load takes 64 contiguous bytes of each of W's 16 rows, the next
+// one the other half of their lines (with 64 bytes a lane instead, 16 from each of 64 places a load, 33 us for 32 rows of 2048
+// to 12288 columns, so 23). A CU takes 14 bytes a clock this way, whatever is in flight: it is for calls that have little to
+// read a CU, and the tiles take the others (plan_of).
 constexpr int kSkinnyWaves = 8;
 template <int MB>
 __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(GemmArgs g) {
@@ -579,7 +653,7 @@ constexpr int64_t kMaxBlocks = ((int64_t)1 << 23) - 8;   // of 512 threads: a gr
 Plan plan_of(int64_t I, int64_t J, int64_t K, bool rows_of_k) {
   Plan p = {};
   p.split = 1;
-  if (rows_of_k && I <= 32) return p;
+  if (rows_of_k && I <= kFewRows) return p;
   const int64_t steps = (K + kStep - 1) / kStep;
   double best = 1e300;
   for (int tile : {256, 128, 64}) {
@@ -600,6 +674,17 @@ Plan plan_of(int64_t I, int64_t J, int64_t K, bool rows_of_k) {
       }
     }
   }
+  // up to 32 rows the kernel for them, by what 1024 k of 16 columns take a CU; the tiles' times above are those of full ones,
+  // bound by the matrix cores (us, skinny / tiles: 16 rows of 2048 to 2048 columns 6.7 / 9.5, of 8192 18.5 / 16.1; 32 of 512 to
+  // 512 4.2 / 5.5, of 2048 to 12288 22.6 / 14.5, of 7680 to 64 21.6 / 12.3)
+  if (rows_of_k && I <= 32) {
+    const int64_t groups = (J + 15) / 16, a_cu = (groups + kCUs - 1) / kCUs;
+    if (1.2 + (double)((K + 1023) / 1024 * a_cu) * (I <= 16 ? 2.2 : a_cu > 1 ? 3.2 : 2.7) <
+        1.2 * best + (p.split > 1 ? 4 : 1)) {
+      p.tile = 0;
+      p.split = 1;
+    }
+  }
   p.part_bytes = p.split > 1 ? (int64_t)p.split * I * J * 4 : 0;
   return p;
 }
@@ -617,6 +702,16 @@ void launch_tiles(const GemmArgs& g, int tile, hipStream_t st) {
 void launch_product(GemmArgs g, bool tra, bool trb, float* part, hipStream_t st) {
   const Plan p = plan_of(g.I, g.J, g.K, !tra && !trb);
   if (p.tile == 0) {
+    if (g.I <= kFewRows) {
+      const dim3 grid((unsigned)(g.J / 8)), block(64 * kRowWaves);
+      switch (g.I) {
+        case 1: hipLaunchKernelGGL(rows_kernel<1>, grid, block, 0, st, g); break;
+        case 2: hipLaunchKernelGGL(rows_kernel<2>, grid, block, 0, st, g); break;
+        case 3: hipLaunchKernelGGL(rows_kernel<3>, grid, block, 0, st, g); break;
+        default: hipLaunchKernelGGL(rows_kernel<4>, grid, block, 0, st, g);
+      }
+      return;
+    }
     const dim3 grid((unsigned)((g.J + 15) / 16));
     if (g.I <= 16) hipLaunchKernelGGL(skinny_kernel<1>, grid, dim3(64 * kSkinnyWaves), 0, st, g);
     else hipLaunchKernelGGL(skinny_kernel<2>, grid, dim3(64 * kSkinnyWaves), 0, st, g);

@@ -80,7 +80,8 @@ def check_backward(got, dy, x, w, z, t, name, bias):
         near(dg, (dyd * a).sum(0), 2 ** -19 * (dyd * z.double()).abs().sum(0), 'dgate')
 
 
-SIZES = [(1, 64, 64), (1, 2048, 520), (16, 72, 8), (17, 256, 1000), (32, 1000, 128), (33, 8, 72), (64, 64, 64), (65, 72, 136),
+SIZES = [(1, 64, 64), (1, 2048, 520), (1, 8, 8), (2, 4104, 24), (3, 520, 136), (4, 2560, 72), (5, 512, 40), (9, 4096, 48),
+         (32, 4096, 64), (16, 72, 8), (17, 256, 1000), (32, 1000, 128), (33, 8, 72), (64, 64, 64), (65, 72, 136),
          (127, 200, 1032), (300, 520, 264), (1000, 1024, 256), (257, 4096, 96), (4100, 264, 2056), (3333, 136, 3336)]
 
 
