@@ -68,7 +68,7 @@ typedef struct or_linear_args {
 } or_linear_args;
 
 /* Bytes of device workspace or_linear needs: fp32 partial products where the call has so few tiles that n_in is split
- * over several work-groups. Negative for sizes it refuses. */
+ * over several work-groups, 0 for others. Negative for sizes it refuses. */
 int64_t or_linear_workspace_size(int64_t n_rows, int32_t n_in, int32_t n_out);
 
 /* Replaces the Linear layers of the Wan transformer block with what follows them (diffusers' WanTransformerBlock and its
@@ -106,7 +106,7 @@ int64_t or_linear_bwd_workspace_size(int64_t n_rows, int32_t n_in, int32_t n_out
 
 /* The gradient of or_linear: dz = dy * gate * act'(z), dx = dz weight, dweight = dz^T x, dbias = sum of dz over rows and
  * dgate = sum of dy * act(z) over rows. Sums are fp32 in a fixed order; dx and dweight are rounded to bf16 once, and dz is
- * rounded to bf16 as an operand of their products (not in dbias). Up to six launches. */
+ * rounded to bf16 as an operand of their products (not in dbias). Up to five launches. */
 int or_linear_bwd(const or_linear_bwd_args* args, void* stream);
 
 #ifdef __cplusplus

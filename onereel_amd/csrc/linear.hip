@@ -142,6 +142,14 @@ struct Operand {
   int64_t stride;                    // elements between its rows (rows of i or j, or rows of k when transposed)
 };
 
+// sums over rows from dz_kernel's partial ones: [2][chunks][n], db and dgate
+struct SumArgs {
+  const float* part;
+  float* out[2];                     // each optional
+  int chunks, n;
+  int blocks;                        // work-groups ahead of a product's that take them; 0: none
+};
+
 struct GemmArgs {
   Operand a, b;
   int64_t I;                         // rows of C
@@ -151,7 +159,26 @@ struct GemmArgs {
   int tiles_i, tiles_j;
   float* part;                       // [split][I][J] when split > 1
   Epilogue e;
+  SumArgs sums;
 };
+
+// 64 columns of one sum for every 4 wavefronts, which deal out its partial rows; st: 64 floats a wavefront
+template <int WAVES>
+__device__ __forceinline__ void column_sums(const SumArgs& g, int block, float* st) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, unit = block * (WAVES / 4) + wave / 4;
+  const int which = unit & 1, col = (unit >> 1) * 64 + lane;
+  float* out = which ? g.out[1] : g.out[0];
+  const bool in = out && col < g.n;
+  float v = 0.0f;
+  if (in) {
+    const float* p = g.part + (int64_t)which * g.chunks * g.n + col;
+#pragma unroll 16
+    for (int b = wave % 4; b < g.chunks; b += 4) v += p[(int64_t)b * g.n];
+  }
+  st[wave * 64 + lane] = v;
+  __syncthreads();
+  if (wave % 4 == 0 && in) out[col] = (v + st[(wave + 1) * 64 + lane]) + (st[(wave + 2) * 64 + lane] + st[(wave + 3) * 64 + lane]);
+}
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const lds_void*)p; }
 
@@ -267,9 +294,9 @@ struct Frag {
 
 // Tiles in groups of 8 rows of tiles: the work-groups of one XCD (index modulo 8) take consecutive tiles, which share
 // their operands' rows in that XCD's L2.
-__device__ __forceinline__ bool tile_of(const GemmArgs& g, int& ti, int& tj, int& part) {
-  const int64_t n = (int64_t)g.tiles_i * g.tiles_j * g.split, per = (n + 7) / 8, j = blockIdx.x >> 3;
-  int64_t x = (blockIdx.x & 7) * per + j;
+__device__ __forceinline__ bool tile_of(const GemmArgs& g, int block, int& ti, int& tj, int& part) {
+  const int64_t n = (int64_t)g.tiles_i * g.tiles_j * g.split, per = (n + 7) / 8, j = block >> 3;
+  int64_t x = (block & 7) * per + j;
   if (j >= per || x >= n) return false;
   part = (int)(x % g.split);
   x /= g.split;
@@ -290,8 +317,12 @@ __global__ __launch_bounds__(128 * WJ) __attribute__((amdgpu_waves_per_eu(NB * (
   constexpr int kPad = TJ / WJ + 4;                        // floats per staged row of the epilogue
   constexpr int kStage = 2 * WJ * 32 * kPad * 4;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[NB * BUF > kStage ? NB * BUF : kStage];
+  if ((int)blockIdx.x < g.sums.blocks) {   // a multiple of 8 of them, so that the others keep their XCDs
+    column_sums<2 * WJ>(g.sums, blockIdx.x, (float*)lds);
+    return;
+  }
   int ti, tj, part;
-  if (!tile_of(g, ti, tj, part)) return;
+  if (!tile_of(g, (int)blockIdx.x - g.sums.blocks, ti, tj, part)) return;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wi = w / WJ, wj = w % WJ;
   const int64_t i0 = (int64_t)ti * TI, j0 = (int64_t)tj * TJ;
@@ -555,7 +586,8 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(GemmArgs g) {
 
 // ------------------------------------------------------------------------------------------------------------------
 // dz = dy * gate * act'(z) and the sums over rows db = sum dz, dgate = sum dy * act(z): 256 columns x 8 to 128 rows a
-// work-group, 8 columns a lane; the work-groups' partial sums are added up in order by a second launch. HBM-bound with
+// work-group, 8 columns a lane; the work-groups' partial sums are added up in order by work-groups ahead of the first product's
+// (a launch of their own took 4 us, and 3 of the host: 333 x 1000 -> 2048 27.9 us in a graph, so 26.0). HBM-bound with
 // many rows; with few of them by the latency of a work-group's rows, so they are dealt to 1024 work-groups or more
 struct DzArgs {
   const uint16_t *dy, *z;
@@ -614,25 +646,9 @@ __global__ __launch_bounds__(kThreads) void dz_kernel(DzArgs g) {
   }
 }
 
-constexpr int kSumWaves = 16;
-__global__ __launch_bounds__(64 * kSumWaves) void column_sum_kernel(DzArgs g) {
-  __shared__ float sum[kSumWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, which = blockIdx.y, col = blockIdx.x * 64 + lane;
-  float* out = which ? g.dgate : g.db;
-  if (!out) return;
-  float v = 0.0f;
-  if (col < g.N) {
-    const float* p = g.part + (int64_t)which * g.chunks * g.N + col;
-#pragma unroll 8
-    for (int b = wave; b < g.chunks; b += kSumWaves) v += p[(int64_t)b * g.N];
-  }
-  sum[wave][lane] = v;
-  __syncthreads();
-  if (wave == 0 && col < g.N) {
-    v = 0.0f;
-    for (int i = 0; i < kSumWaves; ++i) v += sum[i][lane];
-    out[col] = v;
-  }
+__global__ __launch_bounds__(kThreads) void column_sum_kernel(SumArgs g) {
+  __shared__ float st[kThreads];
+  column_sums<kThreads / 64>(g, blockIdx.x, st);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -649,7 +665,7 @@ struct Plan {
 // with two of 64 x 64 and one (128 x 8192 x 2048: 11 us). A work-group's start and epilogue count as 3 steps. Parts of k add
 // the launch that joins them and its traffic (1536 x 8192 in 2 parts: 19 us).
 constexpr int kCUs = 256;
-constexpr int64_t kMaxBlocks = ((int64_t)1 << 23) - 8;   // of 512 threads: a grid has under 2^32
+constexpr int64_t kMaxBlocks = ((int64_t)1 << 23) - (1 << 17);   // of 512 threads: a grid, sums over rows included, has under 2^32
 Plan plan_of(int64_t I, int64_t J, int64_t K, bool rows_of_k) {
   Plan p = {};
   p.split = 1;
@@ -689,10 +705,13 @@ Plan plan_of(int64_t I, int64_t J, int64_t K, bool rows_of_k) {
   return p;
 }
 
+int sum_blocks(int n, int waves) { return (2 * ((n + 63) / 64) * 4 / waves + 7) / 8 * 8; }
+
 template <bool TRA, bool TRB>
-void launch_tiles(const GemmArgs& g, int tile, hipStream_t st) {
+void launch_tiles(GemmArgs g, int tile, hipStream_t st) {
   const int64_t n = (int64_t)g.tiles_i * g.tiles_j * g.split;   // at most kCUs of 128 x 128: one a CU, with room for 4 buffers
-  const dim3 grid((unsigned)((n + 7) / 8 * 8));
+  if (g.sums.part) g.sums.blocks = sum_blocks(g.sums.n, tile == 256 ? 8 : 4);
+  const dim3 grid((unsigned)((n + 7) / 8 * 8 + g.sums.blocks));
   if (tile == 256) hipLaunchKernelGGL((gemm_kernel<256, 256, 4, 2, TRA, TRB>), grid, dim3(512), 0, st, g);
   else if (tile == 128 && n <= kCUs) hipLaunchKernelGGL((gemm_kernel<128, 128, 2, 4, TRA, TRB>), grid, dim3(kThreads), 0, st, g);
   else if (tile == 128) hipLaunchKernelGGL((gemm_kernel<128, 128, 2, 2, TRA, TRB>), grid, dim3(kThreads), 0, st, g);
@@ -777,7 +796,7 @@ using namespace onereel;
 
 extern "C" int64_t or_linear_workspace_size(int64_t n_rows, int32_t n_in, int32_t n_out) {
   if (int rc = check_sizes("or_linear_workspace_size", n_rows, n_out, n_in, OR_ACT_NONE)) return rc;
-  return plan_of(n_rows, n_out, n_in, true).part_bytes + 256;
+  return plan_of(n_rows, n_out, n_in, true).part_bytes;
 }
 
 extern "C" int or_linear(const or_linear_args* p, void* stream) {
@@ -795,7 +814,7 @@ extern "C" int or_linear(const or_linear_args* p, void* stream) {
       !al16(x.preactivation))
     return fail_arg("or_linear: pointers must be 16-byte aligned");
   const int64_t need = or_linear_workspace_size(x.n_rows, x.n_in, x.n_out);
-  if (!x.workspace || !al16(x.workspace) || x.workspace_bytes < need)
+  if (need > 0 && (!x.workspace || !al16(x.workspace) || x.workspace_bytes < need))
     return fail_arg("or_linear: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
   GemmArgs g = {};
   g.a = Operand{(const uint16_t*)x.x, x.x_row_stride};
@@ -841,6 +860,7 @@ extern "C" int or_linear_bwd(const or_linear_bwd_args* p, void* stream) {
   const bool sums = x.dbias || x.dgate, products = x.dx || x.dweight;
   if (!sums && !products) return 0;
   Operand dz{(const uint16_t*)x.dy, x.dy_row_stride};
+  SumArgs s = {};   // ride along with the first product's launch
   if (sums || (scaled && products)) {
     DzArgs d = {};
     d.dy = (const uint16_t*)x.dy;
@@ -859,8 +879,7 @@ extern "C" int or_linear_bwd(const or_linear_bwd_args* p, void* stream) {
     d.chunks = (int)((x.n_rows + d.chunk_rows - 1) / d.chunk_rows);
     if (d.chunks > 0)
       hipLaunchKernelGGL(dz_kernel, dim3((unsigned)((x.n_out + 255) / 256), (unsigned)d.chunks), dim3(kThreads), 0, st, d);
-    if (sums)
-      hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((x.n_out + 63) / 64), 2), dim3(64 * kSumWaves), 0, st, d);
+    if (sums) s = SumArgs{d.part, {x.dbias, x.dgate}, d.chunks, x.n_out, 0};
     if (d.dz) dz = Operand{d.dz, x.n_out};
   }
   if (x.dx && x.n_rows > 0) {
@@ -870,6 +889,8 @@ extern "C" int or_linear_bwd(const or_linear_bwd_args* p, void* stream) {
     g.I = x.n_rows;
     g.J = x.n_in;
     g.K = x.n_out;
+    g.sums = s;
+    s = {};
     g.e.y = (uint16_t*)x.dx;
     g.e.y_stride = x.n_in;
     launch_product(g, false, true, (float*)(ws + l.part), st);
@@ -881,9 +902,12 @@ extern "C" int or_linear_bwd(const or_linear_bwd_args* p, void* stream) {
     g.I = x.n_out;
     g.J = x.n_in;
     g.K = x.n_rows;
+    g.sums = s;
+    s = {};
     g.e.y = (uint16_t*)x.dweight;
     g.e.y_stride = x.n_in;
     launch_product(g, true, true, (float*)(ws + l.part), st);
   }
+  if (s.part) hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)sum_blocks(s.n, kThreads / 64)), dim3(kThreads), 0, st, s);
   return check_hip(hipGetLastError(), "or_linear_bwd launch");
 }

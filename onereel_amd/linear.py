@@ -61,10 +61,11 @@ _SIZES = functools.lru_cache(256)(lambda name, *sizes: int(getattr(L.dit_lib(), 
 
 
 def _workspace(device, name, *sizes):
+    """(a workspace or None, its bytes)"""
     n = _SIZES(name, *sizes)
     if n < 0:
         L.dit_check(getattr(L.dit_lib(), name)(*sizes), name)
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None, n
 
 
 def _sizes(x, weight):
@@ -89,11 +90,11 @@ def _forward(x, weight, bias, act: int, gate, residual, keep: bool):
     M, dev, p = x2.shape[0], x.device, L.ptr
     y = torch.empty(M, n_out, dtype=torch.bfloat16, device=dev)
     z = torch.empty_like(y) if keep else None
-    space = _workspace(dev, 'or_linear_workspace_size', M, n_in, n_out)
+    space, bytes_ = _workspace(dev, 'or_linear_workspace_size', M, n_in, n_out)
     a = L.LinearArgs(x2.data_ptr(), w.data_ptr(), p(b), p(g), p(r), y.data_ptr(), p(z), M, xs, ws, rs, n_out, n_in, n_out,
-                     act, b16, g16, space.data_ptr(), space.numel())
+                     act, b16, g16, p(space), bytes_)
     L.dit_check(L.call(dev, L.dit_lib().or_linear, ctypes.byref(a)), 'or_linear')
-    return y.view(shape), None if z is None else z.view(shape)
+    return (y, z) if len(shape) == 2 else (y.view(shape), None if z is None else z.view(shape))
 
 
 def linear(x, weight, bias=None, activation=None, gate=None, residual=None, keep_preactivation: bool = False):
@@ -140,11 +141,11 @@ def linear_backward(dy, x, weight, bias: bool = False, activation=None, gate=Non
     new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=dev)
     dx, dw = new(torch.bfloat16, M, n_in) if needs[0] else None, new(torch.bfloat16, n_out, n_in) if needs[1] else None
     db, dg = new(torch.float32, n_out) if bias else None, new(torch.float32, n_out) if gate is not None else None
-    space = _workspace(dev, 'or_linear_bwd_workspace_size', M, n_in, n_out, int(act != 0 or g is not None))
+    space, bytes_ = _workspace(dev, 'or_linear_bwd_workspace_size', M, n_in, n_out, int(act != 0 or g is not None))
     a = L.LinearBwdArgs(dy2.data_ptr(), x2.data_ptr(), w.data_ptr(), p(z), p(g), p(dx), p(dw), p(db), p(dg), M, ds, xs, ws,
-                        n_in, n_out, act, g16, space.data_ptr(), space.numel())
+                        n_in, n_out, act, g16, p(space), bytes_)
     L.dit_check(L.call(dev, L.dit_lib().or_linear_bwd, ctypes.byref(a)), 'or_linear_bwd')
-    return None if dx is None else dx.view(x.shape), dw, db, dg
+    return dx if dx is None or x.dim() == 2 else dx.view(x.shape), dw, db, dg
 
 
 class _Linear(torch.autograd.Function):

@@ -158,7 +158,8 @@ def linear_args(**kw):
     (dict(n_in=(1 << 21) + 8), '2\\^21'), (dict(activation=3), 'activation'), (dict(x=None), 'required'), (dict(y=None), 'required'),
     (dict(x_row_stride=56), 'strides'), (dict(weight_row_stride=68), 'strides'), (dict(y_row_stride=1 << 22), 'strides'),
     (dict(residual_row_stride=64), 'strides'), (dict(bias=4100), 'aligned'), (dict(preactivation=4104), 'aligned'),
-    (dict(workspace=None), 'workspace'), (dict(workspace_bytes=10), 'workspace'),
+    (dict(workspace=None, n_in=8192, x_row_stride=8192, weight_row_stride=8192), 'workspace'),
+    (dict(workspace_bytes=10, n_in=8192, x_row_stride=8192, weight_row_stride=8192), 'workspace'),
     (dict(n_rows=1 << 31), 'rows'), (dict(n_rows=1 << 30, n_in=1 << 12, x_row_stride=1 << 12, weight_row_stride=1 << 12), 'tiles'),
 ])
 def test_linear_refuses(kw, message):
@@ -204,8 +205,8 @@ def test_linear_workspace_sizes():
     assert d.or_linear_workspace_size(-1, 64, 64) < 0 and d.or_linear_workspace_size(4, 63, 64) < 0
     assert d.or_linear_bwd_workspace_size(4, 64, 4, 0) < 0
     # whole videos need no partial products forward; a long k with few tiles does, and never more than 32 of them
-    assert d.or_linear_workspace_size(12720, 2048, 8192) <= 256
-    assert 64 * 128 * 4 < d.or_linear_workspace_size(64, 8192, 128) <= 32 * 64 * 128 * 4 + 256
+    assert d.or_linear_workspace_size(12720, 2048, 8192) == 0 and d.or_linear_workspace_size(1, 2048, 12288) == 0
+    assert 64 * 128 * 4 < d.or_linear_workspace_size(64, 8192, 128) <= 32 * 64 * 128 * 4
     # dz in bf16 where there is an activation or a gate
     assert d.or_linear_bwd_workspace_size(12720, 2048, 8192, 1) - d.or_linear_bwd_workspace_size(12720, 2048, 8192, 0) == \
         12720 * 8192 * 2
