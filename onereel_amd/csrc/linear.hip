@@ -488,7 +488,7 @@ __device__ __forceinline__ void fold(float (&acc)[ALL], int lane, int& at) {
 
 // M rows of x, 1 to 4: a work-group takes 8 columns, its wavefronts deal out k in pieces of 512 and read each column's row of W
 // in whole kilobytes; products on the vector units, sums over lanes by halves. Bound by HBM: one
-// row to 12288 columns from 2048 11.6 us (4.3 TB/s), on the matrix cores (below) 14.7; 2 rows of 7680 to 856 columns 6.2 and 11.3,
+// row to 12288 columns from 2048, W in no cache, 11.6 us (4.3 TB/s), on the matrix cores (below) 14.7; 2 rows of 7680 to 856 columns 6.2 and 11.3,
 // 4 rows of 8192 to 2048 11.5 and 13.4; 8 rows of 2048 to 12288 16.8 and 16.4, so up to 4.
 constexpr int kRowWaves = 4, kFewRows = 4;
 template <int M>
