@@ -8,7 +8,7 @@
 // of 5 products would have to add dq into memory from every key tile, with atomics whose order changes the bits; the
 // two passes sum every gradient in registers in a fixed order, so a call gives the same bits every time.
 //
-// - A wavefront owns 32 rows (keys, or queries; 64 queries with heads of 64) of its work-group's tile and keeps their
+// - A wavefront owns 32 rows (keys, or queries; 64 queries in long calls with heads of 64) of its work-group's tile and keeps their
 //   operands and their fp32 gradient in registers; the rows of the other side stream past in blocks of 32 through a ring of
 //   LDS slots filled by LDS DMA, three blocks ahead.
 // - Both products of scores put the streamed rows on the MFMA rows and the owned rows on its columns, so a lane holds
@@ -78,8 +78,10 @@ struct BwdArgs {
 // Blocks of 32 queries that a wavefront owns. One leaves room for two wavefronts on a SIMD, one's exponentials under the
 // other's matrix work: 3 x 9680 queries x 11440 keys, 16 heads of 128, dq 3.41 ms against 3.88 with two blocks (one
 // wavefront); dk and dv 4.80 against 5.36 ms with 32 and 64 keys. With heads of 64, two blocks fit twice too and halve the
-// LDS reads per query: 2 x 3001 x 3001 131 us against 138 (dk and dv with 64 keys do not fit twice: 239 against 198 us).
-constexpr int query_blocks(int D) { return D == 64 ? 2 : 1; }
+// LDS reads per query, one block fits four times: 24 x 9680 x 9680 850 us with two and 890 with one, 2 x 3001 x 3001, 16 heads,
+// 146 and 128, 8 x 700 x 700 16.6 and 12.4. So two where their tiles fill the GPU (dk and dv with 64 keys do not fit twice:
+// 239 against 198 us).
+int query_blocks(int64_t n_q, int H, int D) { return D == 64 && n_q / 256 * H >= 2 * kCUs ? 2 : 1; }
 constexpr int kKeyTile = 128;
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -601,10 +603,9 @@ __device__ __forceinline__ bool item_of(int n_items, int H, int block, int& head
 
 // ------------------------------------------------------------------------------------------------------------------
 // dq: a block owns 128 T queries of one head and streams the keys and values of their segment
-template <int D, bool FEW, bool FINE>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ? 1 : 2, 2))) void bwd_q_kernel(BwdArgs a) {
+template <int D, int T, bool FEW, bool FINE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(FINE ? 1 : 2, D == 64 && T == 1 ? 4 : 2))) void bwd_q_kernel(BwdArgs a) {
   using C = Str<D>;
-  constexpr int T = query_blocks(D);
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * kRing * C::SLOT];
   const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
   QueryItems qi;
@@ -983,6 +984,7 @@ struct Shape {
   int tq, tk;                        // rows of a query tile and of a key tile
   int64_t max_q_items, max_k_items;
   int slots_q, slots_k;
+  bool fine;                         // see shape_of
 };
 
 // Partial gradients of tiles that a head may have: parts_of's limits, of at most `tiles` tiles of at most `blocks` blocks. None in
@@ -992,9 +994,16 @@ int slots_of(int32_t n_seg, int64_t tiles, int64_t blocks, int H) {
   return (int)std::min<int64_t>(kMaxParts / H + 1, tiles * blocks / 6 + 1);
 }
 
+// fine: whether P and dS go into their products as two bf16 numbers, the rounded value and what that rounding left out: in calls
+// of few scores, which latency bounds. A result rounded once has its own rounding and that of its operand, 1.41 times the
+// error of its own rounding alone with many scores and up to 1.55 times with few, where the roundings do not average out;
+// with the second product it is 1.00 times. Kernel times with one product / two: 13.5 / 14.2 us at 2 heads x 64 x 64
+// scores (D 64), 18.8 / 20.3 at 4 x 128 x 128; above the limit 31.5 / 35.6 at 8 x 256 x 256 (D 128), 75.8 / 87.0 at
+// 8 x 1400 x 1400.
 Shape shape_of(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H, int32_t D) {
   Shape s;
-  s.tq = 128 * query_blocks(D);
+  s.fine = (int64_t)H * n_q * max_k <= (int64_t)1 << 18;
+  s.tq = 128 * (s.fine ? 1 : query_blocks(n_q, H, D));
   s.tk = kKeyTile;
   const int64_t q_tiles = n_q / s.tq + n_seg + 1, k_tiles = n_k / s.tk + 2 * (int64_t)n_seg + 1;
   s.slots_q = slots_of(n_seg, q_tiles, ((int64_t)max_k + kBlk - 1) / kBlk, H);
@@ -1029,28 +1038,18 @@ Layout layout_of(const Shape& s, int32_t n_q, int32_t H, int32_t D) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-template <int D, bool FINE>
+template <int D, int T, bool FINE>
 void launch(const BwdArgs& a, const Shape& s, hipStream_t st) {
   auto grid = [](int64_t items) { return dim3((unsigned)((items + 7) / 8 * 8)); };
   const dim3 gq = grid(s.max_q_items * a.H), gk = grid(s.max_k_items * a.H), t(kThreads);
   if (a.n_seg <= kFewSeg) {
-    hipLaunchKernelGGL((bwd_q_kernel<D, true, FINE>), dim3(gq.x + 8), t, 0, st, a);
+    hipLaunchKernelGGL((bwd_q_kernel<D, T, true, FINE>), dim3(gq.x + 8), t, 0, st, a);
   } else {
     hipLaunchKernelGGL(bwd_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
-    if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, false, FINE>), gq, t, 0, st, a);
+    if (a.n_q > 0) hipLaunchKernelGGL((bwd_q_kernel<D, T, false, FINE>), gq, t, 0, st, a);
   }
   if (a.n_k > 0) hipLaunchKernelGGL((bwd_kv_kernel<D, FINE>), gk, t, 0, st, a);
   if (s.slots_q || s.slots_k) hipLaunchKernelGGL(bwd_add_kernel<D>, dim3(8 * kCUs), t, 0, st, a);
-}
-
-// Whether P and dS go into their products as two bf16 numbers, the rounded value and what that rounding left out: in calls
-// of few scores, which latency bounds. A result rounded once has its own rounding and that of its operand, 1.41 times the
-// error of its own rounding alone with many scores and up to 1.55 times with few, where the roundings do not average out;
-// with the second product it is 1.00 times. Kernel times with one product / two: 13.5 / 14.2 us at 2 heads x 64 x 64
-// scores (D 64), 18.8 / 20.3 at 4 x 128 x 128; above the limit 31.5 / 35.6 at 8 x 256 x 256 (D 128), 75.8 / 87.0 at
-// 8 x 1400 x 1400.
-bool is_fine(const or_varlen_bwd_args& x) {
-  return (int64_t)x.H * x.n_q * x.max_k <= (int64_t)1 << 18;
 }
 
 }  // namespace
@@ -1139,8 +1138,8 @@ extern "C" int or_varlen_bwd(const or_varlen_bwd_args* p, void* stream) {
   a.part_q = (float*)(ws + l.part_q);
   a.part_k = (float*)(ws + l.part_k);
   hipStream_t st = (hipStream_t)stream;
-  const bool fine = is_fine(x);
-  if (x.D == 128) fine ? launch<128, true>(a, s, st) : launch<128, false>(a, s, st);
-  else fine ? launch<64, true>(a, s, st) : launch<64, false>(a, s, st);
+  if (x.D == 128) s.fine ? launch<128, 1, true>(a, s, st) : launch<128, 1, false>(a, s, st);
+  else if (s.fine) launch<64, 1, true>(a, s, st);
+  else s.tq == 128 ? launch<64, 1, false>(a, s, st) : launch<64, 2, false>(a, s, st);
   return check_hip(hipGetLastError(), "attention backward launch");
 }

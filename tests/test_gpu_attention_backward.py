@@ -85,6 +85,9 @@ CASES = [
     ([3000, 7000, 40, 900, 0], [8, 1, 1000, 130, 40], 2, 64),
     ([4] * 30 + [700] + [5] * 33, [3] * 30 + [5000] + [6] * 33, 1, 64),    # the most segments that are sorted and split
     ([4] * 30 + [700] + [5] * 34, [3] * 30 + [5000] + [6] * 34, 1, 128),
+    # heads of 64 whose tiles of 256 queries fill the GPU
+    ([700, 33, 256, 1100, 90], [130, 257, 64, 33, 100], 64, 64),
+    ([8] * 300, [5] * 300, 64, 64),
     # many heads and segments: more than one round of work-groups
     ([130] * 33 + [300, 1], [70] * 33 + [513, 200], 16, 64),
     ([130] * 33 + [300, 1], [70] * 33 + [513, 200], 16, 128),
