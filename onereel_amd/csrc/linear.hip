@@ -75,20 +75,17 @@ __device__ __forceinline__ void load8(const void* p, int bf16, int col, float (&
   }
 }
 
-// 1 / (1 + exp(-x)) with v_exp_f32 and v_rcp_f32, good to 2^-22 (a full division costs the epilogue of a 256 x 256 tile as
-// much again as the rest of a GELU: the layer of 12720 x 2048 -> 8192 478 us with it, 455 so)
-__device__ __forceinline__ float logistic(float x) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));
-}
+// 1 / (1 + 2^x) with v_exp_f32 and v_rcp_f32, good to 2^-22 (a full division costs the epilogue of a 256 x 256 tile as
+// much again as the rest of a GELU: the layer of 12720 x 2048 -> 8192 478 us with it, 455 so; the activation asked for once
+// for 8 columns and its constants folded, 480 and 466 in turn)
+__device__ __forceinline__ float falling(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)); }
+constexpr float kLog2e = 1.44269504088896340736f;
+__device__ __forceinline__ float logistic(float x) { return falling(x * -kLog2e); }
 
 // 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3)
 constexpr float kGelu1 = 2 * 0.7978845608028654f, kGelu3 = kGelu1 * 0.044715f;
-
-__device__ __forceinline__ float act_of(float z, int act) {
-  if (act == OR_ACT_SILU) return z * logistic(z);
-  if (act == OR_ACT_GELU_TANH) return z * logistic(z * (kGelu1 + kGelu3 * z * z));
-  return z;
-}
+__device__ __forceinline__ float gelu(float z) { return z * falling(z * fmaf(-kLog2e * kGelu3, z * z, -kLog2e * kGelu1)); }
+__device__ __forceinline__ float silu(float z) { return z * logistic(z); }
 
 // act(z) and act'(z). The derivative is taken at z clamped to +-20, where it has reached 0 or 1 in fp32: no 0 * inf.
 __device__ __forceinline__ void act_grad(float z, int act, float& f, float& d) {
@@ -104,7 +101,7 @@ __device__ __forceinline__ void act_grad(float z, int act, float& f, float& d) {
     d = p + c * p * q * (kGelu1 + 3.0f * kGelu3 * c * c);
   }
   if (z != z) d = z;
-  f = act_of(z, act);
+  f = act == OR_ACT_SILU ? silu(z) : gelu(z);
 }
 
 // 8 columns col .. of one row from the fp32 products v
@@ -116,9 +113,13 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t row, int col,
     for (int i = 0; i < 8; ++i) v[i] += t[i];
   }
   if (e.z) *(u32x4*)(e.z + row * cols + col) = u32x4{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
-  if (e.act != OR_ACT_NONE)
+  if (e.act == OR_ACT_GELU_TANH) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_of(v[i], e.act);
+    for (int i = 0; i < 8; ++i) v[i] = gelu(v[i]);
+  } else if (e.act == OR_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = silu(v[i]);
+  }
   if (e.gate) {
     load8(e.gate, e.gate_bf16, col, t);
 #pragma unroll
