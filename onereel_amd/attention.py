@@ -83,9 +83,12 @@ _MAX_STRIDE = 1 << 24      # of or_varlen_bwd's rows
 def _rows_for(x, H: int, D: int):
     """(x, row stride), x itself where its rows are as the kernels read them, else a copy (a gradient may come expanded or
     transposed)"""
-    shape, stride = x.shape, x.stride()    # asked for once, as in scene._rows2d: a small call's time is the host's
+    shape = x.shape    # asked for once, as in scene._rows2d: a small call's time is the host's
     if len(shape) != 3 or shape[1] != H or shape[2] != D:
         raise _L.HipValueError(f'expected [rows, {H}, {D}], got {tuple(shape)}')
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, H * D
+    stride = x.stride()
     row = stride[0]
     if stride[2] == 1 and stride[1] == D and H * D <= row <= _MAX_STRIDE and row % 8 == 0 and x.data_ptr() % 16 == 0:
         return x, row
