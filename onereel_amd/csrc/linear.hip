@@ -19,8 +19,8 @@
 // - Tiles of 256 x 256 are bound by the matrix cores; smaller tiles and a k axis split over several work-groups (fp32
 //   partial products, added in order by the epilogue's own launch) fill the GPU when there are few tiles. Up to 32 rows
 //   of x take a kernel of their own that streams W once, bound by HBM.
-// Measured (bf16, fp32 sums): 12720 x 2048 -> 8192 with bias, GELU and the pre-activation written 455 us, the product alone
-// 400 to 450 (a library product of that size, without epilogue, 375 to 400); dx 400 us (library 425), dW 360 us (library 460).
+// Measured (bf16, fp32 sums): 12720 x 2048 -> 8192 with bias, GELU and the pre-activation written 426 to 467 us, the product
+// alone 385 (a library product of that size, without epilogue, 361 to 375); dx 400 us (library 425), dW 345 (library 460).
 #include <math.h>
 
 #include <algorithm>
