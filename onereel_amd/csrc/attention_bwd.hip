@@ -117,8 +117,8 @@ constexpr int kFewSeg = 256;
 constexpr int kSorted = 64;
 
 // Parts of a tile that streams `blocks` blocks, in a call whose heads' tiles stream `total` blocks each: the nearest number that
-// gives every one of 256 CUs a share of the call's blocks as long as a part, no part shorter than 8 blocks or so; and where
-// such parts are 48 blocks long, nearly twice as many, since two work-groups on a CU fill each other's gaps. A tile of 2 parts
+// gives every one of 256 CUs a share of the call's blocks as long as a part, no part shorter than 4 blocks or so (with 8, passes
+// of 1 to 2 heads with few segments take 14 to 17 us, so 11 to 14); and where such parts are 48 blocks long, nearly twice as many, since two work-groups on a CU fill each other's gaps. A tile of 2 parts
 // or more has at most blocks / share + 1/2 <= 4/3 blocks / share of them, so a head's split tiles have at most
 // 4/3 total / share, kMaxParts over all heads, and never more than the workspace's slots. 24 calls of 1 to 24 segments of 1
 // to 12720 rows, 1 to 8 heads: 2.4 to 6 times as fast where one segment outweighs the others, 1.5 times on (geometric)
@@ -126,7 +126,7 @@ constexpr int kSorted = 64;
 // part, 103 in 5, 80 in 10.
 constexpr int kMaxParts = 700;
 __device__ __forceinline__ int share_of(int64_t total, int H, int slots) {
-  int64_t share = max((total * H + kCUs - 1) / kCUs, (int64_t)8);
+  int64_t share = max((total * H + kCUs - 1) / kCUs, (int64_t)4);
   if (share >= 48) share = share * 9 / 16;
   return (int)min(max(share, (4 * total + 3 * slots - 1) / (3 * slots)), (int64_t)1 << 30);
 }
@@ -991,7 +991,7 @@ struct Shape {
 // calls of more than 16 rounds of work-groups, whose longest tiles come first.
 int slots_of(int32_t n_seg, int64_t tiles, int64_t blocks, int H) {
   if (n_seg > kSorted || (tiles - n_seg / 2) * H > 32 * kCUs || blocks < 12) return 0;
-  return (int)std::min<int64_t>(kMaxParts / H + 1, tiles * blocks / 6 + 1);
+  return (int)std::min<int64_t>(kMaxParts / H + 1, tiles * blocks / 3 + 1);
 }
 
 // fine: whether P and dS go into their products as two bf16 numbers, the rounded value and what that rounding left out: in calls

@@ -17,8 +17,8 @@
 // - Rows and columns past an operand's end load as zeros through the buffer descriptor (and an offset out of its range
 //   for the pieces past the end of a row that is not the last), so ragged sizes take the same path.
 // - Tiles of 256 x 256 are bound by the matrix cores; smaller tiles and a k axis split over several work-groups (fp32
-//   partial products, added in order by the epilogue's own launch) fill the GPU when there are few tiles. Up to 32 rows
-//   of x take a kernel of their own that streams W once, bound by HBM.
+//   partial products, added in order by the epilogue's own launch) fill the GPU when there are few tiles. Few rows of
+//   x take kernels of their own that stream W once, bound by HBM.
 // Measured (bf16, fp32 sums): 12720 x 2048 -> 8192 with bias, GELU and the pre-activation written 426 to 467 us, the product
 // alone 385 (a library product of that size, without epilogue, 361 to 375); dx 400 us (library 425), dW 345 (library 460).
 #include <math.h>
