@@ -74,13 +74,14 @@ def _qk_forward(q, k, wq, wk, eps, cos, sin, heads):
     if c.shape[0] != S or s.shape[0] != S:
         raise L.HipValueError(f'rotary tables hold {c.shape[0]} rows for {S} tokens')
     w1, w2 = (w.to(torch.bfloat16).contiguous() for w in (wq, wk))
-    qo = torch.empty(S, heads, D, dtype=torch.bfloat16, device=q.device)
+    # in their final shape: a view made inside an autograd function takes no in-place operation
+    qo = torch.empty(*lead, heads, D, dtype=torch.bfloat16, device=q.device)
     ko = torch.empty_like(qo)
     L.check(L.lib().or_rmsnorm_rope(q2.data_ptr(), k2.data_ptr(), w1.data_ptr(), w2.data_ptr(), q2.stride(0),
                                     k2.stride(0), S, C, D, float(eps), c.data_ptr(), s.data_ptr(), None, S,
                                     qo.data_ptr(), ko.data_ptr(), C, C, L.stream_handle(q.device)),
             'or_rmsnorm_rope')
-    return qo.view(*lead, heads, D), ko.view(*lead, heads, D)
+    return qo, ko
 
 
 def rms_norm(x, weight, eps: float):
@@ -96,11 +97,11 @@ def rms_norm(x, weight, eps: float):
     if x2.stride(1) != 1:
         raise L.HipValueError('x rows must be contiguous')
     w = weight.to(torch.bfloat16).contiguous()
-    out = torch.empty(x2.shape, dtype=torch.bfloat16, device=x.device)
+    out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
     L.check(L.lib().or_rmsnorm_rope(x2.data_ptr(), None, w.data_ptr(), None, x2.stride(0), 0, x2.shape[0], C, 128,
                                     float(eps), None, None, None, 0, out.data_ptr(), None, C, 0,
                                     L.stream_handle(x.device)), 'or_rmsnorm_rope')
-    return out.view(x.shape)
+    return out
 
 
 def _grad_rows(x, C: int):

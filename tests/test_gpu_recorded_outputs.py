@@ -1,0 +1,39 @@
+"""Outputs of calls that autograd records take in-place operations, as they do without autograd: they are no views made inside
+a custom autograd function, nor several views of one output."""
+import pytest
+import torch
+
+from helpers import rand_bf16
+from onereel_amd import wan
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason='needs the GPU')]
+DEV = 'cuda'
+
+
+def doubled(call, leaves, grads):
+    """call(*leaves)'s outputs doubled in place: twice the values, and twice the gradients (exact in bf16 and fp32). The inputs
+    need no gradient for the plain call, only the weights as in a model whose parameters have theirs switched on"""
+    plain = [t.clone() for t in call(*(t.detach() for t in leaves))]
+    want = torch.autograd.grad(call(*leaves), leaves, grads)
+    out = call(*leaves)
+    for y in out:
+        y.mul_(2)
+    assert all(torch.equal(y, 2 * p) for y, p in zip(out, plain))
+    got = torch.autograd.grad(out, leaves, grads)
+    assert all(torch.equal(a, 2 * b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('lead', [(), (1,), (2, 1)])
+def test_norms(lead):
+    print(f'in place: norms {lead}', flush=True)
+    S, H, D = 40, 8, 64
+    C, n = H * D, S * len(lead or (1,))
+    q, k, dq, dk = (rand_bf16((n, C), i).to(DEV).view(*lead, -1, C) for i in range(4))
+    wq, wk = (rand_bf16((C,), 7 + i).to(DEV).requires_grad_() for i in range(2))
+    a = torch.rand(n, D // 2, generator=torch.Generator().manual_seed(1), dtype=torch.float64) * 6.3
+    cos, sin = (t.float().repeat_interleave(2, 1).to(DEV) for t in (a.cos(), a.sin()))
+    heads = lambda t: t.view(*t.shape[:-1], H, D)
+    doubled(lambda x, y: wan._qk(q, k, x, y, 1e-6, cos, sin, H), [wq, wk], [heads(dq), heads(dk)])
+    doubled(lambda x: [wan.rms_norm(q, x, 1e-6)], [wq], [dq])
+    x = q.clone().requires_grad_()
+    doubled(lambda x: [wan.rms_norm(x, wq.detach(), 1e-6)], [x], [dq])
