@@ -88,13 +88,14 @@ def _forward(x, weight, bias, act: int, gate, residual, keep: bool):
     r, rs = (None, 0) if residual is None else _rows(residual, n_out, 'residual')
     (b, b16), (g, g16) = _vector(bias, n_out, 'bias'), _vector(gate, n_out, 'gate')
     M, dev, p = x2.shape[0], x.device, L.ptr
-    y = torch.empty(M, n_out, dtype=torch.bfloat16, device=dev)
+    # in its final shape: a view made inside an autograd function takes no in-place operation
+    y = torch.empty(shape, dtype=torch.bfloat16, device=dev)
     z = torch.empty_like(y) if keep else None
     space, bytes_ = _workspace(dev, 'or_linear_workspace_size', M, n_in, n_out)
     a = L.LinearArgs(x2.data_ptr(), w.data_ptr(), p(b), p(g), p(r), y.data_ptr(), p(z), M, xs, ws, rs, n_out, n_in, n_out,
                      act, b16, g16, p(space), bytes_)
     L.dit_check(L.call(dev, L.dit_lib().or_linear, ctypes.byref(a)), 'or_linear')
-    return (y, z) if len(shape) == 2 else (y.view(shape), None if z is None else z.view(shape))
+    return y, z
 
 
 def linear(x, weight, bias=None, activation=None, gate=None, residual=None, keep_preactivation: bool = False):

@@ -5,6 +5,7 @@ import torch
 
 from helpers import rand_bf16
 from onereel_amd import wan
+from onereel_amd.linear import linear, linear_backward
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason='needs the GPU')]
 DEV = 'cuda'
@@ -37,3 +38,19 @@ def test_norms(lead):
     doubled(lambda x: [wan.rms_norm(q, x, 1e-6)], [wq], [dq])
     x = q.clone().requires_grad_()
     doubled(lambda x: [wan.rms_norm(x, wq.detach(), 1e-6)], [x], [dq])
+
+
+@pytest.mark.parametrize('shape', [(48,), (5, 48), (2, 3, 48)])
+@pytest.mark.parametrize('activation', [None, 'silu'])
+def test_linear(shape, activation):
+    print(f'in place: linear {shape} {activation}', flush=True)
+    x, w = rand_bf16(shape, 1).to(DEV), rand_bf16((64, 48), 2).to(DEV)
+    dy = rand_bf16((*shape[:-1], 64), 3).to(DEV)
+    leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+    doubled(lambda a, b: [linear(a, b, activation=activation)], leaves, [dy])
+    y, z = linear(*leaves, activation=activation, keep_preactivation=True)
+    kept = z.clone()
+    z.add_(1)                               # the caller's own
+    assert y.shape == z.shape == dy.shape and torch.equal(z, kept + 1)
+    want = linear_backward(dy, x, w, activation=activation, preactivation=kept)[:2]
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))
