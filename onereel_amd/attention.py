@@ -297,17 +297,39 @@ def _concat(segments):
     return (q, k, v, cu_q, cu_k, max(nq), max(nk)), nq
 
 
+class _Pieces(torch.autograd.Function):
+    """x.split(sizes) as tensors that take in-place operations, which the views of torch's split do not. They are x's memory,
+    which the gradient of the call that made x reads: a piece that has changed is an error in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, sizes):
+        out = torch.unsafe_split_with_sizes(x, sizes)
+        ctx.save_for_backward(*out)
+        return tuple(out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        ctx.saved_tensors       # raises when one has changed
+        return torch.cat(grads), None
+
+
+def _pieces(x, sizes):
+    return _Pieces.apply(x, sizes) if x.requires_grad else x.split(sizes)
+
+
 def packed_lse(segments):
     """as packed, with each segment's log-sum-exp: list of (out, lse [H, n]) (attention.py:56-62)"""
     args, nq = _concat(segments)
     o, lse = varlen_lse(*args, check=False)    # offsets built here from the segments' lengths
-    return list(zip(o.split(nq), lse.split(nq, dim=1)))
+    # a recorded lse is kept for the gradient: the segments get copies
+    return list(zip(_pieces(o, nq), torch.split_with_sizes_copy(lse, nq, 1) if lse.requires_grad else lse.split(nq, dim=1)))
 
 
 def packed(segments):
     """segments: list of (q, k, v) sequences -> list of outputs, one varlen call (attention.py:65-71)"""
     args, nq = _concat(segments)
-    return varlen(*args, check=False).split(nq)    # offsets built here from the segments' lengths
+    return _pieces(varlen(*args, check=False), nq)    # offsets built here from the segments' lengths
 
 
 def _range_args(q, k, v, q_ranges, k_ranges):

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from helpers import rand_bf16
+from onereel_amd import attention as A
 from onereel_amd import wan
 from onereel_amd.linear import linear, linear_backward
 
@@ -54,3 +55,32 @@ def test_linear(shape, activation):
     assert y.shape == z.shape == dy.shape and torch.equal(z, kept + 1)
     want = linear_backward(dy, x, w, activation=activation, preactivation=kept)[:2]
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))
+
+
+@pytest.mark.parametrize('lse', [False, True])
+def test_packed(lse):
+    """every sequence's output takes in-place operations; the gradient, which reads the outputs, then says that they changed
+    (as torch's own operations that keep their result do)"""
+    print(f'in place: packed lse={lse}', flush=True)
+    H, D = 2, 64
+    segments = [tuple(rand_bf16((n, H, D), 10 * s + i).to(DEV).requires_grad_() for i, n in enumerate((nq, nk, nk)))
+                for s, (nq, nk) in enumerate(((9, 33), (1, 4), (70, 20)))]
+    call = lambda: [t for pair in A.packed_lse(segments) for t in pair] if lse else list(A.packed(segments))
+    with torch.no_grad():
+        want = call()
+    out = call()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    out[0].mul_(2)
+    assert torch.equal(out[0], 2 * want[0]) and all(torch.equal(a, b) for a, b in zip(out[1:], want[1:]))
+    with pytest.raises(RuntimeError, match='inplace'):
+        out[-2 if lse else -1].sum().backward()
+    if lse:                                 # the log-sum-exps are the caller's own
+        out = call()
+        want = torch.autograd.grad(out[0::2], segments[0], [torch.ones_like(t) for t in out[0::2]], retain_graph=True)
+        for t in out[1::2]:
+            t.mul_(2)
+        got = torch.autograd.grad(out[0::2], segments[0], [torch.ones_like(t) for t in out[0::2]])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    out = call()
+    torch.autograd.backward(out, [torch.ones_like(t) for t in out])
+    assert all(bool(torch.isfinite(t.grad.float()).all()) for s in segments for t in s)
