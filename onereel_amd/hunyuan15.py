@@ -20,7 +20,7 @@ from . import _lib as L
 from .frame_memory import FrameMemory
 from .layout import SceneLayout
 from .memory import BoundaryMemory, MemoryAttention, frame_plan
-from .scene import ScopePlan, rotate_queries, scene_attention
+from .scene import ScopePlan, rotate_queries, scene_attention, without_gradient
 
 
 @dataclass
@@ -147,7 +147,7 @@ def rotate_tokens(ctx: Context, x: torch.Tensor, cos, sin) -> torch.Tensor:
     if key not in ctx._cache:
         ctx._cache[key] = ScopePlan(SceneLayout(list(lay.lengths), halo=0), ctx.T, None, 0, ctx.scene_rope,
                                     ctx.rope_lengths, False, False, x.device)
-    return rotate_queries(ctx._cache[key], x, cos, sin)
+    return without_gradient('rotate_tokens', rotate_queries(ctx._cache[key], x, cos, sin), x)
 
 
 class Processor:

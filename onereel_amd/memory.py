@@ -34,7 +34,7 @@ import torch
 
 from . import _lib as L
 from .layout import SceneLayout
-from .scene import gather_rows, pack_job, scatter_rows, varlen
+from .scene import gather_rows, pack_job, scatter_rows, varlen, without_gradient
 
 ITERS_INIT, ITERS_UPDATE = 50, 2
 
@@ -362,7 +362,11 @@ class MemoryAttention:
         return hit[1]
 
     def __call__(self, key, q, k, v, p: Plan) -> torch.Tensor:
-        """q [Sq, H, D], k / v [L, H, D] bf16 on the GPU -> [Sq, H, D] (rows outside the plan's queries are zero)"""
+        """q [Sq, H, D], k / v [L, H, D] bf16 on the GPU -> [Sq, H, D] (rows outside the plan's queries are zero). A backward
+        pass that reaches the result raises: there is no gradient."""
+        return without_gradient('the bounded memory', self._attend(key, q, k, v, p), q, k, v)
+
+    def _attend(self, key, q, k, v, p: Plan) -> torch.Tensor:
         Sq, H, D = q.shape
         Lk = k.shape[0]
         if k.shape[1:] != (H, D) or v.shape != k.shape:
@@ -417,7 +421,8 @@ class MemoryAttention:
             st = self._tables(p, H, N + Le, q.device)
             if st.in_place and st.n * H <= 4096 and st.max_key_row < N + Le and st.max_cand < N:
                 rep, valid = self.memory._select(key, k, st.cand32, st.B, H, D)
-                return self._multi_head(st, q, k, v, rep, valid, rep.shape[1], (eq, ek, ev))
+                out = self._multi_head(st, q, k, v, rep, valid, rep.shape[1], (eq, ek, ev))
+                return tuple(without_gradient('the bounded memory', o, *parts) for o in out)
         out = self(key, torch.cat([q, eq]), torch.cat([k, ek]), torch.cat([v, ev]), p)
         return out[:N], out[N:]
 

@@ -10,6 +10,10 @@ launches on the caller's current stream, with no host synchronisation:
     attention            or_varlen_fwd     Q read in place, the own-frame values read in place, output written in place
     zero text padding    or_scatter        ot rows past the valid text (ot = eq.new_zeros in the reference)
 
+The functions here launch kernels on the tensors' memory and have no gradient. `scene_attention` says so when a backward pass
+reaches its outputs; the single launches under it (packing, varlen, write-back) are not known to autograd at all
+(`onereel_amd.attention` has the differentiable calls).
+
 `mode` says what q / k hold: 'raw' (before RoPE: the fused path, the table row of every query and key comes from
 the layout), 'rotated' (already rotated, as the reference's `scene` receives them: shared keys are re-rotated by
 _move_shared's two rotations when the shared frames are moved), or 'none' (no RoPE at all).
@@ -24,6 +28,27 @@ from . import _lib as L
 from .layout import SceneLayout
 
 MODES = ('raw', 'rotated', 'none')
+
+
+class _WithoutGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, out, *inputs):
+        ctx.what = what
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, _):
+        raise L.HipValueError(f'{ctx.what} has no gradient')
+
+
+def without_gradient(what: str, out, *inputs):
+    """out, which kernels without a gradient have made of inputs (None: no tensor), itself. Where autograd records and an input
+    requires a gradient, a backward pass that reaches out raises: left out of the graph, its share of the inputs' gradients
+    would be missing without a word."""
+    if out is not None and torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs):
+        return _WithoutGradient.apply(what, out, *inputs)
+    return out
 
 
 def _desc(lay: SceneLayout, T: int, counts, text_rows: int, scene_rope: bool, rope_lengths, adjacent: bool,
@@ -535,4 +560,4 @@ def scene_attention(plan: ScopePlan, q, k, v, eq, ek, ev, cos=None, sin=None, mo
         op = varlen(qp, kp, vp, plan.cu_q, plan.cu_k, plan.max_q, plan.max_k, k_off=plan.k_off, k_len=plan.k_len,
                     workspace=plan.workspace(H, D))
         scatter(plan, op, ov, ot)
-    return ov, ot
+    return tuple(without_gradient('scene_attention', o, q, k, v, eq, ek, ev) for o in (ov, ot))

@@ -21,7 +21,7 @@ from .comm import frame_tokens  # noqa: F401  (re-exported for callers of the re
 from .frame_memory import FrameMemory
 from .layout import SceneLayout
 from .memory import BoundaryMemory, MemoryAttention, frame_plan
-from .scene import ScopePlan, pack_layer, varlen
+from .scene import ScopePlan, pack_layer, varlen, without_gradient
 
 TEXT_LEN = 512
 
@@ -217,7 +217,7 @@ def _token_ranges(lay, T: int) -> list:
 
 def self_ranges(ctx: Context, q, k, v):
     """all tokens: every scene's keys are one contiguous range read in place, or packed per scene when it reads extra
-    frames (wan.py:110-124)"""
+    frames (wan.py:110-124); those packed scopes have no gradient, a backward pass that reaches their output raises"""
     T, lay = ctx.T, ctx.layout
     if any(lay.extra.get(j) for j in range(lay.n_scenes)):
         key = ('wan_plan', tuple(lay.lengths), lay.halo, lay.sides,
@@ -232,8 +232,9 @@ def self_ranges(ctx: Context, q, k, v):
         kp, vp, _ = pack_layer(plan, k, None, v, None, mode='none', values_in_place=in_place)
         o = torch.empty_like(q)
         vi = dict(v_tok=v, v_lead=plan.v_lead, v_row=plan.v_row, v_runs=plan.v_runs) if in_place else {}
-        return varlen(q, kp, vp, plan.cu_q, plan.cu_k, plan.max_q, plan.max_k, out=o, seg_q_src=plan.seg_q_src,
-                      n_q_video=plan.n_video, sum_q=plan.sum_q, **vi)
+        varlen(q, kp, vp, plan.cu_q, plan.cu_k, plan.max_q, plan.max_k, out=o, seg_q_src=plan.seg_q_src,
+               n_q_video=plan.n_video, sum_q=plan.sum_q, **vi)
+        return without_gradient('self_ranges with extra frames', o, q, k, v)
     k_ranges = []
     for j in range(lay.n_scenes):
         first, end = lay.key_range(j)
