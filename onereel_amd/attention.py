@@ -379,7 +379,8 @@ def merge_lse(o, lse, o_s, lse_s):
     """fold a partial attention result into a running one, in place: o [N, H, D] fp32 and lse [H, N] fp32 are updated
     with o_s [N, H, D] bf16 and lse_s [H, N] fp32 (as varlen_lse returns them). The log-sum-exp merge of ring._merge
     (src/onereel/parallel/ring.py:63-70) and of Processor._far_lse (src/onereel/models/hunyuan15.py:270-275).
-    Returns (o, lse)."""
+    Returns (o, lse). It has no gradient: where autograd records and an argument requires one, a backward pass that reaches
+    the results raises, as does one that needs what they held before."""
     N, H, D = o.shape
     if o.dtype != torch.float32 or lse.dtype != torch.float32 or lse_s.dtype != torch.float32:
         raise _L.HipTypeError('o, lse and lse_s must be float32')
@@ -390,6 +391,8 @@ def merge_lse(o, lse, o_s, lse_s):
     for x in (o, o_s):
         if x.stride(2) != 1 or x.stride(1) != D:
             raise _L.HipValueError('o and o_s rows must hold contiguous [H, D]')
+    for x in (o, lse):
+        _scene.overwritten('merge_lse', x, o, lse, o_s, lse_s)
     _L.check(_L.lib().or_lse_merge(o.data_ptr(), lse.data_ptr(), o_s.data_ptr(), lse_s.data_ptr(), N, H, D,
                                    o.stride(0), o_s.stride(0), _L.stream_handle(o.device)), 'or_lse_merge')
     return o, lse

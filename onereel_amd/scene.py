@@ -42,13 +42,25 @@ class _WithoutGradient(torch.autograd.Function):
         raise L.HipValueError(f'{ctx.what} has no gradient')
 
 
+def _recorded(inputs) -> bool:
+    return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs)
+
+
 def without_gradient(what: str, out, *inputs):
     """out, which kernels without a gradient have made of inputs (None: no tensor), itself. Where autograd records and an input
     requires a gradient, a backward pass that reaches out raises: left out of the graph, its share of the inputs' gradients
     would be missing without a word."""
-    if out is not None and torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs):
-        return _WithoutGradient.apply(what, out, *inputs)
-    return out
+    return _WithoutGradient.apply(what, out, *inputs) if out is not None and _recorded(inputs) else out
+
+
+def overwritten(what: str, x, *inputs):
+    """x, which a kernel without a gradient is about to update in place from inputs: as without_gradient, and autograd knows
+    that x has changed, so the gradient of a call that has kept what x held raises too"""
+    if _recorded(inputs):
+        return _WithoutGradient.apply(what, x, *inputs)
+    if not x.is_inference():
+        torch.autograd.graph.increment_version(x)
+    return x
 
 
 def _desc(lay: SceneLayout, T: int, counts, text_rows: int, scene_rope: bool, rope_lengths, adjacent: bool,

@@ -5,6 +5,7 @@ import torch
 
 from helpers import rand_bf16
 from onereel_amd import _lib as L
+from onereel_amd import attention as A
 from onereel_amd import hunyuan15 as HY
 from onereel_amd import wan
 from onereel_amd import wan_dit as WD
@@ -87,3 +88,35 @@ def test_hunyuan_scopes(memory, fused):
         return p.memory(HY.rotate_tokens(ctx, x[0], cos, sin), HY.rotate_tokens(ctx, x[1], cos, sin), *x[2:])
 
     refused(call, [q, k, v, eq, ek, ev], 'no gradient')
+
+
+def test_merge_of_partial_results():
+    """merge_lse updates its first two arguments in place, the log-sum-exp that varlen_lse kept for its gradient among them"""
+    print('merge', flush=True)
+    n = 50
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    xs = [rand_bf16((n, H, D), i).to(DEV) for i in range(5)]
+
+    def parts(q, k1, v1, k2, v2):
+        o, lse = A.varlen_lse(q, k1, v1, cu, cu, n, n)
+        return (o, o.float(), lse, *A.varlen_lse(q, k2, v2, cu, cu, n, n))
+
+    with torch.no_grad():
+        _, o, lse, *rest = parts(*xs)
+        want = A.merge_lse(o, lse, *rest)
+    leaves = [x.clone().requires_grad_() for x in xs]
+    for i in range(2):
+        _, o, lse, *rest = parts(*leaves)
+        got = A.merge_lse(o, lse, *rest)
+        assert got[0] is o and got[1] is lse and all(torch.equal(a, b) for a, b in zip(got, want))
+        with pytest.raises(L.HipValueError, match='merge_lse'):
+            got[i].sum().backward()
+    # what the first call kept has changed, also where the merge itself was not recorded
+    first, o, lse, *rest = parts(*leaves)
+    with torch.no_grad():
+        A.merge_lse(o, lse, *rest)
+    with pytest.raises(RuntimeError, match='inplace'):
+        first.sum().backward()
+    with torch.inference_mode():
+        _, o, lse, *rest = parts(*xs)
+        assert all(torch.equal(a, b) for a, b in zip(A.merge_lse(o, lse, *rest), want))
