@@ -17,7 +17,8 @@ It runs the attention through onereel_amd.wan's processors:
 GEMMs stay torch ops (hipBLASLt). The block's LayerNorm + modulation and gated residual adds are HIP passes instead of
 chains of torch kernels over fp32 temporaries: every residual add runs in one pass with the LayerNorm that follows it
 (`or_residual_layernorm_modulate`: the next norm of the block, or the next block's first norm, or the output norm),
-and only the first norm runs alone (`or_layernorm_modulate`). Shapes of
+and only the first norm runs alone (`or_layernorm_modulate`). These passes have no gradient: of `WanDiT.forward` only the output
+projection has one, a backward pass that reaches further raises. Shapes of
 Wan2.2-TI2V-5B: hidden 3072 = 24 heads x 128, FFN 14336, 30 blocks, eps 1e-6, patch (1, 2, 2) over 48 latent
 channels, text width 4096 projected to 3072.
 
@@ -39,6 +40,7 @@ from . import _lib as L
 from . import wan
 from .linear import linear
 from .layout import SceneLayout
+from .scene import overwritten, without_gradient
 
 
 @dataclass
@@ -76,13 +78,13 @@ def layernorm_modulate(x, eps, weight=None, bias=None, scale=None, shift=None):
     """bf16 [..., C] -> bf16 LayerNorm(x) [* weight + bias] [* (1 + scale) + shift], fp32 inside, one HIP pass (the
     block's x.float() / layer_norm / modulation / .to(bf16) chain)"""
     x2, C = _rows(x)
-    out = torch.empty(x2.shape, dtype=torch.bfloat16, device=x.device)
+    out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
     w, b, sc, sh = (_vec(t, C) for t in (weight, bias, scale, shift))
     d = L.dit_lib()
     L.dit_check(d.or_layernorm_modulate(x2.data_ptr(), out.data_ptr(), x2.shape[0], C, x2.stride(0), C, float(eps),
                                         L.ptr(w), L.ptr(b), L.ptr(sc), L.ptr(sh), L.stream_handle(x.device)),
                 'or_layernorm_modulate')
-    return out.view(x.shape)
+    return without_gradient('layernorm_modulate', out, x, weight, bias, scale, shift)
 
 
 def gated_residual_(x, a, gate=None):
@@ -92,6 +94,7 @@ def gated_residual_(x, a, gate=None):
     if Ca != C or a2.shape[0] != x2.shape[0]:
         raise L.HipValueError('x and a must have the same rows')
     g = _vec(gate, C)
+    overwritten('gated_residual_', x, x, a, gate)
     d = L.dit_lib()
     L.dit_check(d.or_gated_residual(x2.data_ptr(), a2.data_ptr(), L.ptr(g), x2.shape[0], C, x2.stride(0),
                                     a2.stride(0), L.stream_handle(x.device)), 'or_gated_residual')
@@ -105,14 +108,15 @@ def residual_layernorm_modulate_(x, a, eps, gate=None, weight=None, bias=None, s
     a2, Ca = _rows(a)
     if Ca != C or a2.shape[0] != x2.shape[0]:
         raise L.HipValueError('x and a must have the same rows')
-    out = torch.empty(x2.shape, dtype=torch.bfloat16, device=x.device)
+    overwritten('residual_layernorm_modulate_', x, x, a, gate)
+    out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
     g, w, b, sc, sh = (_vec(t, C) for t in (gate, weight, bias, scale, shift))
     d = L.dit_lib()
     L.dit_check(d.or_residual_layernorm_modulate(x2.data_ptr(), a2.data_ptr(), L.ptr(g), out.data_ptr(), x2.shape[0],
                                                  C, x2.stride(0), a2.stride(0), C, float(eps), L.ptr(w), L.ptr(b),
                                                  L.ptr(sc), L.ptr(sh), L.stream_handle(x.device)),
                 'or_residual_layernorm_modulate')
-    return out.view(x.shape)
+    return without_gradient('residual_layernorm_modulate_', out, x, a, gate, weight, bias, scale, shift)
 
 
 class Linear:

@@ -120,3 +120,36 @@ def test_merge_of_partial_results():
     with torch.inference_mode():
         _, o, lse, *rest = parts(*xs)
         assert all(torch.equal(a, b) for a, b in zip(A.merge_lse(o, lse, *rest), want))
+
+
+def test_inference_pass_of_the_model():
+    """WanDiT.forward updates its rows in place: it has the gradient of the output projection alone"""
+    print('inference pass', flush=True)
+    m = WD.WanDiT(WD.DiTConfig(dim=512, heads=4, ffn=1024, blocks=2, in_channels=4, text_dim=256),
+                  SceneLayout(LENGTHS, halo=1), T, 8, DEV, seed=3)
+    tokens, text = rand_bf16((S, 16), 1).to(DEV), rand_bf16((24, 256), 2).to(DEV)
+    rot = tuple(t.to(DEV) for t in WD.wan_rope_table(sum(LENGTHS), 4, 4, 128))
+    run = lambda: m.forward(tokens, 20.0, text, rot)
+    with torch.no_grad():
+        want = run()
+    m.proj_out.weight.requires_grad_()
+    run().sum().backward()
+    assert m.proj_out.weight.grad.any()
+    for p in (m.blocks[0].ffn_in.weight, m.blocks[1].norm2_w, m.time_in.weight, m.blocks[0].attn2.to_v.weight):
+        p.requires_grad_()
+        out = run()
+        assert torch.equal(out, want)
+        with pytest.raises(L.HipValueError, match='no gradient'):
+            out.sum().backward()
+        p.requires_grad_(False)
+    x, a = rand_bf16((6, 512), 1).to(DEV).requires_grad_(), rand_bf16((6, 512), 2).to(DEV)
+    with pytest.raises(L.HipValueError, match='layernorm_modulate'):
+        WD.layernorm_modulate(x, 1e-6, scale=torch.zeros(512, device=DEV), shift=torch.zeros(512, device=DEV)).sum().backward()
+    with pytest.raises(L.HipValueError, match='gated_residual_'):
+        WD.gated_residual_(x * 1, a).sum().backward()
+    # what an earlier call kept has changed
+    y = (x * 1).mul(3)
+    z = y.exp()
+    WD.gated_residual_(z.detach(), a)
+    with pytest.raises(RuntimeError, match='inplace'):
+        z.sum().backward()
