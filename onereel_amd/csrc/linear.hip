@@ -87,12 +87,13 @@ constexpr float kGelu1 = 2 * 0.7978845608028654f, kGelu3 = kGelu1 * 0.044715f;
 __device__ __forceinline__ float gelu(float z) { return z * falling(z * fmaf(-kLog2e * kGelu3, z * z, -kLog2e * kGelu1)); }
 __device__ __forceinline__ float silu(float z) { return z * logistic(z); }
 
-// act(z) and act'(z). The derivative is taken at z clamped to +-20, where it has reached 0 or 1 in fp32: no 0 * inf.
+// act(z) and act'(z). The derivative is taken at z clamped to where it has reached 0 or 1 in fp32, so that nothing is 0 * inf:
+// +-20 for GELU (within exp(-600) of it), +-100 for SiLU, whose derivative falls as z exp(z) only: -3.9e-8 at -20.
 __device__ __forceinline__ void act_grad(float z, int act, float& f, float& d) {
   f = z;
   d = 1.0f;
   if (act == OR_ACT_NONE) return;
-  const float c = fminf(fmaxf(z, -20.0f), 20.0f);
+  const float far = act == OR_ACT_SILU ? 100.0f : 20.0f, c = fminf(fmaxf(z, -far), far);
   if (act == OR_ACT_SILU) {
     const float p = logistic(c);
     d = p + c * p * (1.0f - p);
