@@ -332,7 +332,7 @@ typedef struct or_varlen_bwd_args {
 } or_varlen_bwd_args;
 
 /* Bytes of device workspace or_varlen_bwd needs: tile tables, two statistics per query row and head, and fp32 partial
- * gradients of the tiles that a call of up to 64 segments may split (up to 160 MB). -1 for sizes it refuses. */
+ * gradients of the tiles that a call of up to 64 segments may split (up to 184 MB). -1 for sizes it refuses. */
 int64_t or_varlen_bwd_workspace_size(int32_t n_seg, int32_t n_q, int32_t n_k, int32_t max_q, int32_t max_k, int32_t H,
                                      int32_t D);
 

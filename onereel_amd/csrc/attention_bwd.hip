@@ -120,7 +120,8 @@ constexpr int kSorted = 64;
 // gives every one of 256 CUs a share of the call's blocks as long as a part, no part shorter than 4 blocks or so (with 8, passes
 // of 1 to 2 heads with few segments take 14 to 17 us, so 11 to 14); and where such parts are 48 blocks long, nearly twice as many, since two work-groups on a CU fill each other's gaps. A tile of 2 parts
 // or more has at most blocks / share + 1/2 <= 4/3 blocks / share of them, so a head's split tiles have at most
-// 4/3 total / share, kMaxParts over all heads, and never more than the workspace's slots. 24 calls of 1 to 24 segments of 1
+// 4/3 total / share, and never more than the workspace's slots: kMaxParts / H + 1, up to 932 over all heads (233 of them), 184 MB
+// of dq, dk and dv. 24 calls of 1 to 24 segments of 1
 // to 12720 rows, 1 to 8 heads: 2.4 to 6 times as fast where one segment outweighs the others, 1.5 times on (geometric)
 // average, as with one number of parts for all tiles; 128 keys against 3 x 9680 queries, 16 heads: 488 us for dk and dv in 1
 // part, 103 in 5, 80 in 10.
