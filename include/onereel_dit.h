@@ -109,6 +109,12 @@ int64_t or_linear_bwd_workspace_size(int64_t n_rows, int32_t n_in, int32_t n_out
  * rounded to bf16 as an operand of their products (not in dbias). Up to five launches. */
 int or_linear_bwd(const or_linear_bwd_args* args, void* stream);
 
+/* How a product is computed at these sizes: product 0 is or_linear's, 1 and 2 are or_linear_bwd's dx and dweight. tile: rows
+ * and columns of a work-group's tile (256, 128 or 64; 0: or_linear's kernels for few rows), buffers: LDS buffers of its ring
+ * (0 with them), split: parts of the summed axis. Host only. */
+int or_linear_plan(int64_t n_rows, int32_t n_in, int32_t n_out, int32_t product, int32_t* tile, int32_t* buffers,
+                   int32_t* split);
+
 #ifdef __cplusplus
 }
 #endif

@@ -136,6 +136,7 @@ DIT_SIGNATURES = {
     'or_gated_residual': (i32, [vp, vp, vp, i64, i32, i64, i64, vp]),
     'or_residual_layernorm_modulate': (i32, [vp, vp, vp, vp, i64, i32, i64, i64, i64, ctypes.c_float, vp, vp, vp, vp,
                                              vp]),
+    'or_linear_plan': (i32, [i64, i32, i32, i32, ctypes.POINTER(i32), ctypes.POINTER(i32), ctypes.POINTER(i32)]),
     'or_linear_workspace_size': (i64, [i64, i32, i32]),
     'or_linear': (i32, [ctypes.POINTER(LinearArgs), vp]),
     'or_linear_bwd_workspace_size': (i64, [i64, i32, i32, i32]),

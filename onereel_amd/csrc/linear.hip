@@ -707,15 +707,18 @@ Plan plan_of(int64_t I, int64_t J, int64_t K, bool rows_of_k) {
   return p;
 }
 
+// LDS buffers of the ring: four where a CU has one work-group, with the room of two
+int buffers_of(int tile, int64_t work_groups) { return tile == 64 || (tile == 128 && work_groups <= kCUs) ? 4 : 2; }
+
 int sum_blocks(int n, int waves) { return (2 * ((n + 63) / 64) * 4 / waves + 7) / 8 * 8; }
 
 template <bool TRA, bool TRB>
 void launch_tiles(GemmArgs g, int tile, hipStream_t st) {
-  const int64_t n = (int64_t)g.tiles_i * g.tiles_j * g.split;   // at most kCUs of 128 x 128: one a CU, with room for 4 buffers
+  const int64_t n = (int64_t)g.tiles_i * g.tiles_j * g.split;
   if (g.sums.part) g.sums.blocks = sum_blocks(g.sums.n, tile == 256 ? 8 : 4);
   const dim3 grid((unsigned)((n + 7) / 8 * 8 + g.sums.blocks));
   if (tile == 256) hipLaunchKernelGGL((gemm_kernel<256, 256, 4, 2, TRA, TRB>), grid, dim3(512), 0, st, g);
-  else if (tile == 128 && n <= kCUs) hipLaunchKernelGGL((gemm_kernel<128, 128, 2, 4, TRA, TRB>), grid, dim3(kThreads), 0, st, g);
+  else if (tile == 128 && buffers_of(tile, n) == 4) hipLaunchKernelGGL((gemm_kernel<128, 128, 2, 4, TRA, TRB>), grid, dim3(kThreads), 0, st, g);
   else if (tile == 128) hipLaunchKernelGGL((gemm_kernel<128, 128, 2, 2, TRA, TRB>), grid, dim3(kThreads), 0, st, g);
   else hipLaunchKernelGGL((gemm_kernel<64, 64, 2, 4, TRA, TRB>), grid, dim3(kThreads), 0, st, g);
 }
@@ -799,6 +802,19 @@ using namespace onereel;
 extern "C" int64_t or_linear_workspace_size(int64_t n_rows, int32_t n_in, int32_t n_out) {
   if (int rc = check_sizes("or_linear_workspace_size", n_rows, n_out, n_in, OR_ACT_NONE)) return rc;
   return plan_of(n_rows, n_out, n_in, true).part_bytes;
+}
+
+extern "C" int or_linear_plan(int64_t n_rows, int32_t n_in, int32_t n_out, int32_t product, int32_t* tile, int32_t* buffers,
+                              int32_t* split) {
+  if (int rc = check_sizes("or_linear_plan", n_rows, n_out, n_in, OR_ACT_NONE)) return rc;
+  if (product < 0 || product > 2 || !tile || !buffers || !split)
+    return fail_arg("or_linear_plan: product must be 0, 1 or 2, and tile, buffers and split are required");
+  const Plan p = product == 0 ? plan_of(n_rows, n_out, n_in, true)
+                 : product == 1 ? plan_of(n_rows, n_in, n_out, false) : plan_of(n_out, n_in, n_rows, false);
+  *tile = p.tile;
+  *buffers = p.tile ? buffers_of(p.tile, (int64_t)p.tiles_i * p.tiles_j * p.split) : 0;
+  *split = p.split;
+  return 0;
 }
 
 extern "C" int or_linear(const or_linear_args* p, void* stream) {
