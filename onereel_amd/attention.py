@@ -56,7 +56,8 @@ def captured_leaves(*xs) -> bool:
     graph adds into its leaves' gradients on the stream of the first pass that used them; when that is another stream (an
     eager pass whose graph still lives), the capture ends the process. So autograd records no such call; the backward entry
     points without autograd can be captured."""
-    return any(x is not None and x.requires_grad and x.is_leaf for x in xs) and torch.cuda.is_current_stream_capturing()
+    return any(x is not None and x.is_cuda and x.requires_grad and x.is_leaf for x in xs) and \
+        torch.cuda.is_current_stream_capturing()
 
 
 def records(what: str, *xs) -> bool:
