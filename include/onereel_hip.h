@@ -340,8 +340,8 @@ int64_t or_varlen_bwd_workspace_size(int32_t n_seg, int32_t n_q, int32_t n_k, in
  * 39-53,74-84, which the reference leaves to FlashAttention's own): with P = exp(scale q k^T - lse) and
  * delta = rowsum(d_o * o) - dlse, dS = P * (d_o v^T - delta), dv = P^T d_o, dq = scale dS k, dk = scale dS^T q, each summed
  * in fp32 over every segment that reads the row and rounded to bf16 once (P and dS are rounded to bf16 as operands). No
- * atomics: a call's results have the same bits every time. Calls of up to 2^18 scores carry what the rounding of P and dS leaves
- * out in a second product. Two launches (dq, dk with dv), a tile planner ahead of them with more than 256 segments, and one
+ * atomics: a call's results have the same bits every time. Calls with H * n_q * max_k up to 2^18 carry what the rounding of P and dS
+ * leaves out in a second product. Two launches (dq, dk with dv), a tile planner ahead of them with more than 256 segments, and one
  * that adds partial gradients in calls that may split tiles. */
 int or_varlen_bwd(const or_varlen_bwd_args* args, void* stream);
 

@@ -6,7 +6,9 @@
 //
 // Two passes, each recomputing P: one over query tiles for dq (3 products), one over key tiles for dk and dv (4). One pass
 // of 5 products would have to add dq into memory from every key tile, with atomics whose order changes the bits; the
-// two passes sum every gradient in registers in a fixed order, so a call gives the same bits every time.
+// two passes sum every gradient in registers in a fixed order, so a call gives the same bits every time. Where a segment's
+// keys fit one tile (cross-attention to a sentence) or its queries do, one pass would need no such sums; those calls take
+// the two passes all the same, and read q and do, or k and v, twice.
 //
 // - A wavefront owns 32 rows (keys, or queries; 64 queries in long calls with heads of 64) of its work-group's tile and keeps their
 //   operands and their fp32 gradient in registers; the rows of the other side stream past in blocks of 32 through a ring of
@@ -16,14 +18,17 @@
 //   Their A operand is the streamed block transposed, read from the same slot by transposing LDS reads. The slot's
 //   swizzle serves both kinds of read without bank conflicts.
 // - P and dS are rounded to bf16 once, as the operands of the bf16 matrix cores (the forward pass rounds its P the same way);
-//   scores, P, dS, delta and all sums are fp32. Calls of few scores carry what that rounding leaves out in a second product.
+//   scores, P, dS, delta and all sums are fp32. Calls of few scores (shape_of) carry what that rounding leaves out in a second
+//   product.
 // - Key rows may belong to several segments (overlapping ranges): the key axis is cut at every range boundary, so that all
 //   rows of a key tile have the same segments, and the tile streams the queries of all of them. Rows past an end load as
 //   zeros: a zero query row adds nothing to dk and dv, and the scores of key rows past the end are set to P = 0.
 // - Tiles with long streamed axes (few queries against long keys, few keys against long queries, one long segment among short
 //   ones) are split; the parts write fp32 partial gradients, and a last launch adds them in order.
-// Measured: 3 x 9680 queries against overlapping 11440 keys, 16 heads of 128: dq 3.27 ms, dk and dv 4.14 ms, 1180 to 1220
-// TFLOP/s of the 7 products executed (a large bf16 product of the vendor library reaches 1390 to 1490 on the same card).
+// Measured: 3 x 9680 queries against overlapping 11440 keys, 16 heads of 128: dq 3.21 ms, dk and dv 4.09 ms, 1240 TFLOP/s of
+// the 7 products executed (a large bf16 product of the vendor library reaches 1360 to 1490 on the same card), the matrix pipes
+// busy 70 % of the cycles. With heads of 64 they are busy 49 % (dq) and 58 % (dk and dv), and the vector units, which have as
+// many exponentials and conversions for half the matrix work, 60 % and 53 % (with heads of 128, 48 % and 39 %).
 #include <math.h>
 
 #include <algorithm>
@@ -112,8 +117,10 @@ __device__ __forceinline__ void seg_k(const BwdArgs& a, int s, int& lo, int& n) 
 constexpr int kFewSeg = 256;
 // Of up to kSorted segments the tiles with the longest streamed axes come first, and long ones are split (parts_of): 12 ragged
 // sequences of 1 to 899 rows, 16 heads of 128, dq in 36 us, 42 in the order of the segments, dk and dv in 36 and 40;
-// 3 x 9680 queries against overlapping ranges, dk and dv, 4.14 ms and 4.33. Calls of more segments have short ones, or items
-// enough to even out.
+// 3 x 9680 queries against overlapping ranges, dk and dv, 4.14 ms and 4.33. A lane ranks one segment, so calls of more are neither
+// sorted nor split. Segments with keys of their own lose nothing by it (64 of 198 rows 184 us, 65 of 195 185, 256 of 49 180);
+// many that read the same keys do, whose tile streams all their queries alone: 64 ranges of 781 queries on the same 128 keys
+// take 407 us, 65 of 769 2475 (one range of 50 000 queries 346).
 constexpr int kSorted = 64;
 
 // Parts of a tile that streams `blocks` blocks, in a call whose heads' tiles stream `total` blocks each: the nearest number that
@@ -996,7 +1003,7 @@ int slots_of(int32_t n_seg, int64_t tiles, int64_t blocks, int H) {
 }
 
 // fine: whether P and dS go into their products as two bf16 numbers, the rounded value and what that rounding left out: in calls
-// of few scores, which latency bounds. A result rounded once has its own rounding and that of its operand, 1.41 times the
+// of few scores, which latency bounds, counted as heads x query rows x the longest segment's keys (the offsets are on the device). A result rounded once has its own rounding and that of its operand, 1.41 times the
 // error of its own rounding alone with many scores and up to 1.55 times with few, where the roundings do not average out;
 // with the second product it is 1.00 times. Kernel times with one product / two: 13.5 / 14.2 us at 2 heads x 64 x 64
 // scores (D 64), 18.8 / 20.3 at 4 x 128 x 128; above the limit 31.5 / 35.6 at 8 x 256 x 256 (D 128), 75.8 / 87.0 at
