@@ -1,0 +1,578 @@
+"""The calls whose time the work of a DiT block around its attention is judged by: the norms before and after a sub-block
+with their modulation, gate and residual (and their gradient), the rotary positions with several axes of queries and keys
+(and their gradient), the linear layers in microscaled 4-bit floating point, and the global norm of a model's gradients with
+their clipping. Sizes are those of the repository's own workloads (HunyuanVideo-1.5 480p: frames of 30 x 53 = 1590 tokens,
+16 heads x 128, width 2048, 8 frames a scene) and ragged ones around them.
+
+listed() names the cases, draw(rng) gives more of the same ranges; prepare makes what a program has in hand before the
+call, run is one pass (in plain torch, or with `own` through the framework's entry points), exact restates it in 64 bits,
+work says what a pass cannot do without. A case is a dict of plain values; lists of lengths are comma-separated text.
+"""
+from __future__ import annotations
+
+import math
+import random
+
+import torch
+
+own = False
+DEV = 'cuda'
+TYPES = {'bf16': torch.bfloat16, 'fp16': torch.float16, 'fp32': torch.float32}
+EPS = 1e-6
+
+
+def listed():
+    return [
+        # a sub-block's output added to one scene's tokens and the next norm, each of 8 frames with its own modulation
+        dict(name='norm-scene', kind='norm', per=1590, groups=8, width=2048, norm='layer', post='', residual=True,
+             gated=True, affine=False, modulated=True, scale=1.0, type='bf16'),
+        # its gradient, of the rows and of the modulation
+        dict(name='norm-bwd-scene', kind='norm_bwd', per=1590, groups=8, width=2048, norm='layer', post='', residual=True,
+             gated=True, affine=False, modulated=True, scale=1.0, type='bf16'),
+        # sandwich norms over a batch of prompts, an odd count of rows and a width that is no power of two, in fp16
+        dict(name='norm-bwd-text', kind='norm_bwd', per=333, groups=1, width=1000, norm='rms', post='rms', residual=True,
+             gated=True, affine=True, modulated=False, scale=0.7, type='fp16'),
+        # queries and keys of one scene: RMSNorm over all heads, then time, row and column of every token
+        dict(name='rotary-scene', kind='rotary', grid='8,30,53', start=0, heads=16, dim=128, dims='44,42,42',
+             pairs='interleaved', normed=True, whole=True, type='bf16'),
+        # its gradient
+        dict(name='rotary-bwd-scene', kind='rotary_bwd', grid='8,30,53', start=0, heads=16, dim=128, dims='44,42,42',
+             pairs='interleaved', normed=True, whole=True, type='bf16'),
+        # an image encoder's patches at interpolated positions, two axes, half-split pairs, fp32
+        dict(name='rotary-image', kind='rotary', grid='9,37', start=0, heads=5, dim=96, dims='48,48', pairs='half',
+             normed=False, whole=False, type='fp32'),
+        # one optimizer step of a 30-block model: gradients in bf16 buckets, clipped into the optimizer's buffers
+        dict(name='clip-model', kind='clip', blocks=30, width=1536, ffn=6144, count=0, largest=0, salt=0, limit=0.3,
+             into=True, type='bf16'),
+        # low-rank adapters: a few hundred small fp32 gradients whose norm is under its limit
+        dict(name='clip-adapters', kind='clip', blocks=0, width=0, ffn=0, count=240, largest=40000, salt=1, limit=4.0,
+             into=False, type='fp32'),
+        # the feed forward's first product over one scene, activations quantised in the call
+        dict(name='mx-ffn', kind='mx', rows=12720, n_in=2048, n_out=8192, act='gelu_tanh', bias=True, gate=False,
+             residual=False),
+        # its second product with the block's gate and residual, a batch of prompts with an odd count of rows
+        dict(name='mx-text', kind='mx', rows=333, n_in=8192, n_out=2048, act='', bias=True, gate=True, residual=True),
+        # the time embedding's projection to the six modulation vectors, one row
+        dict(name='mx-one-row', kind='mx', rows=1, n_in=2048, n_out=12288, act='silu', bias=True, gate=False,
+             residual=False),
+        # a layer's weights quantised and read back
+        dict(name='mx-quantize', kind='mx_quantize', rows=8192, width=2048, type='bf16'),
+    ]
+
+
+# the largest listed cases bound every drawn one
+_MAX_FLOPS, _MAX_BYTES = 4.3e11, 7.0e9
+
+
+def draw(rng):
+    while True:
+        case = _draw(rng)
+        w = work(case)
+        if w['flops'] <= _MAX_FLOPS and w['bytes'] <= _MAX_BYTES:
+            return case
+
+
+def _span(rng, lo, hi):
+    """an integer of [lo, hi], spread over its logarithm"""
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def _ints(text):
+    return [int(x) for x in text.split(',')] if text else []
+
+
+def _draw(rng):
+    kind = rng.choice(['norm', 'norm_bwd', 'rotary', 'rotary_bwd', 'clip', 'mx', 'mx', 'mx_quantize'])
+    dtype = rng.choice(['bf16', 'bf16', 'fp16', 'fp32'])
+    if kind in ('norm', 'norm_bwd'):
+        groups = _span(rng, 1, 300)
+        residual = rng.random() < 0.7
+        return dict(kind=kind, per=_span(rng, 1, 24000 // groups), groups=groups, width=8 * _span(rng, 8, 1024),
+                    norm=rng.choice(['layer', 'rms']), post=rng.choice(['', 'rms', 'layer']) if residual else '',
+                    residual=residual, gated=residual and rng.random() < 0.7, affine=rng.random() < 0.5,
+                    modulated=rng.random() < 0.6, scale=rng.choice([1.0, 0.5]) if residual else 1.0, type=dtype)
+    if kind in ('rotary', 'rotary_bwd'):
+        axes = rng.choice([1, 2, 3, 3])
+        grid = ','.join(str(_span(rng, 1, (20000, 140, 28)[axes - 1])) for _ in range(axes))
+        normed = rng.random() < 0.6
+        dim, heads = rng.choice([64, 128]), rng.choice([8, 16, 32])
+        if not normed:
+            dim, heads = 16 * rng.randint(1, 16), rng.randint(1, 24)
+        pairs = rng.choice(['interleaved', 'half'])
+        # the pairs dealt out to the axes, the last ones left unrotated in some heads
+        left = (dim if rng.random() < 0.7 or dim < 64 else dim - 16) // 2
+        cut = sorted(rng.sample(range(1, left), axes - 1))
+        dims = ','.join(str(2 * (b - a)) for a, b in zip([0] + cut, cut + [left]))
+        return dict(kind=kind, grid=grid, start=rng.choice([0, 0, 100000]), heads=heads, dim=dim, dims=dims, pairs=pairs,
+                    normed=normed, whole=rng.random() < 0.6, type=dtype)
+    if kind == 'clip':
+        return dict(kind=kind, blocks=0, width=0, ffn=0, count=_span(rng, 1, 1000), largest=_span(rng, 1, 4000000),
+                    salt=rng.randrange(1000), limit=rng.choice([0.01, 0.6, 4.0]), into=True, type=dtype)
+    if kind == 'mx':
+        return dict(kind=kind, rows=_span(rng, 1, 16000), n_in=32 * _span(rng, 1, 256), n_out=8 * _span(rng, 1, 1024),
+                    act=rng.choice(['', 'gelu_tanh', 'silu']), bias=rng.random() < 0.7, gate=rng.random() < 0.5,
+                    residual=rng.random() < 0.5)
+    return dict(kind=kind, rows=_span(rng, 1, 16000), width=32 * _span(rng, 1, 256), type=dtype)
+
+
+def work(case):
+    kind = case['kind']
+    e = 4 if case.get('type') == 'fp32' else 2
+    if kind in ('norm', 'norm_bwd'):
+        n = case['per'] * case['groups'] * case['width']
+        if kind == 'norm':
+            return dict(bytes=e * n * (4 if case['residual'] else 2), flops=n * (12 if case['residual'] else 8))
+        # dn, h in and dx out; with a residual dh and a in and da out too
+        return dict(bytes=e * n * (6 if case['residual'] else 3), flops=n * (30 if case['residual'] else 16))
+    if kind in ('rotary', 'rotary_bwd'):
+        rows = math.prod(_ints(case['grid']))
+        n, both = rows * case['heads'] * case['dim'], 2 if case['normed'] else 1
+        moved = 3 if case['normed'] and kind == 'rotary_bwd' else 2
+        return dict(bytes=both * moved * e * n + 4 * rows * len(_ints(case['grid'])), flops=both * (14 if case['normed'] else 4) * n)
+    if kind == 'clip':
+        n = sum(_sizes(case))
+        return dict(bytes=e * n * (2 if case['into'] else 1), flops=3 * n)
+    if kind == 'mx':
+        m, k, n = case['rows'], case['n_in'], case['n_out']
+        return dict(bytes=2 * m * k + n * k // 2 + n * k // 32 + 2 * m * n * (1 + case['residual']), flops=2 * m * n * k)
+    n = case['rows'] * case['width']
+    return dict(bytes=2 * e * n, flops=4 * n)
+
+
+def _sizes(case):
+    """the lengths of the gradients of a clip case: a model's, block by block, or log-uniform ones"""
+    d, f = case['width'], case['ffn']
+    if case['blocks']:
+        block = 8 * [d * d, d] + [d * f, f, f * d, d] + 4 * [d] + [d, d, 6 * d]
+        return case['blocks'] * block
+    rng = random.Random(case['salt'])
+    return [_span(rng, 1, case['largest']) for _ in range(case['count'])]
+
+
+# ------------------------------------------------------------------------------------------------------------------------
+# inputs
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    randn = lambda *shape: torch.randn(*shape, generator=g, device=DEV)
+    kind = case['kind']
+    make = _prepare_norm if kind.startswith('norm') else _prepare_rotary if kind.startswith('rotary') else \
+        _prepare_clip if kind == 'clip' else _prepare_mx
+    return dict(case=case, **make(case, randn))
+
+
+def _activations(randn, rows, width):
+    """rows as a residual stream has them: an offset for every column, some columns far larger than the others"""
+    large = 1 + 12 * (randn(width) > 2.3).float()
+    return randn(rows, width) * large + 0.3 * randn(width)
+
+
+def _prepare_norm(case, randn):
+    rows, C, G, dtype = case['per'] * case['groups'], case['width'], case['groups'], TYPES[case['type']]
+    some = lambda wanted, *shape: 0.3 * randn(*shape) if wanted else None
+    weight = lambda wanted: 1 + 0.1 * randn(C) if wanted else None
+    s = dict(x=_activations(randn, rows, C).to(dtype), a=randn(rows, C).to(dtype) if case['residual'] else None,
+             gate=some(case['gated'], G, C), scale=some(case['modulated'], G, C), shift=some(case['modulated'], G, C),
+             weight=weight(case['affine']), bias=some(case['affine'] and case['norm'] == 'layer', C),
+             post_weight=weight(case['post'] and case['affine']))
+    if case['kind'] == 'norm_bwd':
+        # x is the forward pass's h; gradients as small as they are behind a mean over a video
+        s['dn'] = (randn(rows, C) / 64).to(dtype)
+        s['dh'] = (randn(rows, C) / 64).to(dtype) if case['residual'] else None
+    return s
+
+
+def _prepare_rotary(case, randn):
+    grid, H, D, dtype = _ints(case['grid']), case['heads'], case['dim'], TYPES[case['type']]
+    S, C = math.prod(grid), H * D
+    at = torch.cartesian_prod(*(torch.arange(n, device=DEV) for n in grid)).reshape(S, len(grid))
+    at[:, 0] += case['start']
+    # whole positions, or those of a grid resized to another one
+    s = dict(positions=at.int() if case['whole'] else at.float() * 0.7 + 0.15, dims=tuple(_ints(case['dims'])))
+    s['x'] = [(randn(S, C) * 1.5).to(dtype).view(S, C) for _ in range(2 if case['normed'] else 1)]
+    s['w'] = [(1 + 0.1 * randn(C)).to(dtype) for _ in range(2)] if case['normed'] else None
+    if case['kind'] == 'rotary_bwd':
+        s['dy'] = [(randn(S, H, D) / 64).to(dtype) for _ in s['x']]
+    return s
+
+
+def _prepare_clip(case, randn):
+    sizes, dtype = _sizes(case), TYPES[case['type']]
+    flat = torch.empty(sum(sizes), dtype=dtype, device=DEV)
+    # one bucket, as a data-parallel program has them; piece by piece, the gradients' sizes differ from weight to weight
+    step = 1 << 26
+    for a in range(0, flat.numel(), step):
+        flat[a:a + step] = randn(min(step, flat.numel() - a)) * (1e-3 * (1 + a // step % 3))
+    n = flat.numel()
+    expected = 1e-3 * math.sqrt(sum(min(step, n - a) * (1 + a // step % 3) ** 2 for a in range(0, n, step)))
+    out = torch.empty_like(flat) if case['into'] else None
+    return dict(flat=flat, out=out, grads=list(flat.split(sizes)), outs=list(out.split(sizes)) if case['into'] else None,
+                max_norm=case['limit'] * expected)
+
+
+def _prepare_mx(case, randn):
+    if case['kind'] == 'mx_quantize':
+        # weights of very different rows, some blocks all zero
+        x = randn(case['rows'], case['width']) * torch.exp(2 * randn(case['rows'], 1))
+        x[:, :32] *= (randn(case['rows'], 1) > -1).float()
+        return dict(x=x.to(TYPES[case['type']]))
+    M, K, N = case['rows'], case['n_in'], case['n_out']
+    # weights as they are stored: two e2m1 codes a byte, the even element in the low half, one e8m0 scale for 32 elements
+    codes, scales = _quantized(randn(N, K) * K ** -0.5)
+    s = dict(x=_activations(randn, M, K).bfloat16(), codes=codes[:, 0::2] + 16 * codes[:, 1::2], scales=scales)
+    s['b'] = (0.1 * randn(N)).bfloat16() if case['bias'] else None
+    s['gate'] = 0.5 + 0.5 * randn(N) if case['gate'] else None
+    s['residual'] = randn(M, N).bfloat16() if case['residual'] else None
+    return s
+
+
+# ------------------------------------------------------------------------------------------------------------------------
+# one pass
+
+def run(s):
+    kind = s['case']['kind']
+    if own:
+        return _run_own(s, kind)
+    return {'norm': _norm, 'norm_bwd': _norm_grads, 'rotary': _rotary, 'rotary_bwd': _rotary_grads, 'clip': _clip,
+            'mx': _mx_linear, 'mx_quantize': _mx_values}[kind](s)
+
+
+def _run_own(s, kind):
+    case = s['case']
+    if kind in ('norm', 'norm_bwd'):
+        from onereel_amd import norms
+        pre = dict(norm=case['norm'], weight=s['weight'], bias=s['bias'], scale=s['scale'], shift=s['shift'])
+        add = dict(gate=s['gate'], residual_scale=case['scale'], post_norm=case['post'] or None,
+                   post_weight=s['post_weight'])
+        if kind == 'norm':
+            return norms.residual_norm_modulate(s['x'], s['a'], EPS, **pre, **add) if case['residual'] else \
+                norms.norm_modulate(s['x'], EPS, **pre)
+        return norms.residual_norm_modulate_backward(s['dh'], s['dn'], s['x'], s['a'], EPS, **pre, **add) \
+            if case['residual'] else norms.norm_modulate_backward(s['dn'], s['x'], EPS, **pre)
+    if kind in ('rotary', 'rotary_bwd'):
+        from onereel_amd import rotary
+        axes = rotary.Axes(s['positions'], s['dims'], pairs=case['pairs'])
+        H, D = case['heads'], case['dim']
+        if case['normed']:
+            if kind == 'rotary':
+                return rotary.norm_rotate(*s['x'], *s['w'], EPS, axes, H)
+            return rotary.norm_rotate_backward(*s['dy'], *s['x'], *s['w'], EPS, axes, H)
+        return rotary.rotate(s['x'][0].view(-1, H, D), axes) if kind == 'rotary' else \
+            rotary.rotate_backward(s['dy'][0], axes)
+    if kind == 'clip':
+        from onereel_amd import clip
+        norm = clip.clip_grads_(s['grads'], s['max_norm'], out=s['outs'])
+        return norm, s['out'] if case['into'] else s['flat']
+    from onereel_amd import mxfp4
+    if kind == 'mx_quantize':
+        return mxfp4.quantize(s['x']).dequantize(s['x'].dtype)
+    return mxfp4.linear(s['x'], mxfp4.MXFP4(s['codes'], s['scales']), s['b'], activation=case['act'] or None, gate=s['gate'],
+                        residual=s['residual'])
+
+
+def _rows_of(s, t):
+    """a modulation's vector of every row"""
+    return t.repeat_interleave(s['case']['per'], 0)
+
+
+def _normed(x, kind):
+    """(the normalised rows, what they were multiplied by)"""
+    if kind == 'layer':
+        x = x - x.mean(1, keepdim=True)
+    inv = (x.square().mean(1, keepdim=True) + EPS).rsqrt()
+    return x * inv, inv
+
+
+def _norm(s):
+    case, h = s['case'], s['x'].float()
+    if case['residual']:
+        p = s['a'].float()
+        if case['post']:
+            p = _normed(p, case['post'])[0]
+            p = p if s['post_weight'] is None else p * s['post_weight']
+        h = case['scale'] * h + (p if s['gate'] is None else p * _rows_of(s, s['gate']))
+    n = _normed(h, case['norm'])[0]
+    n = n if s['weight'] is None else n * s['weight']
+    n = n if s['bias'] is None else n + s['bias']
+    if s['scale'] is not None:
+        n = n * (1 + _rows_of(s, s['scale'])) + _rows_of(s, s['shift'])
+    n = n.to(s['x'].dtype)
+    return (h.to(s['x'].dtype), n) if case['residual'] else n
+
+
+def _normed_grad(t, n, inv, kind):
+    """the gradient of the rows from that of their normalised form n"""
+    d = t - n * (t * n).mean(1, keepdim=True)
+    return inv * (d - t.mean(1, keepdim=True) if kind == 'layer' else d)
+
+
+def _group_sums(s, t):
+    return t.view(s['case']['groups'], s['case']['per'], -1).sum(1)
+
+
+def _norm_grads(s):
+    case, dtype, dn = s['case'], s['x'].dtype, s['dn'].float()
+    n, inv = _normed(s['x'].float(), case['norm'])
+    e = dn if s['scale'] is None else dn * (1 + _rows_of(s, s['scale']))
+    d = _normed_grad(e if s['weight'] is None else e * s['weight'], n, inv, case['norm'])
+    grads = []
+    if case['residual']:
+        d = d + s['dh'].float()
+        p, pinv = _normed(s['a'].float(), case['post']) if case['post'] else (s['a'].float(), None)
+        y = p if s['post_weight'] is None else p * s['post_weight']
+        q = d if s['gate'] is None else d * _rows_of(s, s['gate'])
+        u = q if s['post_weight'] is None else q * s['post_weight']
+        grads += [(case['scale'] * d).to(dtype), (_normed_grad(u, p, pinv, case['post']) if case['post'] else u).to(dtype),
+                  None if s['gate'] is None else _group_sums(s, d * y),
+                  None if s['post_weight'] is None else (q * p).sum(0)]
+    else:
+        grads.append(d.to(dtype))
+    grads += [None if s['weight'] is None else (e * n).sum(0), None if s['bias'] is None else e.sum(0)]
+    if s['scale'] is None:
+        return tuple(grads + [None, None])
+    y = n if s['weight'] is None else n * s['weight']
+    y = y if s['bias'] is None else y + s['bias']
+    return tuple(grads + [_group_sums(s, dn * y), _group_sums(s, dn)])
+
+
+def _angles(s):
+    """cos and sin [rows, 1, pairs]; the angles in 64 bits, since those of far positions lose all else"""
+    dev = s['positions'].device
+    freq = torch.cat([1e4 ** (-torch.arange(0, n, 2, device=dev, dtype=torch.float64) / n) for n in s['dims']])
+    axis = torch.repeat_interleave(torch.arange(len(s['dims']), device=dev), torch.tensor([n // 2 for n in s['dims']], device=dev))
+    angle = s['positions'].double()[:, axis] * freq
+    return angle.cos().float()[:, None], angle.sin().float()[:, None]
+
+
+def _turned(s, y, sign):
+    """y [rows, heads, dim] in 32 bits, its pairs rotated"""
+    c, t = _angles(s)
+    t, n = sign * t, sum(s['dims'])
+    turned, rest = y[..., :n], y[..., n:]
+    if s['case']['pairs'] == 'half':
+        a, b = turned[..., :n // 2], turned[..., n // 2:]
+        return torch.cat([a * c - b * t, a * t + b * c, rest], 2)
+    a, b = turned[..., 0::2], turned[..., 1::2]
+    return torch.cat([torch.stack([a * c - b * t, a * t + b * c], 3).flatten(2), rest], 2)
+
+
+def _heads_of(s, y):
+    return y.view(y.shape[0], s['case']['heads'], s['case']['dim'])
+
+
+def _rotary(s):
+    if not s['case']['normed']:
+        return _turned(s, _heads_of(s, s['x'][0].float()), 1).to(s['x'][0].dtype)
+    return tuple(_turned(s, _heads_of(s, _normed(x.float(), 'rms')[0] * w.float()), 1).to(x.dtype)
+                 for x, w in zip(s['x'], s['w']))
+
+
+def _rotary_grads(s):
+    if not s['case']['normed']:
+        return _turned(s, s['dy'][0].float(), -1).to(s['dy'][0].dtype)
+    grads = [_one_rotary_grad(s, *one) for one in zip(s['dy'], s['x'], s['w'])]
+    return tuple(g[0] for g in grads) + tuple(g[1] for g in grads)
+
+
+def _one_rotary_grad(s, dy, x, w):
+    g = _turned(s, dy.float(), -1).flatten(1)
+    n, inv = _normed(x.float(), 'rms')
+    return _normed_grad(g * w.float(), n, inv, 'rms').to(x.dtype), (g * n).sum(0)
+
+
+def _clip(s):
+    # the gradients' sums of squares, added up in 64 bits: a thousand million terms in all
+    norm = torch.stack([g.float().square().sum() for g in s['grads']]).double().sum().sqrt()
+    c = (s['max_norm'] / (norm + 1e-6)).clamp(max=1.0).float()
+    out = s['outs'] or s['grads']
+    _ = [o.copy_(g.float() * c) for g, o in zip(s['grads'], out)]
+    return norm.float(), s['out'] if s['case']['into'] else s['flat']
+
+
+_LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+_UNITS = [2.0 ** (i - 127) for i in range(255)]
+
+
+def _quantized(x):
+    """e2m1 codes [rows, width] and e8m0 scales [rows, width / 32] of x: a block's scale is the power of two that brings its
+    largest value into [4, 8), values go to the nearest of the eight, ties to the even code, past 6 to 6"""
+    b = x.double().view(x.shape[0], -1, 32)
+    exponent = (torch.frexp(b.abs().amax(2)).exponent - 3).clamp(min=-127)
+    exponent = torch.where(b.abs().amax(2) > 0, exponent, -127)
+    v = (b * ((1023 - exponent.long()) << 52).view(torch.float64)[..., None]).flatten(1)    # exp2 is not exact here
+    m = v.abs()
+    code = (m > 0.25).to(torch.uint8) + (m >= 0.75) + (m > 1.25) + (m >= 1.75) + (m > 2.5) + (m >= 3.5) + (m > 5)
+    return code + 8 * (v < 0), (exponent + 127).to(torch.uint8)
+
+
+def _values(codes, scales):
+    """what e2m1 codes and e8m0 scales stand for, in 32 bits"""
+    level = torch.tensor(_LEVELS + tuple(-v for v in _LEVELS), device=codes.device)[codes.int()]
+    unit = torch.tensor(_UNITS, device=codes.device)[scales.int()]
+    return (level.view(codes.shape[0], -1, 32) * unit[..., None]).flatten(1)
+
+
+def _mx_values(s):
+    return _values(*_quantized(s['x'])).to(s['x'].dtype)
+
+
+def _weights(s):
+    return torch.stack([s['codes'] & 15, s['codes'] >> 4], 2).flatten(1)
+
+
+_SQRT, _CUBE = math.sqrt(2 / math.pi), 0.044715
+
+
+def _act(z, name):
+    if name == 'silu':
+        return z / (1 + torch.exp(-z))
+    return 0.5 * z * (1 + torch.tanh(_SQRT * (z + _CUBE * z ** 3))) if name else z
+
+
+def _mx_linear(s):
+    z = _values(*_quantized(s['x'])) @ _values(_weights(s), s['scales']).t()
+    y = _act(z if s['b'] is None else z + s['b'].float(), s['case']['act'])
+    y = y if s['gate'] is None else y * s['gate']
+    return (y if s['residual'] is None else y + s['residual'].float()).bfloat16()
+
+
+# ------------------------------------------------------------------------------------------------------------------------
+# 64 bits, from the definitions: gradients by torch's differentiation of the forward formula
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    return {'norm': _norm_exact, 'norm_bwd': _norm_bwd_exact, 'rotary': _rotary_exact, 'rotary_bwd': _rotary_bwd_exact,
+            'clip': _clip_exact, 'mx': _mx_exact, 'mx_quantize': _mx_quantize_exact}[case['kind']](s)
+
+
+def _standard(x, kind):
+    if kind == 'layer':
+        return (x - x.mean(-1, keepdim=True)) / torch.sqrt(x.var(-1, keepdim=True, unbiased=False) + EPS)
+    return x / torch.sqrt((x * x).sum(-1, keepdim=True) / x.shape[-1] + EPS) if kind else x
+
+
+def _pre_exact(case, h, weight, bias, scale, shift):
+    """the norm before a sub-block, on rows [groups, per, width]"""
+    n = _standard(h, case['norm'])
+    n = n * weight if weight is not None else n
+    n = n + bias if bias is not None else n
+    return n * (scale[:, None] + 1) + shift[:, None] if scale is not None else n
+
+
+def _post_exact(case, a, gate, post_weight):
+    """what is added to the residual stream"""
+    p = _standard(a, case['post'])
+    p = p * post_weight if post_weight is not None else p
+    return p * gate[:, None] if gate is not None else p
+
+
+def _wide(s, *names):
+    return [None if s[n] is None else s[n].double() for n in names]
+
+
+def _norm_exact(s):
+    case = s['case']
+    shape = (case['groups'], case['per'], case['width'])
+    x, a, gate, post_weight = _wide(s, 'x', 'a', 'gate', 'post_weight')
+    h = x.view(shape)
+    if a is not None:
+        h = case['scale'] * h + _post_exact(case, a.view(shape), gate, post_weight)
+    n = _pre_exact(case, h, *_wide(s, 'weight', 'bias', 'scale', 'shift')).view(x.shape)
+    return n if a is None else (h.view(x.shape), n)
+
+
+def _norm_bwd_exact(s):
+    case = s['case']
+    shape = (case['groups'], case['per'], case['width'])
+    names = ('x', 'weight', 'bias', 'scale', 'shift')
+    given = [None if t is None else t.requires_grad_() for t in _wide(s, *names)]
+    n = _pre_exact(case, given[0].view(shape), *given[1:])
+    wanted = [t for t in given if t is not None]
+    found = dict(zip([k for k, t in zip(names, given) if t is not None],
+                     torch.autograd.grad(n, wanted, s['dn'].double().view(shape))))
+    if s['a'] is None:
+        return tuple(found.get(k) for k in names)
+    d = found['x'] + s['dh'].double()
+    more = ('a', 'gate', 'post_weight')
+    given = [None if t is None else t.requires_grad_() for t in _wide(s, *more)]
+    p = _post_exact(case, given[0].view(shape), *given[1:])
+    wanted = [t for t in given if t is not None]
+    found.update(zip([k for k, t in zip(more, given) if t is not None], torch.autograd.grad(p, wanted, d.view(shape))))
+    return (case['scale'] * d,) + tuple(found.get(k) for k in more + names[1:])
+
+
+def _spin_exact(s, y):
+    """pairs as complex numbers, each turned by its angle"""
+    parts, at, turned = torch.split(s['positions'].double(), 1, 1), 0, []
+    n = sum(s['dims'])
+    half = s['case']['pairs'] == 'half'
+    pairs = torch.complex(y[..., :n // 2], y[..., n // 2:n]) if half else \
+        torch.complex(y[..., 0:n:2], y[..., 1:n:2])
+    for p, d in zip(parts, s['dims']):
+        i = torch.arange(d // 2, dtype=torch.float64, device=y.device)
+        angle = p * torch.exp(-2 * i / d * math.log(1e4))
+        turned.append(pairs[..., at:at + d // 2] * torch.polar(torch.ones_like(angle), angle)[:, None])
+        at += d // 2
+    z = torch.cat(turned, 2)
+    parts = [z.real, z.imag] if half else [torch.view_as_real(z).flatten(2)]
+    return torch.cat(parts + [y[..., n:]], 2)
+
+
+def _rotary_of(s, x, w):
+    y = _standard(x, 'rms') * w if w is not None else x
+    return _spin_exact(s, y.view(x.shape[0], s['case']['heads'], s['case']['dim']))
+
+
+def _rotary_exact(s):
+    if not s['case']['normed']:
+        return _rotary_of(s, s['x'][0].double(), None)
+    return tuple(_rotary_of(s, x.double(), w.double()) for x, w in zip(s['x'], s['w']))
+
+
+def _rotary_bwd_exact(s):
+    if not s['case']['normed']:
+        x = torch.zeros_like(s['x'][0], dtype=torch.float64).requires_grad_()
+        return torch.autograd.grad(_rotary_of(s, x, None), x, s['dy'][0].double())[0].view_as(s['dy'][0])
+    grads = []
+    for dy, x, w in zip(s['dy'], s['x'], s['w']):
+        x, w = x.double().requires_grad_(), w.double().requires_grad_()
+        grads.append(torch.autograd.grad(_rotary_of(s, x, w), (x, w), dy.double()))
+    return tuple(g[0] for g in grads) + tuple(g[1] for g in grads)
+
+
+def _clip_exact(s):
+    wide = s['flat'].double()
+    norm = torch.sqrt(torch.dot(wide, wide))
+    return norm, wide.mul_(torch.clamp(s['max_norm'] / (norm + 1e-6), max=1.0))
+
+
+def _nearest_exact(x):
+    """the value that 32 elements' shared power of two and the nearest of the eight levels give, in 64 bits"""
+    b = x.double().reshape(-1, 32)
+    top = b.abs().amax(1, keepdim=True)
+    exponent = (top.view(torch.int64) >> 52) - 1023    # of the largest value, from its bits
+    unit = torch.tensor(_UNITS, dtype=torch.float64, device=x.device)[(exponent + 125).clamp(min=0)]
+    # a value is a multiple of 0.5 units up to 2, of 1 up to 4, of 2 up to 6: rounded to the nearest multiple, ties to even
+    m = b.abs() / unit
+    step = torch.where(m < 2, 0.5, torch.where(m < 4, 1.0, 2.0))
+    return (torch.sign(b) * unit * torch.clamp(torch.round(m / step) * step, max=6.0)).view(x.shape)
+
+
+def _mx_quantize_exact(s):
+    return _nearest_exact(s['x'])
+
+
+def _mx_exact(s):
+    levels = torch.tensor(_LEVELS, dtype=torch.float64, device=DEV)
+    w = torch.empty(s['codes'].shape[0], s['codes'].shape[1] * 2, dtype=torch.float64, device=DEV)
+    for i, c in enumerate((s['codes'] % 16, s['codes'] // 16)):
+        w[:, i::2] = levels[(c % 8).long()] * (1 - 2 * (c // 8).double())
+    w *= torch.tensor(_UNITS, dtype=torch.float64, device=DEV)[s['scales'].long()].repeat_interleave(32, 1)
+    z = _nearest_exact(s['x']) @ w.T
+    if s['b'] is not None:
+        z = z + s['b'].double()
+    y = z * torch.sigmoid(z) if s['case']['act'] == 'silu' else \
+        torch.nn.functional.gelu(z, approximate='tanh') if s['case']['act'] else z
+    if s['gate'] is not None:
+        y = s['gate'].double() * y
+    return y if s['residual'] is None else s['residual'].double() + y
