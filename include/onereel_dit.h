@@ -38,6 +38,85 @@ int or_residual_layernorm_modulate(void* x, const void* a, const float* gate, vo
                                    const float* weight, const float* bias, const float* scale, const float* shift,
                                    void* stream);
 
+/* norms of or_block_norm */
+#define OR_NORM_NONE 0
+#define OR_NORM_LAYER 1       /* (v - mean v) / sqrt(mean (v - mean v)^2 + eps) */
+#define OR_NORM_RMS 2         /* v / sqrt(mean v^2 + eps) */
+
+/* Arguments of or_block_norm: h = residual_scale x + gate post_norm(a) post_weight and
+ * n = (norm(h) weight + bias) (1 + scale) + shift, per row, fp32 inside; h is rounded once, and n comes from h before that.
+ * Without a (then without gate, post_norm, post_weight and h) n is that of x itself. */
+typedef struct or_block_norm_args {
+  const void* x;              /* [n_rows, C], row stride x_row_stride */
+  const void* a;              /* optional [n_rows, C], row stride a_row_stride: the sub-block's output */
+  void* h;                    /* [n_rows, C], contiguous; with a */
+  void* n;                    /* [n_rows, C], contiguous */
+  const float* gate;          /* optional [n_rows / rows_per_group, C]: one vector for rows_per_group consecutive rows */
+  const float* post_weight;   /* optional [C] */
+  const float* weight;        /* optional [C] */
+  const float* bias;          /* optional [C] */
+  const float* scale;         /* optional [n_rows / rows_per_group, C] */
+  const float* shift;         /* optional [n_rows / rows_per_group, C] */
+  int64_t n_rows;             /* up to 2^30 */
+  int64_t rows_per_group;     /* divides n_rows */
+  int64_t x_row_stride;       /* elements; multiples of 8 */
+  int64_t a_row_stride;
+  int32_t C;                  /* a multiple of 8 up to 8192 */
+  int32_t type;               /* OR_TYPE_* of x, a, h and n */
+  int32_t norm;               /* OR_NORM_LAYER or OR_NORM_RMS */
+  int32_t post_norm;          /* OR_NORM_* */
+  float eps;
+  float residual_scale;
+} or_block_norm_args;
+
+/* Replaces the residual add of the Wan transformer block and the norm with modulation that follows it (diffusers'
+ * WanTransformerBlock, third-party; the blocks the processors are installed in, src/onereel/models/wan.py:77-108), as
+ * or_residual_layernorm_modulate does in place, for training (nothing is updated in place), with gate, scale and shift for every
+ * group of rows, RMS norms, a norm of the sub-block's output, and all three element types. One launch. */
+int or_block_norm(const or_block_norm_args* args, void* stream);
+
+/* Arguments of or_block_norm_bwd: the gradient of one or_block_norm call. h is the call's h (its x without a). */
+typedef struct or_block_norm_bwd_args {
+  const void* dh;             /* optional [n_rows, C]: the gradient of h from what else read it; with a */
+  const void* dn;             /* [n_rows, C] */
+  const void* h;              /* [n_rows, C] */
+  const void* a;              /* the call's a or NULL */
+  void* dx;                   /* [n_rows, C], contiguous */
+  void* da;                   /* [n_rows, C], contiguous; with a */
+  const float* gate;          /* the call's parameters */
+  const float* post_weight;
+  const float* weight;
+  const float* bias;
+  const float* scale;
+  float* dgate;               /* each optional: [n_rows / rows_per_group, C], */
+  float* dpost_weight;        /* [C], */
+  float* dweight;             /* [C], */
+  float* dbias;               /* [C], */
+  float* dscale;              /* [n_rows / rows_per_group, C], */
+  float* dshift;              /* [n_rows / rows_per_group, C] */
+  int64_t n_rows;
+  int64_t rows_per_group;
+  int64_t dh_row_stride;      /* elements; multiples of 8 */
+  int64_t dn_row_stride;
+  int64_t h_row_stride;
+  int64_t a_row_stride;
+  int32_t C;
+  int32_t type;               /* OR_TYPE_* of dh, dn, h, a, dx and da */
+  int32_t norm;
+  int32_t post_norm;
+  float eps;
+  float residual_scale;
+  void* workspace;            /* device scratch of or_block_norm_bwd_workspace_size() bytes; with one of the sums over rows */
+  int64_t workspace_bytes;
+} or_block_norm_bwd_args;
+
+/* Bytes of device workspace or_block_norm_bwd needs for the sums over rows. Negative for sizes it refuses. */
+int64_t or_block_norm_bwd_workspace_size(int64_t n_rows, int64_t rows_per_group, int32_t C);
+
+/* The gradient of or_block_norm. Sums are fp32 in a fixed order; dx and da are rounded once. With 0 rows nothing is written.
+ * One launch, two with sums over rows, three with weights' gradients over several groups. */
+int or_block_norm_bwd(const or_block_norm_bwd_args* args, void* stream);
+
 /* activations of or_linear */
 #define OR_ACT_NONE 0
 #define OR_ACT_GELU_TANH 1    /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
@@ -114,6 +193,73 @@ int or_linear_bwd(const or_linear_bwd_args* args, void* stream);
  * (0 with them), split: parts of the summed axis. Host only. */
 int or_linear_plan(int64_t n_rows, int32_t n_in, int32_t n_out, int32_t product, int32_t* tile, int32_t* buffers,
                    int32_t* split);
+
+/* Rows of n elements (a multiple of 32) in microscaled 4-bit floating point (OCP MXFP4): n / 32 scales, each the biased exponent of a
+ * power of two s for 32 elements (255: NaN), and n / 2 bytes of codes, two e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) in
+ * each with the even element in the low half. A block's s is 2^(floor(log2 max|x|) - 2), at least 2^-127; an element is the value
+ * nearest to x / s, ties to the even code, past 6 as 6; a block with an infinity or a NaN gets the scale 255. x: n_rows up to 2^30 of
+ * n up to 2^21 elements of OR_TYPE_*, row stride in elements (a multiple of 8); codes and scales contiguous. */
+int or_mx_quantize(const void* x, int64_t n_rows, int32_t n, int64_t x_row_stride, int32_t type, void* codes, void* scales,
+                   void* stream);
+
+/* The values that codes and scales stand for, into contiguous rows of OR_TYPE_* elements. */
+int or_mx_dequantize(const void* codes, const void* scales, int64_t n_rows, int32_t n, int32_t type, void* out, void* stream);
+
+/* Arguments of or_mx_linear: or_linear with x and the weight in 4 bits. */
+typedef struct or_mx_linear_args {
+  const void* x;              /* bf16 [n_rows, n_in], row stride x_row_stride, quantised by the call; or NULL, then */
+  const void* x_codes;        /* [n_rows, n_in / 2] and */
+  const void* x_scales;       /* [n_rows, n_in / 32], contiguous */
+  const void* weight_codes;   /* [n_out, n_in / 2], contiguous */
+  const void* weight_scales;  /* [n_out, n_in / 32], contiguous */
+  const void* bias;           /* optional fp32 [n_out] (bf16 with bias_bf16) */
+  const void* gate;           /* optional fp32 [n_out] (bf16 with gate_bf16) */
+  const void* residual;       /* optional bf16 [n_rows, n_out], row stride residual_row_stride; may be y itself */
+  void* y;                    /* bf16 [n_rows, n_out], row stride y_row_stride */
+  int64_t n_rows;             /* up to 2^30 */
+  int64_t x_row_stride;       /* elements; multiples of 8 */
+  int64_t residual_row_stride;
+  int64_t y_row_stride;
+  int32_t n_in;               /* a multiple of 32 up to 2^21 */
+  int32_t n_out;              /* a multiple of 8 up to 2^21 */
+  int32_t activation;         /* OR_ACT_* */
+  int32_t bias_bf16;
+  int32_t gate_bf16;
+  void* workspace;            /* device scratch of or_mx_linear_workspace_size() bytes */
+  int64_t workspace_bytes;
+} or_mx_linear_args;
+
+/* Bytes of device workspace or_mx_linear needs (quantized: x comes in 4 bits). Negative for sizes it refuses. */
+int64_t or_mx_linear_workspace_size(int64_t n_rows, int32_t n_in, int32_t n_out, int32_t quantized);
+
+/* Replaces the Linear layers of the Wan transformer block with what follows them, as or_linear does (diffusers'
+ * WanTransformerBlock, third-party; the blocks the processors are installed in, src/onereel/models/wan.py:77-108), for inference
+ * with 4-bit weights and activations: y = residual + gate * act(x weight^T + bias) of the values in 4 bits, fp32 from the products to
+ * the one rounding of y. */
+int or_mx_linear(const or_mx_linear_args* args, void* stream);
+
+/* Arguments of or_clip. The arrays lie in host memory and are read before the call returns. */
+typedef struct or_clip_args {
+  const void* const* x;       /* [n_tensors] device addresses of contiguous elements, aligned to their type */
+  const int64_t* numel;       /* [n_tensors], 0 to 2^40 */
+  const int32_t* type;        /* [n_tensors] OR_TYPE_* */
+  void* const* out;           /* optional [n_tensors] device addresses: x's own (in place) or memory that no x shares; NULL: the
+                                 norm alone */
+  const int32_t* out_type;    /* optional [n_tensors] OR_TYPE_* of out (NULL: as type; that of x where out is x) */
+  int64_t n_tensors;
+  double max_norm;            /* 0 or more */
+  float* norm;                /* device: the norm of all x before scaling */
+  void* workspace;            /* device scratch of or_clip_workspace_size() bytes */
+  int64_t workspace_bytes;
+} or_clip_args;
+
+/* Bytes of device workspace or_clip needs for these tensors. Negative for arguments it refuses. */
+int64_t or_clip_workspace_size(const or_clip_args* args);
+
+/* The clipping of a training step's gradients, which the reference, an inference system, leaves to its trainer (torch's
+ * clip_grad_norm_): norm = sqrt(sum of all x^2) and out = x min(1, max_norm / (norm + 1e-6)); in place, nothing is written where
+ * that factor is 1. Squares are summed in fp64 in a fixed order. Two launches for each 128 tensors. */
+int or_clip(const or_clip_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -13,6 +13,7 @@
  *   or_lse_merge      log-sum-exp merge of two partial attention results (attention split over key sets)
  *   or_rmsnorm_rope   fused RMSNorm + interleaved RoPE of the Wan self-attention's queries and keys
  *   or_varlen_bwd, or_rmsnorm_rope_bwd         the gradients of or_varlen_fwd and or_rmsnorm_rope
+ *   or_rmsnorm_rope_axes, or_rope_axes_rotate  or_rmsnorm_rope, and the rotation alone, from positions on several axes
  *   or_frame_pool     frame memory: per-frame sums of hidden states (deterministic)
  *   or_frame_select   frame memory: k-means (cosine) representatives and their medoids, one workgroup
  *   or_memory_select, or_memory_foreign,
@@ -40,6 +41,11 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* element types of the calls that take more than bf16 */
+#define OR_TYPE_BF16 0
+#define OR_TYPE_FP16 1
+#define OR_TYPE_FP32 2
 
 #define OR_MAX_SCENES 64
 #define OR_MAX_EXTRA 512
@@ -381,6 +387,47 @@ int or_rmsnorm_rope_bwd(const void* dq, const void* dk, const void* q, const voi
                         const float* sin_table, const int32_t* rope_row, int64_t n_rope_rows, void* q_grad,
                         void* k_grad, float* wq_grad, float* wk_grad, void* workspace, int64_t workspace_bytes,
                         void* stream);
+
+#define OR_PAIRS_INTERLEAVED 0   /* dims 2 j and 2 j + 1 of a head */
+#define OR_PAIRS_HALF 1          /* dims j and j + R / 2 of its R rotated dims */
+
+/* Where a call's tokens lie on n_axes axes, and how a head's dims are dealt out to them: axis a rotates dims[a] / 2 pairs, in the
+ * order of the axes, pair i by position * theta[a]^(-2 i / dims[a]). Dims past the axes' are not rotated. Host memory but for
+ * positions. */
+typedef struct or_rope_axes {
+  const void* positions;      /* device [n_positions, n_axes], int32 (fp32 with positions_fp32), contiguous */
+  int64_t n_positions;        /* divides the rows of a call: row r lies at positions[r % n_positions] */
+  int32_t n_axes;             /* 1 to 4 */
+  int32_t positions_fp32;
+  int32_t pairs;              /* OR_PAIRS_*; half-split pairs need a multiple of 8 rotated dims */
+  int32_t dims[4];            /* even, their sum at most the head's dims */
+  double theta[4];
+} or_rope_axes;
+
+/* Replaces the RoPE with tables over frame, row and column of diffusers' Wan attention (WanRotaryPosEmbed's tables handed to the
+ * processors, src/onereel/models/wan.py:91-99) by the rotation from positions: rows of H heads of D dims (a multiple of 8 up to
+ * 512; strides in elements, multiples of 8) of OR_TYPE_* elements into contiguous ones, rotated, or back with inverse (the
+ * gradient). Angles in fp64, fp32 inside, one rounding. out is not x. */
+int or_rope_axes_rotate(const or_rope_axes* axes, const void* x, void* out, int64_t n_rows, int32_t H, int32_t D,
+                        int64_t row_stride, int64_t head_stride, int32_t type, int32_t inverse, void* stream);
+
+/* Replaces _qk (src/onereel/models/wan.py:64-74) as or_rmsnorm_rope does, with positions in place of tables: RMSNorm over each
+ * row of C elements (C / D heads, up to 8192 elements) with weights of the rows' type, then the rotation, of q and (optional) k
+ * into contiguous rows. One launch. */
+int or_rmsnorm_rope_axes(const or_rope_axes* axes, const void* q, const void* k, const void* wq, const void* wk,
+                         int64_t q_row_stride, int64_t k_row_stride, int64_t n_rows, int32_t C, int32_t D, int32_t type,
+                         float eps, void* q_out, void* k_out, void* stream);
+
+/* Bytes of device workspace or_rmsnorm_rope_axes_bwd needs. Negative for sizes it refuses. */
+int64_t or_rmsnorm_rope_axes_bwd_workspace_size(int64_t n_rows, int32_t C);
+
+/* The gradient of or_rmsnorm_rope_axes from those of its outputs (rows of C elements): q_grad and k_grad contiguous in the rows'
+ * type, wq_grad and wk_grad fp32 [C], sums over rows in a fixed order. wk NULL: of q alone. Two launches. */
+int or_rmsnorm_rope_axes_bwd(const or_rope_axes* axes, const void* dq, const void* dk, const void* q, const void* k,
+                             const void* wq, const void* wk, int64_t dq_row_stride, int64_t dk_row_stride,
+                             int64_t q_row_stride, int64_t k_row_stride, int64_t n_rows, int32_t C, int32_t D, int32_t type,
+                             float eps, void* q_grad, void* k_grad, float* wq_grad, float* wk_grad, void* workspace,
+                             int64_t workspace_bytes, void* stream);
 
 /* Replaces the pooling of FrameMemory.collect (src/onereel/frame_memory.py:76-85, index_add_ of one layer's video rows
  * into per-frame sums and counts): for the frame-major rows r of hs (bf16, row stride row_stride elements, C wide),

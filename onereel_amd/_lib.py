@@ -98,6 +98,44 @@ class LinearBwdArgs(ctypes.Structure):
                [('workspace', vp), ('workspace_bytes', i64)]
 
 
+# element types (OR_TYPE_*), norms of or_block_norm (OR_NORM_*)
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+NORMS = {None: 0, 'layer': 1, 'rms': 2}
+
+
+class BlockNormArgs(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ('x', 'a', 'h', 'n', 'gate', 'post_weight', 'weight', 'bias', 'scale', 'shift')] + \
+               [(n, i64) for n in ('n_rows', 'rows_per_group', 'x_row_stride', 'a_row_stride')] + \
+               [(n, i32) for n in ('C', 'type', 'norm', 'post_norm')] + \
+               [(n, ctypes.c_float) for n in ('eps', 'residual_scale')]
+
+
+class BlockNormBwdArgs(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ('dh', 'dn', 'h', 'a', 'dx', 'da', 'gate', 'post_weight', 'weight', 'bias', 'scale', 'dgate',
+                                  'dpost_weight', 'dweight', 'dbias', 'dscale', 'dshift')] + \
+               [(n, i64) for n in ('n_rows', 'rows_per_group', 'dh_row_stride', 'dn_row_stride', 'h_row_stride',
+                                   'a_row_stride')] + \
+               [(n, i32) for n in ('C', 'type', 'norm', 'post_norm')] + \
+               [(n, ctypes.c_float) for n in ('eps', 'residual_scale')] + [('workspace', vp), ('workspace_bytes', i64)]
+
+
+class MxLinearArgs(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ('x', 'x_codes', 'x_scales', 'weight_codes', 'weight_scales', 'bias', 'gate', 'residual', 'y')] + \
+               [(n, i64) for n in ('n_rows', 'x_row_stride', 'residual_row_stride', 'y_row_stride')] + \
+               [(n, i32) for n in ('n_in', 'n_out', 'activation', 'bias_bf16', 'gate_bf16')] + \
+               [('workspace', vp), ('workspace_bytes', i64)]
+
+
+class ClipArgs(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ('x', 'numel', 'type', 'out', 'out_type')] + \
+               [('n_tensors', i64), ('max_norm', ctypes.c_double), ('norm', vp), ('workspace', vp), ('workspace_bytes', i64)]
+
+
+class RopeAxes(ctypes.Structure):
+    _fields_ = [('positions', vp), ('n_positions', i64), ('n_axes', i32), ('positions_fp32', i32), ('pairs', i32),
+                ('dims', i32 * 4), ('theta', ctypes.c_double * 4)]
+
+
 # every exported symbol with its ctypes signature: include/onereel_hip.h
 SIGNATURES = {
     'or_layout_plan': (i32, [ctypes.POINTER(LayoutDesc), ctypes.POINTER(LayoutSizes)]),
@@ -116,6 +154,12 @@ SIGNATURES = {
                               i64, vp]),
     'or_rmsnorm_rope_bwd_workspace_size': (i64, [i64, i32]),
     'or_rmsnorm_rope_bwd': (i32, [vp] * 6 + [i64] * 5 + [i32, i32, ctypes.c_float, vp, vp, vp, i64] + [vp] * 5 + [i64, vp]),
+    'or_rope_axes_rotate': (i32, [ctypes.POINTER(RopeAxes), vp, vp, i64, i32, i32, i64, i64, i32, i32, vp]),
+    'or_rmsnorm_rope_axes': (i32, [ctypes.POINTER(RopeAxes), vp, vp, vp, vp, i64, i64, i64, i32, i32, i32, ctypes.c_float, vp,
+                                   vp, vp]),
+    'or_rmsnorm_rope_axes_bwd_workspace_size': (i64, [i64, i32]),
+    'or_rmsnorm_rope_axes_bwd': (i32, [ctypes.POINTER(RopeAxes)] + [vp] * 6 + [i64] * 5 + [i32, i32, i32, ctypes.c_float] +
+                                 [vp] * 5 + [i64, vp]),
     'or_frame_pool': (i32, [vp, i64, i32, i64, i64, i32, i32, vp, vp, vp]),
     'or_frame_select_host': (i32, [vp, i32, i32, vp, i32, i32, i32, vp, vp, vp]),
     'or_frame_select': (i32, [vp, i32, i32, vp, i32, i32, i32, vp, vp, vp]),
@@ -141,6 +185,15 @@ DIT_SIGNATURES = {
     'or_linear': (i32, [ctypes.POINTER(LinearArgs), vp]),
     'or_linear_bwd_workspace_size': (i64, [i64, i32, i32, i32]),
     'or_linear_bwd': (i32, [ctypes.POINTER(LinearBwdArgs), vp]),
+    'or_mx_quantize': (i32, [vp, i64, i32, i64, i32, vp, vp, vp]),
+    'or_mx_dequantize': (i32, [vp, vp, i64, i32, i32, vp, vp]),
+    'or_mx_linear_workspace_size': (i64, [i64, i32, i32, i32]),
+    'or_mx_linear': (i32, [ctypes.POINTER(MxLinearArgs), vp]),
+    'or_clip_workspace_size': (i64, [ctypes.POINTER(ClipArgs)]),
+    'or_clip': (i32, [ctypes.POINTER(ClipArgs), vp]),
+    'or_block_norm': (i32, [ctypes.POINTER(BlockNormArgs), vp]),
+    'or_block_norm_bwd_workspace_size': (i64, [i64, i64, i32]),
+    'or_block_norm_bwd': (i32, [ctypes.POINTER(BlockNormBwdArgs), vp]),
 }
 
 # libonereel_bench.so: include/onereel_bench.h

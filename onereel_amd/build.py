@@ -19,8 +19,8 @@ LIB = PKG / 'libonereel_hip.so'
 DIT_LIB = PKG / 'libonereel_dit.so'
 BENCH_LIB = PKG / 'libonereel_bench.so'
 OBJ = PKG / 'csrc' / '_obj'
-SOURCES = ['layout.hip', 'gather.hip', 'attention.hip', 'attention_bwd.hip', 'merge.hip', 'norm_rope.hip', 'frame_memory.hip', 'memory.hip']
-DIT_SOURCES = ['dit_fused.hip', 'linear.hip']
+SOURCES = ['layout.hip', 'gather.hip', 'attention.hip', 'attention_bwd.hip', 'merge.hip', 'norm_rope.hip', 'rope_axes.hip', 'frame_memory.hip', 'memory.hip']
+DIT_SOURCES = ['dit_fused.hip', 'linear.hip', 'block_norm.hip', 'clip.hip', 'mxfp4.hip']
 BENCH_SOURCES = ['mfma_ceiling.hip']
 # attention: no NaN operands reach the softmax max, so fmax needs no quieting of its inputs (v_max3_f32 directly)
 SOURCE_FLAGS = {'attention.hip': ['-fno-honor-nans']}

@@ -1,0 +1,593 @@
+// The norms before and after a sub-block (attention, feed forward), fused with its gate and residual, and their gradient. Built
+// into libonereel_dit.so (include/onereel_dit.h). Per row of C elements, in fp32, with one vector of gate, scale and shift for
+// every group of `per` consecutive rows (a frame, a scene, or all rows):
+//
+//   p = Post(a) * wp        h = r x + gate p        n = (Norm(h) w + b) (1 + scale) + shift
+//
+// Norm is (v - m) / sqrt(mean (v - m)^2 + eps) (layer) or v / sqrt(mean v^2 + eps) (RMS), Post one of them or nothing. h is
+// rounded once, and n comes from h before that rounding. The gradient reads the rounded h and a (xh, ah: what the two norms
+// make of them, s and sa the factors they multiply by):
+//
+//   t = dn W, W = w (1 + scale)         d = dh + s (t - mean t - xh mean(t xh))        dx = r d
+//   u = d G,  G = gate wp               da = sa (u - mean u - ah mean(u ah))           (without Post: da = u)
+//   A = sum dn xh, B = sum dn, D = sum d ah over the rows of a group:
+//   dshift = B, dscale = w A + b B, dgate = wp D;   dw = sum (1 + scale) A, db = sum (1 + scale) B, dwp = sum gate D over groups
+//
+// (the terms mean t and mean u are the layer norm's alone). Three column sums serve all six parameters' gradients.
+//
+// HBM-bound: x and a are read and h and n written once, h, a, dh and dn are read and dx and da written once. A work-group takes
+// rows of one group, each of its threads 8 columns of them, so that the parameters stay in registers, folded into two or three
+// vectors; a row's sums go over lanes within a wavefront, then through LDS: one barrier for a batch of rows, since each wavefront
+// hands on its own mean and the squares around that, which are joined without cancellation. In the gradient a thread adds up its
+// columns' A, B and D over its work-group's rows, in a fixed order; a second launch joins the work-groups' sums.
+#include <math.h>
+
+#include <algorithm>
+
+#include "../../include/onereel_dit.h"
+#include "rows.h"
+
+namespace onereel {
+
+namespace {
+
+constexpr int kMaxC = 8192;            // 1024 threads of 8 columns
+constexpr int kMaxWaves = 16;
+constexpr int kRows = 2;               // rows of a batch
+constexpr int kMaxPartRows = 256;      // rows whose sums a thread adds up one after the other
+
+struct NormArgs {
+  const void *x, *a;
+  void *h, *n;
+  const float *gate, *post_weight, *weight, *bias, *scale, *shift;   // gate, scale, shift: [groups][C]
+  int64_t per, x_stride, a_stride;
+  int64_t spans;                       // groups x parts
+  int C, parts, norm, post;            // parts: work-groups of a group of rows
+  float eps, r;
+};
+
+// 8 columns of a vector of parameters, or `other` where there is none
+__device__ __forceinline__ void param8(const float* p, int64_t at, bool in, float other, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = other;
+  if (p && in) {
+    const f32x4 a = *(const f32x4*)(p + at), b = *(const f32x4*)(p + at + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < 4 ? a[i] : b[i - 4];
+  }
+}
+
+// a wavefront's columns of a row of C: their mean and the sum of squares around it (RMS: around 0), and what else it hands on
+struct Share {
+  float mean, square, t, tx;
+};
+
+// columns of wavefront w of a row of C
+__device__ __forceinline__ int wave_columns(int C, int w) { return min(512, C - 512 * w); }
+
+__device__ __forceinline__ void moments(const float (&v)[8], bool in, int columns, int norm, Share& s) {
+  float sum = 0.0f;
+  s.mean = 0.0f;
+  if (norm == OR_NORM_LAYER) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += v[i];
+    s.mean = wave_sum(in ? sum : 0.0f) / (float)columns;
+    sum = 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += (v[i] - s.mean) * (v[i] - s.mean);
+  s.square = wave_sum(in ? sum : 0.0f);
+}
+
+// mean and 1 / sqrt(mean square + eps) of a row from its wavefronts' shares
+__device__ __forceinline__ void join_moments(const Share* s, int waves, int C, float eps, float& mean, float& inv) {
+  float sum = 0.0f;
+  for (int w = 0; w < waves; ++w) sum += s[w].mean * (float)wave_columns(C, w);
+  mean = sum / (float)C;
+  float square = 0.0f;
+  for (int w = 0; w < waves; ++w) {
+    const float d = s[w].mean - mean;
+    square += s[w].square + d * d * (float)wave_columns(C, w);
+  }
+  inv = 1.0f / sqrtf(square / (float)C + eps);
+}
+
+// the rows [first, last) of work-group b
+struct Span {
+  int64_t group, first, last;
+  int part;
+};
+__device__ __forceinline__ Span span_of(int64_t block, int parts, int64_t per) {
+  Span s;
+  s.group = block / parts;
+  s.part = (int)(block - s.group * parts);
+  s.first = s.group * per + per * s.part / parts;
+  s.last = s.group * per + per * (s.part + 1) / parts;
+  return s;
+}
+
+template <typename T, bool RES>
+__global__ __launch_bounds__(1024) void block_norm_kernel(NormArgs g) {
+  __shared__ Share post_share[2][kRows][kMaxWaves], share[2][kRows][kMaxWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, col = 8 * threadIdx.x, C = g.C;
+  const bool in = col < C;
+  const int columns = wave_columns(C, wave);
+  int turn = 0;
+  for (int64_t span = blockIdx.x; span < g.spans; span += gridDim.x) {
+  const Span s = span_of(span, g.parts, g.per);
+  const int64_t at = s.group * C + col;
+  float G[8], W[8], B[8], t[8];
+  param8(g.gate, at, in, 1.0f, G);
+  param8(g.post_weight, col, in, 1.0f, t);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) G[i] *= t[i];
+  param8(g.weight, col, in, 1.0f, W);
+  param8(g.bias, col, in, 0.0f, B);
+  param8(g.scale, at, in, 0.0f, t);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    W[i] *= 1.0f + t[i];
+    B[i] *= 1.0f + t[i];
+  }
+  param8(g.shift, at, in, 0.0f, t);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) B[i] += t[i];
+  for (int64_t r0 = s.first; r0 < s.last; r0 += kRows, turn ^= 1) {
+    float h[kRows][8], p[kRows][8];
+    Piece<T, 8> x[kRows], a[kRows];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      x[k].zero();
+      a[k].zero();
+      if (in && r0 + k < s.last) {
+        x[k].load(g.x, (r0 + k) * g.x_stride + col);
+        if constexpr (RES) a[k].load(g.a, (r0 + k) * g.a_stride + col);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) x[k].get(h[k]);
+    if constexpr (RES) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) a[k].get(p[k]);
+      if (g.post != OR_NORM_NONE) {
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          Share m;
+          moments(p[k], in, columns, g.post, m);
+          if (lane == 0) post_share[turn][k][wave] = m;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          float mean, inv;
+          join_moments(post_share[turn][k], waves, C, g.eps, mean, inv);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[k][i] = (p[k][i] - mean) * inv;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[k][i] = g.r * h[k][i] + p[k][i] * G[i];
+        if (in && r0 + k < s.last) Piece<T, 8>::store(g.h, (r0 + k) * C + col, h[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      Share m;
+      moments(h[k], in, columns, g.norm, m);
+      if (lane == 0) share[turn][k][wave] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      float mean, inv, n[8];
+      join_moments(share[turn][k], waves, C, g.eps, mean, inv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) n[i] = (h[k][i] - mean) * inv * W[i] + B[i];
+      if (in && r0 + k < s.last) Piece<T, 8>::store(g.n, (r0 + k) * C + col, n);
+    }
+  }
+  }
+}
+
+struct NormBwdArgs {
+  const void *dh, *dn, *h, *a;         // dh optional
+  void *dx, *da;
+  const float *gate, *post_weight, *weight, *bias, *scale;
+  float *dgate, *dpost_weight, *dweight, *dbias, *dscale, *dshift;   // each optional
+  float* part;                         // [groups * parts][3][C]: A, B, D
+  float* group_part;                   // [groups][3][C]: the groups' terms of dweight, dbias, dpost_weight
+  int64_t per, groups, dh_stride, dn_stride, h_stride, a_stride;
+  int C, parts, norm, post;
+  float eps, r;
+};
+
+template <typename T, bool RES>
+__global__ __launch_bounds__(1024) void block_norm_bwd_kernel(NormBwdArgs g) {
+  __shared__ Share share[2][kRows][kMaxWaves], post_share[2][kRows][kMaxWaves];
+  __shared__ float back[2][kRows][kMaxWaves][2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, col = 8 * threadIdx.x, C = g.C;
+  const bool in = col < C;
+  const int columns = wave_columns(C, wave);
+  int turn = 0;
+  for (int64_t span = blockIdx.x; span < g.groups * g.parts; span += gridDim.x) {
+  const Span s = span_of(span, g.parts, g.per);
+  const int64_t at = s.group * C + col;
+  float G[8], W[8], v[8], A[8], B[8], D[8];
+  param8(g.gate, at, in, 1.0f, G);
+  param8(g.post_weight, col, in, 1.0f, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) G[i] *= v[i];
+  param8(g.weight, col, in, 1.0f, W);
+  param8(g.scale, at, in, 0.0f, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    W[i] *= 1.0f + v[i];
+    A[i] = B[i] = D[i] = 0.0f;
+  }
+  for (int64_t r0 = s.first; r0 < s.last; r0 += kRows, turn ^= 1) {
+    Piece<T, 8> hp[kRows], np[kRows], dp[kRows], ap[kRows];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      hp[k].zero();
+      np[k].zero();
+      dp[k].zero();
+      ap[k].zero();
+      if (in && r0 + k < s.last) {
+        hp[k].load(g.h, (r0 + k) * g.h_stride + col);
+        np[k].load(g.dn, (r0 + k) * g.dn_stride + col);
+        if constexpr (RES) {
+          if (g.dh) dp[k].load(g.dh, (r0 + k) * g.dh_stride + col);
+          ap[k].load(g.a, (r0 + k) * g.a_stride + col);
+        }
+      }
+    }
+    float h[kRows][8], n[kRows][8], a[kRows][8];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      Share m;
+      hp[k].get(h[k]);
+      np[k].get(n[k]);
+      moments(h[k], in, columns, g.norm, m);
+      float t = 0.0f, tx = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        t += n[k][i] * W[i];
+        tx += n[k][i] * W[i] * (h[k][i] - m.mean);
+      }
+      m.t = g.norm == OR_NORM_LAYER ? wave_sum(in ? t : 0.0f) : 0.0f;
+      m.tx = wave_sum(in ? tx : 0.0f);
+      if (lane == 0) share[turn][k][wave] = m;
+      if constexpr (RES) {
+        ap[k].get(a[k]);
+        if (g.post != OR_NORM_NONE) {
+          moments(a[k], in, columns, g.post, m);
+          if (lane == 0) post_share[turn][k][wave] = m;
+        }
+      }
+    }
+    __syncthreads();
+    float u[kRows][8], post_inv[kRows];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      float mean, inv, t = 0.0f, tx = 0.0f, d[8];
+      join_moments(share[turn][k], waves, C, g.eps, mean, inv);
+      for (int w = 0; w < waves; ++w) {
+        const Share m = share[turn][k][w];
+        t += m.t;
+        tx += m.tx + (m.mean - mean) * m.t;
+      }
+      t /= (float)C;
+      tx *= inv / (float)C;
+      dp[k].get(d);
+      const bool row = in && r0 + k < s.last;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float xh = (h[k][i] - mean) * inv;
+        A[i] += row ? n[k][i] * xh : 0.0f;
+        B[i] += n[k][i];
+        d[i] += inv * (n[k][i] * W[i] - t - xh * tx);
+        u[k][i] = d[i] * G[i];
+      }
+      if constexpr (RES) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = g.r * d[i];
+        if (row) Piece<T, 8>::store(g.dx, (r0 + k) * C + col, x);
+        if (g.post != OR_NORM_NONE) {
+          join_moments(post_share[turn][k], waves, C, g.eps, mean, post_inv[k]);
+          float su = 0.0f, sux = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            a[k][i] = (a[k][i] - mean) * post_inv[k];
+            su += u[k][i];
+            sux += u[k][i] * a[k][i];
+          }
+          su = g.post == OR_NORM_LAYER ? wave_sum(in ? su : 0.0f) : 0.0f;
+          sux = wave_sum(in ? sux : 0.0f);
+          if (lane == 0) {
+            back[turn][k][wave][0] = su;
+            back[turn][k][wave][1] = sux;
+          }
+        } else if (row) {
+          Piece<T, 8>::store(g.da, (r0 + k) * C + col, u[k]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) D[i] += row ? d[i] * a[k][i] : 0.0f;
+      } else if (row) {
+        Piece<T, 8>::store(g.dx, (r0 + k) * C + col, d);
+      }
+    }
+    if constexpr (RES) {
+      if (g.post != OR_NORM_NONE) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          float su = 0.0f, sux = 0.0f;
+          for (int w = 0; w < waves; ++w) {
+            su += back[turn][k][w][0];
+            sux += back[turn][k][w][1];
+          }
+          su /= (float)C;
+          sux /= (float)C;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) u[k][i] = post_inv[k] * (u[k][i] - su - a[k][i] * sux);
+          if (in && r0 + k < s.last) Piece<T, 8>::store(g.da, (r0 + k) * C + col, u[k]);
+        }
+      }
+    }
+  }
+  if (!g.part || !in) continue;
+  float* out = g.part + span * 3 * C + col;
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    *(f32x4*)(out + i) = f32x4{A[i], A[i + 1], A[i + 2], A[i + 3]};
+    *(f32x4*)(out + C + i) = f32x4{B[i], B[i + 1], B[i + 2], B[i + 3]};
+    *(f32x4*)(out + 2 * C + i) = f32x4{D[i], D[i + 1], D[i + 2], D[i + 3]};
+  }
+  }
+}
+
+// a group's sums of 64 columns, its work-groups' dealt out to 16 wavefronts; then its parameters' gradients, or their terms
+constexpr int kSumWaves = 16;
+__global__ __launch_bounds__(64 * kSumWaves) void block_norm_sums_kernel(NormBwdArgs g) {
+  __shared__ float sum[3][kSumWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+  for (int64_t group = blockIdx.y; group < g.groups; group += gridDim.y) {
+    float v[3] = {};
+    if (col < g.C) {
+      const float* p = g.part + group * g.parts * 3 * g.C + col;
+#pragma unroll 8
+      for (int b = wave; b < g.parts; b += kSumWaves)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) v[i] += p[((int64_t)b * 3 + i) * g.C];
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sum[i][wave][lane] = v[i];
+    __syncthreads();
+    if (wave == 0 && col < g.C) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        v[i] = 0.0f;
+        for (int w = 0; w < kSumWaves; ++w) v[i] += sum[i][w][lane];
+      }
+      const int64_t at = group * g.C + col;
+      const float w = g.weight ? g.weight[col] : 1.0f, b = g.bias ? g.bias[col] : 0.0f, e = g.scale ? 1.0f + g.scale[at] : 1.0f;
+      const float gate = g.gate ? g.gate[at] : 1.0f, wp = g.post_weight ? g.post_weight[col] : 1.0f;
+      if (g.dscale) g.dscale[at] = w * v[0] + b * v[1];
+      if (g.dshift) g.dshift[at] = v[1];
+      if (g.dgate) g.dgate[at] = wp * v[2];
+      const float term[3] = {e * v[0], e * v[1], gate * v[2]};
+      if (g.groups == 1) {
+        if (g.dweight) g.dweight[col] = term[0];
+        if (g.dbias) g.dbias[col] = term[1];
+        if (g.dpost_weight) g.dpost_weight[col] = term[2];
+      } else if (g.group_part) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) g.group_part[(group * 3 + i) * g.C + col] = term[i];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// the sums over groups
+__global__ __launch_bounds__(64 * kSumWaves) void block_norm_weights_kernel(NormBwdArgs g) {
+  __shared__ float sum[kSumWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane, which = blockIdx.y;
+  float* out = which == 0 ? g.dweight : which == 1 ? g.dbias : g.dpost_weight;
+  if (!out) return;
+  float v = 0.0f;
+  if (col < g.C) {
+#pragma unroll 8
+    for (int64_t b = wave; b < g.groups; b += kSumWaves) v += g.group_part[(b * 3 + which) * g.C + col];
+  }
+  sum[wave][lane] = v;
+  __syncthreads();
+  if (wave != 0 || col >= g.C) return;
+  v = 0.0f;
+  for (int w = 0; w < kSumWaves; ++w) v += sum[w][lane];
+  out[col] = v;
+}
+
+bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+int threads_of(int C) { return (C / 8 + 63) / 64 * 64; }
+
+// work-groups of a group of rows: `wanted` in all, each with two batches of rows or more
+int64_t parts_of(int64_t per, int64_t groups, int wanted) {
+  return std::max<int64_t>(1, std::min<int64_t>((wanted + groups - 1) / groups, per / (2 * kRows)));
+}
+
+int check_sizes(const char* what, int64_t rows, int64_t per, int32_t C, int32_t type) {
+  if (!known_type(type)) return fail_arg("%s: unknown element type %d", what, type);
+  if (C < 8 || C % 8 || C > kMaxC) return fail_arg("%s: rows of a multiple of 8 elements up to %d (got %d)", what, kMaxC, C);
+  if (rows < 0 || rows > (int64_t)1 << 30) return fail_arg("%s: 0 to 2^30 rows (got %lld)", what, (long long)rows);
+  if (rows > 0 && (per < 1 || rows % per)) return fail_arg("%s: rows_per_group must divide the rows", what);
+  return 0;
+}
+
+int check_norms(const char* what, int norm, int post) {
+  if (norm != OR_NORM_LAYER && norm != OR_NORM_RMS) return fail_arg("%s: norm must be OR_NORM_LAYER or OR_NORM_RMS", what);
+  if (post != OR_NORM_NONE && post != OR_NORM_LAYER && post != OR_NORM_RMS) return fail_arg("%s: unknown post_norm %d", what, post);
+  return 0;
+}
+
+int bad_rows(const char* what, const void* p, int64_t stride, int C) {
+  if (!p) return fail_arg("%s is required", what);
+  if (!al16(p) || stride < C || stride % 8) return fail_arg("%s: 16-byte aligned rows, a multiple of 8 elements apart, that cover C", what);
+  return 0;
+}
+
+// Work-groups of the gradient. Each writes 3 sums of C columns, which the second launch reads, so there are as few as keep the
+// GPU's loads in flight; and no thread adds up more than kMaxPartRows rows in a row.
+int64_t bwd_parts(int64_t per, int64_t groups) { return std::max(parts_of(per, groups, 512), (per + kMaxPartRows - 1) / kMaxPartRows); }
+
+int64_t part_bytes(int64_t rows, int64_t per, int C) {
+  const int64_t groups = rows / per;
+  return groups * bwd_parts(per, groups) * 3 * C * 4;
+}
+
+constexpr int64_t kMaxBlocks = 1 << 20;   // of up to 1024 threads: a grid has under 2^32 of them
+
+template <typename T>
+void launch(const NormArgs& g, hipStream_t st) {
+  const dim3 grid((unsigned)std::min(g.spans, kMaxBlocks)), block((unsigned)threads_of(g.C));
+  if (g.a) hipLaunchKernelGGL((block_norm_kernel<T, true>), grid, block, 0, st, g);
+  else hipLaunchKernelGGL((block_norm_kernel<T, false>), grid, block, 0, st, g);
+}
+
+template <typename T>
+void launch_bwd(const NormBwdArgs& g, hipStream_t st) {
+  const dim3 grid((unsigned)std::min(g.groups * g.parts, kMaxBlocks)), block((unsigned)threads_of(g.C));
+  if (g.a) hipLaunchKernelGGL((block_norm_bwd_kernel<T, true>), grid, block, 0, st, g);
+  else hipLaunchKernelGGL((block_norm_bwd_kernel<T, false>), grid, block, 0, st, g);
+}
+
+}  // namespace
+}  // namespace onereel
+
+using namespace onereel;
+
+extern "C" int or_block_norm(const or_block_norm_args* p, void* stream) {
+  if (!p) return fail_arg("or_block_norm: args is NULL");
+  const or_block_norm_args& x = *p;
+  if (int rc = check_sizes("or_block_norm", x.n_rows, x.rows_per_group, x.C, x.type)) return rc;
+  if (int rc = check_norms("or_block_norm", x.norm, x.post_norm)) return rc;
+  if (x.n_rows == 0) return 0;
+  if (int rc = bad_rows("or_block_norm: x", x.x, x.x_row_stride, x.C)) return rc;
+  if (int rc = bad_rows("or_block_norm: n", x.n, x.C, x.C)) return rc;
+  if (x.a) {
+    if (int rc = bad_rows("or_block_norm: a", x.a, x.a_row_stride, x.C)) return rc;
+    if (int rc = bad_rows("or_block_norm: h", x.h, x.C, x.C)) return rc;
+  } else if (x.gate || x.post_weight || x.post_norm != OR_NORM_NONE) {
+    return fail_arg("or_block_norm: gate, post_norm and post_weight belong to a");
+  }
+  if (x.post_weight && x.post_norm == OR_NORM_NONE) return fail_arg("or_block_norm: post_weight belongs to a post_norm");
+  if (!al16(x.gate) || !al16(x.post_weight) || !al16(x.weight) || !al16(x.bias) || !al16(x.scale) || !al16(x.shift))
+    return fail_arg("or_block_norm: parameters must be 16-byte aligned");
+  NormArgs g = {};
+  g.x = x.x;
+  g.a = x.a;
+  g.h = x.h;
+  g.n = x.n;
+  g.gate = x.gate;
+  g.post_weight = x.post_weight;
+  g.weight = x.weight;
+  g.bias = x.bias;
+  g.scale = x.scale;
+  g.shift = x.shift;
+  g.per = x.rows_per_group;
+  g.x_stride = x.x_row_stride;
+  g.a_stride = x.a_row_stride;
+  g.C = x.C;
+  g.norm = x.norm;
+  g.post = x.post_norm;
+  g.eps = x.eps;
+  g.r = x.residual_scale;
+  const int64_t groups = x.n_rows / g.per;
+  g.parts = (int)parts_of(g.per, groups, 2048);
+  g.spans = groups * g.parts;
+  hipStream_t st = (hipStream_t)stream;
+  if (x.type == OR_TYPE_BF16) launch<Bf16>(g, st);
+  else if (x.type == OR_TYPE_FP16) launch<_Float16>(g, st);
+  else launch<float>(g, st);
+  return check_hip(hipGetLastError(), "block_norm_kernel launch");
+}
+
+extern "C" int64_t or_block_norm_bwd_workspace_size(int64_t n_rows, int64_t rows_per_group, int32_t C) {
+  if (int rc = check_sizes("or_block_norm_bwd_workspace_size", n_rows, rows_per_group, C, OR_TYPE_BF16)) return rc;
+  if (n_rows == 0) return 0;
+  const int64_t groups = n_rows / rows_per_group;
+  return part_bytes(n_rows, rows_per_group, C) + (groups > 1 ? groups * 3 * C * 4 : 0);
+}
+
+extern "C" int or_block_norm_bwd(const or_block_norm_bwd_args* p, void* stream) {
+  if (!p) return fail_arg("or_block_norm_bwd: args is NULL");
+  const or_block_norm_bwd_args& x = *p;
+  if (int rc = check_sizes("or_block_norm_bwd", x.n_rows, x.rows_per_group, x.C, x.type)) return rc;
+  if (int rc = check_norms("or_block_norm_bwd", x.norm, x.post_norm)) return rc;
+  if (x.n_rows == 0) return 0;
+  if (int rc = bad_rows("or_block_norm_bwd: h", x.h, x.h_row_stride, x.C)) return rc;
+  if (int rc = bad_rows("or_block_norm_bwd: dn", x.dn, x.dn_row_stride, x.C)) return rc;
+  if (int rc = bad_rows("or_block_norm_bwd: dx", x.dx, x.C, x.C)) return rc;
+  if (x.a) {
+    if (int rc = bad_rows("or_block_norm_bwd: a", x.a, x.a_row_stride, x.C)) return rc;
+    if (int rc = bad_rows("or_block_norm_bwd: da", x.da, x.C, x.C)) return rc;
+    if (x.dh)
+      if (int rc = bad_rows("or_block_norm_bwd: dh", x.dh, x.dh_row_stride, x.C)) return rc;
+  } else if (x.gate || x.post_weight || x.post_norm != OR_NORM_NONE || x.dh || x.dgate || x.dpost_weight) {
+    return fail_arg("or_block_norm_bwd: dh, gate, post_norm and post_weight belong to a");
+  }
+  if (x.post_weight && x.post_norm == OR_NORM_NONE) return fail_arg("or_block_norm_bwd: post_weight belongs to a post_norm");
+  if (!al16(x.gate) || !al16(x.post_weight) || !al16(x.weight) || !al16(x.scale))
+    return fail_arg("or_block_norm_bwd: parameters must be 16-byte aligned");
+  const int64_t need = or_block_norm_bwd_workspace_size(x.n_rows, x.rows_per_group, x.C);
+  const bool sums = x.dgate || x.dpost_weight || x.dweight || x.dbias || x.dscale || x.dshift;
+  if (sums && (!x.workspace || !al16(x.workspace) || x.workspace_bytes < need))
+    return fail_arg("or_block_norm_bwd: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
+  NormBwdArgs g = {};
+  g.dh = x.dh;
+  g.dn = x.dn;
+  g.h = x.h;
+  g.a = x.a;
+  g.dx = x.dx;
+  g.da = x.da;
+  g.gate = x.gate;
+  g.post_weight = x.post_weight;
+  g.weight = x.weight;
+  g.bias = x.bias;
+  g.scale = x.scale;
+  g.dgate = x.dgate;
+  g.dpost_weight = x.dpost_weight;
+  g.dweight = x.dweight;
+  g.dbias = x.dbias;
+  g.dscale = x.dscale;
+  g.dshift = x.dshift;
+  g.per = x.rows_per_group;
+  g.groups = x.n_rows / g.per;
+  g.dh_stride = x.dh_row_stride;
+  g.dn_stride = x.dn_row_stride;
+  g.h_stride = x.h_row_stride;
+  g.a_stride = x.a_row_stride;
+  g.C = x.C;
+  g.parts = (int)bwd_parts(g.per, g.groups);
+  g.norm = x.norm;
+  g.post = x.post_norm;
+  g.eps = x.eps;
+  g.r = x.residual_scale;
+  if (sums) g.part = (float*)x.workspace;
+  const bool weights = x.dweight || x.dbias || x.dpost_weight;
+  if (weights && g.groups > 1) g.group_part = (float*)((char*)x.workspace + part_bytes(x.n_rows, g.per, g.C));
+  hipStream_t st = (hipStream_t)stream;
+  if (x.type == OR_TYPE_BF16) launch_bwd<Bf16>(g, st);
+  else if (x.type == OR_TYPE_FP16) launch_bwd<_Float16>(g, st);
+  else launch_bwd<float>(g, st);
+  if (sums) {
+    const unsigned columns = (unsigned)((g.C + 63) / 64);
+    const dim3 grid(columns, (unsigned)std::min<int64_t>(g.groups, 4096));
+    hipLaunchKernelGGL(block_norm_sums_kernel, grid, dim3(64 * kSumWaves), 0, st, g);
+    if (g.group_part) hipLaunchKernelGGL(block_norm_weights_kernel, dim3(columns, 3), dim3(64 * kSumWaves), 0, st, g);
+  }
+  return check_hip(hipGetLastError(), "or_block_norm_bwd launch");
+}
