@@ -88,6 +88,20 @@ def test_ties_borders_and_ends_of_the_range(dtype):
     assert torch.equal(m.dequantize(torch.float32).cpu(), want.float())
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize('order', ['in order', 'mixed', 'near'])
+def test_every_16_bit_value(dtype, order):
+    print(f'quantize every {dtype} {order}', flush=True)
+    bits = torch.arange(65536, dtype=torch.int32)
+    if order == 'mixed':
+        bits = bits[torch.randperm(65536, generator=torch.Generator().manual_seed(2))]
+    if order == 'near':              # blocks of few exponents, so that most elements are neither 0 nor at the end of the range
+        bits = bits.view(512, 128).t().reshape(-1)
+        bits = bits.view(-1, 16, 2).transpose(1, 2).reshape(-1)
+    x = bits.to(torch.int16).view(dtype).view(64, 1024).to(DEV)
+    check_quantized(x)
+
+
 def test_not_finite_blocks():
     print('quantize not finite', flush=True)
     for dtype in TYPES:
