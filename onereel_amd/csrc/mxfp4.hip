@@ -648,7 +648,7 @@ __global__ __launch_bounds__(kThreads) void mx_prepare_kernel(PrepareArgs g) {
 
 bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 constexpr int64_t kMaxStride = 1 << 21;
-constexpr int kFewRows = 16;
+constexpr int kFewRows = 32;
 constexpr int kCUs = 256;
 constexpr int64_t kMaxBlocks = (int64_t)1 << 22;   // of 512 threads: a grid has under 2^32
 
@@ -717,9 +717,15 @@ Plan plan_of(int64_t I, int64_t J, int64_t K) {
       }
     }
   }
+  // Up to 32 rows the kernel for them, by what 2048 k of 16 columns take a CU for that many rows; the tiles' launches and the one
+  // ahead of them take 2 us more than its own (us, it and the tiles: one row of 2048 to 12288 columns 7.5 and 10.4, of 8192 to 2048 8.6
+  // and 12.1; 16 rows of 2048 to 12288 11.4 and 10.4, of 512 to 512 4.0 and 7.1; 32 of 512 to 512 4.8 and 7.4, of 8192 to 512 23 and 12).
   if (I <= kFewRows) {
-    p.tile = 0;
-    p.split = 1;
+    const int64_t a_cu = ((J + 15) / 16 + kCUs - 1) / kCUs;
+    if (std::max(0.5, K / 2048.0) * a_cu * (1.5 + 0.11 * I) < best + 2.2) {
+      p.tile = 0;
+      p.split = 1;
+    }
   }
   return p;
 }
