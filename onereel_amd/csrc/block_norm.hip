@@ -106,88 +106,95 @@ __device__ __forceinline__ Span span_of(int64_t block, int parts, int64_t per) {
   return s;
 }
 
-template <typename T, bool RES>
-__global__ __launch_bounds__(1024) void block_norm_kernel(NormArgs g) {
-  __shared__ Share post_share[2][kRows][kMaxWaves], share[2][kRows][kMaxWaves];
+// What a row has beside x: nothing, a sub-block's output, or one with a norm of its own
+enum { kNoResidual, kResidual, kPostNorm };
+
+// Work-groups of up to N threads take R rows at a time (fewer registers where a work-group is large).
+template <typename T, int KIND, int N, int R>
+__global__ __launch_bounds__(N) void block_norm_kernel(NormArgs g) {
+  __shared__ Share post_share[2][R][kMaxWaves], share[2][R][kMaxWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, col = 8 * threadIdx.x, C = g.C;
   const bool in = col < C;
   const int columns = wave_columns(C, wave);
   int turn = 0;
   for (int64_t span = blockIdx.x; span < g.spans; span += gridDim.x) {
-  const Span s = span_of(span, g.parts, g.per);
-  const int64_t at = s.group * C + col;
-  float G[8], W[8], B[8], t[8];
-  param8(g.gate, at, in, 1.0f, G);
-  param8(g.post_weight, col, in, 1.0f, t);
+    const Span s = span_of(span, g.parts, g.per);
+    const int64_t at = s.group * C + col;
+    float G[8], W[8], B[8], t[8];
+    if constexpr (KIND != kNoResidual) param8(g.gate, at, in, 1.0f, G);
+    if constexpr (KIND == kPostNorm) {
+      param8(g.post_weight, col, in, 1.0f, t);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) G[i] *= t[i];
-  param8(g.weight, col, in, 1.0f, W);
-  param8(g.bias, col, in, 0.0f, B);
-  param8(g.scale, at, in, 0.0f, t);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    W[i] *= 1.0f + t[i];
-    B[i] *= 1.0f + t[i];
-  }
-  param8(g.shift, at, in, 0.0f, t);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) B[i] += t[i];
-  for (int64_t r0 = s.first; r0 < s.last; r0 += kRows, turn ^= 1) {
-    float h[kRows][8], p[kRows][8];
-    Piece<T, 8> x[kRows], a[kRows];
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      x[k].zero();
-      a[k].zero();
-      if (in && r0 + k < s.last) {
-        x[k].load(g.x, (r0 + k) * g.x_stride + col);
-        if constexpr (RES) a[k].load(g.a, (r0 + k) * g.a_stride + col);
-      }
+      for (int i = 0; i < 8; ++i) G[i] *= t[i];
     }
+    param8(g.weight, col, in, 1.0f, W);
+    param8(g.bias, col, in, 0.0f, B);
+    param8(g.scale, at, in, 0.0f, t);
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) x[k].get(h[k]);
-    if constexpr (RES) {
+    for (int i = 0; i < 8; ++i) {
+      W[i] *= 1.0f + t[i];
+      B[i] *= 1.0f + t[i];
+    }
+    param8(g.shift, at, in, 0.0f, t);
 #pragma unroll
-      for (int k = 0; k < kRows; ++k) a[k].get(p[k]);
-      if (g.post != OR_NORM_NONE) {
+    for (int i = 0; i < 8; ++i) B[i] += t[i];
+    for (int64_t r0 = s.first; r0 < s.last; r0 += R, turn ^= 1) {
+      float h[R][8];
+      Piece<T, 8> x[R], a[R];
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) {
-          Share m;
-          moments(p[k], in, columns, g.post, m);
-          if (lane == 0) post_share[turn][k][wave] = m;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kRows; ++k) {
-          float mean, inv;
-          join_moments(post_share[turn][k], waves, C, g.eps, mean, inv);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) p[k][i] = (p[k][i] - mean) * inv;
+      for (int k = 0; k < R; ++k) {
+        x[k].zero();
+        a[k].zero();
+        if (in && r0 + k < s.last) {
+          x[k].load(g.x, (r0 + k) * g.x_stride + col);
+          if constexpr (KIND != kNoResidual) a[k].load(g.a, (r0 + k) * g.a_stride + col);
         }
       }
 #pragma unroll
-      for (int k = 0; k < kRows; ++k) {
+      for (int k = 0; k < R; ++k) x[k].get(h[k]);
+      if constexpr (KIND != kNoResidual) {
+        float p[R][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[k][i] = g.r * h[k][i] + p[k][i] * G[i];
-        if (in && r0 + k < s.last) Piece<T, 8>::store(g.h, (r0 + k) * C + col, h[k]);
+        for (int k = 0; k < R; ++k) a[k].get(p[k]);
+        if constexpr (KIND == kPostNorm) {
+#pragma unroll
+          for (int k = 0; k < R; ++k) {
+            Share m;
+            moments(p[k], in, columns, g.post, m);
+            if (lane == 0) post_share[turn][k][wave] = m;
+          }
+          __syncthreads();
+#pragma unroll
+          for (int k = 0; k < R; ++k) {
+            float mean, inv;
+            join_moments(post_share[turn][k], waves, C, g.eps, mean, inv);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[k][i] = (p[k][i] - mean) * inv;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[k][i] = g.r * h[k][i] + p[k][i] * G[i];
+          if (in && r0 + k < s.last) Piece<T, 8>::store(g.h, (r0 + k) * C + col, h[k]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        Share m;
+        moments(h[k], in, columns, g.norm, m);
+        if (lane == 0) share[turn][k][wave] = m;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        float mean, inv, n[8];
+        join_moments(share[turn][k], waves, C, g.eps, mean, inv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n[i] = (h[k][i] - mean) * inv * W[i] + B[i];
+        if (in && r0 + k < s.last) Piece<T, 8>::store(g.n, (r0 + k) * C + col, n);
       }
     }
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      Share m;
-      moments(h[k], in, columns, g.norm, m);
-      if (lane == 0) share[turn][k][wave] = m;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      float mean, inv, n[8];
-      join_moments(share[turn][k], waves, C, g.eps, mean, inv);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) n[i] = (h[k][i] - mean) * inv * W[i] + B[i];
-      if (in && r0 + k < s.last) Piece<T, 8>::store(g.n, (r0 + k) * C + col, n);
-    }
-  }
   }
 }
 
@@ -203,127 +210,131 @@ struct NormBwdArgs {
   float eps, r;
 };
 
-template <typename T, bool RES>
-__global__ __launch_bounds__(1024) void block_norm_bwd_kernel(NormBwdArgs g) {
-  __shared__ Share share[2][kRows][kMaxWaves], post_share[2][kRows][kMaxWaves];
-  __shared__ float back[2][kRows][kMaxWaves][2];
+template <typename T, int KIND, int N, int R>
+__global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
+  __shared__ Share share[2][R][kMaxWaves], post_share[2][R][kMaxWaves];
+  __shared__ float back[2][R][kMaxWaves][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, col = 8 * threadIdx.x, C = g.C;
   const bool in = col < C;
   const int columns = wave_columns(C, wave);
   int turn = 0;
   for (int64_t span = blockIdx.x; span < g.groups * g.parts; span += gridDim.x) {
-  const Span s = span_of(span, g.parts, g.per);
-  const int64_t at = s.group * C + col;
-  float G[8], W[8], v[8], A[8], B[8], D[8];
-  param8(g.gate, at, in, 1.0f, G);
-  param8(g.post_weight, col, in, 1.0f, v);
+    const Span s = span_of(span, g.parts, g.per);
+    const int64_t at = s.group * C + col;
+    float G[8], W[8], v[8], A[8], B[8], D[8];
+    if constexpr (KIND != kNoResidual) param8(g.gate, at, in, 1.0f, G);
+    if constexpr (KIND == kPostNorm) {
+      param8(g.post_weight, col, in, 1.0f, v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) G[i] *= v[i];
-  param8(g.weight, col, in, 1.0f, W);
-  param8(g.scale, at, in, 0.0f, v);
+      for (int i = 0; i < 8; ++i) G[i] *= v[i];
+    }
+    param8(g.weight, col, in, 1.0f, W);
+    param8(g.scale, at, in, 0.0f, v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    W[i] *= 1.0f + v[i];
-    A[i] = B[i] = D[i] = 0.0f;
-  }
-  for (int64_t r0 = s.first; r0 < s.last; r0 += kRows, turn ^= 1) {
-    Piece<T, 8> hp[kRows], np[kRows], dp[kRows], ap[kRows];
+    for (int i = 0; i < 8; ++i) {
+      W[i] *= 1.0f + v[i];
+      A[i] = B[i] = D[i] = 0.0f;
+    }
+    for (int64_t r0 = s.first; r0 < s.last; r0 += R, turn ^= 1) {
+      Piece<T, 8> hp[R], np[R], dp[R], ap[R];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      hp[k].zero();
-      np[k].zero();
-      dp[k].zero();
-      ap[k].zero();
-      if (in && r0 + k < s.last) {
-        hp[k].load(g.h, (r0 + k) * g.h_stride + col);
-        np[k].load(g.dn, (r0 + k) * g.dn_stride + col);
-        if constexpr (RES) {
-          if (g.dh) dp[k].load(g.dh, (r0 + k) * g.dh_stride + col);
-          ap[k].load(g.a, (r0 + k) * g.a_stride + col);
+      for (int k = 0; k < R; ++k) {
+        hp[k].zero();
+        np[k].zero();
+        dp[k].zero();
+        ap[k].zero();
+        if (in && r0 + k < s.last) {
+          hp[k].load(g.h, (r0 + k) * g.h_stride + col);
+          np[k].load(g.dn, (r0 + k) * g.dn_stride + col);
+          if constexpr (KIND != kNoResidual) {
+            if (g.dh) dp[k].load(g.dh, (r0 + k) * g.dh_stride + col);
+            ap[k].load(g.a, (r0 + k) * g.a_stride + col);
+          }
         }
       }
-    }
-    float h[kRows][8], n[kRows][8], a[kRows][8];
+      // the elements are unpacked from their words again after the barrier, so that only the words stay live across it
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      Share m;
-      hp[k].get(h[k]);
-      np[k].get(n[k]);
-      moments(h[k], in, columns, g.norm, m);
-      float t = 0.0f, tx = 0.0f;
+      for (int k = 0; k < R; ++k) {
+        Share m;
+        float h[8], n[8];
+        hp[k].get(h);
+        np[k].get(n);
+        moments(h, in, columns, g.norm, m);
+        float t = 0.0f, tx = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        t += n[k][i] * W[i];
-        tx += n[k][i] * W[i] * (h[k][i] - m.mean);
-      }
-      m.t = g.norm == OR_NORM_LAYER ? wave_sum(in ? t : 0.0f) : 0.0f;
-      m.tx = wave_sum(in ? tx : 0.0f);
-      if (lane == 0) share[turn][k][wave] = m;
-      if constexpr (RES) {
-        ap[k].get(a[k]);
-        if (g.post != OR_NORM_NONE) {
-          moments(a[k], in, columns, g.post, m);
+        for (int i = 0; i < 8; ++i) {
+          t += n[i] * W[i];
+          tx += n[i] * W[i] * (h[i] - m.mean);
+        }
+        m.t = g.norm == OR_NORM_LAYER ? wave_sum(in ? t : 0.0f) : 0.0f;
+        m.tx = wave_sum(in ? tx : 0.0f);
+        if (lane == 0) share[turn][k][wave] = m;
+        if constexpr (KIND == kPostNorm) {
+          ap[k].get(h);
+          moments(h, in, columns, g.post, m);
           if (lane == 0) post_share[turn][k][wave] = m;
         }
       }
-    }
-    __syncthreads();
-    float u[kRows][8], post_inv[kRows];
+      __syncthreads();
+      float u[R][8], ah[R][8], post_inv[R];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      float mean, inv, t = 0.0f, tx = 0.0f, d[8];
-      join_moments(share[turn][k], waves, C, g.eps, mean, inv);
-      for (int w = 0; w < waves; ++w) {
-        const Share m = share[turn][k][w];
-        t += m.t;
-        tx += m.tx + (m.mean - mean) * m.t;
-      }
-      t /= (float)C;
-      tx *= inv / (float)C;
-      dp[k].get(d);
-      const bool row = in && r0 + k < s.last;
+      for (int k = 0; k < R; ++k) {
+        float mean, inv, t = 0.0f, tx = 0.0f, h[8], n[8], d[8], a[8];
+        join_moments(share[turn][k], waves, C, g.eps, mean, inv);
+        for (int w = 0; w < waves; ++w) {
+          const Share m = share[turn][k][w];
+          t += m.t;
+          tx += m.tx + (m.mean - mean) * m.t;
+        }
+        t /= (float)C;
+        tx *= inv / (float)C;
+        hp[k].get(h);
+        np[k].get(n);
+        dp[k].get(d);
+        const bool row = in && r0 + k < s.last;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float xh = (h[k][i] - mean) * inv;
-        A[i] += row ? n[k][i] * xh : 0.0f;
-        B[i] += n[k][i];
-        d[i] += inv * (n[k][i] * W[i] - t - xh * tx);
-        u[k][i] = d[i] * G[i];
-      }
-      if constexpr (RES) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = g.r * d[i];
-        if (row) Piece<T, 8>::store(g.dx, (r0 + k) * C + col, x);
-        if (g.post != OR_NORM_NONE) {
-          join_moments(post_share[turn][k], waves, C, g.eps, mean, post_inv[k]);
-          float su = 0.0f, sux = 0.0f;
+        for (int i = 0; i < 8; ++i) {
+          const float xh = (h[i] - mean) * inv;
+          A[i] += row ? n[i] * xh : 0.0f;
+          B[i] += n[i];
+          d[i] += inv * (n[i] * W[i] - t - xh * tx);
+        }
+        if constexpr (KIND == kNoResidual) {
+          if (row) Piece<T, 8>::store(g.dx, (r0 + k) * C + col, d);
+        } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            a[k][i] = (a[k][i] - mean) * post_inv[k];
-            su += u[k][i];
-            sux += u[k][i] * a[k][i];
+            u[k][i] = d[i] * G[i];
+            h[i] = g.r * d[i];
           }
-          su = g.post == OR_NORM_LAYER ? wave_sum(in ? su : 0.0f) : 0.0f;
-          sux = wave_sum(in ? sux : 0.0f);
-          if (lane == 0) {
-            back[turn][k][wave][0] = su;
-            back[turn][k][wave][1] = sux;
-          }
-        } else if (row) {
-          Piece<T, 8>::store(g.da, (r0 + k) * C + col, u[k]);
-        }
+          if (row) Piece<T, 8>::store(g.dx, (r0 + k) * C + col, h);
+          ap[k].get(a);
+          if constexpr (KIND == kPostNorm) {
+            join_moments(post_share[turn][k], waves, C, g.eps, mean, post_inv[k]);
+            float su = 0.0f, sux = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) D[i] += row ? d[i] * a[k][i] : 0.0f;
-      } else if (row) {
-        Piece<T, 8>::store(g.dx, (r0 + k) * C + col, d);
+            for (int i = 0; i < 8; ++i) {
+              a[i] = ah[k][i] = (a[i] - mean) * post_inv[k];
+              su += u[k][i];
+              sux += u[k][i] * a[i];
+            }
+            su = g.post == OR_NORM_LAYER ? wave_sum(in ? su : 0.0f) : 0.0f;
+            sux = wave_sum(in ? sux : 0.0f);
+            if (lane == 0) {
+              back[turn][k][wave][0] = su;
+              back[turn][k][wave][1] = sux;
+            }
+          } else if (row) {
+            Piece<T, 8>::store(g.da, (r0 + k) * C + col, u[k]);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) D[i] += row ? d[i] * a[i] : 0.0f;
+        }
       }
-    }
-    if constexpr (RES) {
-      if (g.post != OR_NORM_NONE) {
+      if constexpr (KIND == kPostNorm) {
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) {
+        for (int k = 0; k < R; ++k) {
           float su = 0.0f, sux = 0.0f;
           for (int w = 0; w < waves; ++w) {
             su += back[turn][k][w][0];
@@ -332,20 +343,19 @@ __global__ __launch_bounds__(1024) void block_norm_bwd_kernel(NormBwdArgs g) {
           su /= (float)C;
           sux /= (float)C;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) u[k][i] = post_inv[k] * (u[k][i] - su - a[k][i] * sux);
+          for (int i = 0; i < 8; ++i) u[k][i] = post_inv[k] * (u[k][i] - su - ah[k][i] * sux);
           if (in && r0 + k < s.last) Piece<T, 8>::store(g.da, (r0 + k) * C + col, u[k]);
         }
       }
     }
-  }
-  if (!g.part || !in) continue;
-  float* out = g.part + span * 3 * C + col;
+    if (!g.part || !in) continue;
+    float* out = g.part + span * 3 * C + col;
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    *(f32x4*)(out + i) = f32x4{A[i], A[i + 1], A[i + 2], A[i + 3]};
-    *(f32x4*)(out + C + i) = f32x4{B[i], B[i + 1], B[i + 2], B[i + 3]};
-    *(f32x4*)(out + 2 * C + i) = f32x4{D[i], D[i + 1], D[i + 2], D[i + 3]};
-  }
+    for (int i = 0; i < 8; i += 4) {
+      *(f32x4*)(out + i) = f32x4{A[i], A[i + 1], A[i + 2], A[i + 3]};
+      *(f32x4*)(out + C + i) = f32x4{B[i], B[i + 1], B[i + 2], B[i + 3]};
+      *(f32x4*)(out + 2 * C + i) = f32x4{D[i], D[i + 1], D[i + 2], D[i + 3]};
+    }
   }
 }
 
@@ -414,9 +424,9 @@ __global__ __launch_bounds__(64 * kSumWaves) void block_norm_weights_kernel(Norm
 bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 int threads_of(int C) { return (C / 8 + 63) / 64 * 64; }
 
-// work-groups of a group of rows: `wanted` in all, each with two batches of rows or more
+// work-groups of a group of rows: `wanted` in all, each with a batch of rows or more
 int64_t parts_of(int64_t per, int64_t groups, int wanted) {
-  return std::max<int64_t>(1, std::min<int64_t>((wanted + groups - 1) / groups, per / (2 * kRows)));
+  return std::max<int64_t>(1, std::min<int64_t>((wanted + groups - 1) / groups, per / kRows));
 }
 
 int check_sizes(const char* what, int64_t rows, int64_t per, int32_t C, int32_t type) {
@@ -450,18 +460,38 @@ int64_t part_bytes(int64_t rows, int64_t per, int C) {
 
 constexpr int64_t kMaxBlocks = 1 << 20;   // of up to 1024 threads: a grid has under 2^32 of them
 
-template <typename T>
-void launch(const NormArgs& g, hipStream_t st) {
+template <typename T, int KIND, int N>
+void launch_kind(const NormArgs& g, hipStream_t st) {
   const dim3 grid((unsigned)std::min(g.spans, kMaxBlocks)), block((unsigned)threads_of(g.C));
-  if (g.a) hipLaunchKernelGGL((block_norm_kernel<T, true>), grid, block, 0, st, g);
-  else hipLaunchKernelGGL((block_norm_kernel<T, false>), grid, block, 0, st, g);
+  hipLaunchKernelGGL((block_norm_kernel<T, KIND, N, kRows>), grid, block, 0, st, g);
 }
 
-template <typename T>
-void launch_bwd(const NormBwdArgs& g, hipStream_t st) {
+template <typename T, int KIND, int N>
+void launch_kind(const NormBwdArgs& g, hipStream_t st) {
   const dim3 grid((unsigned)std::min(g.groups * g.parts, kMaxBlocks)), block((unsigned)threads_of(g.C));
-  if (g.a) hipLaunchKernelGGL((block_norm_bwd_kernel<T, true>), grid, block, 0, st, g);
-  else hipLaunchKernelGGL((block_norm_bwd_kernel<T, false>), grid, block, 0, st, g);
+  hipLaunchKernelGGL((block_norm_bwd_kernel<T, KIND, N, (N > 512 ? 1 : kRows)>), grid, block, 0, st, g);
+}
+
+template <typename T, int KIND, typename G>
+void launch_width(const G& g, hipStream_t st) {
+  const int n = threads_of(g.C);
+  if (n <= 256) launch_kind<T, KIND, 256>(g, st);
+  else if (n <= 512) launch_kind<T, KIND, 512>(g, st);
+  else launch_kind<T, KIND, 1024>(g, st);
+}
+
+template <typename T, typename G>
+void launch_type(const G& g, hipStream_t st) {
+  if (!g.a) launch_width<T, kNoResidual>(g, st);
+  else if (g.post == OR_NORM_NONE) launch_width<T, kResidual>(g, st);
+  else launch_width<T, kPostNorm>(g, st);
+}
+
+template <typename G>
+void launch(const G& g, int type, hipStream_t st) {
+  if (type == OR_TYPE_BF16) launch_type<Bf16>(g, st);
+  else if (type == OR_TYPE_FP16) launch_type<_Float16>(g, st);
+  else launch_type<float>(g, st);
 }
 
 }  // namespace
@@ -509,9 +539,7 @@ extern "C" int or_block_norm(const or_block_norm_args* p, void* stream) {
   g.parts = (int)parts_of(g.per, groups, 2048);
   g.spans = groups * g.parts;
   hipStream_t st = (hipStream_t)stream;
-  if (x.type == OR_TYPE_BF16) launch<Bf16>(g, st);
-  else if (x.type == OR_TYPE_FP16) launch<_Float16>(g, st);
-  else launch<float>(g, st);
+  launch(g, x.type, st);
   return check_hip(hipGetLastError(), "block_norm_kernel launch");
 }
 
@@ -580,9 +608,7 @@ extern "C" int or_block_norm_bwd(const or_block_norm_bwd_args* p, void* stream) 
   const bool weights = x.dweight || x.dbias || x.dpost_weight;
   if (weights && g.groups > 1) g.group_part = (float*)((char*)x.workspace + part_bytes(x.n_rows, g.per, g.C));
   hipStream_t st = (hipStream_t)stream;
-  if (x.type == OR_TYPE_BF16) launch_bwd<Bf16>(g, st);
-  else if (x.type == OR_TYPE_FP16) launch_bwd<_Float16>(g, st);
-  else launch_bwd<float>(g, st);
+  launch(g, x.type, st);
   if (sums) {
     const unsigned columns = (unsigned)((g.C + 63) / 64);
     const dim3 grid(columns, (unsigned)std::min<int64_t>(g.groups, 4096));
