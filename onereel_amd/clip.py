@@ -8,10 +8,15 @@ from __future__ import annotations
 
 import array
 import ctypes
+import operator
 
 import torch
 
 from . import _lib as L
+
+
+_T = torch.Tensor
+_DTYPE, _DEVICE, _ADDRESS, _NUMEL, _SHAPE = operator.attrgetter('dtype'), _T.get_device, _T.data_ptr, _T.numel, operator.attrgetter('shape')
 
 
 def _dense(t) -> bool:
@@ -26,86 +31,86 @@ def _dense(t) -> bool:
     return True
 
 
-def _check(tensors, what: str, device=None):
-    for t in tensors:
-        if t.dtype not in L.TYPES or not t.is_cuda:
-            raise L.HipTypeError(f'{what} must be bf16, fp16 or fp32 GPU tensors, got {t.dtype} on {t.device}')
-        device = t.device if device is None else device
-        if t.device != device:
-            raise L.HipTypeError('all tensors of a call must be on one GPU')
-    return device
+def _addresses(tensors, what: str, at: int):
+    """(addresses, lengths, types) of the tensors as the library takes them, and their GPU's index (at: the one it has to be,
+    None for any)"""
+    # one C call for each tensor and question: a model has hundreds of them, and their launches take less than a loop over them
+    dtypes, devices = list(map(_DTYPE, tensors)), set(map(_DEVICE, tensors))
+    if not L.TYPES.keys() >= set(dtypes) or devices and min(devices) < 0:
+        t = next(t for t in tensors if t.dtype not in L.TYPES or t.get_device() < 0)
+        raise L.HipTypeError(f'{what} must be bf16, fp16 or fp32 GPU tensors, got {t.dtype} on {t.device}')
+    if at is not None:
+        devices.add(at)
+    if len(devices) > 1:
+        raise L.HipTypeError('all tensors of a call must be on one GPU')
+    kinds = array.array('i', map(L.TYPES.__getitem__, dtypes))
+    return (array.array('Q', map(_ADDRESS, tensors)), array.array('q', map(_NUMEL, tensors)), kinds), \
+        devices.pop() if devices else None
 
 
-def _apart(written, read):
-    """raises where a tensor to write shares memory with another one, or with one to read that it does not take the place of"""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), True) for t in written if t.numel()]
-    spans += [(r.data_ptr(), r.data_ptr() + r.numel() * r.element_size(), False) for r, w in zip(read, written)
-              if r.numel() and (r.data_ptr() != w.data_ptr() or r.dtype != w.dtype)]
-    end = end_written = 0
-    for first, last, writes in sorted(spans):
-        if first < (end if writes else end_written):
-            raise L.HipValueError('tensors that are written must not share memory with one another or with what is read')
-        end, end_written = max(end, last), max(end_written, last) if writes else end_written
-
-
-def _call(tensors, device, max_norm=0.0, out=None):
-    n = len(tensors)
-    x = array.array('Q', [t.data_ptr() for t in tensors])
-    numel = array.array('q', [t.numel() for t in tensors])
-    types = array.array('i', [L.TYPES[t.dtype] for t in tensors])
-    o = None if out is None else array.array('Q', [t.data_ptr() for t in out])
-    out_types = None if out is None else array.array('i', [L.TYPES[t.dtype] for t in out])
-    at = lambda values: None if values is None or not n else values.buffer_info()[0]
+def _call(sources, out, at: int, max_norm: float = 0.0):
+    """or_clip of two results of _addresses (out None: the norm alone)"""
+    p = lambda values: values.buffer_info()[0]
+    n, device = len(sources[0]), torch.device('cuda', at)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    args = L.ClipArgs(at(x), at(numel), at(types), at(o), at(out_types), n, max_norm, norm.data_ptr(), None, 0)
-    size = int(L.dit_lib().or_clip_workspace_size(ctypes.byref(args)))
+    args = L.ClipArgs(*map(p, sources), out and p(out[0]), out and p(out[2]), n, max_norm, norm.data_ptr(), None, 0)
+    size = L.dit_lib().or_clip_workspace_size(ctypes.byref(args))
     if size < 0:
         L.dit_check(size, 'or_clip_workspace_size')
-    space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    args.workspace, args.workspace_bytes = L.ptr(space), size
+    if size:
+        space = torch.empty(size, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = space.data_ptr(), size
     L.dit_check(L.call(device, L.dit_lib().or_clip, ctypes.byref(args)), 'or_clip')
     return norm
 
 
+def _zero():
+    return torch.zeros((), dtype=torch.float32, device='cuda')
+
+
 def grad_norm(tensors):
     """The 2-norm of all elements of the tensors (an iterable; 0 without any), an fp32 scalar on their GPU"""
-    tensors = [t.detach() for t in tensors]
-    device = _check(tensors, 'tensors')
-    if device is None:
-        return torch.zeros((), dtype=torch.float32, device='cuda')
-    return _call([t if _dense(t) else t.contiguous() for t in tensors], device)
+    tensors = list(tensors)
+    if not all(map(_T.is_contiguous, tensors)):
+        tensors = [t if _dense(t) else t.detach().contiguous() for t in tensors]
+    sources, at = _addresses(tensors, 'tensors', None)
+    return _zero() if at is None else _call(sources, None, at)
 
 
 def clip_grads_(tensors, max_norm: float, out=None):
     """Scales the tensors by c = min(1, max_norm / (norm + 1e-6)), norm being the 2-norm of all their elements together, in place
     or, with out (one tensor of the same shape for each, of any of the types), into those. Returns the norm before clipping, an
     fp32 scalar on the GPU. A norm that is infinite or NaN does to the tensors what the formula says, as in torch: zeros and NaN, or
-    NaN throughout. The tensors (those of out) must not share memory, and each fill its own."""
-    tensors = [t.detach() for t in tensors]
+    NaN throughout. Tensors that are written must not share memory with one another or with what is read (but for the tensor that
+    they take the place of), and each fill its own."""
+    tensors = list(tensors)
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise L.HipValueError(f'max_norm must be 0 or more, got {max_norm}')
-    device = _check(tensors, 'tensors')
     if out is None:
-        written = tensors
-        if not all(_dense(t) for t in tensors):
+        if not all(map(_T.is_contiguous, tensors)) and not all(map(_dense, tensors)):
             raise L.HipValueError('tensors that are scaled in place must fill their memory: expanded or strided ones do not')
-        sources = tensors
+        sources, at = _addresses(tensors, 'tensors', None)
+        written = sources
     else:
-        written = [t.detach() for t in out]
-        if len(written) != len(tensors) or any(a.shape != b.shape for a, b in zip(written, tensors)):
+        if not all(map(_T.is_contiguous, tensors)):
+            tensors = [t.detach().contiguous() for t in tensors]
+        out = list(out)
+        if len(out) != len(tensors) or list(map(_SHAPE, out)) != list(map(_SHAPE, tensors)):
             raise L.HipValueError('out must hold a tensor of the same shape for each of the tensors')
-        _check(written, 'out', device)
-        if not all(t.is_contiguous() for t in written):
+        if not all(map(_T.is_contiguous, out)):
             raise L.HipValueError('out must be contiguous')
-        sources = [t.contiguous() for t in tensors]
-    _apart(written, sources)
-    if device is None:
-        return torch.zeros((), dtype=torch.float32, device='cuda')
-    for t in out if out is not None else tensors:
-        if not t.is_inference():
-            torch.autograd.graph.increment_version(t)
-    return _call(sources, device, max_norm, written)
+        sources, at = _addresses(tensors, 'tensors', None)
+        written, _ = _addresses(out, 'out', at)
+    if at is None:
+        return _zero()
+    norm = _call(sources, written, at, max_norm)
+    changed = tensors if out is None else out
+    try:
+        torch.autograd.graph.increment_version(changed)
+    except RuntimeError:               # inference tensors among them, which have no version
+        torch.autograd.graph.increment_version([t for t in changed if not t.is_inference()])
+    return norm
 
 
 def clip_grad_norm_(parameters, max_norm: float):

@@ -13,6 +13,8 @@
 #include <math.h>
 
 #include <algorithm>
+#include <new>
+#include <vector>
 
 #include "../../include/onereel_dit.h"
 #include "rows.h"
@@ -92,13 +94,6 @@ __device__ __forceinline__ void put8(T* x, int64_t at, int64_t n, bool wide, con
     }
 }
 
-__device__ __forceinline__ void get(int type, const void* x, int64_t at, int64_t n, float (&v)[8]) {
-  const bool wide = ((uintptr_t)x & 15) == 0;
-  if (type == OR_TYPE_BF16) get8((const Bf16*)x, at, n, wide, v);
-  else if (type == OR_TYPE_FP16) get8((const _Float16*)x, at, n, wide, v);
-  else get8((const float*)x, at, n, wide, v);
-}
-
 __device__ __forceinline__ double wave_sum64(double v) {
   for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
   return v;
@@ -114,21 +109,48 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
   return v;
 }
 
+// Pieces [p, end) of a tensor of n elements, several at a time where they are whole: the loads of all of them first
+constexpr int kAtOnce = 4;
+
+template <typename T>
+__device__ __forceinline__ double squares(const T* x, int64_t n, int64_t p, int64_t end) {
+  const bool wide = ((uintptr_t)x & 15) == 0;
+  double sum = 0.0;
+  float v[8];
+  auto add = [&] {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += (double)v[i] * (double)v[i];
+  };
+  const int64_t whole = wide ? min(end, n / kPiece) : 0;
+  for (; p + kAtOnce <= whole; p += kAtOnce) {
+    Piece<T, 8> r[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) r[k].load(x, (p + k) * kPiece + 8 * threadIdx.x);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      r[k].get(v);
+      add();
+    }
+  }
+  for (; p < end; ++p) {
+    get8(x, p * kPiece + 8 * threadIdx.x, n, wide, v);
+    add();
+  }
+  return sum;
+}
+
 __global__ __launch_bounds__(kThreads) void grad_norm_kernel(Tensors t, double* part) {
   __shared__ double shared[kThreads / 64];
   const int64_t last = piece_of(t, blockIdx.x + 1);
   int64_t p = piece_of(t, blockIdx.x);
-  int k = tensor_of(t, p);
   double sum = 0.0;
-  while (p < last) {
-    while (t.first[k + 1] <= p) ++k;
-    const int64_t end = min(last, (int64_t)t.first[k + 1]), n = t.n[k];
-    for (; p < end; ++p) {
-      float v[8];
-      get(t.type[k] & 15, t.x[k], (p - t.first[k]) * kPiece + 8 * threadIdx.x, n, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum += (double)v[i] * (double)v[i];
-    }
+  for (int k = tensor_of(t, p); p < last; ++k) {
+    const int64_t at = t.first[k], end = min(last, (int64_t)t.first[k + 1]), n = t.n[k];
+    const int type = t.type[k] & 15;
+    if (type == OR_TYPE_BF16) sum += squares((const Bf16*)t.x[k], n, p - at, end - at);
+    else if (type == OR_TYPE_FP16) sum += squares((const _Float16*)t.x[k], n, p - at, end - at);
+    else sum += squares((const float*)t.x[k], n, p - at, end - at);
+    p = end;
   }
   sum = block_sum(sum, shared);
   if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -147,6 +169,44 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(ClipArgs c) {
   if (threadIdx.x == 0) *c.norm = (float)norm;
 }
 
+// Pieces [first, p) of a tensor, from the last one down
+template <typename T, typename O>
+__device__ __forceinline__ void scale(const T* x, O* out, int64_t n, int64_t first, int64_t p, float factor) {
+  const bool wide = ((uintptr_t)x & 15) == 0, wide_out = ((uintptr_t)out & 15) == 0;
+  float v[8];
+  auto one = [&](int64_t q) {
+    const int64_t at = q * kPiece + 8 * threadIdx.x;
+    get8(x, at, n, wide, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= factor;
+    put8(out, at, n, wide_out, v);
+  };
+  const int64_t whole = wide && wide_out ? n / kPiece : 0;
+  for (; p > first && p > whole; --p) one(p - 1);
+  for (; p - kAtOnce >= first; p -= kAtOnce) {
+    Piece<T, 8> r[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) r[k].load(x, (p - 1 - k) * kPiece + 8 * threadIdx.x);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      r[k].get(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= factor;
+      Piece<O, 8>::store(out, (p - 1 - k) * kPiece + 8 * threadIdx.x, v);
+    }
+  }
+  for (; p > first; --p) one(p - 1);
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_into(const T* x, void* out, int type, int64_t n, int64_t first, int64_t p, float factor) {
+  if (type == OR_TYPE_BF16) scale(x, (Bf16*)out, n, first, p, factor);
+  else if (type == OR_TYPE_FP16) scale(x, (_Float16*)out, n, first, p, factor);
+  else scale(x, (float*)out, n, first, p, factor);
+}
+
+// The launches, tensors and pieces in the opposite order of the first kernel's: what that has read last is still in the last-level
+// cache.
 __global__ __launch_bounds__(kThreads) void clip_kernel(Tensors t, ClipArgs c) {
   __shared__ double shared[kThreads / 64];
   const double norm = norm_of(c, shared);
@@ -154,29 +214,17 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(Tensors t, ClipArgs c) {
   // the comparison keeps a NaN, as min(1, NaN) of torch's clamp does: gradients with a NaN among them all become NaN
   const double ratio = c.max_norm / (norm + 1e-6);
   const float factor = ratio > 1.0 ? 1.0f : (float)ratio;
-  const int64_t last = piece_of(t, blockIdx.x + 1);
-  int64_t p = piece_of(t, blockIdx.x);
-  int k = tensor_of(t, p);
-  while (p < last) {
-    while (t.first[k + 1] <= p) ++k;
-    const int64_t end = min(last, (int64_t)t.first[k + 1]), n = t.n[k];
-    if (factor == 1.0f && t.out[k] == t.x[k]) {
-      p = end;
-      continue;
+  const int64_t first = piece_of(t, blockIdx.x);
+  int64_t p = piece_of(t, blockIdx.x + 1);
+  for (int k = tensor_of(t, p - 1); p > first; --k) {
+    const int64_t at = t.first[k], begin = max(first, at), n = t.n[k];
+    if (factor != 1.0f || t.out[k] != t.x[k]) {
+      const int type = t.type[k] & 15, to = t.type[k] >> 4;
+      if (type == OR_TYPE_BF16) scale_into((const Bf16*)t.x[k], t.out[k], to, n, begin - at, p - at, factor);
+      else if (type == OR_TYPE_FP16) scale_into((const _Float16*)t.x[k], t.out[k], to, n, begin - at, p - at, factor);
+      else scale_into((const float*)t.x[k], t.out[k], to, n, begin - at, p - at, factor);
     }
-    for (; p < end; ++p) {
-      float v[8];
-      const int64_t at = (p - t.first[k]) * kPiece + 8 * threadIdx.x;
-      get(t.type[k] & 15, t.x[k], at, n, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= factor;
-      void* o = t.out[k];
-      const bool wide = ((uintptr_t)o & 15) == 0;
-      const int type = t.type[k] >> 4;
-      if (type == OR_TYPE_BF16) put8((Bf16*)o, at, n, wide, v);
-      else if (type == OR_TYPE_FP16) put8((_Float16*)o, at, n, wide, v);
-      else put8((float*)o, at, n, wide, v);
-    }
+    p = begin;
   }
 }
 
@@ -198,45 +246,66 @@ int check_tensors(const char* what, const or_clip_args& a) {
   return 0;
 }
 
-int64_t pieces_of(int64_t n) { return (n + kPiece - 1) / kPiece; }
-
-// Work-groups of a launch: as many as a second reader of their partial sums may cost, each with two pieces or more
-int blocks_of(int64_t pieces) { return (int)std::max<int64_t>(1, std::min<int64_t>(kBlocks, (pieces + 1) / 2)); }
-
-// the launches' tensors, one after the other; f(tensors) for each. A tensor of 2^31 pieces or more, and a launch of so many, are
-// divided.
-template <typename F>
-int64_t each_launch(const or_clip_args& a, const F& f) {
-  constexpr int64_t kMost = (int64_t)1 << 30;   // pieces of a launch
-  int64_t launches = 0;
-  Tensors t;
-  t.count = 0;
-  t.first[0] = 0;
-  auto flush = [&] {
-    if (!t.count) return;
-    t.blocks = blocks_of(t.first[t.count]);
-    f(t);
-    ++launches;
-    t.count = 0;
+// What is written shares memory neither with other such tensors nor with what is read, but for the tensor that it takes the place of.
+int check_apart(const or_clip_args& a) {
+  struct Span {
+    uintptr_t first, last;
+    bool writes;
   };
+  std::vector<Span> spans;
+  spans.reserve(2 * a.n_tensors);
   for (int64_t i = 0; i < a.n_tensors; ++i) {
     if (a.numel[i] == 0) continue;
-    int64_t at = 0;
-    while (at < a.numel[i]) {
-      if (t.count == kTensors || (t.count && t.first[t.count] == kMost)) flush();
+    const uintptr_t x = (uintptr_t)a.x[i], o = (uintptr_t)a.out[i];
+    spans.push_back({o, o + a.numel[i] * type_size(a.out_type ? a.out_type[i] : a.type[i]), true});
+    if (o != x) spans.push_back({x, x + a.numel[i] * type_size(a.type[i]), false});
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& p, const Span& q) { return p.first < q.first; });
+  uintptr_t end = 0, written = 0;
+  for (const Span& s : spans) {
+    if (s.first < (s.writes ? end : written)) return fail_arg("or_clip: tensors that are written must not share memory with one another or with what is read");
+    end = std::max(end, s.last);
+    if (s.writes) written = std::max(written, s.last);
+  }
+  return 0;
+}
+
+int64_t pieces_of(int64_t n) { return (n + kPiece - 1) / kPiece; }
+
+// Work-groups of a launch: as many as a second reader of their partial sums may cost
+int blocks_of(int64_t pieces) { return (int)std::min<int64_t>(kBlocks, pieces); }
+
+// the launches' tensors. A tensor with more pieces than a launch numbers is divided.
+std::vector<Tensors> launches_of(const or_clip_args& a) {
+  constexpr int64_t kMost = (int64_t)1 << 30;   // pieces of a launch
+  std::vector<Tensors> all;
+  for (int64_t i = 0; i < a.n_tensors; ++i) {
+    const int size = type_size(a.type[i]), out_type = a.out_type ? a.out_type[i] : a.type[i];
+    for (int64_t at = 0; at < a.numel[i];) {
+      if (all.empty() || all.back().count == kTensors || all.back().first[all.back().count] == kMost) {
+        all.emplace_back();
+        all.back().count = all.back().first[0] = 0;
+      }
+      Tensors& t = all.back();
       const int64_t n = std::min(a.numel[i] - at, (kMost - t.first[t.count]) * kPiece);
-      const int size = type_size(a.type[i]), out_type = a.out_type ? a.out_type[i] : a.type[i];
       t.x[t.count] = (const char*)a.x[i] + at * size;
       t.out[t.count] = a.out ? (char*)a.out[i] + at * type_size(out_type) : nullptr;
       t.n[t.count] = n;
       t.type[t.count] = (uint8_t)(a.type[i] | out_type << 4);
       t.first[t.count + 1] = (int32_t)(t.first[t.count] + pieces_of(n));
       ++t.count;
+      t.blocks = blocks_of(t.first[t.count]);
       at += n;
     }
   }
-  flush();
-  return launches;
+  return all;
+}
+
+// how many partial sums there are
+int64_t parts_of(const std::vector<Tensors>& launches) {
+  int64_t n = 0;
+  for (const Tensors& t : launches) n += t.blocks;
+  return n;
 }
 
 }  // namespace
@@ -244,41 +313,45 @@ int64_t each_launch(const or_clip_args& a, const F& f) {
 
 using namespace onereel;
 
-extern "C" int64_t or_clip_workspace_size(const or_clip_args* p) {
+extern "C" int64_t or_clip_workspace_size(const or_clip_args* p) try {
   if (!p) return fail_arg("or_clip_workspace_size: args is NULL");
   if (int rc = check_tensors("or_clip_workspace_size", *p)) return rc;
-  int64_t parts = 0;
-  each_launch(*p, [&](const Tensors& t) { parts += t.blocks; });
-  return parts * 8;
+  return parts_of(launches_of(*p)) * 8;
+} catch (const std::bad_alloc&) {
+  return fail_arg("or_clip_workspace_size: out of host memory");
 }
 
-extern "C" int or_clip(const or_clip_args* p, void* stream) {
+extern "C" int or_clip(const or_clip_args* p, void* stream) try {
   if (!p) return fail_arg("or_clip: args is NULL");
   const or_clip_args& a = *p;
-  const int64_t need = or_clip_workspace_size(p);
-  if (need < 0) return (int)need;
+  if (int rc = check_tensors("or_clip", a)) return rc;
+  if (a.out)
+    if (int rc = check_apart(a)) return rc;
   if (!a.norm || ((uintptr_t)a.norm & 3)) return fail_arg("or_clip: norm is required");
   if (a.out && !(a.max_norm >= 0)) return fail_arg("or_clip: max_norm must be 0 or more");
-  if (need > 0 && (!a.workspace || ((uintptr_t)a.workspace & 15) || a.workspace_bytes < need))
-    return fail_arg("or_clip: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
-  hipStream_t st = (hipStream_t)stream;
+  const std::vector<Tensors> launches = launches_of(a);
   ClipArgs c = {};
+  c.parts = parts_of(launches);
+  if (c.parts > 0 && (!a.workspace || ((uintptr_t)a.workspace & 15) || a.workspace_bytes < c.parts * 8))
+    return fail_arg("or_clip: a 16-byte aligned workspace of %lld bytes is needed", (long long)c.parts * 8);
   c.part = (double*)a.workspace;
-  c.parts = need / 8;
   c.norm = a.norm;
   c.max_norm = a.max_norm;
+  hipStream_t st = (hipStream_t)stream;
   double* part = c.part;
-  each_launch(a, [&](const Tensors& t) {
+  for (const Tensors& t : launches) {
     hipLaunchKernelGGL(grad_norm_kernel, dim3(t.blocks), dim3(kThreads), 0, st, t, part);
     part += t.blocks;
-  });
-  if (!a.out || c.parts == 0) {
+  }
+  if (!a.out || launches.empty()) {
     hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, st, c);
   } else {
-    each_launch(a, [&](const Tensors& t) {
-      hipLaunchKernelGGL(clip_kernel, dim3(t.blocks), dim3(kThreads), 0, st, t, c);
-      c.norm = nullptr;   // the first launch has written it
-    });
+    for (auto t = launches.rbegin(); t != launches.rend(); ++t) {
+      hipLaunchKernelGGL(clip_kernel, dim3(t->blocks), dim3(kThreads), 0, st, *t, c);
+      c.norm = nullptr;   // the first launch writes it
+    }
   }
   return check_hip(hipGetLastError(), "or_clip launch");
+} catch (const std::bad_alloc&) {
+  return fail_arg("or_clip: out of host memory");
 }
