@@ -6,7 +6,7 @@ key offset and length). With extra frames (frame memory) each scene's keys are p
 pack-gather kernels instead. With `Context.memory` = M > 0, scene j's queries read scene j plus M representatives
 per head of the other scenes' boundary keys (`onereel_amd.memory`, wan.py:100-101,154-173). Cross-attention: scene
 j's queries read only sentence j, all scenes in one varlen launch. The RMSNorm + interleaved RoPE of `_qk`
-(wan.py:64-74) is one HIP launch for q and k (`or_rmsnorm_rope`).
+(wan.py:64-74) is one HIP launch for q and k (`or_rmsnorm_rope`; with positions in place of tables, `onereel_amd.rotary`).
 """
 from __future__ import annotations
 
@@ -21,6 +21,8 @@ from .comm import frame_tokens  # noqa: F401  (re-exported for callers of the re
 from .frame_memory import FrameMemory
 from .layout import SceneLayout
 from .memory import BoundaryMemory, MemoryAttention, frame_plan
+from .mxfp4 import MXFP4
+from .rotary import Axes, norm_rotate
 from .scene import ScopePlan, pack_layer, varlen, without_gradient
 
 TEXT_LEN = 512
@@ -267,7 +269,8 @@ def cross_ranges(ctx: Context, q, k, v):
 
 
 class Processor:
-    """kind 'self' or 'cross' (wan.py:77-108). One GPU: the whole token range."""
+    """kind 'self' or 'cross' (wan.py:77-108). One GPU: the whole token range. rotary_emb: the (cos, sin) tables, or the positions
+    (`rotary.Axes`); hidden_states may come in 4 bits (`mxfp4.MXFP4`) where the projections take it so."""
 
     def __init__(self, ctx: Context, kind: str, orig=None, layer: int = 0):
         assert kind in ('self', 'cross'), kind
@@ -282,10 +285,11 @@ class Processor:
             q, k, v = (x[0].to(torch.bfloat16).contiguous() for x in (q, k, v))
             o = cross_ranges(self.ctx, q, k, v)
         else:
-            cos, sin = rotary_emb
             q, k, v = attn.to_q(hidden_states), attn.to_k(hidden_states), attn.to_v(hidden_states)
-            q, k = _qk(q, k, attn.norm_q.weight, attn.norm_k.weight, attn.norm_q.eps, cos, sin, H)
+            w = attn.norm_q.weight, attn.norm_k.weight, attn.norm_q.eps
+            q, k = norm_rotate(q, k, *w, rotary_emb, H) if isinstance(rotary_emb, Axes) else _qk(q, k, *w, *rotary_emb, H)
             v = v.unflatten(2, (H, -1))
             q, k, v = (x[0].to(torch.bfloat16).contiguous() for x in (q, k, v))
             o = memory_self(self.ctx, q, k, v, self.layer) if self.ctx.memory else self_ranges(self.ctx, q, k, v)
-        return attn.to_out[1](attn.to_out[0](o.flatten(1, 2)[None].type_as(hidden_states)))
+        o = o.flatten(1, 2)[None]
+        return attn.to_out[1](attn.to_out[0](o if isinstance(hidden_states, MXFP4) else o.type_as(hidden_states)))

@@ -25,7 +25,12 @@ channels, text width 4096 projected to 3072.
 `WanDiT.differentiable_forward` is the same pass for fine-tuning, with gradients of every weight: the projections and the
 feed forward are `linear` calls (bias, GELU, gate and residual in their epilogues), the attention and its norms the
 differentiable calls of the processors (halo scopes; the packed frame-memory scopes and the bounded memory have no
-gradient), the LayerNorm + modulation torch operations in fp32. Nothing is updated in place.
+gradient), the LayerNorm + modulation `norms` calls. Nothing is updated in place. `clip_gradients` is what a training step does
+between the backward pass and the optimizer.
+
+Both passes take one timestep for all tokens, or one for each latent frame (a conditioning frame at 0 beside noisy ones), whose
+modulation and gates then differ from frame to frame (`norms.residual_norm_modulate`), and rotary tables or positions
+(`rotary.grid`). `quantize` turns the inference pass's blocks to 4-bit weights and activations (`onereel_amd.mxfp4`).
 """
 from __future__ import annotations
 
@@ -37,7 +42,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib as L
-from . import wan
+from . import clip, mxfp4, norms, wan
 from .linear import linear
 from .layout import SceneLayout
 from .scene import overwritten, without_gradient
@@ -123,23 +128,27 @@ class Linear:
     def __init__(self, n_in, n_out, std, gen, device):
         self.weight = (torch.randn(n_out, n_in, generator=gen, device=device) * std).to(torch.bfloat16)
         self.bias = (torch.randn(n_out, generator=gen, device=device) * std).to(torch.bfloat16)
+        self.quantized = None            # the weight in 4 bits, for the inference pass
 
     def __call__(self, x):
+        if self.quantized is not None:
+            return mxfp4.linear(x, self.quantized, self.bias)
         return F.linear(x, self.weight, self.bias)
 
     def gelu_tanh(self, x):
         """GELU(x W^T + b, approximate='tanh') with the activation in the GEMM's epilogue (hipBLASLt through
         torch._addmm_activation): the activation is applied to the fp32 accumulator and the [.., n_out] output is
         written once, instead of a separate GELU pass over it"""
+        if self.quantized is not None:
+            return mxfp4.linear(x, self.quantized, self.bias, activation='gelu_tanh')
         x2 = x.reshape(-1, x.shape[-1])
         y = torch._addmm_activation(self.bias, x2, self.weight.t(), use_gelu=True)
         return y.view(*x.shape[:-1], y.shape[-1])
 
 
 def _norm(x, eps, weight=None, bias=None, scale=None, shift=None):
-    """layernorm_modulate in torch operations, for autograd"""
-    y = F.layer_norm(x.float(), x.shape[-1:], weight, bias, eps)
-    return (y if scale is None else y * (1 + scale) + shift).to(torch.bfloat16)
+    """layernorm_modulate with gradients"""
+    return norms.norm_modulate(x, eps, weight=weight, bias=bias, scale=scale, shift=shift)
 
 
 def _apply(layer, x, **epilogue):
@@ -169,13 +178,13 @@ class Attention:
 
 
 class _Projections:
-    """an Attention as a processor sees it in the differentiable pass: projections by or_linear, the output's left to the
-    caller, who has its gate and residual"""
+    """an Attention as a processor sees it in the differentiable pass: projections by or_linear, the output's (unless `out`) left
+    to the caller, who has its gate and residual"""
 
-    def __init__(self, attn: Attention):
+    def __init__(self, attn: Attention, out: bool = False):
         self.heads, self.norm_q, self.norm_k = attn.heads, attn.norm_q, attn.norm_k
         self.to_q, self.to_k, self.to_v = (functools.partial(_apply, l) for l in (attn.to_q, attn.to_k, attn.to_v))
-        self.to_out = [lambda x: x, lambda x: x]
+        self.to_out = [functools.partial(_apply, attn.to_out[0]) if out else lambda x: x, lambda x: x]
 
 
 class Block:
@@ -192,8 +201,13 @@ class Block:
         self.scale_shift_table = torch.randn(6, d, generator=gen, device=device) / d ** 0.5
 
     def modulation(self, temb6):
-        """(shift, scale, gate, c_shift, c_scale, c_gate), each [1, dim] fp32"""
+        """(shift, scale, gate, c_shift, c_scale, c_gate), each [1, dim] fp32; of temb6 [6, frames, dim] each [frames, dim]"""
+        if temb6.dim() == 3:
+            return (self.scale_shift_table[:, None] + temb6).unbind(0)
         return (self.scale_shift_table + temb6).chunk(6, 0)
+
+    def linears(self):
+        return [l for a in (self.attn1, self.attn2) for l in (a.to_q, a.to_k, a.to_v, a.to_out[0])] + [self.ffn_in, self.ffn_out]
 
     def __call__(self, x, n, mod, text, rotary, p_self, p_cross):
         """x [1, S, dim] bf16, updated in place; n: LayerNorm(x) * (1 + scale) + shift of this block's modulation
@@ -201,11 +215,28 @@ class Block:
         together with the next LayerNorm (the block's own residual adds run with the norms that follow them)."""
         eps = self.cfg.eps
         shift, scale, gate, c_shift, c_scale, c_gate = mod
-        n = residual_layernorm_modulate_(x, p_self(self.attn1, n, rotary_emb=rotary), eps, gate=gate,
+        n = residual_layernorm_modulate_(x, p_self(self.attn1, self._shared(n), rotary_emb=rotary), eps, gate=gate,
                                          weight=self.norm2_w, bias=self.norm2_b)
         n = residual_layernorm_modulate_(x, p_cross(self.attn2, n, encoder_hidden_states=text), eps, scale=c_scale,
                                          shift=c_shift)
         return self.ffn_out(self.ffn_in.gelu_tanh(n)), c_gate
+
+    def _shared(self, n):
+        """the rows that queries, keys and values are projected from, quantised once for the three"""
+        return n if self.attn1.to_q.quantized is None else mxfp4.quantize(n)
+
+    def grouped(self, x, n, mod, text, rotary, p_self, p_cross, apply=None):
+        """__call__ with the modulation and gates of each frame, on new tensors: (x, the feed forward's output, its gate). apply:
+        _apply for a differentiable pass"""
+        eps = self.cfg.eps
+        _, _, gate, c_shift, c_scale, c_gate = mod
+        attn1, attn2 = (self.attn1, self.attn2) if apply is None else (_Projections(self.attn1, True), _Projections(self.attn2, True))
+        o = p_self(attn1, n if apply else self._shared(n), rotary_emb=rotary)
+        x, n = norms.residual_norm_modulate(x, o, eps, gate=gate, weight=self.norm2_w, bias=self.norm2_b)
+        x, n = norms.residual_norm_modulate(x, p_cross(attn2, n, encoder_hidden_states=text), eps, scale=c_scale, shift=c_shift)
+        if apply is None:
+            return x, self.ffn_out(self.ffn_in.gelu_tanh(n)), c_gate
+        return x, apply(self.ffn_out, apply(self.ffn_in, n, activation='gelu_tanh')), c_gate
 
     def differentiable(self, x, mod, text, rotary, p_self, p_cross):
         """x [1, S, dim] bf16 -> the block's output, a new tensor, with gradients of x and of every weight"""
@@ -219,9 +250,7 @@ class Block:
         return _apply(self.ffn_out, h, gate=c_gate, residual=x)
 
     def parameters(self):
-        layers = [l for a in (self.attn1, self.attn2) for l in (a.to_q, a.to_k, a.to_v, a.to_out[0])]
-        layers += [self.ffn_in, self.ffn_out]
-        return [p for l in layers for p in (l.weight, l.bias)] + \
+        return [p for l in self.linears() for p in (l.weight, l.bias)] + \
             [n.weight for a in (self.attn1, self.attn2) for n in (a.norm_q, a.norm_k)] + \
             [self.norm2_w, self.norm2_b, self.scale_shift_table]
 
@@ -250,9 +279,33 @@ class WanDiT:
         self.p_self = wan.Processor(self.ctx, 'self')
         self.p_cross = wan.Processor(self.ctx, 'cross')
 
-    def forward(self, tokens, t: float, text, rotary):
-        """tokens [S, in_channels * patch] bf16 (the patchified latent, frame-major), text [n_scenes * text_len,
-        text_dim] bf16 (sentence j in rows j * text_len ..), rotary (cos, sin) [1, S, 1, D] fp32 -> [S, in * patch]"""
+    def quantize(self):
+        """The blocks' projections and feed forwards in 4 bits (MXFP4) for `forward` from here on, from the present weights; the
+        embeddings and the output projection stay in bf16. `differentiable_forward` keeps the bf16 weights."""
+        for l in (l for b in self.blocks for l in b.linears()):
+            l.quantized = mxfp4.quantize(l.weight)
+        return self
+
+    def clip_gradients(self, max_norm: float):
+        """the gradients of `parameters()` scaled to a norm of at most max_norm (clip.clip_grad_norm_): their norm before that"""
+        return clip.clip_grad_norm_(self.parameters(), max_norm)
+
+    def _per_frame(self, t):
+        """the timesteps of the latent frames, or None where t is one for all"""
+        if isinstance(t, (int, float)) or isinstance(t, torch.Tensor) and t.dim() == 0:
+            return None
+        t = [float(x) for x in t]
+        if len(t) != self.ctx.layout.n_frames:
+            raise L.HipValueError(f'{len(t)} timesteps for {self.ctx.layout.n_frames} latent frames')
+        return t
+
+    def forward(self, tokens, t, text, rotary):
+        """tokens [S, in_channels * patch] bf16 (the patchified latent, frame-major), t the timestep, or one for each latent frame,
+        text [n_scenes * text_len, text_dim] bf16 (sentence j in rows j * text_len ..), rotary (cos, sin) [1, S, 1, D] fp32 or a
+        rotary.Axes -> [S, in * patch]"""
+        frames = self._per_frame(t)
+        if frames is not None:
+            return self._forward_frames(tokens, frames, text, rotary)
         d = self.cfg.dim
         x = self.patch_embed(tokens)[None]
         temb = self.time_out(F.silu(self.time_in(timestep_features(t, self.cfg.freq_dim, tokens.device)
@@ -270,10 +323,30 @@ class WanDiT:
             n = residual_layernorm_modulate_(x, f, eps, gate=gate, scale=scale, shift=shift)
         return self.proj_out(n)[0]
 
-    def differentiable_forward(self, tokens, t: float, text, rotary):
+    def _forward_frames(self, tokens, frames, text, rotary, apply=None):
+        """forward, or with apply differentiable_forward, with a timestep for each latent frame"""
+        d, eps, run = self.cfg.dim, self.cfg.eps, apply or (lambda layer, x: layer(x))
+        x = run(self.patch_embed, tokens)[None]
+        features = torch.stack([timestep_features(t, self.cfg.freq_dim, tokens.device) for t in frames]).to(torch.bfloat16)
+        temb = run(self.time_out, F.silu(run(self.time_in, features)))
+        temb6 = run(self.time_proj, F.silu(temb)).view(-1, 6, d).transpose(0, 1).float().contiguous()
+        ctx_text = run(self.text_out, F.gelu(run(self.text_in, text), approximate='tanh'))[None]
+        mods = [blk.modulation(temb6) for blk in self.blocks]
+        out_shift, out_scale = (self.scale_shift_table[:, None] + temb.float()).unbind(0)
+        n = norms.norm_modulate(x, eps, scale=mods[0][1], shift=mods[0][0])
+        for i, blk in enumerate(self.blocks):
+            x, f, gate = blk.grouped(x, n, mods[i], ctx_text, rotary, self.p_self, self.p_cross, apply)
+            shift, scale = (mods[i + 1][0], mods[i + 1][1]) if i + 1 < len(self.blocks) else (out_shift, out_scale)
+            x, n = norms.residual_norm_modulate(x, f, eps, gate=gate, scale=scale, shift=shift)
+        return run(self.proj_out, n)[0]
+
+    def differentiable_forward(self, tokens, t, text, rotary):
         """forward with gradients of tokens, text and `parameters()` (those of them that require one)"""
         if self.ctx.memory or any(self.ctx.layout.extra.get(j) for j in range(self.ctx.layout.n_scenes)):
             raise L.HipValueError('the frame-memory scopes and the bounded memory have no gradient: train with halo scopes')
+        frames = self._per_frame(t)
+        if frames is not None:
+            return self._forward_frames(tokens, frames, text, rotary, _apply)
         d, eps = self.cfg.dim, self.cfg.eps
         x = _apply(self.patch_embed, tokens)[None]
         features = timestep_features(t, self.cfg.freq_dim, tokens.device).to(torch.bfloat16)[None]
