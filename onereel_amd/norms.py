@@ -54,6 +54,12 @@ def _vector(t, C: int, what: str, groups=None):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _like(t):
+    """a new contiguous tensor of t's shape and type, in its final shape: a view made inside an autograd function takes no in-place
+    operation"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _norm(name, none: bool = False) -> int:
     if name not in L.NORMS or name is None and not none:
         raise L.HipValueError(f'a norm must be one of {[n for n in L.NORMS if none or n]}, got {name!r}')
@@ -95,9 +101,7 @@ def _forward(x, a, eps, norm, gate, residual_scale, post_norm, post_weight, weig
     x2, xs = _rows(x, shape, x.dtype, 'x')
     a2, as_ = (None, 0) if a is None else _rows(a, shape, x.dtype, 'a')
     p, dev = L.ptr, x.device
-    # in their final shape: a view made inside an autograd function takes no in-place operation
-    n = torch.empty(shape, dtype=x.dtype, device=dev)
-    h = None if a is None else torch.empty_like(n)
+    n, h = _like(x), None if a is None else _like(x)
     args = L.BlockNormArgs(x2.data_ptr(), p(a2), p(h), n.data_ptr(), p(g), p(pw), p(w), p(b), p(sc), p(sh), rows, per, xs, as_,
                            C, L.TYPES[x.dtype], *kinds, eps, residual_scale)
     L.dit_check(L.call(dev, L.dit_lib().or_block_norm, ctypes.byref(args)), 'or_block_norm')
@@ -120,11 +124,9 @@ def _backward(dh, dn, h, a, eps, norm, gate, residual_scale, post_norm, post_wei
     n2, ns = _rows(dn, shape, h.dtype, 'dn')
     a2, as_ = (None, 0) if a is None else _rows(a, shape, h.dtype, 'a')
     d2, ds = (None, 0) if dh is None else _rows(dh, shape, h.dtype, 'dh')
-    dx = torch.empty(shape, dtype=h.dtype, device=dev)
-    da = None if a is None else torch.empty_like(dx)
-    make = torch.empty if rows else torch.zeros
-    grads = [make(t.shape, dtype=torch.float32, device=dev) if t is not None and need else None
-             for t, need in zip(given, needs)]
+    dx, da = _like(h), None if a is None else _like(h)
+    make = torch.empty_like if rows else torch.zeros_like
+    grads = [make(t) if t is not None and need else None for t, need in zip(given, needs)]
     p = L.ptr
     size, space = 0, None
     if any(t is not None for t in grads):

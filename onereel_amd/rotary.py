@@ -20,6 +20,13 @@ from .attention import records
 PAIRS = {'interleaved': 0, 'half': 1}
 
 
+@functools.lru_cache(256)
+def _four(dims: tuple, theta: tuple):
+    """dims and theta of up to 4 axes as the library takes them"""
+    fill = (0,) * (4 - len(dims))
+    return (L.i32 * 4)(*dims, *fill), (ctypes.c_double * 4)(*theta, *fill)
+
+
 class Axes:
     """Positions [S, n] of S tokens on n (1 to 4) axes, int32 or fp32 on the GPU (whole or fractional, of any size; one axis may
     come as [S]), and the dims of a head that each axis rotates: an even count, together up to the head's; the dims past them
@@ -43,10 +50,9 @@ class Axes:
         self.positions, self.dims, self.theta, self.pairs = positions.contiguous(), dims, theta, pairs
 
     def _struct(self):
-        four = lambda values: (*values, *([0] * (4 - len(values))))
         p = self.positions
         return L.RopeAxes(p.data_ptr(), p.shape[0], len(self.dims), int(p.dtype == torch.float32), PAIRS[self.pairs],
-                          (L.i32 * 4)(*four(self.dims)), (ctypes.c_double * 4)(*four(self.theta)))
+                          *_four(self.dims, self.theta))
 
 
 def split_dims(head_dim: int) -> tuple:
@@ -100,7 +106,7 @@ def _rotate(x, axes, inverse: bool):
         x3 = x3.clone(memory_format=torch.contiguous_format)
         s = x3.stride()
     # in its final shape: a view made inside an autograd function takes no in-place operation
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
     a = axes._struct()
     L.check(L.call(x.device, L.lib().or_rope_axes_rotate, ctypes.byref(a), x3.data_ptr(), out.data_ptr(), x3.shape[0], H, D,
                    s[0], s[1], L.TYPES[x.dtype], int(inverse)), 'or_rope_axes_rotate')
@@ -191,8 +197,8 @@ def norm_rotate_backward(dq, dk, q, k, wq, wk, eps: float, axes: Axes, heads: in
     (q2, qs), (k2, ks), (dq2, dqs), (dk2, dks) = (_rows(t, C) for t in (q, k, dq, dk))
     w = [_weight(t, q, C) for t in (wq, wk)]
     S, dev = q2.shape[0], q.device
-    gq, gk = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=q.dtype, device=dev)
-    gw = [torch.empty(C, dtype=torch.float32, device=dev) for _ in range(2)]
+    gq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    gk, gw = torch.empty_like(gq), [torch.empty(C, dtype=torch.float32, device=dev) for _ in range(2)]
     n = _SIZES(S, C)
     if n < 0:
         L.check(L.lib().or_rmsnorm_rope_axes_bwd_workspace_size(S, C), 'or_rmsnorm_rope_axes_bwd_workspace_size')
