@@ -613,37 +613,40 @@ __global__ __launch_bounds__(kThreads) void mx_prepare_kernel(PrepareArgs g) {
   using U = ScaleUnit<SB>;
   __shared__ __attribute__((aligned(16))) uint8_t st[256];
   const bool weights = (int)blockIdx.x >= g.a_blocks;
-  const int64_t unit = weights ? (int)blockIdx.x - g.a_blocks : (int)blockIdx.x;
   const int64_t rows = weights ? g.n_out : g.q.rows, all = weights ? g.b_rows : g.a_rows;
-  const int step = (int)(unit % g.steps), blocks = g.q.K / kBlock, tid = threadIdx.x;
-  // group of 128 rows, and the first of 8 rows in each 32 of it
-  const int64_t u = unit / g.steps, r0 = u / 4 * kScaleRows + u % 4 * 8;
-  if (weights || !g.q.x) {
-    const uint8_t* from = weights ? g.w_scales : g.q.scales;
-    const int f = tid >> 6, l = tid >> 3 & 7, k = tid & 7, block = 8 * step + k;
-    const int64_t row = r0 + l + 32 * f;
-    st[U::place(l, f, k)] = row < rows && block < blocks ? from[row * blocks + block] : 0;
-  } else {
-    const int l = tid >> 5, c = tid & 31, at = 256 * step + 8 * c;
-    const bool in = at < g.q.K;        // all four lanes of a block, or none
-    Piece<Bf16, 8> p[4];
-#pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      p[f].zero();
+  const int blocks = g.q.K / kBlock, tid = threadIdx.x, work_groups = weights ? (int)gridDim.x - g.a_blocks : g.a_blocks;
+  for (int64_t unit = weights ? (int)blockIdx.x - g.a_blocks : (int)blockIdx.x; unit < all / 32 * g.steps; unit += work_groups) {
+    const int step = (int)(unit % g.steps);
+    // group of 128 rows, and the first of 8 rows in each 32 of it
+    const int64_t u = unit / g.steps, r0 = u / 4 * kScaleRows + u % 4 * 8;
+    if (weights || !g.q.x) {
+      const uint8_t* from = weights ? g.w_scales : g.q.scales;
+      const int f = tid >> 6, l = tid >> 3 & 7, k = tid & 7, block = 8 * step + k;
       const int64_t row = r0 + l + 32 * f;
-      if (in && row < rows) p[f].load(g.q.x, row * g.q.x_stride + at);
-    }
+      st[U::place(l, f, k)] = row < rows && block < blocks ? from[row * blocks + block] : 0;
+    } else {
+      const int l = tid >> 5, c = tid & 31, at = 256 * step + 8 * c;
+      const bool in = at < g.q.K;        // all four lanes of a block, or none
+      Piece<Bf16, 8> p[4];
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      const int64_t row = r0 + l + 32 * f;
-      uint32_t codes, scale;
-      quantize8(p[f], codes, scale);
-      if (in && row < rows) ((uint32_t*)g.q.codes)[row * (g.q.K / 8) + at / 8] = codes;
-      if ((c & 3) == 0) st[U::place(l, f, c >> 2)] = in && row < rows ? (uint8_t)scale : 0;
+      for (int f = 0; f < 4; ++f) {
+        p[f].zero();
+        const int64_t row = r0 + l + 32 * f;
+        if (in && row < rows) p[f].load(g.q.x, row * g.q.x_stride + at);
+      }
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const int64_t row = r0 + l + 32 * f;
+        uint32_t codes, scale;
+        quantize8(p[f], codes, scale);
+        if (in && row < rows) ((uint32_t*)g.q.codes)[row * (g.q.K / 8) + at / 8] = codes;
+        if ((c & 3) == 0) st[U::place(l, f, c >> 2)] = in && row < rows ? (uint8_t)scale : 0;
+      }
     }
+    __syncthreads();
+    U::write(st, weights ? g.b_scales : g.a_scales, all, r0, step, tid);
+    __syncthreads();
   }
-  __syncthreads();
-  U::write(st, weights ? g.b_scales : g.a_scales, all, r0, step, tid);
 }
 
 bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
@@ -692,28 +695,27 @@ constexpr int kTileRows = 256;         // the scales' layouts come in whole tile
 // 256 -> 8192 73); 1.2 (steps + 3.8) with two of 128 x 128 a CU and 0.65 (steps + 7) with one, whose four buffers then fit (4096 x
 // 2048 -> 2048 22, 1024 x 8192 -> 2048 30); 0.5 (steps + 5.9) and 0.42 (steps + 2.6) with two of 64 x 64 and one (1024 x 8192 -> 2048 26, 333
 // x 8192 -> 2048 19). Parts of k add the launch that joins them and its traffic (64 x 8192 -> 512 in 4 parts 12.0, in one 16.3).
+double time_of(int tile, int64_t n, double steps) {
+  const int64_t one = (n + kCUs - 1) / kCUs, two = (n + 2 * kCUs - 1) / (2 * kCUs);
+  if (tile == 256) return 2.1 * (steps + 3.6) * one;
+  if (tile == 128) return n <= kCUs ? 0.65 * (steps + 7) : 1.2 * (steps + 3.8) * two;
+  return n <= kCUs ? 0.42 * (steps + 2.6) : 0.5 * (steps + 5.9) * two;
+}
+
 Plan plan_of(int64_t I, int64_t J, int64_t K) {
   Plan p = {};
-  p.split = 1;
-  const int64_t steps = (K + kStepElements - 1) / kStepElements;
   double best = 1e300;
+  const int64_t steps = (K + kStepElements - 1) / kStepElements;
   for (int tile : {256, 128, 64}) {
     const int64_t ti = (I + tile - 1) / tile, tj = (J + tile - 1) / tile;
     for (int split : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (split > 1 && steps / split < 4) break;
-      const int64_t n = ti * tj * split, one = (n + kCUs - 1) / kCUs, two = (n + 2 * kCUs - 1) / (2 * kCUs);
+      const int64_t n = ti * tj * split;
       if (n > kMaxBlocks) break;
-      const double of_tile = (double)((steps + split - 1) / split);
-      const double time = (tile == 256 ? 2.1 * (of_tile + 3.6) * one
-                           : tile == 128 ? (n <= kCUs ? 0.65 * (of_tile + 7) : 1.2 * (of_tile + 3.8) * two)
-                                         : (n <= kCUs ? 0.42 * (of_tile + 2.6) : 0.5 * (of_tile + 5.9) * two)) +
-                          (split > 1 ? 3 + (8.0 * split + 2) * I * J / 4e6 : 0);
+      const double time = time_of(tile, n, (double)((steps + split - 1) / split)) + (split > 1 ? 3 + (8.0 * split + 2) * I * J / 4e6 : 0);
       if (time < best) {
         best = time;
-        p.tile = tile;
-        p.tiles_i = (int)ti;
-        p.tiles_j = (int)tj;
-        p.split = split;
+        p = Plan{tile, (int)ti, (int)tj, split};
       }
     }
   }
@@ -722,10 +724,7 @@ Plan plan_of(int64_t I, int64_t J, int64_t K) {
   // and 12.1; 16 rows of 2048 to 12288 11.4 and 10.4, of 512 to 512 4.0 and 7.1; 32 of 512 to 512 4.8 and 7.4, of 8192 to 512 23 and 12).
   if (I <= kFewRows) {
     const int64_t a_cu = ((J + 15) / 16 + kCUs - 1) / kCUs;
-    if (std::max(0.5, K / 2048.0) * a_cu * (1.5 + 0.11 * I) < best + 2.2) {
-      p.tile = 0;
-      p.split = 1;
-    }
+    if (std::max(0.5, K / 2048.0) * a_cu * (1.5 + 0.11 * I) < best + 2.2) p = Plan{0, 0, 0, 1};
   }
   return p;
 }
@@ -856,17 +855,20 @@ extern "C" int or_mx_linear(const or_mx_linear_args* p, void* stream) {
   r.b_rows = l.b_rows;
   r.n_out = x.n_out;
   r.steps = l.steps;
-  r.a_blocks = (int)((l.a_rows / 32) * r.steps);
-  const unsigned w_blocks = (unsigned)(l.b_rows / 32 * r.steps);
+  const int64_t a_units = l.a_rows / 32 * r.steps, w_units = l.b_rows / 32 * r.steps;
+  r.a_blocks = (int)std::min<int64_t>(a_units, kMaxBlocks);
+  const unsigned w_blocks = (unsigned)std::min<int64_t>(w_units, kMaxBlocks);
   hipLaunchKernelGGL(mx_prepare_kernel<kSB>, dim3(r.a_blocks + w_blocks), dim3(kThreads), 0, st, r);
   g.a_scales = r.a_scales;
   g.b_scales = r.b_scales;
   g.a_rows = l.a_rows;
   g.b_rows = l.b_rows;
+  g.part = (float*)(ws + l.part);
   g.split = plan.split;
   g.tiles_i = plan.tiles_i;
   g.tiles_j = plan.tiles_j;
-  g.part = (float*)(ws + l.part);
+  // (The rows of a last round that fills few CUs in smaller tiles, in a launch after the others': 12720 x 2048 -> 8192, 1600 tiles in 6.25
+  // rounds, 155 and 13 us, one launch 172.)
   const int64_t n = (int64_t)g.tiles_i * g.tiles_j * g.split;
   const unsigned blocks = (unsigned)((n + 7) / 8 * 8);
   if (plan.tile == 256) launch_tiles<256, 256, 2, 4, 2>(g, blocks, st);
@@ -874,8 +876,8 @@ extern "C" int or_mx_linear(const or_mx_linear_args* p, void* stream) {
   else if (plan.tile == 128) launch_tiles<128, 128, 2, 2, 2>(g, blocks, st);
   else launch_tiles<64, 64, 2, 2, 4>(g, blocks, st);
   if (g.split > 1) {
-    const int64_t blocks = std::min<int64_t>((g.I * g.J / 8 + kThreads - 1) / kThreads, 8192);
-    hipLaunchKernelGGL(mx_join_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, g);
+    const int64_t joins = std::min<int64_t>((g.I * g.J / 8 + kThreads - 1) / kThreads, 8192);
+    hipLaunchKernelGGL(mx_join_kernel, dim3((unsigned)joins), dim3(kThreads), 0, st, g);
   }
   return check_hip(hipGetLastError(), "or_mx_linear launch");
 }
