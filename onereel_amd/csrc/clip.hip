@@ -13,7 +13,7 @@
 #include <math.h>
 
 #include <algorithm>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "../../include/onereel_dit.h"
@@ -317,8 +317,8 @@ extern "C" int64_t or_clip_workspace_size(const or_clip_args* p) try {
   if (!p) return fail_arg("or_clip_workspace_size: args is NULL");
   if (int rc = check_tensors("or_clip_workspace_size", *p)) return rc;
   return parts_of(launches_of(*p)) * 8;
-} catch (const std::bad_alloc&) {
-  return fail_arg("or_clip_workspace_size: out of host memory");
+} catch (const std::exception& e) {
+  return fail_arg("or_clip_workspace_size: %s", e.what());
 }
 
 extern "C" int or_clip(const or_clip_args* p, void* stream) try {
@@ -352,6 +352,6 @@ extern "C" int or_clip(const or_clip_args* p, void* stream) try {
     }
   }
   return check_hip(hipGetLastError(), "or_clip launch");
-} catch (const std::bad_alloc&) {
-  return fail_arg("or_clip: out of host memory");
+} catch (const std::exception& e) {
+  return fail_arg("or_clip: %s", e.what());
 }

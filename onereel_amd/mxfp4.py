@@ -38,6 +38,7 @@ class MXFP4:
                                   f'{tuple(codes.shape)} and {tuple(scales.shape)}')
         codes = codes.contiguous()
         self.codes, self.scales = codes if codes.data_ptr() % 16 == 0 else codes.clone(), scales.contiguous()
+        self._of = None      # what was quantised, where autograd recorded that
 
     @property
     def shape(self):
@@ -57,13 +58,14 @@ class MXFP4:
         n = shape[-1]
         L.dit_check(L.call(dev, L.dit_lib().or_mx_dequantize, self.codes.data_ptr(), self.scales.data_ptr(), out.numel() // n, n,
                            L.TYPES[dtype], out.data_ptr()), 'or_mx_dequantize')
-        return out
+        return without_gradient('MXFP4.dequantize', out, self._of)
 
 
 def quantize(x) -> MXFP4:
     """x [.., n] (bf16, fp16 or fp32, n a multiple of 32) in 4 bits: a block's scale is the power of two that brings its largest
     magnitude into [4, 8), elements go to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4 and 6 times it, ties to the even code, past 6 to
-    6. A block with an infinity or a NaN becomes NaN."""
+    6. A block with an infinity or a NaN becomes NaN. Without a gradient: a backward pass that reaches what is made of the result
+    raises, where autograd records and x requires one."""
     if x.dtype not in L.TYPES or not x.is_cuda:
         raise L.HipTypeError(f'expected a bf16, fp16 or fp32 GPU tensor, got {x.dtype} on {x.device}')
     shape = x.shape
@@ -78,7 +80,10 @@ def quantize(x) -> MXFP4:
     scales = torch.empty(*shape[:-1], n // BLOCK, dtype=torch.uint8, device=dev)
     L.dit_check(L.call(dev, L.dit_lib().or_mx_quantize, x2.data_ptr(), x2.shape[0], n, row, L.TYPES[x.dtype], codes.data_ptr(),
                        scales.data_ptr()), 'or_mx_quantize')
-    return MXFP4(codes, scales)
+    m = MXFP4(codes, scales)
+    if torch.is_grad_enabled() and x.requires_grad:
+        m._of = x
+    return m
 
 
 _SIZES = functools.lru_cache(256)(lambda *sizes: int(L.dit_lib().or_mx_linear_workspace_size(*sizes)))
@@ -117,4 +122,4 @@ def linear(x, weight: MXFP4, bias=None, activation=None, gate=None, residual=Non
                        weight.codes.data_ptr(), weight.scales.data_ptr(), p(b), p(g), p(r), y.data_ptr(), M, xs, rs, n_out, n_in,
                        n_out, act, b16, g16, p(space), size)
     L.dit_check(L.call(dev, L.dit_lib().or_mx_linear, ctypes.byref(a)), 'or_mx_linear')
-    return without_gradient('mxfp4.linear', y, None if ready else x, bias, gate, residual)
+    return without_gradient('mxfp4.linear', y, x._of if ready else x, weight._of, bias, gate, residual)

@@ -37,6 +37,8 @@ class Axes:
     def __init__(self, positions, dims, theta=10000.0, pairs: str = 'interleaved'):
         if positions.dtype not in (torch.int32, torch.float32):
             raise L.HipTypeError(f'positions must be int32 or fp32, got {positions.dtype}')
+        if positions.requires_grad:
+            raise L.HipValueError('positions have no gradient: detach them')
         dims = tuple(int(d) for d in dims)
         n = len(dims)
         theta = tuple(float(t) for t in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * n

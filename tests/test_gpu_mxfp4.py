@@ -267,6 +267,19 @@ def test_a_backward_pass_raises():
         y.sum().backward()
 
 
+def test_a_backward_pass_through_quantised_tensors_raises():
+    x, w, b, _, _ = layer(4, 64, 16)
+    made = [mxfp4.linear(mxfp4.quantize(x.clone().requires_grad_()), w), mxfp4.quantize(x.clone().requires_grad_()).dequantize(),
+            mxfp4.linear(x, mxfp4.quantize(torch.ones(16, 64, device=DEV, requires_grad=True))),
+            mxfp4.linear(x, w, b.clone().requires_grad_())]
+    for y in made:
+        with pytest.raises(L.HipValueError, match='no gradient'):
+            y.float().sum().backward()
+    with torch.no_grad():
+        assert not mxfp4.linear(mxfp4.quantize(x.clone().requires_grad_()), w).requires_grad
+    assert not mxfp4.linear(mxfp4.quantize(x), w, b).requires_grad
+
+
 def test_refusals():
     x, w, b, gate, r = layer(4, 64, 16)
     c, s = w.codes, w.scales

@@ -269,7 +269,7 @@ def test_refusals():
            lambda: rotary.rotate(x, rotary.Axes(p, (8, 8), theta=math.inf)), lambda: rotary.rotate(x, rotary.Axes(p, (8, 8), theta=-1.0)),
            lambda: rotary.rotate(x, rotary.Axes(p, (4, 8), pairs='half')), lambda: rotary.rotate(x[:5], axes),
            lambda: rotary.rotate(x[..., :12], axes), lambda: rotary.rotate(x.double(), axes), lambda: rotary.rotate(q, axes),
-           lambda: rotary.rotate(x, (p, p)), lambda: rotary.rotate(x, rotary.Axes(p.cpu(), (8, 8))),
+           lambda: rotary.rotate(x, (p, p)), lambda: rotary.Axes(p.float().requires_grad_(), (8, 8)), lambda: rotary.rotate(x, rotary.Axes(p.cpu(), (8, 8))),
            lambda: rotary.norm_rotate(q, q, w, w, EPS, axes, 3), lambda: rotary.norm_rotate(q, q[:, :16], w, w, EPS, axes, 2),
            lambda: rotary.norm_rotate(q, q, w[:16], w, EPS, axes, 2), lambda: rotary.norm_rotate(q, q.float(), w, w, EPS, axes, 2),
            lambda: rotary.norm_rotate(q, q, w, w.cpu(), EPS, axes, 2), lambda: rotary.norm_rotate(q[:4], q[:4], w, w, EPS, axes, 2),
