@@ -57,7 +57,7 @@ __device__ __forceinline__ float2 angle_of(const Axes& x, int64_t row, int j, do
   int a = 0;
 #pragma unroll
   for (int i = 1; i < kMaxAxes; ++i) a = i < x.n_axes && j >= x.first[i] ? i : a;
-  const int64_t at = row % x.n_positions * x.n_axes + a;
+  const int64_t at = (row < x.n_positions ? row : row % x.n_positions) * x.n_axes + a;   // the division is for batches alone
   const double p = x.whole ? (double)((const int32_t*)x.position)[at] : (double)((const float*)x.position)[at];
   double turns = p * turn;
   turns -= rint(turns);
@@ -240,6 +240,8 @@ __global__ __launch_bounds__(1024) void norm_rope_axes_kernel(NormedArgs g) {
   }
 }
 
+// (One row at a time, its loads and angles under way ahead of the last one's sums and one barrier a row: 70.5 us, so 69.2, for q and k of
+// 12720 rows of 2048.)
 template <typename T, bool HALF>
 __global__ __launch_bounds__(1024) void norm_rope_axes_bwd_kernel(NormedArgs g) {
   __shared__ float2 angle[2][kRows][kMaxPairs];
