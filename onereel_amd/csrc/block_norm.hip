@@ -333,7 +333,8 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
   }
 }
 
-// a group's sums of 64 columns, its work-groups' dealt out to 16 wavefronts; then its parameters' gradients, or their terms
+// a group's sums of 64 columns, its work-groups' dealt out to 16 wavefronts; then its parameters' gradients, or their terms. (16
+// columns a work-group and four times as many of them: 7.2 us, so 5.1, for 8 groups of 64 work-groups and 2048 columns.)
 constexpr int kSumWaves = 16;
 __global__ __launch_bounds__(64 * kSumWaves) void block_norm_sums_kernel(NormBwdArgs g) {
   __shared__ float sum[3][kSumWaves][64];

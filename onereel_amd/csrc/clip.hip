@@ -10,6 +10,10 @@
 // A launch takes the addresses and lengths of up to kTensors tensors as its arguments, so nothing is copied to the device ahead
 // of it. Its work-groups deal out the tensors' elements evenly, whatever their sizes: pieces of kPiece elements, a tensor's last
 // one shorter, numbered through all tensors of the launch; a work-group takes consecutive pieces.
+//
+// 1.13e9 bf16 elements in 810 tensors, clipped into others: 1352 us for three passes over 2.27 GB (5.0 TB/s, the
+// rate of a copy of 1 GB here 5.15 to 5.5). 240 fp32 tensors of up to 40000 elements, in two launches of each kernel: 88 us, which is
+// the host's checks and addresses; 6.8, 5.4, 4.1 and 4.6 us on the GPU.
 #include <math.h>
 
 #include <algorithm>

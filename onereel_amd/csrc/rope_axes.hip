@@ -18,6 +18,9 @@
 //
 // HBM-bound: rows are read once and written once. The cosines and sines of a batch of tokens go through LDS, one of a token's
 // pairs a thread, since the heads share them; in the normed form they are ready at the barrier that the rows' sums need anyway.
+// 12720 tokens of 16 heads of 128 in bf16, q and k, among other work: normed 39.7 us for 208 MB (5.2 TB/s, the rate of a copy of 1 GB
+// here 5.15 to 5.5), its gradient 67.7 us for 313 MB (63 in the first launch, 5.0 TB/s, and 5 in the sum of dw). A call for few
+// tokens is the launch: 5.2 us on the GPU for 333 tokens of 5 heads of 96 in fp32, 12.6 with the host.
 #include <math.h>
 
 #include <algorithm>
@@ -183,7 +186,8 @@ __device__ __forceinline__ float sum_shares(const float* s, int waves) {
   return v;
 }
 
-// blockIdx.y picks q or k. A thread has one unit of every row; the work-group takes kRows rows at a time.
+// blockIdx.y picks q or k. A thread has one unit of every row; the work-group takes kRows rows at a time, so that their loads are under
+// way together.
 template <typename T, bool HALF>
 __global__ __launch_bounds__(1024) void norm_rope_axes_kernel(NormedArgs g) {
   __shared__ float2 angle[2][kRows][kMaxPairs];
