@@ -255,10 +255,11 @@ class Block:
             [self.norm2_w, self.norm2_b, self.scale_shift_table]
 
 
-def timestep_features(t: float, n: int, device) -> torch.Tensor:
-    """sinusoidal features of timestep t: [cos(t f_i), sin(t f_i)] with f_i = 10000^(-i / (n / 2))"""
+def timestep_features(t, n: int, device) -> torch.Tensor:
+    """sinusoidal features of timestep t, or of each of t [frames, 1]: [cos(t f_i), sin(t f_i)] with f_i = 10000^(-i / (n / 2))"""
     f = torch.exp(-math.log(10000.0) * torch.arange(n // 2, device=device, dtype=torch.float32) / (n // 2))
-    return torch.cat([torch.cos(t * f), torch.sin(t * f)])
+    t = t if isinstance(t, torch.Tensor) else float(t)
+    return torch.cat([torch.cos(t * f), torch.sin(t * f)], -1)
 
 
 class WanDiT:
@@ -282,28 +283,30 @@ class WanDiT:
     def quantize(self):
         """The blocks' projections and feed forwards in 4 bits (MXFP4) for `forward` from here on, from the present weights; the
         embeddings and the output projection stay in bf16. `differentiable_forward` keeps the bf16 weights."""
-        for l in (l for b in self.blocks for l in b.linears()):
-            l.quantized = mxfp4.quantize(l.weight)
+        layers = [l for b in self.blocks for l in b.linears()]
+        for l, q in zip(layers, [mxfp4.quantize(l.weight) for l in layers]):      # all of them, or none where one raises
+            l.quantized = q
         return self
 
     def clip_gradients(self, max_norm: float):
         """the gradients of `parameters()` scaled to a norm of at most max_norm (clip.clip_grad_norm_): their norm before that"""
         return clip.clip_grad_norm_(self.parameters(), max_norm)
 
-    def _per_frame(self, t):
-        """the timesteps of the latent frames, or None where t is one for all"""
-        if isinstance(t, (int, float)) or isinstance(t, torch.Tensor) and t.dim() == 0:
+    def _per_frame(self, t, device):
+        """the timesteps of the latent frames [frames, 1] fp32, or None where t is one for all: a number, or a tensor or array of
+        one element"""
+        if not isinstance(t, (list, tuple)) and math.prod(getattr(t, 'shape', ())) == 1:
             return None
-        t = [float(x) for x in t]
-        if len(t) != self.ctx.layout.n_frames:
-            raise L.HipValueError(f'{len(t)} timesteps for {self.ctx.layout.n_frames} latent frames')
-        return t
+        t = torch.as_tensor(t, dtype=torch.float32, device=device)
+        if t.shape != (self.ctx.layout.n_frames,):
+            raise L.HipValueError(f'timesteps of shape {tuple(t.shape)} for {self.ctx.layout.n_frames} latent frames')
+        return t[:, None]
 
     def forward(self, tokens, t, text, rotary):
         """tokens [S, in_channels * patch] bf16 (the patchified latent, frame-major), t the timestep, or one for each latent frame,
         text [n_scenes * text_len, text_dim] bf16 (sentence j in rows j * text_len ..), rotary (cos, sin) [1, S, 1, D] fp32 or a
         rotary.Axes -> [S, in * patch]"""
-        frames = self._per_frame(t)
+        frames = self._per_frame(t, tokens.device)
         if frames is not None:
             return self._forward_frames(tokens, frames, text, rotary)
         d = self.cfg.dim
@@ -327,7 +330,7 @@ class WanDiT:
         """forward, or with apply differentiable_forward, with a timestep for each latent frame"""
         d, eps, run = self.cfg.dim, self.cfg.eps, apply or (lambda layer, x: layer(x))
         x = run(self.patch_embed, tokens)[None]
-        features = torch.stack([timestep_features(t, self.cfg.freq_dim, tokens.device) for t in frames]).to(torch.bfloat16)
+        features = timestep_features(frames, self.cfg.freq_dim, tokens.device).to(torch.bfloat16)
         temb = run(self.time_out, F.silu(run(self.time_in, features)))
         temb6 = run(self.time_proj, F.silu(temb)).view(-1, 6, d).transpose(0, 1).float().contiguous()
         ctx_text = run(self.text_out, F.gelu(run(self.text_in, text), approximate='tanh'))[None]
@@ -344,7 +347,7 @@ class WanDiT:
         """forward with gradients of tokens, text and `parameters()` (those of them that require one)"""
         if self.ctx.memory or any(self.ctx.layout.extra.get(j) for j in range(self.ctx.layout.n_scenes)):
             raise L.HipValueError('the frame-memory scopes and the bounded memory have no gradient: train with halo scopes')
-        frames = self._per_frame(t)
+        frames = self._per_frame(t, tokens.device)
         if frames is not None:
             return self._forward_frames(tokens, frames, text, rotary, _apply)
         d, eps = self.cfg.dim, self.cfg.eps

@@ -6,6 +6,7 @@ sqrt(44) 2^-8 = 2.6e-2. A bias's gradient may be off by as much of |sum| + sqrt(
 rows in general (the modulation's tables)."""
 import math
 
+import numpy as np
 import pytest
 import torch
 import torch.nn.functional as F
@@ -205,3 +206,31 @@ def test_norm_rotate_in_the_processor_shares_scenes_positions():
     a = m.forward(tokens, 20.0, text, table)
     b = m.forward(tokens, 20.0, text, rotary.Axes(within, axes.dims))
     assert relative(b, a) <= BOUND and not torch.equal(m.forward(tokens, 20.0, text, tables()), a)
+
+
+def test_what_one_timestep_may_come_as():
+    """numbers of any kind and tensors or arrays of one element are one timestep for all; a tensor on the GPU is one for each frame
+    without the host reading it, so that such a pass can be captured"""
+    print('dit operators: kinds of timesteps', flush=True)
+    m = model()
+    tokens, text, axes, _ = inputs()
+    with torch.no_grad():
+        want = m.forward(tokens, 300.0, text, axes)
+        for t in (300, np.float32(300), np.int64(300), np.array(300.0), torch.tensor(300.0, device=DEV), torch.tensor([300.0], device=DEV)):
+            assert torch.equal(m.forward(tokens, t, text, axes), want)
+        want = m.forward(tokens, STEPS, text, axes)
+        steps = torch.tensor(STEPS, device=DEV)
+        for t in (tuple(STEPS), np.array(STEPS), torch.tensor(STEPS), steps):
+            assert torch.equal(m.forward(tokens, t, text, axes), want)
+        for t in (steps[:3], steps[None], steps.repeat(2), []):
+            with pytest.raises(ValueError, match='timesteps'):
+                m.forward(tokens, t, text, axes)
+
+
+def test_a_model_is_quantised_whole_or_not_at_all():
+    """a feed forward of 1032 columns does not divide into blocks of 32: no layer is left in 4 bits"""
+    cfg = WD.DiTConfig(dim=512, heads=4, ffn=1032, blocks=1, in_channels=4, text_dim=256, std=0.05)
+    m = WD.WanDiT(cfg, SceneLayout(LENGTHS, halo=HALO), T, TEXT_LEN, DEV, seed=3)
+    with pytest.raises(ValueError, match='multiple of 32'):
+        m.quantize()
+    assert all(l.quantized is None for b in m.blocks for l in b.linears())
