@@ -243,20 +243,22 @@ __global__ __launch_bounds__(64 * kRowWaves) void mx_rows_kernel(MxArgs g) {
   }
 }
 
-// The tiles' scales. A step of SB bytes of a row has SB / 16 blocks, SB / 32 of them for the lanes of each half h of a wavefront
-// (lanes 32 h ..), which multiply blocks h, 2 + h, .. of their rows, 32 apart. So the scales of 128 rows lie as
-// [step][row % 32][h][row / 32 % 4][SB / 32]: a step's lie together, and a lane reads those of 4 (or 2) of its rows at once. Blocks
-// past the end of a row get the scale 0: what their place holds in LDS are zeros, but not every scale keeps a zero a zero.
+// The tiles' scales. A step of kSB bytes of a row has 8 blocks, 4 of them for the lanes of each half h of a wavefront (lanes 32 h ..),
+// which multiply blocks h, 2 + h, .. of their rows, 32 apart. So the scales of 128 rows lie as [step][row % 32][h][row / 32 % 4][4]:
+// a step's lie together, and a lane reads those of 4 (or 2, or 1) of its rows at once. Blocks past the end of a row get the scale 0:
+// what their place holds in LDS are zeros, but not every scale keeps a zero a zero.
 constexpr int kScaleRows = 128;
+constexpr int kSB = 128, kStepElements = 2 * kSB, kStepBlocks = kSB / 16;
+constexpr int KS = kSB / 32;           // of them, those of one half of the lanes: products of 64 elements in a step
 
-// One operand's tile of N rows x SB bytes in LDS, chunk c (16 bytes, a block) of row r at position c ^ swz(r). A load of the
+// One operand's tile of N rows x kSB bytes in LDS, chunk c (16 bytes, a block) of row r at position c ^ swz(r). A load of the
 // work-group takes ROWS rows; a lane's place among them is the same in each.
-template <int N, int THREADS, int SB>
+template <int N, int THREADS>
 struct MxTile {
-  static constexpr int CH = SB / 16, BYTES = N * SB, ROWS = THREADS / CH, LOADS = N / ROWS;
-  static constexpr int SCALES = (N > kScaleRows ? N : kScaleRows) * CH;   // whole groups of rows
+  static constexpr int BYTES = N * kSB, ROWS = THREADS / kStepBlocks, LOADS = N / ROWS;
+  static constexpr int SCALES = (N > kScaleRows ? N : kScaleRows) * kStepBlocks;   // whole groups of rows
   static constexpr int SCALE_LOADS = (SCALES + 4 * THREADS - 1) / (4 * THREADS);
-  static __device__ __forceinline__ int swz(int r) { return SB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+  static __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
   static_assert(LOADS >= 1 && N % ROWS == 0 && ROWS % 16 == 0, "tile");   // 16 rows: the swizzle's period
   const uint8_t *p, *s;
   int rows, left, wide;                // rows that end the tile; bytes of k left, and of this step
@@ -265,19 +267,19 @@ struct MxTile {
   __device__ __forceinline__ void start(const uint8_t* codes, const uint8_t* scales, int64_t scale_rows, uint32_t stride, int64_t n0,
                                         int64_t n, int step0, int end) {
     row_bytes = stride;
-    p = codes + n0 * stride + (int64_t)step0 * SB;
-    s = scales + ((int64_t)step0 * scale_rows + n0 / kScaleRows * kScaleRows) * CH;
-    scale_pitch = scale_rows * CH;
+    p = codes + n0 * stride + (int64_t)step0 * kSB;
+    s = scales + ((int64_t)step0 * scale_rows + n0 / kScaleRows * kScaleRows) * kStepBlocks;
+    scale_pitch = scale_rows * kStepBlocks;
     rows = (int)min(n - n0, (int64_t)N);
-    left = end - step0 * SB;
+    left = end - step0 * kSB;
     wide = 0;
   }
   // the step to load from now on
-  __device__ __forceinline__ void step() { wide = min(max(left, 0), SB); }
+  __device__ __forceinline__ void step() { wide = min(max(left, 0), kSB); }
   __device__ __forceinline__ void next() {
-    p += SB;
+    p += kSB;
     s += scale_pitch;
-    left -= SB;
+    left -= kSB;
   }
   __device__ __forceinline__ i32x4 codes(int i) const {
     const int n = rows - i * ROWS;
@@ -293,11 +295,11 @@ __device__ __forceinline__ void dma4(const i32x4& r, uint32_t off, uint32_t m0) 
                : "memory");
 }
 
-template <int TI, int TJ, int WI, int WJ, int NB, int SB>
+template <int TI, int TJ, int WI, int WJ, int NB>
 struct MxShape {
   static constexpr int THREADS = 64 * WI * WJ;
-  using TA = MxTile<TI, THREADS, SB>;
-  using TB = MxTile<TJ, THREADS, SB>;
+  using TA = MxTile<TI, THREADS>;
+  using TB = MxTile<TJ, THREADS>;
   static constexpr int FI = TI / WI / 32, FJ = TJ / WJ / 32;
   static constexpr int SCALE_A = 4 * THREADS * TA::SCALE_LOADS, SCALE_B = 4 * THREADS * TB::SCALE_LOADS;   // bytes that their loads write
   static constexpr int BUF = TA::BYTES + TB::BYTES + SCALE_A + SCALE_B;
@@ -365,24 +367,22 @@ struct Finish {
 
 // The structure of the bf16 product (linear.hip): a ring of NB buffers filled by LDS DMA, one barrier a step, two sets of
 // fragments, one read while the other is multiplied. A lane's 16 bytes of a row are one block, its scale a byte of a register.
-// A work-group takes one tile after the other, as if their steps were one long row of them: the first steps of the next tile are
-// loaded while the last ones of this one are multiplied and while its results are written.
-template <int TI, int TJ, int WI, int WJ, int NB, int SB>
+template <int TI, int TJ, int WI, int WJ, int NB>
 __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(1, 2))) void mx_tile_kernel(MxArgs g) {
-  using S = MxShape<TI, TJ, WI, WJ, NB, SB>;
+  using S = MxShape<TI, TJ, WI, WJ, NB>;
   using TA = typename S::TA;
   using TB = typename S::TB;
-  constexpr int FI = S::FI, FJ = S::FJ, HK = SB / 64, KS = SB / 32;
+  constexpr int FI = S::FI, FJ = S::FJ, HK = KS / 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[S::LDS];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wi = w / WJ, wj = w % WJ, l32 = lane & 31, h = lane >> 5;
-  const int row_bytes = g.K / 2, steps = (row_bytes + SB - 1) / SB;
+  const int row_bytes = g.K / 2, steps = (row_bytes + kSB - 1) / kSB;
 
   Place work;
   if (!place_of(g, blockIdx.x, steps, work)) return;
   TA la;
   TB lb;
-  const int end = min(work.last * SB, row_bytes);
+  const int end = min(work.last * kSB, row_bytes);
   la.start(g.a, g.a_scales, g.a_rows, row_bytes, (int64_t)work.ti * TI, g.I, work.first, end);
   lb.start(g.b, g.b_scales, g.b_rows, row_bytes, (int64_t)work.tj * TJ, g.J, work.first, end);
   auto next_step = [&] {
@@ -391,16 +391,16 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(1,
   };
 
   const uint32_t base = lds_addr(lds), m0 = base + w * 1024, m0s = base + TA::BYTES + TB::BYTES + w * 256;
-  const int chunk = (tid % TA::CH) ^ TA::swz(tid / TA::CH);
-  const uint32_t off = (uint32_t)(tid / TA::CH) * (uint32_t)row_bytes + chunk * 16;
+  const int chunk = (tid % kStepBlocks) ^ TA::swz(tid / kStepBlocks);
+  const uint32_t off = (uint32_t)(tid / kStepBlocks) * (uint32_t)row_bytes + chunk * 16;
   // addresses of the fragments of a buffer: one a step of 64 elements, the blocks of 32 rows are immediates from it
   const int swz = TA::swz(l32);
   uint32_t at[KS];
 #pragma unroll
-  for (int k = 0; k < KS; ++k) at[k] = l32 * SB + ((2 * k + h) ^ swz) * 16;
-  const uint32_t at_a = base + wi * (TI / WI) * SB, at_b = base + TA::BYTES + wj * (TJ / WJ) * SB;
+  for (int k = 0; k < KS; ++k) at[k] = l32 * kSB + ((2 * k + h) ^ swz) * 16;
+  const uint32_t at_a = base + wi * (TI / WI) * kSB, at_b = base + TA::BYTES + wj * (TJ / WJ) * kSB;
   // a wavefront's rows from `row` on in their group of 128
-  auto scale_at = [&](int row) { return (row / kScaleRows) * kScaleRows * TA::CH + (l32 * 2 + h) * 4 * KS + row % kScaleRows / 32 * KS; };
+  auto scale_at = [&](int row) { return (row / kScaleRows) * kScaleRows * kStepBlocks + (l32 * 2 + h) * 4 * KS + row % kScaleRows / 32 * KS; };
   const uint32_t at_sa = base + TA::BYTES + TB::BYTES + scale_at(wi * (TI / WI) + (work.ti * (TI % kScaleRows)) % kScaleRows);
   const uint32_t at_sb = base + TA::BYTES + TB::BYTES + S::SCALE_A + scale_at(wj * (TJ / WJ) + (work.tj * (TJ % kScaleRows)) % kScaleRows);
 
@@ -446,8 +446,8 @@ __global__ __launch_bounds__(64 * WI * WJ) __attribute__((amdgpu_waves_per_eu(1,
   };
   auto read = [&](int x, auto s_) {    // fragment x of set s
     constexpr int s = decltype(s_)::value;
-    if (x < HK * FJ) b[s][x / FJ][x % FJ] = *(lds_u32x4*)(uintptr_t)(pb[x / FJ] + x % FJ * 32 * SB);
-    else a[s][(x - HK * FJ) / FI][(x - HK * FJ) % FI] = *(lds_u32x4*)(uintptr_t)(pa[(x - HK * FJ) / FI] + (x - HK * FJ) % FI * 32 * SB);
+    if (x < HK * FJ) b[s][x / FJ][x % FJ] = *(lds_u32x4*)(uintptr_t)(pb[x / FJ] + x % FJ * 32 * kSB);
+    else a[s][(x - HK * FJ) / FI][(x - HK * FJ) % FI] = *(lds_u32x4*)(uintptr_t)(pa[(x - HK * FJ) / FI] + (x - HK * FJ) % FI * 32 * kSB);
   };
   // KS bytes of each block of 32 rows, packed
   constexpr int WA = FI * KS / 4, WB = FJ * KS / 4;
@@ -600,24 +600,11 @@ struct PrepareArgs {
 
 // One unit is 32 rows (8 neighbouring ones of each 32 of 128) x 256 elements: rows r0 + l + 32 f, whose scales lie together in each
 // step. They are collected in LDS in that order.
-template <int SB>
-struct ScaleUnit {
-  static constexpr int KS = SB / 32, STEPS = 128 / SB, BYTES = 8 * 2 * 4 * KS;   // bytes of a step
-  static __device__ __forceinline__ int place(int l, int f, int block) {        // block 0 .. 7 of the 256 elements
-    const int step = block / (2 * KS), in = block % (2 * KS);
-    return step * BYTES + ((l * 2 + (in & 1)) * 4 + f) * KS + (in >> 1);
-  }
-  static __device__ __forceinline__ void write(const uint8_t* st, uint8_t* to, int64_t rows, int64_t r0, int step, int tid) {
-    if (tid >= STEPS * BYTES / 4) return;
-    const int s = tid / (BYTES / 4), i = tid % (BYTES / 4);
-    ((uint32_t*)(to + (((int64_t)step * STEPS + s) * rows + r0 / kScaleRows * kScaleRows) * 2 * KS + r0 % kScaleRows * 8 * KS))[i] = ((const uint32_t*)st)[tid];
-  }
-};
+constexpr int kUnitBytes = 8 * 2 * 4 * KS;
+__device__ __forceinline__ int unit_place(int l, int f, int block) { return ((l * 2 + (block & 1)) * 4 + f) * KS + (block >> 1); }
 
-template <int SB>
 __global__ __launch_bounds__(kThreads) void mx_prepare_kernel(PrepareArgs g) {
-  using U = ScaleUnit<SB>;
-  __shared__ __attribute__((aligned(16))) uint8_t st[256];
+  __shared__ __attribute__((aligned(16))) uint8_t st[kUnitBytes];
   const bool weights = (int)blockIdx.x >= g.a_blocks;
   const int64_t rows = weights ? g.n_out : g.q.rows, all = weights ? g.b_rows : g.a_rows;
   const int blocks = g.q.K / kBlock, tid = threadIdx.x, work_groups = weights ? (int)gridDim.x - g.a_blocks : g.a_blocks;
@@ -629,7 +616,7 @@ __global__ __launch_bounds__(kThreads) void mx_prepare_kernel(PrepareArgs g) {
       const uint8_t* from = weights ? g.w_scales : g.q.scales;
       const int f = tid >> 6, l = tid >> 3 & 7, k = tid & 7, block = 8 * step + k;
       const int64_t row = r0 + l + 32 * f;
-      st[U::place(l, f, k)] = row < rows && block < blocks ? from[row * blocks + block] : 0;
+      st[unit_place(l, f, k)] = row < rows && block < blocks ? from[row * blocks + block] : 0;
     } else {
       const int l = tid >> 5, c = tid & 31, at = 256 * step + 8 * c;
       const bool in = at < g.q.K;        // all four lanes of a block, or none
@@ -646,11 +633,12 @@ __global__ __launch_bounds__(kThreads) void mx_prepare_kernel(PrepareArgs g) {
         uint32_t codes, scale;
         quantize8(p[f], codes, scale);
         if (in && row < rows) ((uint32_t*)g.q.codes)[row * (g.q.K / 8) + at / 8] = codes;
-        if ((c & 3) == 0) st[U::place(l, f, c >> 2)] = in && row < rows ? (uint8_t)scale : 0;
+        if ((c & 3) == 0) st[unit_place(l, f, c >> 2)] = in && row < rows ? (uint8_t)scale : 0;
       }
     }
     __syncthreads();
-    U::write(st, weights ? g.b_scales : g.a_scales, all, r0, step, tid);
+    uint8_t* to = (weights ? g.b_scales : g.a_scales) + (step * all + r0 / kScaleRows * kScaleRows) * kStepBlocks + r0 % kScaleRows * 8 * KS;
+    if (tid < kUnitBytes / 4) ((uint32_t*)to)[tid] = ((const uint32_t*)st)[tid];
     __syncthreads();
   }
 }
@@ -692,8 +680,6 @@ struct Plan {
   int tiles_i, tiles_j, split;
 };
 
-constexpr int kSB = 128;               // bytes of a step: 256 elements
-constexpr int kStepElements = 2 * kSB;
 constexpr int kTileRows = 256;         // the scales' layouts come in whole tiles of any size
 
 // The tile and the parts of k that a product takes least time with, by what a step of 256 k was measured to take a round of
@@ -756,8 +742,8 @@ Layout layout_of(const Plan& p, int64_t M, int64_t N, int64_t K, bool quantized)
     l.a_rows = (M + kTileRows - 1) / kTileRows * kTileRows;
     l.b_rows = (N + kTileRows - 1) / kTileRows * kTileRows;
     if (!quantized) l.codes = take(M * (K / 2));
-    l.a_scales = take(l.a_rows * l.steps * (kSB / 16));
-    l.b_scales = take(l.b_rows * l.steps * (kSB / 16));
+    l.a_scales = take(l.a_rows * l.steps * kStepBlocks);
+    l.b_scales = take(l.b_rows * l.steps * kStepBlocks);
     if (p.split > 1) l.part = take((int64_t)p.split * M * N * 4);
   }
   l.bytes = at;
@@ -766,7 +752,7 @@ Layout layout_of(const Plan& p, int64_t M, int64_t N, int64_t K, bool quantized)
 
 template <int TI, int TJ, int WI, int WJ, int NB>
 void launch_tiles(const MxArgs& g, unsigned blocks, hipStream_t st) {
-  hipLaunchKernelGGL((mx_tile_kernel<TI, TJ, WI, WJ, NB, kSB>), dim3(blocks), dim3(64 * WI * WJ), 0, st, g);
+  hipLaunchKernelGGL((mx_tile_kernel<TI, TJ, WI, WJ, NB>), dim3(blocks), dim3(64 * WI * WJ), 0, st, g);
 }
 
 }  // namespace
@@ -864,7 +850,7 @@ extern "C" int or_mx_linear(const or_mx_linear_args* p, void* stream) {
   const int64_t a_units = l.a_rows / 32 * r.steps, w_units = l.b_rows / 32 * r.steps;
   r.a_blocks = (int)std::min<int64_t>(a_units, kMaxBlocks);
   const unsigned w_blocks = (unsigned)std::min<int64_t>(w_units, kMaxBlocks);
-  hipLaunchKernelGGL(mx_prepare_kernel<kSB>, dim3(r.a_blocks + w_blocks), dim3(kThreads), 0, st, r);
+  hipLaunchKernelGGL(mx_prepare_kernel, dim3(r.a_blocks + w_blocks), dim3(kThreads), 0, st, r);
   g.a_scales = r.a_scales;
   g.b_scales = r.b_scales;
   g.a_rows = l.a_rows;
