@@ -1,5 +1,6 @@
 /*
- * onereel_dit.h: C ABI of libonereel_dit.so, the linear layers and fused elementwise kernels of the Wan-shaped DiT block
+ * onereel_dit.h: C ABI of libonereel_dit.so, the linear layers (bf16 and 4-bit), norms and fused elementwise kernels of the
+ * Wan-shaped DiT block, and the clipping of its gradients
  * (onereel_amd/wan_dit.py): a random-init model that runs the scene-attention processors end to end so that a
  * denoising step's time can be measured. These kernels are not on the scene-attention path (libonereel_hip.so,
  * include/onereel_hip.h); the library links against libonereel_hip.so and reports errors through its or_last_error.
