@@ -13,6 +13,7 @@ import operator
 import torch
 
 from . import _lib as L
+from .scene import without_gradient
 
 
 _T = torch.Tensor
@@ -36,14 +37,17 @@ def _addresses(tensors, what: str, at: int):
     None for any)"""
     # one C call for each tensor and question: a model has hundreds of them, and their launches take less than a loop over them
     dtypes, devices = list(map(_DTYPE, tensors)), set(map(_DEVICE, tensors))
-    if not L.TYPES.keys() >= set(dtypes) or devices and min(devices) < 0:
+    distinct = set(dtypes)
+    if not L.TYPES.keys() >= distinct or devices and min(devices) < 0:
         t = next(t for t in tensors if t.dtype not in L.TYPES or t.get_device() < 0)
         raise L.HipTypeError(f'{what} must be bf16, fp16 or fp32 GPU tensors, got {t.dtype} on {t.device}')
     if at is not None:
         devices.add(at)
     if len(devices) > 1:
         raise L.HipTypeError('all tensors of a call must be on one GPU')
-    kinds = array.array('i', map(L.TYPES.__getitem__, dtypes))
+    kinds = array.array('i', map(L.TYPES.__getitem__, distinct if len(distinct) == 1 else dtypes))
+    if len(distinct) == 1:
+        kinds *= len(tensors)
     return (array.array('Q', map(_ADDRESS, tensors)), array.array('q', map(_NUMEL, tensors)), kinds), \
         devices.pop() if devices else None
 
@@ -69,12 +73,13 @@ def _zero():
 
 
 def grad_norm(tensors):
-    """The 2-norm of all elements of the tensors (an iterable; 0 without any), an fp32 scalar on their GPU"""
-    tensors = list(tensors)
+    """The 2-norm of all elements of the tensors (an iterable; 0 without any), an fp32 scalar on their GPU. It has no gradient: where
+    autograd records and one of them requires a gradient, a backward pass that reaches it raises."""
+    given = tensors = list(tensors)
     if not all(map(_T.is_contiguous, tensors)):
         tensors = [t if _dense(t) else t.detach().contiguous() for t in tensors]
     sources, at = _addresses(tensors, 'tensors', None)
-    return _zero() if at is None else _call(sources, None, at)
+    return _zero() if at is None else without_gradient('clip.grad_norm', _call(sources, None, at), *given)
 
 
 def clip_grads_(tensors, max_norm: float, out=None):

@@ -205,3 +205,15 @@ def test_graph_replays_and_streams():
             clip.clip_grads_(mine, 100.0)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for mine in sets for a, b in zip(mine, keep))
+
+
+def test_a_norm_that_autograd_would_record_has_no_gradient():
+    w = torch.randn(40, device=DEV, requires_grad=True)
+    norm = clip.grad_norm([w, torch.ones(3, device=DEV)])
+    want = torch.cat([w.detach().double(), torch.ones(3, device=DEV, dtype=torch.float64)]).norm()
+    assert abs(norm.item() - want.item()) <= 1e-6 * want.item()
+    with pytest.raises(L.HipValueError, match='clip.grad_norm'):
+        (norm + w.sum()).backward()
+    with torch.no_grad():
+        assert not clip.grad_norm([w]).requires_grad
+    assert not clip.grad_norm([w.detach()]).requires_grad
