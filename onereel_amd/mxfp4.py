@@ -38,11 +38,8 @@ class MXFP4:
                                   f'{tuple(codes.shape)} and {tuple(scales.shape)}')
         codes = codes.contiguous()
         self.codes, self.scales = codes if codes.data_ptr() % 16 == 0 else codes.clone(), scales.contiguous()
+        self.shape = torch.Size((*codes.shape[:-1], n))
         self._of = None      # what was quantised, where autograd recorded that
-
-    @property
-    def shape(self):
-        return torch.Size((*self.codes.shape[:-1], 2 * self.codes.shape[-1]))
 
     @property
     def device(self):
@@ -98,14 +95,15 @@ def linear(x, weight: MXFP4, bias=None, activation=None, gate=None, residual=Non
     if not isinstance(weight, MXFP4):
         raise L.HipTypeError(f'weight must be an MXFP4, got {type(weight).__name__}')
     ready = isinstance(x, MXFP4)
-    if len(weight.shape) != 2 or not len(x.shape) or x.shape[-1] != weight.shape[1]:
-        raise L.HipValueError(f'x {tuple(x.shape)} does not fit a weight of {tuple(weight.shape)}')
-    n_out, n_in = weight.shape
+    rows, of = x.shape, weight.shape
+    if len(of) != 2 or not rows or rows[-1] != of[1]:
+        raise L.HipValueError(f'x {tuple(rows)} does not fit a weight of {tuple(of)}')
+    n_out, n_in = of
     if n_out < 8 or n_out % 8:
         raise L.HipValueError(f'n_out must be a multiple of 8, got {n_out}')
     first = x.codes if ready else x
     _on_one_gpu(first, weight.codes, bias, gate, residual)
-    shape = (*x.shape[:-1], n_out)
+    shape = (*rows[:-1], n_out)
     if residual is not None and tuple(residual.shape) != shape:
         raise L.HipValueError(f'the residual must be {shape}, got {tuple(residual.shape)}')
     x2, xs = (None, 0) if ready else _rows(x, n_in, 'x')

@@ -43,7 +43,11 @@ class _WithoutGradient(torch.autograd.Function):
 
 
 def _recorded(inputs) -> bool:
-    return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs)
+    if torch.is_grad_enabled():
+        for x in inputs:
+            if x is not None and x.requires_grad:
+                return True
+    return False
 
 
 def without_gradient(what: str, out, *inputs):
