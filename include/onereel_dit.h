@@ -115,7 +115,7 @@ typedef struct or_block_norm_bwd_args {
 int64_t or_block_norm_bwd_workspace_size(int64_t n_rows, int64_t rows_per_group, int32_t C);
 
 /* The gradient of or_block_norm. Sums are fp32 in a fixed order; dx and da are rounded once. With 0 rows nothing is written.
- * One launch, two with sums over rows, three with weights' gradients over several groups. */
+ * One launch; with sums over rows up to three. The parameters' gradients lie at 16-byte aligned addresses. */
 int or_block_norm_bwd(const or_block_norm_bwd_args* args, void* stream);
 
 /* activations of or_linear */

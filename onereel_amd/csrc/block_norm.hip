@@ -17,9 +17,10 @@
 //
 // HBM-bound: x and a are read and h and n written once, h, a, dh and dn are read and dx and da written once. A work-group takes
 // rows of one group, each of its threads 8 columns of them, so that the parameters stay in registers, folded into two or three
-// vectors; a row's sums go over lanes within a wavefront, then through LDS: one barrier for a batch of rows, since each wavefront
+// vectors; a row's sums go over lanes within a wavefront, then through LDS: one barrier a row, since each wavefront
 // hands on its own mean and the squares around that, which are joined without cancellation. In the gradient a thread adds up its
-// columns' A, B and D over its work-group's rows, in a fixed order; a second launch joins the work-groups' sums. 12720 x 2048 in bf16
+// columns' A, B and D over its work-group's rows, in a fixed order; a second launch joins the work-groups' sums, unless there are so
+// many groups that each is one work-group's, which then makes the group's gradients by itself. 12720 x 2048 in bf16
 // with gate, scale and shift of 8 groups, among other work: forward 41.2 us for 208 MB (5.1 TB/s, the rate of a copy of 1 GB here
 // 5.15 to 5.5); gradient 71.3 us for 313 MB, 65 of them in the first launch (4.8 TB/s) and 5 in the column sums.
 #include <math.h>
@@ -191,19 +192,62 @@ struct NormBwdArgs {
   const float *gate, *post_weight, *weight, *bias, *scale;
   float *dgate, *dpost_weight, *dweight, *dbias, *dscale, *dshift;   // each optional
   float* part;                         // [groups * parts][3][C]: A, B, D
-  float* group_part;                   // [groups][3][C]: the groups' terms of dweight, dbias, dpost_weight
+  float* terms;                        // [n_terms][3][C] of dweight, dbias, dpost_weight: of a group, or (alone) of a work-group
+  int64_t n_terms;
   int64_t per, groups, dh_stride, dn_stride, h_stride, a_stride;
   int C, parts, norm, post;
+  unsigned blocks;
+  bool alone;
   float eps, r;
 };
 
-template <typename T, int KIND, int N>
+__device__ __forceinline__ void put8(float* p, const float (&v)[8]) {
+  *(f32x4*)p = f32x4{v[0], v[1], v[2], v[3]};
+  *(f32x4*)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+}
+
+// The gradients of a group's own 8 columns from their sums, and their terms of the weights' gradients, added up in LDS
+__device__ __forceinline__ void alone8(const NormBwdArgs& g, int64_t at, int col, const float (&A)[8], const float (&B)[8],
+                                       const float (&D)[8], float* term) {
+  float x[8], y[8];
+  if (g.dshift) put8(g.dshift + at, B);
+  if (g.dscale) {
+    param8(g.weight, col, true, 1.0f, x);
+    param8(g.bias, col, true, 0.0f, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * A[i] + y[i] * B[i];
+    put8(g.dscale + at, x);
+  }
+  if (g.dgate) {
+    param8(g.post_weight, col, true, 1.0f, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= D[i];
+    put8(g.dgate + at, x);
+  }
+  if (!g.terms) return;
+  param8(g.scale, at, true, 0.0f, x);
+  param8(g.gate, at, true, 1.0f, y);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    term[col + i] += (1.0f + x[i]) * A[i];
+    term[g.C + col + i] += (1.0f + x[i]) * B[i];
+    term[2 * g.C + col + i] += y[i] * D[i];
+  }
+}
+
+// ALONE: a group has one work-group, which makes its gradients by itself
+template <typename T, int KIND, int N, bool ALONE>
 __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
   __shared__ Share share[2][kMaxWaves], post_share[2][kMaxWaves];
   __shared__ float back[2][kMaxWaves][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, col = 8 * threadIdx.x, C = g.C;
   const bool in = col < C;
   const int columns = wave_columns(C, wave);
+  extern __shared__ __attribute__((aligned(16))) float term[];        // alone: [3][C], each thread's columns its own
+  if (ALONE && g.terms && in) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *(f32x4*)(term + i * C + col) = *(f32x4*)(term + i * C + col + 4) = f32x4{0, 0, 0, 0};
+  }
   int turn = 0;
   for (int64_t span = blockIdx.x; span < g.groups * g.parts; span += gridDim.x) {
     const Span s = span_of(span, g.parts, g.per);
@@ -322,7 +366,12 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
         for (int i = 0; i < 8; ++i) D[i] += d[i] * a[i];
       }
     }
-    if (!g.part || !in) continue;
+    if (!in) continue;
+    if constexpr (ALONE) {
+      alone8(g, at, col, A, B, D, term);
+      continue;
+    }
+    if (!g.part) continue;
     float* out = g.part + span * 3 * C + col;
 #pragma unroll
     for (int i = 0; i < 8; i += 4) {
@@ -331,31 +380,42 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
       *(f32x4*)(out + 2 * C + i) = f32x4{D[i], D[i + 1], D[i + 2], D[i + 3]};
     }
   }
+  if (!ALONE || !g.terms || !in) return;
+  float* out = g.terms + (int64_t)blockIdx.x * 3 * C + col;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    *(f32x4*)(out + i * C) = *(f32x4*)(term + i * C + col);
+    *(f32x4*)(out + i * C + 4) = *(f32x4*)(term + i * C + col + 4);
+  }
 }
 
-// a group's sums of 64 columns, its work-groups' dealt out to 16 wavefronts; then its parameters' gradients, or their terms. (16
+// The groups' sums of 64 columns, those of a group's work-groups dealt out to WAVES of 16 wavefronts: all of them, or 4 for up to 8
+// work-groups; then its parameters' gradients, or their terms. (16
 // columns a work-group and four times as many of them: 7.2 us, so 5.1, for 8 groups of 64 work-groups and 2048 columns.)
 constexpr int kSumWaves = 16;
+template <int WAVES>
 __global__ __launch_bounds__(64 * kSumWaves) void block_norm_sums_kernel(NormBwdArgs g) {
   __shared__ float sum[3][kSumWaves][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
-  for (int64_t group = blockIdx.y; group < g.groups; group += gridDim.y) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = wave / WAVES * WAVES, col = blockIdx.x * 64 + lane;
+  for (int64_t base = (int64_t)blockIdx.y * (kSumWaves / WAVES); base < g.groups; base += (int64_t)gridDim.y * (kSumWaves / WAVES)) {
+    const int64_t group = base + wave / WAVES;
+    const bool in = col < g.C && group < g.groups;
     float v[3] = {};
-    if (col < g.C) {
+    if (in) {
       const float* p = g.part + group * g.parts * 3 * g.C + col;
 #pragma unroll 8
-      for (int b = wave; b < g.parts; b += kSumWaves)
+      for (int b = wave - first; b < g.parts; b += WAVES)
 #pragma unroll
         for (int i = 0; i < 3; ++i) v[i] += p[((int64_t)b * 3 + i) * g.C];
     }
 #pragma unroll
     for (int i = 0; i < 3; ++i) sum[i][wave][lane] = v[i];
     __syncthreads();
-    if (wave == 0 && col < g.C) {
+    if (wave == first && in) {
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
         v[i] = 0.0f;
-        for (int w = 0; w < kSumWaves; ++w) v[i] += sum[i][w][lane];
+        for (int w = 0; w < WAVES; ++w) v[i] += sum[i][first + w][lane];
       }
       const int64_t at = group * g.C + col;
       const float w = g.weight ? g.weight[col] : 1.0f, b = g.bias ? g.bias[col] : 0.0f, e = g.scale ? 1.0f + g.scale[at] : 1.0f;
@@ -368,16 +428,16 @@ __global__ __launch_bounds__(64 * kSumWaves) void block_norm_sums_kernel(NormBwd
         if (g.dweight) g.dweight[col] = term[0];
         if (g.dbias) g.dbias[col] = term[1];
         if (g.dpost_weight) g.dpost_weight[col] = term[2];
-      } else if (g.group_part) {
+      } else if (g.terms) {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) g.group_part[(group * 3 + i) * g.C + col] = term[i];
+        for (int i = 0; i < 3; ++i) g.terms[(group * 3 + i) * g.C + col] = term[i];
       }
     }
     __syncthreads();
   }
 }
 
-// the sums over groups
+// the sums of the terms
 __global__ __launch_bounds__(64 * kSumWaves) void block_norm_weights_kernel(NormBwdArgs g) {
   __shared__ float sum[kSumWaves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane, which = blockIdx.y;
@@ -386,7 +446,7 @@ __global__ __launch_bounds__(64 * kSumWaves) void block_norm_weights_kernel(Norm
   float v = 0.0f;
   if (col < g.C) {
 #pragma unroll 8
-    for (int64_t b = wave; b < g.groups; b += kSumWaves) v += g.group_part[(b * 3 + which) * g.C + col];
+    for (int64_t b = wave; b < g.n_terms; b += kSumWaves) v += g.terms[(b * 3 + which) * g.C + col];
   }
   sum[wave][lane] = v;
   __syncthreads();
@@ -433,12 +493,26 @@ int bad_rows(const char* what, const void* p, int64_t stride, int C) {
 // GPU's loads in flight; and no thread adds up more than kMaxPartRows rows in a row.
 int64_t bwd_parts(int64_t per, int64_t groups) { return std::max(parts_of(per, groups, kBwdBlocks), (per + kMaxPartRows - 1) / kMaxPartRows); }
 
-int64_t part_bytes(int64_t rows, int64_t per, int C) {
-  const int64_t groups = rows / per;
-  return groups * bwd_parts(per, groups) * 3 * C * 4;
-}
-
 constexpr int64_t kMaxBlocks = 1 << 20;   // of up to 1024 threads: a grid has under 2^32 of them
+
+// Where the gradient's sums lie in the workspace: those of the work-groups, unless each group has but one, and the terms of the
+// weights' gradients. A group that is one work-group's has its gradients from there: 12720 x 2048 in 1590 groups 94 us, in as many as
+// rows 203 (467 and 3180 through the second launch); 1024 or 2048 work-groups instead of 512 93 and 235, 99 and 206.
+struct BwdPlan {
+  int64_t groups, parts, blocks, part_bytes, n_terms, bytes;
+  bool alone;
+};
+BwdPlan bwd_plan(int64_t rows, int64_t per, int C) {
+  BwdPlan p = {};
+  p.groups = rows / per;
+  p.parts = bwd_parts(per, p.groups);
+  p.alone = p.groups > 1 && p.parts == 1;
+  p.blocks = std::min({p.groups * p.parts, p.alone ? std::max<int64_t>(kBwdBlocks, p.groups / kMaxPartRows) : kMaxBlocks, kMaxBlocks});
+  p.part_bytes = p.alone ? 0 : p.groups * p.parts * 3 * C * 4;
+  p.n_terms = p.alone ? p.blocks : p.groups > 1 ? p.groups : 0;
+  p.bytes = p.part_bytes + p.n_terms * 3 * C * 4;
+  return p;
+}
 
 template <typename T, int KIND, int N>
 void launch_kind(const NormArgs& g, hipStream_t st) {
@@ -448,8 +522,9 @@ void launch_kind(const NormArgs& g, hipStream_t st) {
 
 template <typename T, int KIND, int N>
 void launch_kind(const NormBwdArgs& g, hipStream_t st) {
-  const dim3 grid((unsigned)std::min(g.groups * g.parts, kMaxBlocks)), block((unsigned)threads_of(g.C));
-  hipLaunchKernelGGL((block_norm_bwd_kernel<T, KIND, N>), grid, block, 0, st, g);
+  const dim3 grid(g.blocks), block((unsigned)threads_of(g.C));
+  if (g.alone) hipLaunchKernelGGL((block_norm_bwd_kernel<T, KIND, N, true>), grid, block, g.terms ? 3 * g.C * 4 : 0, st, g);
+  else hipLaunchKernelGGL((block_norm_bwd_kernel<T, KIND, N, false>), grid, block, 0, st, g);
 }
 
 template <typename T, int KIND, typename G>
@@ -526,8 +601,7 @@ extern "C" int or_block_norm(const or_block_norm_args* p, void* stream) {
 extern "C" int64_t or_block_norm_bwd_workspace_size(int64_t n_rows, int64_t rows_per_group, int32_t C) {
   if (int rc = check_sizes("or_block_norm_bwd_workspace_size", n_rows, rows_per_group, C, OR_TYPE_BF16)) return rc;
   if (n_rows == 0) return 0;
-  const int64_t groups = n_rows / rows_per_group;
-  return part_bytes(n_rows, rows_per_group, C) + (groups > 1 ? groups * 3 * C * 4 : 0);
+  return bwd_plan(n_rows, rows_per_group, C).bytes;
 }
 
 extern "C" int or_block_norm_bwd(const or_block_norm_bwd_args* p, void* stream) {
@@ -550,7 +624,10 @@ extern "C" int or_block_norm_bwd(const or_block_norm_bwd_args* p, void* stream) 
   if (x.post_weight && x.post_norm == OR_NORM_NONE) return fail_arg("or_block_norm_bwd: post_weight belongs to a post_norm");
   if (!al16(x.gate) || !al16(x.post_weight) || !al16(x.weight) || !al16(x.scale))
     return fail_arg("or_block_norm_bwd: parameters must be 16-byte aligned");
-  const int64_t need = or_block_norm_bwd_workspace_size(x.n_rows, x.rows_per_group, x.C);
+  if (!al16(x.dgate) || !al16(x.dpost_weight) || !al16(x.dweight) || !al16(x.dbias) || !al16(x.dscale) || !al16(x.dshift))
+    return fail_arg("or_block_norm_bwd: the parameters' gradients must be 16-byte aligned");
+  const BwdPlan plan = bwd_plan(x.n_rows, x.rows_per_group, x.C);
+  const int64_t need = plan.bytes;
   const bool sums = x.dgate || x.dpost_weight || x.dweight || x.dbias || x.dscale || x.dshift;
   if (sums && (!x.workspace || !al16(x.workspace) || x.workspace_bytes < need))
     return fail_arg("or_block_norm_bwd: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
@@ -573,27 +650,32 @@ extern "C" int or_block_norm_bwd(const or_block_norm_bwd_args* p, void* stream) 
   g.dscale = x.dscale;
   g.dshift = x.dshift;
   g.per = x.rows_per_group;
-  g.groups = x.n_rows / g.per;
+  g.groups = plan.groups;
   g.dh_stride = x.dh_row_stride;
   g.dn_stride = x.dn_row_stride;
   g.h_stride = x.h_row_stride;
   g.a_stride = x.a_row_stride;
   g.C = x.C;
-  g.parts = (int)bwd_parts(g.per, g.groups);
+  g.parts = (int)plan.parts;
+  g.blocks = (unsigned)plan.blocks;
+  g.alone = plan.alone && sums;
   g.norm = x.norm;
   g.post = x.post_norm;
   g.eps = x.eps;
   g.r = x.residual_scale;
-  if (sums) g.part = (float*)x.workspace;
+  if (sums && !g.alone) g.part = (float*)x.workspace;
   const bool weights = x.dweight || x.dbias || x.dpost_weight;
-  if (weights && g.groups > 1) g.group_part = (float*)((char*)x.workspace + part_bytes(x.n_rows, g.per, g.C));
+  g.n_terms = plan.n_terms;
+  if (weights && g.groups > 1) g.terms = (float*)((char*)x.workspace + plan.part_bytes);
   hipStream_t st = (hipStream_t)stream;
   launch(g, x.type, st);
-  if (sums) {
-    const unsigned columns = (unsigned)((g.C + 63) / 64);
-    const dim3 grid(columns, (unsigned)std::min<int64_t>(g.groups, 4096));
-    hipLaunchKernelGGL(block_norm_sums_kernel, grid, dim3(64 * kSumWaves), 0, st, g);
-    if (g.group_part) hipLaunchKernelGGL(block_norm_weights_kernel, dim3(columns, 3), dim3(64 * kSumWaves), 0, st, g);
+  const unsigned columns = (unsigned)((g.C + 63) / 64);
+  if (g.part) {
+    const int waves = g.parts > 8 ? kSumWaves : 4;
+    const dim3 grid(columns, (unsigned)std::min<int64_t>((g.groups * waves + kSumWaves - 1) / kSumWaves, 4096));
+    if (waves == kSumWaves) hipLaunchKernelGGL(block_norm_sums_kernel<kSumWaves>, grid, dim3(64 * kSumWaves), 0, st, g);
+    else hipLaunchKernelGGL(block_norm_sums_kernel<4>, grid, dim3(64 * kSumWaves), 0, st, g);
   }
+  if (g.terms) hipLaunchKernelGGL(block_norm_weights_kernel, dim3(columns, 3), dim3(64 * kSumWaves), 0, st, g);
   return check_hip(hipGetLastError(), "or_block_norm_bwd launch");
 }

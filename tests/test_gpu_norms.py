@@ -366,3 +366,22 @@ def test_refusals():
         with pytest.raises(L.HipPathError):
             f()
             print(k)
+
+
+@pytest.mark.parametrize('rows,C,groups', [(2100, 64, 2100), (1400, 8192, 700), (3 * 1300, 520, 1300), (30 * 40, 1000, 40), (7 * 170, 2048, 170),
+                                           (20 * 5, 8, 5), (9 * 600, 4096, 600)])
+@pytest.mark.parametrize('norm,post,dtype', [('layer', None, torch.bfloat16), ('rms', 'layer', torch.float32)])
+def test_many_groups(rows, C, groups, norm, post, dtype):
+    """as many groups as fill the GPU, each one work-group's, and numbers of them on both sides of that"""
+    print(f'norms {rows} x {C}, {groups} groups, {dtype}', flush=True)
+    i = inputs(rows, C, groups, dtype, True, True, post, True, True, seed=rows)
+    got = run(i, norm, post, 0.7)
+    # the parameters' gradients are the same whichever of them are asked for
+    x, a = (i[k].clone().requires_grad_(k == 'x') for k in ('x', 'a'))
+    for wanted in (('scale',), ('w',), ('gate', 'b'), ()):
+        p = {k: (v if v is None else v.clone().requires_grad_(k in wanted)) for k, v in i.items() if k in ('gate', 'wp', 'w', 'b', 'scale', 'shift')}
+        h, n = norms.residual_norm_modulate(x, a, EPS, norm, p['gate'], 0.7, post, p['wp'], p['w'], p['b'], p['scale'], p['shift'])
+        grads = torch.autograd.grad((h, n), [x] + [p[k] for k in wanted], (i['dh'], i['dn']))
+        order = {'gate': 2, 'wp': 3, 'w': 4, 'b': 5, 'scale': 6, 'shift': 7}
+        for g, k in zip(grads, ('x', *wanted)):
+            assert torch.equal(g, got[order[k] if k != 'x' else 0]), (wanted, k)
