@@ -1,5 +1,6 @@
 """Build libonereel_hip.so (gfx950) in-tree with hipcc: one object per HIP source, then one shared library; and,
-linked against it, libonereel_dit.so (the linear layers, norms and elementwise kernels of the Wan-shaped DiT, gradient clipping) and libonereel_bench.so (bench.py's
+linked against it, libonereel_dit.so (the linear layers, norms and elementwise kernels of the Wan-shaped DiT, gradient
+clipping) and libonereel_bench.so (bench.py's
 measurement kernels).
 
     python -m onereel_amd.build            # or __graft_entry__.build()
