@@ -36,8 +36,7 @@ namespace {
 
 constexpr int kMaxC = 8192;            // 1024 threads of 8 columns
 constexpr int kMaxWaves = 16;
-// work-groups in all (12720 x 2048, 8 groups: forward 768 39.9 us, 1024 40.3, 2048 42.1; gradient 512 71.9, 768 74.5, 1024 76.1)
-constexpr int kBlocks = 768, kBwdBlocks = 512;
+constexpr int kCUs = 256, kBwdBlocks = 512;
 constexpr int kMaxPartRows = 256;      // rows whose sums a thread adds up one after the other
 
 struct NormArgs {
@@ -83,18 +82,23 @@ __device__ __forceinline__ void moments(const float (&v)[8], bool in, int column
   s.square = wave_sum(in ? sum : 0.0f);
 }
 
-// mean and 1 / sqrt(mean square + eps) of a row from its wavefronts' shares
-__device__ __forceinline__ void join_moments(const Share* s, int waves, int C, float eps, float& mean, float& inv) {
-  float sum = 0.0f;
-  for (int w = 0; w < waves; ++w) sum += s[w].mean * (float)wave_columns(C, w);
-  mean = sum / (float)C;
-  float square = 0.0f;
-  for (int w = 0; w < waves; ++w) {
-    const float d = s[w].mean - mean;
-    square += s[w].square + d * d * (float)wave_columns(C, w);
+// The wavefronts' shares are joined by 16 lanes, each with one of them (every 16 lanes of every wavefront do the same): one read of
+// LDS and sums over lanes. (Loops over the shares, one read after the other: 4096 x
+// 8192 63.9 us, so 55.4, with a norm ahead 98 and 62; the gradient of 12720 x 4096 147 and 137, with a norm ahead of 2048 91 and 76.)
+struct Joiner {
+  int wave, waves;
+  float columns;                       // of the lane's share; 0 past the last
+  __device__ __forceinline__ Joiner(int C) : wave(threadIdx.x & 15), waves(blockDim.x >> 6) {
+    columns = wave < waves ? (float)wave_columns(C, wave) : 0.0f;
   }
-  inv = 1.0f / sqrtf(square / (float)C + eps);
-}
+  __device__ __forceinline__ Share take(const Share* s) const { return wave < waves ? s[wave] : Share{}; }
+  // mean and 1 / sqrt(mean square + eps) of a row
+  __device__ __forceinline__ void moments(const Share& s, int C, float eps, float& mean, float& inv) const {
+    mean = row_sum(s.mean * columns) / (float)C;
+    const float d = s.mean - mean;
+    inv = 1.0f / sqrtf(row_sum(s.square + d * d * columns) / (float)C + eps);
+  }
+};
 
 // the rows [first, last) of work-group b
 struct Span {
@@ -118,9 +122,10 @@ enum { kNoResidual, kResidual, kPostNorm };
 template <typename T, int KIND, int N>
 __global__ __launch_bounds__(N) void block_norm_kernel(NormArgs g) {
   __shared__ Share post_share[2][kMaxWaves], share[2][kMaxWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, col = 8 * threadIdx.x, C = g.C;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = 8 * threadIdx.x, C = g.C;
   const bool in = col < C;
   const int columns = wave_columns(C, wave);
+  const Joiner join(C);
   int turn = 0;
   for (int64_t span = blockIdx.x; span < g.spans; span += gridDim.x) {
     const Span s = span_of(span, g.parts, g.per);
@@ -165,7 +170,7 @@ __global__ __launch_bounds__(N) void block_norm_kernel(NormArgs g) {
           moments(p, in, columns, g.post, m);
           if (lane == 0) post_share[turn][wave] = m;
           __syncthreads();
-          join_moments(post_share[turn], waves, C, g.eps, mean, inv);
+          join.moments(join.take(post_share[turn]), C, g.eps, mean, inv);
 #pragma unroll
           for (int i = 0; i < 8; ++i) p[i] = (p[i] - mean) * inv;
         }
@@ -178,7 +183,7 @@ __global__ __launch_bounds__(N) void block_norm_kernel(NormArgs g) {
       moments(h, in, columns, g.norm, m);
       if (lane == 0) share[turn][wave] = m;
       __syncthreads();
-      join_moments(share[turn], waves, C, g.eps, mean, inv);
+      join.moments(join.take(share[turn]), C, g.eps, mean, inv);
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[i] = (h[i] - mean) * inv * W[i] + B[i];
       if (in) Piece<T, 8>::store(g.n, r * C + col, h);
@@ -240,9 +245,10 @@ template <typename T, int KIND, int N, bool ALONE>
 __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
   __shared__ Share share[2][kMaxWaves], post_share[2][kMaxWaves];
   __shared__ float back[2][kMaxWaves][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, col = 8 * threadIdx.x, C = g.C;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = 8 * threadIdx.x, C = g.C;
   const bool in = col < C;
   const int columns = wave_columns(C, wave);
+  const Joiner join(C);
   extern __shared__ __attribute__((aligned(16))) float term[];        // alone: [3][C], each thread's columns its own
   if (ALONE && g.terms && in) {
 #pragma unroll
@@ -307,15 +313,10 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
         if (lane == 0) post_share[turn][wave] = m;
       }
       __syncthreads();
-      join_moments(share[turn], waves, C, g.eps, mean, inv);
-      t = tx = 0.0f;
-      for (int w = 0; w < waves; ++w) {
-        const Share x = share[turn][w];
-        t += x.t;
-        tx += x.tx + (x.mean - mean) * x.t;
-      }
-      t /= (float)C;
-      tx *= inv / (float)C;
+      m = join.take(share[turn]);
+      join.moments(m, C, g.eps, mean, inv);
+      t = g.norm == OR_NORM_LAYER ? row_sum(m.t) / (float)C : 0.0f;
+      tx = row_sum(m.tx + (m.mean - mean) * m.t) * inv / (float)C;
       float d[8];
       now.d.get(d);
 #pragma unroll
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
         }
         if (in) Piece<T, 8>::store(g.dx, r * C + col, h);
         if constexpr (KIND == kPostNorm) {
-          join_moments(post_share[turn], waves, C, g.eps, mean, inv);
+          join.moments(join.take(post_share[turn]), C, g.eps, mean, inv);
           float su = 0.0f, sux = 0.0f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -351,13 +352,9 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
             back[turn][wave][1] = sux;
           }
           __syncthreads();
-          su = sux = 0.0f;
-          for (int w = 0; w < waves; ++w) {
-            su += back[turn][w][0];
-            sux += back[turn][w][1];
-          }
-          su /= (float)C;
-          sux /= (float)C;
+          const bool has = join.wave < join.waves;
+          su = g.post == OR_NORM_LAYER ? row_sum(has ? back[turn][join.wave][0] : 0.0f) / (float)C : 0.0f;
+          sux = row_sum(has ? back[turn][join.wave][1] : 0.0f) / (float)C;
 #pragma unroll
           for (int i = 0; i < 8; ++i) u[i] = inv * (u[i] - su - a[i] * sux);
         }
@@ -459,15 +456,23 @@ __global__ __launch_bounds__(64 * kSumWaves) void block_norm_weights_kernel(Norm
 bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 int threads_of(int C) { return (C / 8 + 63) / 64 * 64; }
 
-// work-groups of a group of rows: `wanted` in all, each with a row or more
-int64_t parts_of(int64_t per, int64_t groups, int wanted) {
-  return std::max<int64_t>(1, std::min<int64_t>((wanted + groups - 1) / groups, per));
+// Work-groups of a group of `per` rows: as many as give each CU the least to do, a work-group's own start being worth a row; all of
+// them at least `wavefronts` a CU, to keep enough loads in flight, and `fewest` to `most` work-groups a CU.
+int64_t parts_of(int64_t per, int64_t groups, int C, int wavefronts, int fewest, int most) {
+  const int64_t waves = threads_of(C) / 64;
+  int64_t best = 1, least = INT64_MAX;
+  for (int k = fewest; k <= most; ++k) {
+    const int64_t parts = std::min(per, kCUs * k / groups), n = parts * groups;
+    if (parts < 1 || (n * waves < (int64_t)kCUs * wavefronts && parts < per && k < most)) continue;
+    const int64_t cost = (n + kCUs - 1) / kCUs * ((per + parts - 1) / parts + 1);
+    if (cost < least) {
+      least = cost;
+      best = parts;
+    }
+    if (parts == per) break;
+  }
+  return best;
 }
-
-// The forward's work-groups in all: narrow rows take few threads a work-group, so more of them keep the loads in flight
-// (12000 rows of 64 and of 512 columns: 768 work-groups 15.0 and 16.1 us, as many wavefronts as 768 of 2048 columns have
-// 7.9 and 9.8); wide ones keep 768 (4096 columns: 84.1 us, as many wavefronts 93.3). The gradient's two are even (35.5, 37.1).
-int fwd_blocks(int C) { return std::max(kBlocks, kBlocks * 256 / threads_of(C)); }
 
 int check_sizes(const char* what, int64_t rows, int64_t per, int32_t C, int32_t type) {
   if (!known_type(type)) return fail_arg("%s: unknown element type %d", what, type);
@@ -491,7 +496,18 @@ int bad_rows(const char* what, const void* p, int64_t stride, int C) {
 
 // Work-groups of the gradient. Each writes 3 sums of C columns, which the second launch reads, so there are as few as keep the
 // GPU's loads in flight; and no thread adds up more than kMaxPartRows rows in a row.
-int64_t bwd_parts(int64_t per, int64_t groups) { return std::max(parts_of(per, groups, kBwdBlocks), (per + kMaxPartRows - 1) / kMaxPartRows); }
+//
+// A group of few rows is one work-group's where the rows that this takes one after the other cost less than a second launch over
+// many groups' sums, a row about as much as 24 groups (in one work-group each and divided, us: 240 groups of 10 x 1536 26 and 36, 100 of
+// 4 x 8192 36 and 62, 173 of 3 x 3232 27 and 53; 240 of 53 x 2048 95 and 98, 80 of 20 x 4096 63 and 45, 16
+// of 16 x 2048 50 and 16). From 256 rows on a
+// work-group has two or more (333 x 1000 in 167 work-groups 12.5 us, 333 13.8; 512 x 2048 14.7, 19.6; 76 x 3584 in 38 13.2, 76 12.3).
+int64_t bwd_parts(int64_t per, int64_t groups, int C) {
+  const int64_t rows = per * groups, turns = (rows + kBwdBlocks - 1) / kBwdBlocks;
+  if (groups > 1 && (per - turns) * 24 <= groups) return (per + kMaxPartRows - 1) / kMaxPartRows;
+  const int64_t parts = std::min(parts_of(per, groups, C, 8, threads_of(C) < 1024 ? 2 : 1, 3), rows < 256 ? per : (per + 1) / 2);
+  return std::max(parts, (per + kMaxPartRows - 1) / kMaxPartRows);
+}
 
 constexpr int64_t kMaxBlocks = 1 << 20;   // of up to 1024 threads: a grid has under 2^32 of them
 
@@ -505,7 +521,7 @@ struct BwdPlan {
 BwdPlan bwd_plan(int64_t rows, int64_t per, int C) {
   BwdPlan p = {};
   p.groups = rows / per;
-  p.parts = bwd_parts(per, p.groups);
+  p.parts = bwd_parts(per, p.groups, C);
   p.alone = p.groups > 1 && p.parts == 1;
   p.blocks = std::min({p.groups * p.parts, p.alone ? std::max<int64_t>(kBwdBlocks, p.groups / kMaxPartRows) : kMaxBlocks, kMaxBlocks});
   p.part_bytes = p.alone ? 0 : p.groups * p.parts * 3 * C * 4;
@@ -591,7 +607,7 @@ extern "C" int or_block_norm(const or_block_norm_args* p, void* stream) {
   g.eps = x.eps;
   g.r = x.residual_scale;
   const int64_t groups = x.n_rows / g.per;
-  g.parts = (int)parts_of(g.per, groups, fwd_blocks(g.C));
+  g.parts = (int)parts_of(g.per, groups, g.C, 12, 1, 12);
   g.spans = groups * g.parts;
   hipStream_t st = (hipStream_t)stream;
   launch(g, x.type, st);

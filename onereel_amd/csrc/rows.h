@@ -119,6 +119,15 @@ struct Piece<float, 8> {
   }
 };
 
+// sum over 16 neighbouring lanes, the same in each of them
+__device__ __forceinline__ float row_sum(float v) {
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, false));   // quad_perm 1032
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, false));   // quad_perm 2301
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, false));  // row_half_mirror
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, false));  // row_mirror
+  return v;
+}
+
 inline int type_size(int type) { return type == OR_TYPE_FP32 ? 4 : 2; }
 inline bool known_type(int type) { return type == OR_TYPE_BF16 || type == OR_TYPE_FP16 || type == OR_TYPE_FP32; }
 
