@@ -180,10 +180,10 @@ struct NormedArgs {
   float eps;
 };
 
+// the wavefronts' shares, one to each of 16 lanes
 __device__ __forceinline__ float sum_shares(const float* s, int waves) {
-  float v = 0.0f;
-  for (int w = 0; w < waves; ++w) v += s[w];
-  return v;
+  const int w = threadIdx.x & 15;
+  return row_sum(w < waves ? s[w] : 0.0f);
 }
 
 // blockIdx.y picks q or k. A thread has one unit of every row; the work-group takes kRows rows at a time, so that their loads are under
