@@ -68,13 +68,13 @@ struct Share {
 // columns of wavefront w of a row of C
 __device__ __forceinline__ int wave_columns(int C, int w) { return min(512, C - 512 * w); }
 
-__device__ __forceinline__ void moments(const float (&v)[8], bool in, int columns, int norm, Share& s) {
+__device__ __forceinline__ void moments(const float (&v)[8], bool in, float a_column, int norm, Share& s) {
   float sum = 0.0f;
   s.mean = 0.0f;
   if (norm == OR_NORM_LAYER) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += v[i];
-    s.mean = wave_sum(in ? sum : 0.0f) / (float)columns;
+    s.mean = wave_sum(in ? sum : 0.0f) * a_column;
     sum = 0.0f;
   }
 #pragma unroll
@@ -87,16 +87,16 @@ __device__ __forceinline__ void moments(const float (&v)[8], bool in, int column
 // 8192 63.9 us, so 55.4, with a norm ahead 98 and 62; the gradient of 12720 x 4096 147 and 137, with a norm ahead of 2048 91 and 76.)
 struct Joiner {
   int wave, waves;
-  float columns;                       // of the lane's share; 0 past the last
-  __device__ __forceinline__ Joiner(int C) : wave(threadIdx.x & 15), waves(blockDim.x >> 6) {
+  float columns, a_column;             // of the lane's share, 0 past the last; 1 / C
+  __device__ __forceinline__ Joiner(int C) : wave(threadIdx.x & 15), waves(blockDim.x >> 6), a_column(1.0f / (float)C) {
     columns = wave < waves ? (float)wave_columns(C, wave) : 0.0f;
   }
   __device__ __forceinline__ Share take(const Share* s) const { return wave < waves ? s[wave] : Share{}; }
   // mean and 1 / sqrt(mean square + eps) of a row
-  __device__ __forceinline__ void moments(const Share& s, int C, float eps, float& mean, float& inv) const {
-    mean = row_sum(s.mean * columns) / (float)C;
+  __device__ __forceinline__ void moments(const Share& s, float eps, float& mean, float& inv) const {
+    mean = row_sum(s.mean * columns) * a_column;
     const float d = s.mean - mean;
-    inv = 1.0f / sqrtf(row_sum(s.square + d * d * columns) / (float)C + eps);
+    inv = rsqrtf(row_sum(s.square + d * d * columns) * a_column + eps);
   }
 };
 
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(N) void block_norm_kernel(NormArgs g) {
   __shared__ Share post_share[2][kMaxWaves], share[2][kMaxWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = 8 * threadIdx.x, C = g.C;
   const bool in = col < C;
-  const int columns = wave_columns(C, wave);
+  const float a_column = 1.0f / (float)wave_columns(C, wave);
   const Joiner join(C);
   int turn = 0;
   for (int64_t span = blockIdx.x; span < g.spans; span += gridDim.x) {
@@ -167,10 +167,10 @@ __global__ __launch_bounds__(N) void block_norm_kernel(NormArgs g) {
         a.get(p);
         if (r + 1 < s.last) load(r + 1);
         if constexpr (KIND == kPostNorm) {
-          moments(p, in, columns, g.post, m);
+          moments(p, in, a_column, g.post, m);
           if (lane == 0) post_share[turn][wave] = m;
           __syncthreads();
-          join.moments(join.take(post_share[turn]), C, g.eps, mean, inv);
+          join.moments(join.take(post_share[turn]), g.eps, mean, inv);
 #pragma unroll
           for (int i = 0; i < 8; ++i) p[i] = (p[i] - mean) * inv;
         }
@@ -180,10 +180,10 @@ __global__ __launch_bounds__(N) void block_norm_kernel(NormArgs g) {
       } else if (r + 1 < s.last) {
         load(r + 1);
       }
-      moments(h, in, columns, g.norm, m);
+      moments(h, in, a_column, g.norm, m);
       if (lane == 0) share[turn][wave] = m;
       __syncthreads();
-      join.moments(join.take(share[turn]), C, g.eps, mean, inv);
+      join.moments(join.take(share[turn]), g.eps, mean, inv);
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[i] = (h[i] - mean) * inv * W[i] + B[i];
       if (in) Piece<T, 8>::store(g.n, r * C + col, h);
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
   __shared__ float back[2][kMaxWaves][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = 8 * threadIdx.x, C = g.C;
   const bool in = col < C;
-  const int columns = wave_columns(C, wave);
+  const float a_column = 1.0f / (float)wave_columns(C, wave);
   const Joiner join(C);
   extern __shared__ __attribute__((aligned(16))) float term[];        // alone: [3][C], each thread's columns its own
   if (ALONE && g.terms && in) {
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
       Share m;
       now.h.get(h);
       now.n.get(n);
-      moments(h, in, columns, g.norm, m);
+      moments(h, in, a_column, g.norm, m);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         t += n[i] * W[i];
@@ -309,14 +309,14 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
       float a[8];
       if constexpr (KIND != kNoResidual) now.a.get(a);
       if constexpr (KIND == kPostNorm) {
-        moments(a, in, columns, g.post, m);
+        moments(a, in, a_column, g.post, m);
         if (lane == 0) post_share[turn][wave] = m;
       }
       __syncthreads();
       m = join.take(share[turn]);
-      join.moments(m, C, g.eps, mean, inv);
-      t = g.norm == OR_NORM_LAYER ? row_sum(m.t) / (float)C : 0.0f;
-      tx = row_sum(m.tx + (m.mean - mean) * m.t) * inv / (float)C;
+      join.moments(m, g.eps, mean, inv);
+      t = g.norm == OR_NORM_LAYER ? row_sum(m.t) * join.a_column : 0.0f;
+      tx = row_sum(m.tx + (m.mean - mean) * m.t) * inv * join.a_column;
       float d[8];
       now.d.get(d);
 #pragma unroll
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
         }
         if (in) Piece<T, 8>::store(g.dx, r * C + col, h);
         if constexpr (KIND == kPostNorm) {
-          join.moments(join.take(post_share[turn]), C, g.eps, mean, inv);
+          join.moments(join.take(post_share[turn]), g.eps, mean, inv);
           float su = 0.0f, sux = 0.0f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -353,8 +353,8 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
           }
           __syncthreads();
           const bool has = join.wave < join.waves;
-          su = g.post == OR_NORM_LAYER ? row_sum(has ? back[turn][join.wave][0] : 0.0f) / (float)C : 0.0f;
-          sux = row_sum(has ? back[turn][join.wave][1] : 0.0f) / (float)C;
+          su = g.post == OR_NORM_LAYER ? row_sum(has ? back[turn][join.wave][0] : 0.0f) * join.a_column : 0.0f;
+          sux = row_sum(has ? back[turn][join.wave][1] : 0.0f) * join.a_column;
 #pragma unroll
           for (int i = 0; i < 8; ++i) u[i] = inv * (u[i] - su - a[i] * sux);
         }
@@ -457,14 +457,16 @@ bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 int threads_of(int C) { return (C / 8 + 63) / 64 * 64; }
 
 // Work-groups of a group of `per` rows: as many as give each CU the least to do, a work-group's own start being worth a row; all of
-// them at least `wavefronts` a CU, to keep enough loads in flight, and `fewest` to `most` work-groups a CU.
-int64_t parts_of(int64_t per, int64_t groups, int C, int wavefronts, int fewest, int most) {
-  const int64_t waves = threads_of(C) / 64;
+// them at least `wavefronts` a CU, to keep enough loads in flight, and `fewest` to `most` work-groups a CU, of whose wavefronts a CU
+// has room for `room` at a time.
+int64_t parts_of(int64_t per, int64_t groups, int C, int wavefronts, int room, int fewest, int most) {
+  const int64_t waves = threads_of(C) / 64, at_once = std::max<int64_t>(1, room / waves);
   int64_t best = 1, least = INT64_MAX;
   for (int k = fewest; k <= most; ++k) {
     const int64_t parts = std::min(per, kCUs * k / groups), n = parts * groups;
     if (parts < 1 || (n * waves < (int64_t)kCUs * wavefronts && parts < per && k < most)) continue;
-    const int64_t cost = (n + kCUs - 1) / kCUs * ((per + parts - 1) / parts + 1);
+    const int64_t a_cu = (n + kCUs - 1) / kCUs, turns = a_cu <= at_once ? a_cu : (n + kCUs * at_once - 1) / (kCUs * at_once) * at_once;
+    const int64_t cost = turns * ((per + parts - 1) / parts + 1);
     if (cost < least) {
       least = cost;
       best = parts;
@@ -505,7 +507,7 @@ int bad_rows(const char* what, const void* p, int64_t stride, int C) {
 int64_t bwd_parts(int64_t per, int64_t groups, int C) {
   const int64_t rows = per * groups, turns = (rows + kBwdBlocks - 1) / kBwdBlocks;
   if (groups > 1 && (per - turns) * 24 <= groups) return (per + kMaxPartRows - 1) / kMaxPartRows;
-  const int64_t parts = std::min(parts_of(per, groups, C, 8, threads_of(C) < 1024 ? 2 : 1, 3), rows < 256 ? per : (per + 1) / 2);
+  const int64_t parts = std::min(parts_of(per, groups, C, 8, threads_of(C) <= 512 ? 12 : 16, threads_of(C) < 1024 ? 2 : 1, 3), rows < 256 ? per : (per + 1) / 2);
   return std::max(parts, (per + kMaxPartRows - 1) / kMaxPartRows);
 }
 
@@ -607,7 +609,7 @@ extern "C" int or_block_norm(const or_block_norm_args* p, void* stream) {
   g.eps = x.eps;
   g.r = x.residual_scale;
   const int64_t groups = x.n_rows / g.per;
-  g.parts = (int)parts_of(g.per, groups, g.C, 12, 1, 12);
+  g.parts = (int)parts_of(g.per, groups, g.C, 12, 20, 1, 12);
   g.spans = groups * g.parts;
   hipStream_t st = (hipStream_t)stream;
   launch(g, x.type, st);
