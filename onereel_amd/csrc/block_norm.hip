@@ -22,7 +22,7 @@
 // columns' A, B and D over its work-group's rows, in a fixed order; a second launch joins the work-groups' sums, unless there are so
 // many groups that each is one work-group's, which then makes the group's gradients by itself. 12720 x 2048 in bf16
 // with gate, scale and shift of 8 groups, among other work: forward 41.2 us for 208 MB (5.1 TB/s, the rate of a copy of 1 GB here
-// 5.15 to 5.5); gradient 71.3 us for 313 MB, 65 of them in the first launch (4.8 TB/s) and 5 in the column sums.
+// 5.15 to 5.5); gradient 71.2 us for 313 MB, 65 of them in the first launch (4.8 TB/s) and 5 in the column sums.
 #include <math.h>
 
 #include <algorithm>
@@ -456,19 +456,23 @@ __global__ __launch_bounds__(64 * kSumWaves) void block_norm_weights_kernel(Norm
 bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 int threads_of(int C) { return (C / 8 + 63) / 64 * 64; }
 
-// Work-groups of a group of `per` rows: as many as give each CU the least to do, a work-group's own start being worth a row; all of
-// them at least `wavefronts` a CU, to keep enough loads in flight, and `fewest` to `most` work-groups a CU, of whose wavefronts a CU
-// has room for `room` at a time.
-int64_t parts_of(int64_t per, int64_t groups, int C, int wavefronts, int room, int fewest, int most) {
-  const int64_t waves = threads_of(C) / 64, at_once = std::max<int64_t>(1, room / waves);
-  int64_t best = 1, least = INT64_MAX;
-  for (int k = fewest; k <= most; ++k) {
-    const int64_t parts = std::min(per, kCUs * k / groups), n = parts * groups;
-    if (parts < 1 || (n * waves < (int64_t)kCUs * wavefronts && parts < per && k < most)) continue;
-    const int64_t a_cu = (n + kCUs - 1) / kCUs, turns = a_cu <= at_once ? a_cu : (n + kCUs * at_once - 1) / (kCUs * at_once) * at_once;
-    const int64_t cost = turns * ((per + parts - 1) / parts + 1);
-    if (cost < least) {
-      least = cost;
+// Work-groups of a group of `per` rows, up to `most` a CU: as many as keep a CU shortest, of whose wavefronts it has room for 16 at a
+// time, a work-group's own start being worth a row. What a row takes follows the wavefronts on the fullest of the four SIMDs, and is
+// no shorter than with `least` on each, which the loads under way need.
+// (768 work-groups and more for the forward, 512 for the gradient, rounded up to whole ones a group, on the left: 113 groups of 189 x
+// 2424 with a norm ahead 117 and 102 us, 4096 x 8192 64 and 55; gradients of 24 groups of 880 x 1536 106 and 92, 100 of 200 x 2048 131
+// and 118, 4096 x 8192 111 and 95. Up to four a CU for the gradient: 24 of 880 x 1536 105.)
+int64_t parts_of(int64_t per, int64_t groups, int C, int least, int most) {
+  const int64_t waves = threads_of(C) / 64, at_once = std::max<int64_t>(1, 16 / waves);
+  const auto load = [&](int64_t n) { return n ? std::max<int64_t>(least, (n * waves + 3) / 4) : 0; };
+  int64_t best = 1, shortest = INT64_MAX;
+  for (int k = 1; k <= most; ++k) {
+    const int64_t parts = std::min(per, kCUs * k / groups);
+    if (parts < 1) continue;
+    const int64_t a_cu = (parts * groups + kCUs - 1) / kCUs;
+    const int64_t cost = (a_cu / at_once * load(at_once) + load(a_cu % at_once)) * ((per + parts - 1) / parts + 1);
+    if (cost < shortest) {
+      shortest = cost;
       best = parts;
     }
     if (parts == per) break;
@@ -507,7 +511,7 @@ int bad_rows(const char* what, const void* p, int64_t stride, int C) {
 int64_t bwd_parts(int64_t per, int64_t groups, int C) {
   const int64_t rows = per * groups, turns = (rows + kBwdBlocks - 1) / kBwdBlocks;
   if (groups > 1 && (per - turns) * 24 <= groups) return (per + kMaxPartRows - 1) / kMaxPartRows;
-  const int64_t parts = std::min(parts_of(per, groups, C, 8, threads_of(C) <= 512 ? 12 : 16, threads_of(C) < 1024 ? 2 : 1, 3), rows < 256 ? per : (per + 1) / 2);
+  const int64_t parts = std::min(parts_of(per, groups, C, 2, 3), rows < 256 ? per : (per + 1) / 2);
   return std::max(parts, (per + kMaxPartRows - 1) / kMaxPartRows);
 }
 
@@ -609,7 +613,7 @@ extern "C" int or_block_norm(const or_block_norm_args* p, void* stream) {
   g.eps = x.eps;
   g.r = x.residual_scale;
   const int64_t groups = x.n_rows / g.per;
-  g.parts = (int)parts_of(g.per, groups, g.C, 12, 20, 1, 12);
+  g.parts = (int)parts_of(g.per, groups, g.C, 3, 12);
   g.spans = groups * g.parts;
   hipStream_t st = (hipStream_t)stream;
   launch(g, x.type, st);
