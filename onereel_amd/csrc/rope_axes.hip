@@ -18,8 +18,8 @@
 //
 // HBM-bound: rows are read once and written once. The cosines and sines of a batch of tokens go through LDS, one of a token's
 // pairs a thread, since the heads share them; in the normed form they are ready at the barrier that the rows' sums need anyway.
-// 12720 tokens of 16 heads of 128 in bf16, q and k, among other work: normed 39.7 us for 208 MB (5.2 TB/s, the rate of a copy of 1 GB
-// here 5.15 to 5.5), its gradient 67.7 us for 313 MB (63 in the first launch, 5.0 TB/s, and 5 in the sum of dw). A call for few
+// 12720 tokens of 16 heads of 128 in bf16, q and k, among other work: normed 39.6 us for 208 MB (5.2 TB/s, the rate of a copy of 1 GB
+// here 5.15 to 5.5), its gradient 65.7 us for 313 MB (61 in the first launch, 5.1 TB/s, and 5 in the sum of dw). A call for few
 // tokens is the launch: 5.2 us on the GPU for 333 tokens of 5 heads of 96 in fp32, 12.6 with the host.
 #include <math.h>
 
@@ -196,6 +196,7 @@ __global__ __launch_bounds__(1024) void norm_rope_axes_kernel(NormedArgs g) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, which = blockIdx.y;
   const int half = g.D / 2, units = g.D / 8, h = threadIdx.x / units;
   const bool in = 8 * (int)threadIdx.x < g.C;
+  const float a_column = 1.0f / (float)g.C;
   int lo, hi, j;
   unit_of<HALF>(g.axes, threadIdx.x - h * units, lo, hi, j);
   lo += h * g.D;
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(1024) void norm_rope_axes_kernel(NormedArgs g) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      const float inv = 1.0f / sqrtf(sum_shares(share[now][k], waves) / (float)g.C + g.eps);
+      const float inv = rsqrtf(sum_shares(share[now][k], waves) * a_column + g.eps);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[k][i] *= inv * w[i];
       if (in && r0 + k < g.rows) {
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(1024) void norm_rope_axes_kernel(NormedArgs g) {
   }
 }
 
-// (One row at a time, its loads and angles under way ahead of the last one's sums and one barrier a row: 70.5 us, so 69.2, for q and k of
+// (One row at a time, its loads and angles under way ahead of the last one's sums and one barrier a row: 70.5 us, two rows and two barriers 69.2 then, for q and k of
 // 12720 rows of 2048.)
 template <typename T, bool HALF>
 __global__ __launch_bounds__(1024) void norm_rope_axes_bwd_kernel(NormedArgs g) {
@@ -254,6 +255,7 @@ __global__ __launch_bounds__(1024) void norm_rope_axes_bwd_kernel(NormedArgs g) 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, which = blockIdx.y;
   const int half = g.D / 2, units = g.D / 8, h = threadIdx.x / units;
   const bool in = 8 * (int)threadIdx.x < g.C;
+  const float a_column = 1.0f / (float)g.C;
   int lo, hi, j;
   unit_of<HALF>(g.axes, threadIdx.x - h * units, lo, hi, j);
   lo += h * g.D;
@@ -306,8 +308,8 @@ __global__ __launch_bounds__(1024) void norm_rope_axes_bwd_kernel(NormedArgs g) 
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      const float inv = 1.0f / sqrtf(sum_shares(share[now][k], waves) / (float)g.C + g.eps);
-      const float m = sum_shares(share_x[now][k], waves) / (float)g.C * inv * inv;    // mean(t n) inv
+      const float inv = rsqrtf(sum_shares(share[now][k], waves) * a_column + g.eps);
+      const float m = sum_shares(share_x[now][k], waves) * a_column * inv * inv;    // mean(t n) inv
       const bool row = in && r0 + k < g.rows;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
