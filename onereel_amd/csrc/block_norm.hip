@@ -293,18 +293,27 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
     for (int64_t r = s.first; r < s.last; ++r, turn ^= 1) {
       now = next;
       if (r + 1 < s.last) load(next, r + 1);
-      float h[8], n[8], t = 0.0f, tx = 0.0f, mean, inv;
-      Share m;
+      float h[8], n[8], t = 0.0f, tx = 0.0f, sum = 0.0f, mean, inv;
+      Share m = {};
       now.h.get(h);
       now.n.get(n);
-      moments(h, in, a_column, g.norm, m);
+      if (g.norm == OR_NORM_LAYER) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          sum += h[i];
+          t += n[i] * W[i];
+        }
+        wave_sums(in ? sum : 0.0f, in ? t : 0.0f, m.mean, m.t);
+        m.mean *= a_column;
+        sum = 0.0f;
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        t += n[i] * W[i];
-        tx += n[i] * W[i] * (h[i] - m.mean);
+        const float c = h[i] - m.mean;
+        sum += c * c;
+        tx += n[i] * W[i] * c;
       }
-      m.t = g.norm == OR_NORM_LAYER ? wave_sum(in ? t : 0.0f) : 0.0f;
-      m.tx = wave_sum(in ? tx : 0.0f);
+      wave_sums(in ? sum : 0.0f, in ? tx : 0.0f, m.square, m.tx);
       if (lane == 0) share[turn][wave] = m;
       float a[8];
       if constexpr (KIND != kNoResidual) now.a.get(a);
@@ -345,8 +354,7 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
             su += u[i];
             sux += u[i] * a[i];
           }
-          su = g.post == OR_NORM_LAYER ? wave_sum(in ? su : 0.0f) : 0.0f;
-          sux = wave_sum(in ? sux : 0.0f);
+          wave_sums(in ? su : 0.0f, in ? sux : 0.0f, su, sux);
           if (lane == 0) {
             back[turn][wave][0] = su;
             back[turn][wave][1] = sux;

@@ -128,6 +128,17 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
+// sums of two values over the 64 lanes of a wavefront, the same in each of them: the halves swap one for the other, so that one
+// register goes through the rest for both
+__device__ __forceinline__ void wave_sums(float a, float b, float& sum_a, float& sum_b) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  const float v = row_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+  const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  const float r = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+  sum_a = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(r), 0));
+  sum_b = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(r), 32));
+}
+
 inline int type_size(int type) { return type == OR_TYPE_FP32 ? 4 : 2; }
 inline bool known_type(int type) { return type == OR_TYPE_BF16 || type == OR_TYPE_FP16 || type == OR_TYPE_FP32; }
 
