@@ -394,9 +394,10 @@ __global__ __launch_bounds__(N) void block_norm_bwd_kernel(NormBwdArgs g) {
   }
 }
 
-// The groups' sums of 64 columns, those of a group's work-groups dealt out to WAVES of 16 wavefronts: all of them, or 4 for up to 8
-// work-groups; then its parameters' gradients, or their terms. (16
-// columns a work-group and four times as many of them: 7.2 us, so 5.1, for 8 groups of 64 work-groups and 2048 columns.)
+// The groups' sums of 64 columns, those of a group's work-groups dealt out to WAVES of 16 wavefronts: all of them, or one for up to 8
+// work-groups (the whole gradient of 240 groups of 53 x 2048 with 3 each 81.5 us, so, 93.9 with 4 wavefronts a group; 80 of 20 x 4096
+// 29.9 and 35.3). Then its parameters' gradients, or their terms. (16 columns a work-group and four times as many of them: 7.2 us, so
+// 5.1, for 8 groups of 64 work-groups and 2048 columns.)
 constexpr int kSumWaves = 16;
 template <int WAVES>
 __global__ __launch_bounds__(64 * kSumWaves) void block_norm_sums_kernel(NormBwdArgs g) {
@@ -512,9 +513,8 @@ int bad_rows(const char* what, const void* p, int64_t stride, int C) {
 // GPU's loads in flight; and no thread adds up more than kMaxPartRows rows in a row.
 //
 // A group of few rows is one work-group's where the rows that this takes one after the other cost less than a second launch over
-// many groups' sums, a row about as much as 24 groups (in one work-group each and divided, us: 240 groups of 10 x 1536 26 and 36, 100 of
-// 4 x 8192 36 and 62, 173 of 3 x 3232 27 and 53; 240 of 53 x 2048 95 and 98, 80 of 20 x 4096 63 and 45, 16
-// of 16 x 2048 50 and 16). From 256 rows on a
+// many groups' sums, a row about as much as 24 groups (in one work-group each and divided, us: 300 groups of 20 x 2048 46 and 51, 100 of
+// 4 x 8192 32 and 36; 160 of 12 x 512 17.5 and 15.2, 80 of 20 x 4096 40 and 30, 99 of 13 x 5432 73 and 57). From 256 rows on a
 // work-group has two or more (333 x 1000 in 167 work-groups 12.5 us, 333 13.8; 512 x 2048 14.7, 19.6; 76 x 3584 in 38 13.2, 76 12.3).
 int64_t bwd_parts(int64_t per, int64_t groups, int C) {
   const int64_t rows = per * groups, turns = (rows + kBwdBlocks - 1) / kBwdBlocks;
@@ -701,10 +701,10 @@ extern "C" int or_block_norm_bwd(const or_block_norm_bwd_args* p, void* stream) 
   launch(g, x.type, st);
   const unsigned columns = (unsigned)((g.C + 63) / 64);
   if (g.part) {
-    const int waves = g.parts > 8 ? kSumWaves : 4;
+    const int waves = g.parts > 8 ? kSumWaves : 1;
     const dim3 grid(columns, (unsigned)std::min<int64_t>((g.groups * waves + kSumWaves - 1) / kSumWaves, 4096));
     if (waves == kSumWaves) hipLaunchKernelGGL(block_norm_sums_kernel<kSumWaves>, grid, dim3(64 * kSumWaves), 0, st, g);
-    else hipLaunchKernelGGL(block_norm_sums_kernel<4>, grid, dim3(64 * kSumWaves), 0, st, g);
+    else hipLaunchKernelGGL(block_norm_sums_kernel<1>, grid, dim3(64 * kSumWaves), 0, st, g);
   }
   if (g.terms) hipLaunchKernelGGL(block_norm_weights_kernel, dim3(columns, 3), dim3(64 * kSumWaves), 0, st, g);
   return check_hip(hipGetLastError(), "or_block_norm_bwd launch");
