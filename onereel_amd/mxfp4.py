@@ -24,18 +24,23 @@ BLOCK = 32
 class MXFP4:
     """A tensor [.., n] in 4 bits: codes uint8 [.., n / 2], two e2m1 values a byte with the even element in the low half, and
     scales uint8 [.., n / 32], the biased exponent of each 32 elements' power of two (255: NaN). Both contiguous on one GPU; n a
-    multiple of 32. `quantize` makes one; one can be made of stored codes and scales too."""
+    multiple of 32. `quantize` makes one; one can be made of stored codes and scales too, of bytes or of the 64-bit integers that
+    torch makes of sums of bytes with Python's numbers and of lists of those (their low 8 bits, copied)."""
 
     def __init__(self, codes, scales):
         for t, what in ((codes, 'codes'), (scales, 'scales')):
-            if t.dtype != torch.uint8 or not t.is_cuda:
-                raise L.HipTypeError(f'{what} must be a uint8 GPU tensor, got {t.dtype} on {t.device}')
+            if t.dtype not in (torch.uint8, torch.int64) or not t.is_cuda:
+                raise L.HipTypeError(f'{what} must be a uint8 (or int64) GPU tensor, got {t.dtype} on {t.device}')
         if codes.device != scales.device:
             raise L.HipTypeError('all tensors of a call must be on one GPU')
         n = 2 * codes.shape[-1] if codes.dim() else 0
         if not n or n % BLOCK or scales.shape != (*codes.shape[:-1], n // BLOCK):
             raise L.HipValueError(f'codes [.., n / 2] and scales [.., n / 32] of a multiple of 32 elements n are needed, got '
                                   f'{tuple(codes.shape)} and {tuple(scales.shape)}')
+        if codes.dtype != torch.uint8:
+            codes = codes.to(torch.uint8)
+        if scales.dtype != torch.uint8:
+            scales = scales.to(torch.uint8)
         codes = codes.contiguous()
         self.codes, self.scales = codes if codes.data_ptr() % 16 == 0 else codes.clone(), scales.contiguous()
         self.shape = torch.Size((*codes.shape[:-1], n))
