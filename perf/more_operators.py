@@ -219,8 +219,7 @@ def _prepare_mx(case, randn):
     M, K, N = case['rows'], case['n_in'], case['n_out']
     # weights as they are stored: two e2m1 codes a byte, the even element in the low half, one e8m0 scale for 32 elements
     codes, scales = _quantized(randn(N, K) * K ** -0.5)
-    s = dict(x=_activations(randn, M, K).bfloat16(), codes=(codes[:, 0::2] + 16 * codes[:, 1::2]).to(torch.uint8),
-             scales=scales)
+    s = dict(x=_activations(randn, M, K).bfloat16(), codes=codes[:, 0::2] + 16 * codes[:, 1::2], scales=scales)
     s['b'] = (0.1 * randn(N)).bfloat16() if case['bias'] else None
     s['gate'] = 0.5 + 0.5 * randn(N) if case['gate'] else None
     s['residual'] = randn(M, N).bfloat16() if case['residual'] else None
