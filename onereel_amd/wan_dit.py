@@ -292,21 +292,23 @@ class WanDiT:
         """the gradients of `parameters()` scaled to a norm of at most max_norm (clip.clip_grad_norm_): their norm before that"""
         return clip.clip_grad_norm_(self.parameters(), max_norm)
 
-    def _per_frame(self, t, device):
-        """the timesteps of the latent frames [frames, 1] fp32, or None where t is one for all: a number, or a tensor or array of
-        one element"""
+    def _timesteps(self, t, device):
+        """(t, None) where t is one timestep for all, a number, or a tensor or array of one element in any shape: as a number, or a
+        tensor that features on the device can be multiplied by; else (None, the timesteps of the latent frames [frames, 1] fp32)"""
         if not isinstance(t, (list, tuple)) and math.prod(getattr(t, 'shape', ())) == 1:
-            return None
+            if isinstance(t, torch.Tensor):
+                return (t.reshape(1).to(device) if t.dim() else t), None
+            return float(t.item() if getattr(t, 'shape', ()) else t), None
         t = torch.as_tensor(t, dtype=torch.float32, device=device)
         if t.shape != (self.ctx.layout.n_frames,):
             raise L.HipValueError(f'timesteps of shape {tuple(t.shape)} for {self.ctx.layout.n_frames} latent frames')
-        return t[:, None]
+        return None, t[:, None]
 
     def forward(self, tokens, t, text, rotary):
         """tokens [S, in_channels * patch] bf16 (the patchified latent, frame-major), t the timestep, or one for each latent frame,
         text [n_scenes * text_len, text_dim] bf16 (sentence j in rows j * text_len ..), rotary (cos, sin) [1, S, 1, D] fp32 or a
         rotary.Axes -> [S, in * patch]"""
-        frames = self._per_frame(t, tokens.device)
+        t, frames = self._timesteps(t, tokens.device)
         if frames is not None:
             return self._forward_frames(tokens, frames, text, rotary)
         d = self.cfg.dim
@@ -347,7 +349,7 @@ class WanDiT:
         """forward with gradients of tokens, text and `parameters()` (those of them that require one)"""
         if self.ctx.memory or any(self.ctx.layout.extra.get(j) for j in range(self.ctx.layout.n_scenes)):
             raise L.HipValueError('the frame-memory scopes and the bounded memory have no gradient: train with halo scopes')
-        frames = self._per_frame(t, tokens.device)
+        t, frames = self._timesteps(t, tokens.device)
         if frames is not None:
             return self._forward_frames(tokens, frames, text, rotary, _apply)
         d, eps = self.cfg.dim, self.cfg.eps
