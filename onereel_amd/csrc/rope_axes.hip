@@ -113,17 +113,19 @@ struct Unit {
   }
 };
 
-// the pairs of a unit, rotated by their angles (sign 1) or back (-1)
+// The first `left` pairs of a unit, rotated by their angles (sign 1) or back (-1). The others are left as they are: a product with a
+// sine of 0 would make a NaN of an infinity beside them.
 template <bool HALF>
-__device__ __forceinline__ void turn8(float (&v)[8], const float2* angle, float sign) {
+__device__ __forceinline__ void turn8(float (&v)[8], const float2* angle, int left, float sign) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float c = angle[i].x, s = sign * angle[i].y;
     float& a = v[HALF ? i : 2 * i];
     float& b = v[HALF ? 4 + i : 2 * i + 1];
     const float x = a * c - b * s, y = a * s + b * c;
-    a = x;
-    b = y;
+    const bool turned = i < left;
+    a = turned ? x : a;
+    b = turned ? y : b;
   }
 }
 
@@ -161,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RotateArgs g) {
       float v[8];
       x.load(g.x, (r0 + t) * g.row_stride + h * g.head_stride, lo, hi);
       x.get(v);
-      turn8<HALF>(v, angle + t * half + j, g.sign);
+      turn8<HALF>(v, angle + t * half + j, g.axes.pairs - j, g.sign);
       Unit<T, HALF>::store(g.out, ((r0 + t) * g.H + h) * g.D, lo, hi, v);
     }
   }
@@ -238,7 +240,7 @@ __global__ __launch_bounds__(1024) void norm_rope_axes_kernel(NormedArgs g) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[k][i] *= inv * w[i];
       if (in && r0 + k < g.rows) {
-        turn8<HALF>(v[k], angle[now][k] + j, 1.0f);
+        turn8<HALF>(v[k], angle[now][k] + j, g.axes.pairs - j, 1.0f);
         Unit<T, HALF>::store(g.out[which], (r0 + k) * g.C, lo, hi, v[k]);
       }
     }
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(1024) void norm_rope_axes_bwd_kernel(NormedArgs g) 
     for (int k = 0; k < kRows; ++k) {
       x[k].get(v[k]);
       d[k].get(e[k]);
-      turn8<HALF>(e[k], angle[now][k] + (in ? j : 0), -1.0f);
+      turn8<HALF>(e[k], angle[now][k] + (in ? j : 0), g.axes.pairs - j, -1.0f);
       float ss = 0.0f, tx = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
