@@ -52,11 +52,24 @@ def _addresses(tensors, what: str, at: int):
         devices.pop() if devices else None
 
 
-def _call(sources, out, at: int, max_norm: float = 0.0):
-    """or_clip of two results of _addresses (out None: the norm alone)"""
+def _refuse(changed):
+    """what autograd cannot follow a change of, where it records one"""
+    for t in changed:
+        view = t._is_view()
+        if t.is_inference() or t.requires_grad and (t._base if view else t).is_leaf or \
+                view and torch._C._autograd._get_creation_meta(t) != torch._C._autograd.CreationMeta.DEFAULT:
+            raise L.HipValueError('where autograd records a call, it scales no leaf that requires a gradient, no inference tensor and no '
+                                  'view that was made without autograd or as one of several: call it under torch.no_grad()')
+
+
+def _norm_on(at: int):
+    return torch.empty((), dtype=torch.float32, device=torch.device('cuda', at))
+
+
+def _call(sources, out, norm, max_norm: float = 0.0):
+    """or_clip of two results of _addresses (out None: the norm alone) into the scalar norm"""
     p = lambda values: values.buffer_info()[0]
-    n, device = len(sources[0]), torch.device('cuda', at)
-    norm = torch.empty((), dtype=torch.float32, device=device)
+    n, device = len(sources[0]), norm.device
     args = L.ClipArgs(*map(p, sources), out and p(out[0]), out and p(out[2]), n, max_norm, norm.data_ptr(), None, 0)
     size = L.dit_lib().or_clip_workspace_size(ctypes.byref(args))
     if size < 0:
@@ -79,7 +92,7 @@ def grad_norm(tensors):
     if not all(map(_T.is_contiguous, tensors)):
         tensors = [t if _dense(t) else t.detach().contiguous() for t in tensors]
     sources, at = _addresses(tensors, 'tensors', None)
-    return _zero() if at is None else without_gradient('clip.grad_norm', _call(sources, None, at), *given)
+    return _zero() if at is None else without_gradient('clip.grad_norm', _call(sources, None, _norm_on(at)), *given)
 
 
 def clip_grads_(tensors, max_norm: float, out=None):
@@ -87,8 +100,10 @@ def clip_grads_(tensors, max_norm: float, out=None):
     or, with out (one tensor of the same shape for each, of any of the types), into those. Returns the norm before clipping, an
     fp32 scalar on the GPU. A norm that is infinite or NaN does to the tensors what the formula says, as in torch: zeros and NaN, or
     NaN throughout. Tensors that are written must not share memory with one another or with what is read (but for the tensor that
-    they take the place of), and each fill its own."""
-    tensors = list(tensors)
+    they take the place of), and each fill its own. Nothing here has a gradient: where autograd records and one of the tensors requires
+    one, a backward pass that reaches the norm or what was written raises, and what autograd could not follow a change of (a leaf
+    that requires one) is refused."""
+    given = tensors = list(tensors)
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise L.HipValueError(f'max_norm must be 0 or more, got {max_norm}')
@@ -109,8 +124,17 @@ def clip_grads_(tensors, max_norm: float, out=None):
         written, _ = _addresses(out, 'out', at)
     if at is None:
         return _zero()
-    norm = _call(sources, written, at, max_norm)
-    changed = tensors if out is None else out
+    changed, norm = tensors if out is None else out, _norm_on(at)
+    # one C call for all, as above
+    recorded = torch.is_grad_enabled() and torch._C._any_requires_grad(*given, *(out or ()))
+    if recorded:
+        _refuse(changed)
+    _call(sources, written, norm, max_norm)
+    if recorded:
+        norm = without_gradient('clip.clip_grads_', norm, *given, *changed)
+        for t in changed:              # which counts their versions up too
+            without_gradient('clip.clip_grads_', t, norm)
+        return norm
     try:
         torch.autograd.graph.increment_version(changed)
     except RuntimeError:               # inference tensors among them, which have no version
@@ -120,6 +144,7 @@ def clip_grads_(tensors, max_norm: float, out=None):
 
 def clip_grad_norm_(parameters, max_norm: float):
     """torch.nn.utils.clip_grad_norm_ of the parameters' gradients (those that have one): scaled in place, returns their norm
-    before that, an fp32 scalar on the GPU"""
+    before that, an fp32 scalar on the GPU. As there, autograd does not record it. A parameter is given once."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    return clip_grads_([p.grad for p in parameters if p.grad is not None], max_norm)
+    with torch.no_grad():
+        return clip_grads_([p.grad for p in parameters if p.grad is not None], max_norm)
