@@ -73,7 +73,8 @@ typedef struct or_block_norm_args {
 /* Replaces the residual add of the Wan transformer block and the norm with modulation that follows it (diffusers'
  * WanTransformerBlock, third-party; the blocks the processors are installed in, src/onereel/models/wan.py:77-108), as
  * or_residual_layernorm_modulate does in place, for training (nothing is updated in place), with gate, scale and shift for every
- * group of rows, RMS norms, a norm of the sub-block's output, and all three element types. One launch. */
+ * group of rows, RMS norms, a norm of the sub-block's output, and all three element types. One launch. Rows and parameters lie at
+ * 16-byte aligned addresses. */
 int or_block_norm(const or_block_norm_args* args, void* stream);
 
 /* Arguments of or_block_norm_bwd: the gradient of one or_block_norm call. h is the call's h (its x without a). */
@@ -115,7 +116,7 @@ typedef struct or_block_norm_bwd_args {
 int64_t or_block_norm_bwd_workspace_size(int64_t n_rows, int64_t rows_per_group, int32_t C);
 
 /* The gradient of or_block_norm. Sums are fp32 in a fixed order; dx and da are rounded once. With 0 rows nothing is written.
- * One launch; with sums over rows up to three. The parameters' gradients lie at 16-byte aligned addresses. */
+ * One launch; with sums over rows up to three. Rows, parameters and the parameters' gradients lie at 16-byte aligned addresses. */
 int or_block_norm_bwd(const or_block_norm_bwd_args* args, void* stream);
 
 /* activations of or_linear */

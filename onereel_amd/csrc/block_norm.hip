@@ -652,7 +652,7 @@ extern "C" int or_block_norm_bwd(const or_block_norm_bwd_args* p, void* stream) 
     return fail_arg("or_block_norm_bwd: dh, gate, post_norm and post_weight belong to a");
   }
   if (x.post_weight && x.post_norm == OR_NORM_NONE) return fail_arg("or_block_norm_bwd: post_weight belongs to a post_norm");
-  if (!al16(x.gate) || !al16(x.post_weight) || !al16(x.weight) || !al16(x.scale))
+  if (!al16(x.gate) || !al16(x.post_weight) || !al16(x.weight) || !al16(x.bias) || !al16(x.scale))
     return fail_arg("or_block_norm_bwd: parameters must be 16-byte aligned");
   if (!al16(x.dgate) || !al16(x.dpost_weight) || !al16(x.dweight) || !al16(x.dbias) || !al16(x.dscale) || !al16(x.dshift))
     return fail_arg("or_block_norm_bwd: the parameters' gradients must be 16-byte aligned");
