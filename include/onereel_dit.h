@@ -234,6 +234,10 @@ typedef struct or_mx_linear_args {
 /* Bytes of device workspace or_mx_linear needs (quantized: x comes in 4 bits). Negative for sizes it refuses. */
 int64_t or_mx_linear_workspace_size(int64_t n_rows, int32_t n_in, int32_t n_out, int32_t quantized);
 
+/* How or_mx_linear computes a product of these sizes, as or_linear_plan tells of or_linear: tile (256, 128 or 64; 0: the kernel for
+ * few rows), LDS buffers of its ring (0 with that), parts of n_in. Host only. */
+int or_mx_linear_plan(int64_t n_rows, int32_t n_in, int32_t n_out, int32_t* tile, int32_t* buffers, int32_t* split);
+
 /* Replaces the Linear layers of the Wan transformer block with what follows them, as or_linear does (diffusers'
  * WanTransformerBlock, third-party; the blocks the processors are installed in, src/onereel/models/wan.py:77-108), for inference
  * with 4-bit weights and activations: y = residual + gate * act(x weight^T + bias) of the values in 4 bits, fp32 from the products to

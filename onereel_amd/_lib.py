@@ -188,6 +188,7 @@ DIT_SIGNATURES = {
     'or_mx_quantize': (i32, [vp, i64, i32, i64, i32, vp, vp, vp]),
     'or_mx_dequantize': (i32, [vp, vp, i64, i32, i32, vp, vp]),
     'or_mx_linear_workspace_size': (i64, [i64, i32, i32, i32]),
+    'or_mx_linear_plan': (i32, [i64, i32, i32, ctypes.POINTER(i32), ctypes.POINTER(i32), ctypes.POINTER(i32)]),
     'or_mx_linear': (i32, [ctypes.POINTER(MxLinearArgs), vp]),
     'or_clip_workspace_size': (i64, [ctypes.POINTER(ClipArgs)]),
     'or_clip': (i32, [ctypes.POINTER(ClipArgs), vp]),

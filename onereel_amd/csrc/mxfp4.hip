@@ -817,6 +817,16 @@ extern "C" int64_t or_mx_linear_workspace_size(int64_t n_rows, int32_t n_in, int
   return layout_of(plan_of(n_rows, n_out, n_in), n_rows, n_out, n_in, quantized != 0).bytes;
 }
 
+extern "C" int or_mx_linear_plan(int64_t n_rows, int32_t n_in, int32_t n_out, int32_t* tile, int32_t* buffers, int32_t* split) {
+  if (int rc = check_product("or_mx_linear_plan", n_rows, n_in, n_out)) return rc;
+  if (!tile || !buffers || !split) return fail_arg("or_mx_linear_plan: tile, buffers and split are required");
+  const Plan p = plan_of(n_rows, n_out, n_in);
+  *tile = p.tile;
+  *buffers = p.tile ? buffers_of(p.tile, (int64_t)p.tiles_i * p.tiles_j * p.split) : 0;
+  *split = p.split;
+  return 0;
+}
+
 extern "C" int or_mx_linear(const or_mx_linear_args* p, void* stream) {
   if (!p) return fail_arg("or_mx_linear: args is NULL");
   const or_mx_linear_args& x = *p;
