@@ -21,8 +21,8 @@
 // hands on its own mean and the squares around that, which are joined without cancellation. In the gradient a thread adds up its
 // columns' A, B and D over its work-group's rows, in a fixed order; a second launch joins the work-groups' sums, unless there are so
 // many groups that each is one work-group's, which then makes the group's gradients by itself. 12720 x 2048 in bf16
-// with gate, scale and shift of 8 groups, among other work: forward 41.2 us for 208 MB (5.1 TB/s, the rate of a copy of 1 GB here
-// 5.15 to 5.5); gradient 71.2 us for 313 MB, 65 of them in the first launch (4.8 TB/s) and 5 in the column sums.
+// with gate, scale and shift of 8 groups, among other work: forward 40.3 us for 208 MB (5.2 TB/s, the rate of a copy of 1 GB here
+// 5.15 to 5.5); gradient 70.2 us for 313 MB, 65 of them in the first launch (4.8 TB/s) and 5 in the column sums.
 #include <math.h>
 
 #include <algorithm>

@@ -10,11 +10,12 @@
 // x / s is exact (a power of two), so the choice of the code has no rounding but its own, and no result depends on the order of
 // anything. The products of codes are exact too; sums and scales are the matrix cores', in fp32.
 //
-// Quantising and reading back are HBM-bound: 8192 x 2048 in bf16 8.9 and 8.3 us for 42 MB (4.8 and 5.1 TB/s). The product of few rows
-// reads W once (1 x 2048 -> 12288 8.4 us for 13 MB, a launch and its latency; 12.6 with the host), that of many is bound by the matrix
-// cores and by what feeds them from LDS: 8192^3 300 us (3.67 PFLOP/s; matrix pipes busy 51% of the time at 1.84 GHz; without loads from HBM
-// 236, without reads of LDS 255, with neither 204, the bare matrix instructions 193), 12720 x 2048 -> 8192 with bias and GELU 178
-// and 16.5 for the launch ahead of it, where the 7 rounds of tiles (6.25 of them full) each pay an epilogue and a start for 8 steps.
+// Quantising and reading back are HBM-bound: 8192 x 2048 in bf16 9.4 and 8.8 us for 42 MB (4.5 and 4.8 TB/s). The product of few rows
+// reads W once (1 x 2048 -> 12288 7.6 us for 13 MB, a launch and its latency; 12 with the host), that of many is bound by the matrix
+// cores and by what feeds them from LDS: 8192^3 in 260 to 270 us (4.1 PFLOP/s; matrix pipes busy 55% of the time at 1.82 GHz; of an
+// earlier 288 without loads from HBM 236, without reads of LDS 255, with neither 204, the bare matrix instructions 193), 12720 x 2048 ->
+// 8192 with bias and GELU in 171, where the 7 rounds of tiles (6.25 of them full) each pay an epilogue and a start for 8 steps, and 16 to
+// 19 for the launch ahead of it, which quantises x (the call 183; with x in 4 bits 174).
 #include <algorithm>
 #include <type_traits>
 
@@ -895,7 +896,7 @@ extern "C" int or_mx_linear(const or_mx_linear_args* p, void* stream) {
   g.tiles_i = plan.tiles_i;
   g.tiles_j = plan.tiles_j;
   // (The rows of a last round that fills few CUs in smaller tiles, in a launch after the others': 12720 x 2048 -> 8192, 1600 tiles in 6.25
-  // rounds, 155 and 13 us, one launch 172.)
+  // rounds, 155 and 13 us, one launch 171.)
   const int64_t n = (int64_t)g.tiles_i * g.tiles_j * g.split;
   const unsigned blocks = (unsigned)((n + 7) / 8 * 8);
   if (plan.tile == 256) launch_tiles<256, 256, 2, 4, 2>(g, blocks, st);

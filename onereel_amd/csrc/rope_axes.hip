@@ -18,8 +18,9 @@
 //
 // HBM-bound: rows are read once and written once. The cosines and sines of a batch of tokens go through LDS, one of a token's
 // pairs a thread, since the heads share them; in the normed form they are ready at the barrier that the rows' sums need anyway.
-// 12720 tokens of 16 heads of 128 in bf16, q and k, among other work: normed 39.6 us for 208 MB (5.2 TB/s, the rate of a copy of 1 GB
-// here 5.15 to 5.5), its gradient 65.7 us for 313 MB (61 in the first launch, 5.1 TB/s, and 5 in the sum of dw). A call for few
+// 12720 tokens of 16 heads of 128 in bf16, q and k, among other work: normed 38.2 us for 208 MB (5.4 TB/s, the rate of a copy of 1 GB
+// here 5.15 to 5.5), its gradient 65.5 us for 313 MB (61 in the first launch, 5.1 TB/s, and 5 in the sum of dw); one tensor rotated
+// alone 19 us for 104 MB, either way (5.5 TB/s), of 63600 tokens 106 us (4.9). A call for few
 // tokens is the launch: 5.2 us on the GPU for 333 tokens of 5 heads of 96 in fp32, 12.6 with the host.
 #include <math.h>
 
